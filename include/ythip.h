@@ -494,6 +494,127 @@ int ythip_argmax_finish(const float* parts, int n_parts, int32_t* token, int32_t
 int ythip_rope_tables(int dim, int max_len, float theta, float* cosv, float* sinv);
 
 /* ------------------------------------------------------------------------
+ * Paged KV cache. No counterpart in the reference, whose KVCache is one ring of rows a
+ * sequence (example/qwen3/src/qwen3.cpp:57-126): sequences hold pages of a shared pool, so
+ * that they grow without moving, share a prompt's rows and give them back.
+ *   pools    K and V [pages][Hkv][page][d], element strides pool_str = (page, head, row) of
+ *            both, d contiguous, rows 16-byte aligned; page = rows of a page, a power of two
+ *            from 16 to 32768. Several layers: [layers][pages]...
+ *   key sums fp32 [pages][Hkv][d], a page's K rows in use added up (sparse attention's scores)
+ *   table    int32 [B][columns], row stride ld_table: row r of sequence b lies in page
+ *            table[b][r / page] at r % page. An id outside [0, pages) is never an address: its
+ *            rows are hidden (attention) or not written (append)
+ *   kv_len   int32 [B], rows in use (clamped to [0, columns * page])
+ *   ref      int32 [pages], the sequences that hold a page; 0: free
+ * All of it lives on the device and is read when the kernels run, so captured HIP graphs
+ * follow it. Pages are taken lowest free first, in the order of the sequences or pairs, so
+ * every result is determined by the arguments. `status`, an int32 on the device or NULL,
+ * collects bits for what was left undone; the call's own status is about its arguments.
+ * ---------------------------------------------------------------------- */
+enum ythip_cache_status {
+    YTHIP_CACHE_ERR_INDEX = 1, /* a sequence, page id, length or count out of range */
+    YTHIP_CACHE_ERR_BUSY = 2,  /* fork: dst holds rows already, or is named twice */
+    YTHIP_CACHE_ERR_FULL = 4   /* no free page, or the table row is too short */
+};
+
+/*
+ * Attention of T new tokens a sequence over its cached rows and the new tokens' own K / V:
+ *   O[b,h,t] = sum over visible j of p_j V_j,  p = softmax(scale * Q[b,h,t] . K_j)
+ * visible: every cached row j < kv_len[b], and of the new tokens those on t's path: t,
+ * parents[b][t], its parent, ... until a value outside [0, child) (a drafted tree; T <= 4096);
+ * parents NULL: 0..t (one token, or a chunk of a prompt). Kn / Vn NULL: cached rows alone.
+ * Query head h reads KV head h / (Hq / Hkv). new_len (device int32[B], NULL: T) gives the new
+ * tokens of each sequence: rows t >= new_len[b] of O are left as they were. A row that sees
+ * nothing, or only scores of -inf, is zero; K and V of what a row does not see never reach
+ * it, NaN and infinities included. scale == 0: 1 / sqrt(d). d in {64, 128}; strides (batch,
+ * head, token), d contiguous, 16-byte aligned rows. Any of Q's type. Workspace:
+ * ythip_paged_attn_workspace_size bytes (0: NULL is accepted).
+ */
+size_t ythip_paged_attn_workspace_size(int dtype, int B, int Hq, int Hkv, int T, int d, int columns, int page);
+int ythip_paged_attn(int dtype, int B, int Hq, int Hkv, int T, int d, const void* Q, const int64_t q_str[3],
+                     const void* Kn, const int64_t kn_str[3], const void* Vn, const int64_t vn_str[3],
+                     const void* Kp, const void* Vp, const int64_t pool_str[3], int pages, int page,
+                     const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len,
+                     const int32_t* parents, int64_t ld_parents, const int32_t* new_len, void* O,
+                     const int64_t o_str[3], float scale, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * ythip_paged_attn over the cached rows of top_k pages, chosen for each new token t and KV
+ * head h by score(i) = (sum of Q[b, h's query heads, t]) . sums[table[b][i]][h] in 64 bits,
+ * over i < ceil(kv_len[b] / page): the last of them always, then the highest scores, equal
+ * ones (and NaN, the lowest) by the lower i. The new tokens are visible as above. sel
+ * (contiguous int32 [B][Hkv][T][top_k]) receives the chosen i ascending, then -1 (-1 alone
+ * for t >= new_len[b]). sums: strides (page, head). top_k <= 4096, columns <= 65536.
+ */
+size_t ythip_paged_attn_sparse_workspace_size(int dtype, int B, int Hq, int Hkv, int T, int d, int columns, int page,
+                                              int top_k);
+int ythip_paged_attn_sparse(int dtype, int B, int Hq, int Hkv, int T, int d, const void* Q, const int64_t q_str[3],
+                            const void* Kn, const int64_t kn_str[3], const void* Vn, const int64_t vn_str[3],
+                            const void* Kp, const void* Vp, const int64_t pool_str[3], int pages, int page,
+                            const float* sums, const int64_t sums_str[2], const int32_t* table, int64_t ld_table,
+                            int columns, const int32_t* kv_len, const int32_t* parents, int64_t ld_parents,
+                            const int32_t* new_len, int top_k, int32_t* sel, void* O, const int64_t o_str[3],
+                            float scale, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Rows into the pages (KVCache::append, example/qwen3/src/qwen3.cpp:70-88, over a table), of
+ * all layers at once: cached row kv_len[b] + i of sequence b takes row path[b][i] of Kn / Vn
+ * (path NULL: row i), i < n_new[b] (NULL: T, the rows of Kn). The table must hold the pages
+ * (ythip_cache_grow); kv_len is the length before. A path entry outside [0, T) writes zeros.
+ * sums (NULL: none), strides (layer, page, head): the sums of every page written to, over its
+ * rows in use, anew. Strides: new_str of both Kn and Vn (layer, batch, head, token), pool_str
+ * (layer, page, head, row). d * element size a multiple of 16, at most 4096. No two sequences
+ * may write one page (ythip_cache_fork sees to that).
+ */
+int ythip_cache_append(int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn,
+                       const int64_t new_str[4], void* Kp, void* Vp, const int64_t pool_str[4], int pages, int page,
+                       float* sums, const int64_t sums_str[3], const int32_t* table, int64_t ld_table, int columns,
+                       const int32_t* kv_len, const int32_t* n_new, const int32_t* path, int64_t ld_path,
+                       void* stream);
+
+/*
+ * The page bookkeeping: each call reads (ref, table, len) and writes (ref_out, table_out,
+ * len_out) whole, in place where they are the same pointers (then ld_out == ld_table).
+ * At most 4096 sequences in a growing table, 4096 pairs in a fork.
+ * grow: sequence b gets the free pages that n_new[b] more rows need, and that length. One
+ *   that is out of range or finds too few pages keeps what it has (pages are handed out in
+ *   the order of b, and after one that finds too few no other gets any).
+ * fork: sequence dst[i], which must be empty, becomes a copy of src[i]: it shares the whole
+ *   pages (ref + 1) and takes a copy of the partial last one in a free page. All pairs read
+ *   the state before the call; a refused pair leaves its dst empty.
+ * free: the pages of seqs[i] lose a user, its row becomes -1, its length 0. An empty one and
+ *   a second mention change nothing.
+ * compact: the pages in use from `live` (their number, int32[1]) on move to the free ones
+ *   below it, both ascending, in every pool; ref and table follow. Freed places keep their
+ *   old bytes.
+ * copy_pages: page src[i] over page dst[i] of every pool. No dst may be another's src or dst.
+ */
+typedef struct ythip_page_pool {
+    void* data;           /* [layers][pages], a page contiguous */
+    int64_t layer_stride; /* bytes, as page_stride and page_bytes; multiples of 4 */
+    int64_t page_stride;
+    int64_t page_bytes;
+} ythip_page_pool;
+int ythip_cache_grow(int B, int columns, int pages, int page, const int32_t* ref, const int32_t* table,
+                     int64_t ld_table, const int32_t* len, const int32_t* n_new, int32_t* ref_out, int32_t* table_out,
+                     int64_t ld_out, int32_t* len_out, int32_t* status, void* stream);
+size_t ythip_cache_fork_workspace_size(int n);
+int ythip_cache_fork(int B, int columns, int pages, int page, const int32_t* ref, const int32_t* table,
+                     int64_t ld_table, const int32_t* len, int n, const int32_t* src, const int32_t* dst,
+                     int32_t* ref_out, int32_t* table_out, int64_t ld_out, int32_t* len_out, int n_pools, int layers,
+                     const ythip_page_pool* pools, int32_t* status, void* workspace, size_t ws_bytes, void* stream);
+int ythip_cache_free(int B, int columns, int pages, int page, const int32_t* ref, const int32_t* table,
+                     int64_t ld_table, const int32_t* len, int n, const int32_t* seqs, int32_t* ref_out,
+                     int32_t* table_out, int64_t ld_out, int32_t* len_out, int32_t* status, void* stream);
+size_t ythip_cache_compact_workspace_size(int pages);
+int ythip_cache_compact(int B, int columns, int pages, int page, const int32_t* ref, const int32_t* table,
+                        int64_t ld_table, const int32_t* len, int32_t* ref_out, int32_t* table_out, int64_t ld_out,
+                        int32_t* live, int n_pools, int layers, const ythip_page_pool* pools, void* workspace,
+                        size_t ws_bytes, void* stream);
+int ythip_cache_copy_pages(int pages, int n, const int32_t* src, const int32_t* dst, int n_pools, int layers,
+                           const ythip_page_pool* pools, int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------
  * .yt checkpoint files (yt::io::YTensorIO, include/ytensor_io.hpp:81-180,
  * src/ytensor_io.inl) read straight into device memory and written from it.
  * Host-side calls: paths and the info/tensor descriptors are HOST memory,

@@ -25,6 +25,20 @@ from .ops import (  # noqa: F401
     scaled_dot_product_attention,
     silu_mul,
 )
+from .paged import (  # noqa: F401
+    CACHE_ERR_BUSY,
+    CACHE_ERR_FULL,
+    CACHE_ERR_INDEX,
+    cache_append,
+    cache_compact,
+    cache_copy_pages,
+    cache_fork,
+    cache_free,
+    cache_grow,
+    paged_attention,
+    paged_sparse_attention,
+    paged_workspace_bytes,
+)
 
 
 def load():
@@ -37,4 +51,6 @@ __all__ = [
     "YthipError", "lib", "gemm", "matmul", "linear", "scaled_dot_product_attention",
     "decode_attention", "rms_norm", "rms_norm_rope", "silu_mul", "embedding", "argmax_step",
     "gemv_fused", "gemv_swiglu", "gemv_attn_merge", "argmax_finish", "io", "masked_matmul", "gemm_masked",
+    "paged_attention", "paged_sparse_attention", "paged_workspace_bytes", "cache_grow", "cache_append", "cache_fork",
+    "cache_free", "cache_compact", "cache_copy_pages", "CACHE_ERR_INDEX", "CACHE_ERR_BUSY", "CACHE_ERR_FULL",
 ]

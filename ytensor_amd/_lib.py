@@ -39,7 +39,14 @@ class YtTensor(ctypes.Structure):
                 ("shape", ctypes.POINTER(ctypes.c_int32)), ("data", ctypes.c_void_p)]
 
 
+class PagePool(ctypes.Structure):
+    """struct ythip_page_pool (include/ythip.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("layer_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("page_bytes", ctypes.c_int64)]
+
+
 _U64 = ctypes.c_uint64
+_PP = ctypes.POINTER(PagePool)
 
 # Every symbol include/ythip.h declares, with its ctypes signature.
 SIGNATURES = {
@@ -88,6 +95,22 @@ SIGNATURES = {
     "ythip_gemv_attn_merge": (_I, [_I, _I, _I, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _F, _F, _P, _I, _P]),
     "ythip_argmax_finish": (_I, [_P, _I, _P, _P, _P, _P]),
     "ythip_rope_tables": (_I, [_I, _I, _F, _P, _P]),
+    "ythip_paged_attn_workspace_size": (ctypes.c_size_t, [_I] * 8),
+    "ythip_paged_attn": (_I, [_I, _I, _I, _I, _I, _I, _P, _LP, _P, _LP, _P, _LP, _P, _P, _LP, _I, _I, _P, _L, _I, _P,
+                              _P, _L, _P, _P, _LP, _F, _P, ctypes.c_size_t, _P]),
+    "ythip_paged_attn_sparse_workspace_size": (ctypes.c_size_t, [_I] * 9),
+    "ythip_paged_attn_sparse": (_I, [_I, _I, _I, _I, _I, _I, _P, _LP, _P, _LP, _P, _LP, _P, _P, _LP, _I, _I, _P, _LP,
+                                     _P, _L, _I, _P, _P, _L, _P, _I, _P, _P, _LP, _F, _P, ctypes.c_size_t, _P]),
+    "ythip_cache_append": (_I, [_I, _I, _I, _I, _I, _I, _P, _P, _LP, _P, _P, _LP, _I, _I, _P, _LP, _P, _L, _I, _P, _P,
+                                _P, _L, _P]),
+    "ythip_cache_grow": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _P, _P, _P, _L, _P, _P, _P]),
+    "ythip_cache_fork_workspace_size": (ctypes.c_size_t, [_I]),
+    "ythip_cache_fork": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _I, _P, _P, _P, _P, _L, _P, _I, _I, _PP, _P, _P,
+                              ctypes.c_size_t, _P]),
+    "ythip_cache_free": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _I, _P, _P, _P, _L, _P, _P, _P]),
+    "ythip_cache_compact_workspace_size": (ctypes.c_size_t, [_I]),
+    "ythip_cache_compact": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _P, _P, _L, _P, _I, _I, _PP, _P, ctypes.c_size_t, _P]),
+    "ythip_cache_copy_pages": (_I, [_I, _I, _P, _P, _I, _I, _PP, _P, _P]),
     "ythip_yt_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "ythip_yt_close": (_I, [_P]),
     "ythip_yt_count": (_I, [_P]),

@@ -1,0 +1,735 @@
+// paged_cache.hip — the paged KV cache's bookkeeping and row movement for gfx950: append,
+// grow, fork, free, compact, copy (include/ythip.h). Everything is decided on the device
+// from (ref, table, len), so no call waits for the host and all of them can be captured.
+//
+// Shape of the work: what a call decides (which free page goes to whom) is a prefix sum over
+// the page counts, done by one workgroup; what it moves (whole pages of every layer, rows) is
+// a second launch over all CUs, bound by HBM (a page is read once and written once).
+
+#include <climits>
+
+#include "launch.hpp"
+
+namespace ythip {
+namespace {
+
+constexpr int PLAN_THREADS = 1024;  // the deciding workgroup
+constexpr int PLAN_ROWS = 4;        // pages a thread looks at per step
+constexpr int MAX_SEQS = 4096;      // sequences of a grow, pairs of a fork: their prefix sums lie in LDS
+constexpr int MAX_COLUMNS = 65536;
+constexpr int MAX_POOLS = 4;
+constexpr int COPY_BYTES = 16384;  // of a page, a workgroup of 256 threads: four 16-byte loads in flight each
+
+__device__ __forceinline__ int pages_of(int rows, int shift) { return (int)(((int64_t)rows + (1ll << shift) - 1) >> shift); }
+__device__ __forceinline__ void flag(int32_t* status, int bits) {
+    if (status != nullptr) atomicOr(status, bits);
+}
+
+// Sum of v over the threads before this one, and over all; every thread of the workgroup calls it.
+__device__ __forceinline__ int block_scan(int v, int* lds, int& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int inc = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int x = __shfl_up(inc, off, 64);
+        if (lane >= off) inc += x;
+    }
+    __syncthreads();  // the last call's totals are read
+    if (lane == 63) lds[wave] = inc;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < PLAN_THREADS / 64; ++w) {
+        const int x = lds[w];
+        before += w < wave ? x : 0;
+        all += x;
+    }
+    total = all;
+    return before + inc - v;
+}
+
+// Calls found(rank, page) for the free pages in ascending order until `want` of them were met
+// (the last step may pass it); returns how many were met.
+template <class F>
+__device__ __forceinline__ int scan_free(const int32_t* ref, int pages, int want, int* lds, F&& found) {
+    int met = 0;
+    for (int base = 0; base < pages && met < want; base += PLAN_THREADS * PLAN_ROWS) {
+        const int p0 = base + (int)threadIdx.x * PLAN_ROWS;
+        bool is_free[PLAN_ROWS];
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < PLAN_ROWS; ++k) {
+            is_free[k] = p0 + k < pages && ref[p0 + k] <= 0;
+            c += is_free[k];
+        }
+        int total;
+        int r = met + block_scan(c, lds, total);
+#pragma unroll
+        for (int k = 0; k < PLAN_ROWS; ++k)
+            if (is_free[k]) found(r++, p0 + k);
+        met += total;
+    }
+    return met;
+}
+
+// (ref, table, len) into the arrays that a call writes, where those are others.
+struct StateArgs {
+    int B, columns, pages;
+    const int32_t *ref, *table, *len;
+    int64_t ld, ld_out;
+    int32_t *ref_out, *table_out, *len_out;
+};
+__global__ __launch_bounds__(256) void cache_state_copy(StateArgs a) {
+    const int64_t step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (a.ref_out != a.ref)
+        for (int64_t i = at; i < a.pages; i += step) a.ref_out[i] = a.ref[i];
+    if (a.len_out != a.len)
+        for (int64_t i = at; i < a.B; i += step) a.len_out[i] = a.len[i];
+    if (a.table_out != a.table)
+        for (int64_t i = at; i < (int64_t)a.B * a.columns; i += step) {
+            const int64_t b = i / a.columns, c = i % a.columns;
+            a.table_out[b * a.ld_out + c] = a.table[b * a.ld + c];
+        }
+}
+
+struct GrowArgs {
+    int B, columns, pages, shift;
+    const int32_t* n_new;
+    int32_t *ref, *table, *len;  // in place
+    int64_t ld;
+    int32_t* status;
+};
+// The prefix sum of the pages that the sequences need gives each its ranks among the free
+// pages; a free page's rank then finds its sequence by bisection.
+__global__ __launch_bounds__(PLAN_THREADS) void cache_grow_kernel(GrowArgs a) {
+    constexpr int LIST = 4096;  // more pages than that: the free ones are looked up twice
+    __shared__ int s_off[MAX_SEQS + 1], s_have[MAX_SEQS], s_list[LIST], s_scan[PLAN_THREADS / 64];
+    const int64_t cap = (int64_t)a.columns << a.shift;
+    int want = 0;
+    for (int base = 0; base < a.B; base += PLAN_THREADS) {
+        const int b = base + (int)threadIdx.x;
+        int need = 0;
+        if (b < a.B) {
+            const int len = a.len[b], n = a.n_new[b];
+            const bool sane = len >= 0 && n >= 0, fits = (int64_t)len + n <= cap;
+            if (!sane) flag(a.status, YTHIP_CACHE_ERR_INDEX);
+            else if (!fits) flag(a.status, YTHIP_CACHE_ERR_FULL);
+            const int have = sane ? pages_of(len, a.shift) : 0;
+            if (sane && fits) need = pages_of(len + n, a.shift) - have;
+            s_have[b] = sane && fits ? have : -1;
+        }
+        int total;
+        const int off = want + block_scan(need, s_scan, total);
+        if (b < a.B) s_off[b] = off;
+        want += total;
+    }
+    if (threadIdx.x == 0) s_off[a.B] = want;
+    __syncthreads();
+    const int met = scan_free(a.ref, a.pages, want, s_scan, [&](int r, int p) {
+        if (r < LIST) s_list[r] = p;
+    });
+    const int got = met < want ? met : want;
+    __syncthreads();
+    auto give = [&](int r, int p) {
+        if (r >= got) return;
+        int lo = 0, hi = a.B;  // s_off[lo] <= r < s_off[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_off[mid] <= r) lo = mid;
+            else hi = mid;
+        }
+        if (s_off[lo + 1] > got) return;  // its sequence finds too few
+        a.table[lo * a.ld + s_have[lo] + (r - s_off[lo])] = p;
+        a.ref[p] = 1;
+    };
+    if (got <= LIST) {
+        for (int r = threadIdx.x; r < got; r += PLAN_THREADS) give(r, s_list[r]);
+    } else {
+        // a page's count is read before any of the same step's is written, and never again
+        scan_free(a.ref, a.pages, got, s_scan, give);
+    }
+    for (int b = threadIdx.x; b < a.B; b += PLAN_THREADS) {
+        if (s_have[b] < 0) continue;
+        if (s_off[b + 1] == s_off[b] || s_off[b + 1] <= got) a.len[b] += a.n_new[b];
+        else flag(a.status, YTHIP_CACHE_ERR_FULL);
+    }
+}
+
+struct PoolSet {
+    char* data[MAX_POOLS];
+    int64_t ls[MAX_POOLS], ps[MAX_POOLS], bytes[MAX_POOLS];
+    int chunks[MAX_POOLS];  // COPY_BYTES pieces of a page
+    bool wide[MAX_POOLS];   // 16-byte moves
+    int n, layers;
+};
+
+// Piece `chunk` of page `from` over page `to`.
+__device__ __forceinline__ void copy_piece(const PoolSet& ps, int k, int layer, int from, int to, int chunk) {
+    const int64_t at = (int64_t)layer * ps.ls[k], b0 = (int64_t)chunk * COPY_BYTES;
+    const char* src = ps.data[k] + at + from * ps.ps[k] + b0;
+    char* dst = ps.data[k] + at + to * ps.ps[k] + b0;
+    const int64_t left = ps.bytes[k] - b0;
+    const int bytes = left < COPY_BYTES ? (int)left : COPY_BYTES;
+    if (ps.wide[k]) {
+        constexpr int N = COPY_BYTES / (256 * 16);
+        const u32x4* s = reinterpret_cast<const u32x4*>(src);
+        u32x4* d = reinterpret_cast<u32x4*>(dst);
+        const int n = bytes >> 4;
+        u32x4 v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i * 256 + (int)threadIdx.x < n) v[i] = s[i * 256 + threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i * 256 + (int)threadIdx.x < n) d[i * 256 + threadIdx.x] = v[i];
+    } else {
+        const uint32_t* s = reinterpret_cast<const uint32_t*>(src);
+        uint32_t* d = reinterpret_cast<uint32_t*>(dst);
+        for (int i = threadIdx.x; i < bytes >> 2; i += 256) d[i] = s[i];
+    }
+}
+
+// Unit u of the copies of `n` pages in all pools: which pool, layer, page and piece.
+struct Unit {
+    int k, layer, i, chunk;
+};
+__device__ __forceinline__ bool unit_of(const PoolSet& ps, int n, int64_t u, Unit& x) {
+    for (x.k = 0; x.k < ps.n; ++x.k) {
+        const int64_t mine = (int64_t)n * ps.layers * ps.chunks[x.k];
+        if (u < mine) {
+            x.chunk = (int)(u % ps.chunks[x.k]);
+            u /= ps.chunks[x.k];
+            x.i = (int)(u % n);
+            x.layer = (int)(u / n);
+            return true;
+        }
+        u -= mine;
+    }
+    return false;
+}
+
+struct ForkArgs {
+    int B, columns, pages, shift, n;
+    const int32_t *src, *dst;
+    int32_t *ref, *table, *len;  // in place
+    int64_t ld;
+    int4* plan;  // per pair: source, destination (-1: refused), whole pages, the fresh page (-1: none)
+    int32_t* status;
+};
+__global__ __launch_bounds__(PLAN_THREADS) void cache_fork_plan(ForkArgs a) {
+    __shared__ int s_dst[MAX_SEQS], s_who[MAX_SEQS], s_page[MAX_SEQS], s_scan[PLAN_THREADS / 64];
+    for (int i = threadIdx.x; i < a.n; i += PLAN_THREADS) s_dst[i] = a.dst[i];
+    __syncthreads();
+    const int64_t cap = (int64_t)a.columns << a.shift;
+    int want = 0;
+    for (int base = 0; base < a.n; base += PLAN_THREADS) {
+        const int i = base + (int)threadIdx.x;
+        int need = 0, bits = 0;
+        int4 pl = {-1, -1, 0, -1};
+        if (i < a.n) {
+            const int s = a.src[i], d = s_dst[i];
+            if (s < 0 || s >= a.B || d < 0 || d >= a.B) {
+                bits = YTHIP_CACHE_ERR_INDEX;
+            } else {
+                const int len = a.len[s];
+                bool twice = false;
+                for (int j = 0; j < i && !twice; ++j) twice = s_dst[j] == d;
+                if (len < 0 || len > cap) bits = YTHIP_CACHE_ERR_INDEX;
+                else if (twice || a.len[d] != 0) bits = YTHIP_CACHE_ERR_BUSY;
+                else {
+                    pl = int4{s, d, len >> a.shift, -1};
+                    need = (len & ((1 << a.shift) - 1)) != 0;
+                }
+            }
+            if (bits) flag(a.status, bits);
+        }
+        int total;
+        const int r = want + block_scan(need, s_scan, total);
+        if (need) s_who[r] = i;
+        if (i < a.n) a.plan[i] = pl;
+        want += total;
+    }
+    __syncthreads();
+    const int met = scan_free(a.ref, a.pages, want, s_scan, [&](int r, int p) {
+        if (r < want) s_page[r] = p;
+    });
+    const int got = met < want ? met : want;
+    __syncthreads();  // every length is read
+    for (int r = threadIdx.x; r < want; r += PLAN_THREADS) {
+        const int i = s_who[r];
+        int4 pl = a.plan[i];
+        if (r < got) {
+            pl.w = s_page[r];
+            a.ref[pl.w] = 1;
+        } else {
+            pl.y = -1;
+            flag(a.status, YTHIP_CACHE_ERR_FULL);
+        }
+        a.plan[i] = pl;
+    }
+    __syncthreads();
+    // a dst is empty, so no pair that takes rows reads a length written here
+    for (int i = threadIdx.x; i < a.n; i += PLAN_THREADS) {
+        const int4 pl = a.plan[i];
+        if (pl.y < 0) continue;
+        const int rest = pl.w >= 0 ? a.len[pl.x] & ((1 << a.shift) - 1) : 0;
+        if (pl.z > 0 || rest > 0) a.len[pl.y] = (pl.z << a.shift) + rest;
+    }
+}
+
+// Workgroups [0, n): pair i's row and page counts; the others its partial page, in every pool.
+__global__ __launch_bounds__(256) void cache_fork_copy(ForkArgs a, PoolSet ps) {
+    const int w = blockIdx.x;
+    if (w < a.n) {
+        const int4 pl = a.plan[w];
+        if (pl.y < 0) return;
+        const int32_t* from = a.table + pl.x * a.ld;
+        int32_t* to = a.table + pl.y * a.ld;
+        for (int c = threadIdx.x; c < pl.z; c += 256) {
+            const int p = from[c];
+            to[c] = p;
+            if (p >= 0 && p < a.pages) atomicAdd(a.ref + p, 1);
+            else flag(a.status, YTHIP_CACHE_ERR_INDEX);
+        }
+        if (threadIdx.x == 0 && pl.w >= 0) to[pl.z] = pl.w;
+        return;
+    }
+    Unit u;
+    if (!unit_of(ps, a.n, w - a.n, u)) return;
+    const int4 pl = a.plan[u.i];
+    if (pl.y < 0 || pl.w < 0) return;
+    const int from = a.table[pl.x * a.ld + pl.z];
+    if (from < 0 || from >= a.pages) {
+        if (threadIdx.x == 0) flag(a.status, YTHIP_CACHE_ERR_INDEX);
+        return;
+    }
+    copy_piece(ps, u.k, u.layer, from, pl.w, u.chunk);
+}
+
+struct FreeArgs {
+    int B, columns, pages, shift;
+    const int32_t* seqs;
+    int32_t *ref, *table, *len;  // in place
+    int64_t ld;
+    int32_t* status;
+};
+// One workgroup a mention; the one that finds rows takes them all (an exchange of the length).
+__global__ __launch_bounds__(256) void cache_free_kernel(FreeArgs a) {
+    __shared__ int s_len;
+    const int s = a.seqs[blockIdx.x];
+    if (s < 0 || s >= a.B) {
+        if (threadIdx.x == 0) flag(a.status, YTHIP_CACHE_ERR_INDEX);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        const int len = atomicExch(a.len + s, 0);
+        if (len < 0) flag(a.status, YTHIP_CACHE_ERR_INDEX);
+        s_len = len;
+    }
+    __syncthreads();
+    if (s_len <= 0) return;
+    const int held = min(pages_of(s_len, a.shift), a.columns);
+    int32_t* row = a.table + s * a.ld;
+    for (int c = threadIdx.x; c < a.columns; c += 256) {
+        if (c < held) {
+            const int p = row[c];
+            if (p < 0 || p >= a.pages) {
+                flag(a.status, YTHIP_CACHE_ERR_INDEX);
+            } else if (atomicSub(a.ref + p, 1) <= 0) {  // it had no user
+                atomicAdd(a.ref + p, 1);
+                flag(a.status, YTHIP_CACHE_ERR_INDEX);
+            }
+        }
+        row[c] = -1;
+    }
+}
+
+struct CompactArgs {
+    int B, columns, pages, shift;
+    const int32_t *ref, *table, *len;
+    int64_t ld, ld_out;
+    int32_t *ref_out, *table_out, *live;
+    int32_t* count;  // moves
+    int32_t *map, *from, *to;
+};
+__global__ __launch_bounds__(PLAN_THREADS) void cache_compact_plan(CompactArgs a) {
+    __shared__ int s_scan[PLAN_THREADS / 64];
+    int mine = 0, live;
+    for (int p = threadIdx.x; p < a.pages; p += PLAN_THREADS) mine += a.ref[p] > 0;
+    block_scan(mine, s_scan, live);
+    // the free pages below `live` and the used ones from there on: as many of each, and a
+    // page is at most one of them, so both counts go through one scan
+    int holes = 0, moves = 0;
+    for (int base = 0; base < a.pages; base += PLAN_THREADS * PLAN_ROWS) {
+        const int p0 = base + (int)threadIdx.x * PLAN_ROWS;
+        bool hole[PLAN_ROWS], move[PLAN_ROWS];
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < PLAN_ROWS; ++k) {
+            const int p = p0 + k, r = p < a.pages ? a.ref[p] : 0;
+            hole[k] = p < live && r <= 0;
+            move[k] = p >= live && r > 0;
+            c += (hole[k] ? 1 : 0) + (move[k] ? 1 << 16 : 0);
+            if (p < a.pages) {
+                if (a.ref_out != a.ref) a.ref_out[p] = r;
+                a.map[p] = p;
+            }
+        }
+        int total;
+        const int r = block_scan(c, s_scan, total);
+        int h = holes + (r & 0xffff), m = moves + (r >> 16);
+#pragma unroll
+        for (int k = 0; k < PLAN_ROWS; ++k) {
+            if (hole[k]) a.to[h++] = p0 + k;
+            if (move[k]) a.from[m++] = p0 + k;
+        }
+        holes += total & 0xffff;
+        moves += total >> 16;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < moves; i += PLAN_THREADS) {
+        const int f = a.from[i], t = a.to[i];
+        a.ref_out[t] = a.ref[f];
+        a.ref_out[f] = 0;
+        a.map[f] = t;
+    }
+    if (threadIdx.x == 0) {
+        *a.count = moves;
+        *a.live = live;
+    }
+}
+
+__global__ __launch_bounds__(256) void cache_compact_move(CompactArgs a, PoolSet ps) {
+    const int64_t entries = (int64_t)a.B * a.columns, step = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += step) {
+        const int64_t b = i / a.columns;
+        const int c = (int)(i % a.columns), p = a.table[b * a.ld + c], len = a.len[b];
+        const bool held = len > 0 && c < pages_of(len, a.shift) && p >= 0 && p < a.pages;
+        a.table_out[b * a.ld_out + c] = held ? a.map[p] : p;
+    }
+    const int n = *a.count;
+    if (n <= 0) return;
+    Unit u;
+    for (int64_t w = blockIdx.x; unit_of(ps, n, w, u); w += gridDim.x)
+        copy_piece(ps, u.k, u.layer, a.from[u.i], a.to[u.i], u.chunk);
+}
+
+__global__ __launch_bounds__(256) void cache_copy_kernel(int pages, int n, const int32_t* src, const int32_t* dst,
+                                                         PoolSet ps, int32_t* status) {
+    Unit u;
+    if (!unit_of(ps, n, blockIdx.x, u)) return;
+    const int from = src[u.i], to = dst[u.i];
+    if (from < 0 || from >= pages || to < 0 || to >= pages) {
+        if (threadIdx.x == 0) flag(status, YTHIP_CACHE_ERR_INDEX);
+        return;
+    }
+    copy_piece(ps, u.k, u.layer, from, to, u.chunk);
+}
+
+struct AppendArgs {
+    int layers, B, Hkv, T, pages, shift, slots, columns;
+    const char *Kn, *Vn;
+    char *Kp, *Vp;
+    int64_t ns0, ns1, ns2, ns3;  // bytes
+    int64_t ps0, ps1, ps2, ps3;
+    float* sums;
+    int64_t ss0, ss1, ss2;  // elements
+    const int32_t *table, *kv_len, *n_new, *path;
+    int64_t ld_table, ld_path;
+    int chunks;  // 16-byte chunks of a row
+};
+// A workgroup takes one page that the new rows of one (layer, sequence, KV head) touch:
+// thread = (row group, 16-byte chunk), so that a row moves as one run of bytes. It writes the
+// new rows and, for the key sums, adds every row in use to fp32 partials in registers, then the
+// row groups in order, so the sum is determined by the page's rows alone.
+template <class T>
+__global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
+    constexpr int VN = Vec<T>::n;
+    __shared__ float s_sum[256 * VN];
+    int w = blockIdx.x;
+    const int i = w % a.slots;
+    w /= a.slots;
+    const int h = w % a.Hkv;
+    w /= a.Hkv;
+    const int b = w % a.B, l = w / a.B;
+    const int page = 1 << a.shift;
+    const int len = a.kv_len[b];
+    int n = a.n_new != nullptr ? min(a.n_new[b], a.T) : a.T;
+    if (len < 0 || n <= 0) return;
+    const int slot = (len >> a.shift) + i;
+    const int64_t end = (int64_t)len + n;  // rows in use afterwards
+    if (slot >= a.columns || ((int64_t)slot << a.shift) >= end) return;
+    const int p = a.table[b * a.ld_table + slot];
+    if (p < 0 || p >= a.pages) return;
+    const int r0 = slot << a.shift;                              // the page's first row
+    const int lo = max(len - r0, 0), hi = (int)min(end - r0, (int64_t)page);  // its new rows
+    const int rows = 256 / a.chunks;                             // rows at a time
+    const int rg = (int)threadIdx.x / a.chunks, ch = (int)threadIdx.x % a.chunks;
+    const bool works = rg < rows;
+    char* kp = a.Kp + l * a.ps0 + p * a.ps1 + h * a.ps2 + ch * 16;
+    char* vp = a.Vp + l * a.ps0 + p * a.ps1 + h * a.ps2 + ch * 16;
+    const char* kn = a.Kn + l * a.ns0 + b * a.ns1 + h * a.ns2 + ch * 16;
+    const char* vn = a.Vn + l * a.ns0 + b * a.ns1 + h * a.ns2 + ch * 16;
+    float acc[VN];
+#pragma unroll
+    for (int e = 0; e < VN; ++e) acc[e] = 0.f;
+    auto add = [&](u32x4 v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (VN == 4) acc[e] += __uint_as_float(v[e]);
+            else {
+                acc[2 * e] += lo_as_f32(T{}, v[e]);
+                acc[2 * e + 1] += hi_as_f32(T{}, v[e]);
+            }
+        }
+    };
+    for (int r = works ? rg : hi; r < hi; r += rows) {
+        if (r < lo) {
+            if (a.sums != nullptr) add(*reinterpret_cast<const u32x4*>(kp + r * a.ps3));
+            continue;
+        }
+        const int j = r0 + r - len;
+        const int from = a.path != nullptr ? a.path[b * a.ld_path + j] : j;
+        u32x4 k = {0u, 0u, 0u, 0u}, v = {0u, 0u, 0u, 0u};
+        if (from >= 0 && from < a.T) {
+            k = *reinterpret_cast<const u32x4*>(kn + from * a.ns3);
+            v = *reinterpret_cast<const u32x4*>(vn + from * a.ns3);
+        }
+        *reinterpret_cast<u32x4*>(kp + r * a.ps3) = k;
+        *reinterpret_cast<u32x4*>(vp + r * a.ps3) = v;
+        if (a.sums != nullptr) add(k);
+    }
+    if (a.sums == nullptr) return;
+    const int d = a.chunks * VN;
+    if (works) {
+#pragma unroll
+        for (int e = 0; e < VN; ++e) s_sum[rg * d + ch * VN + e] = acc[e];
+    }
+    __syncthreads();
+    float* out = a.sums + l * a.ss0 + p * a.ss1 + h * a.ss2;
+    for (int e = threadIdx.x; e < d; e += 256) {
+        float t = 0.f;
+        for (int g = 0; g < rows; ++g) t += s_sum[g * d + e];
+        out[e] = t;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+int page_shift(int page) {
+    for (int s = 4; s <= 15; ++s)
+        if (page == 1 << s) return s;
+    return -1;
+}
+
+int check_table(const char* who, int B, int columns, int pages, int page, const void* table, int64_t ld,
+                const void* len) {
+    if (B < 0 || columns < 0 || pages < 0) return fail(YTHIP_EINVAL, "%s: negative size", who);
+    if (page_shift(page) < 0) return fail(YTHIP_EINVAL, "%s: a page of %d rows (a power of two from 16 to 32768)", who, page);
+    if (columns > MAX_COLUMNS || (int64_t)columns * page > INT_MAX)
+        return fail(YTHIP_EUNSUPPORTED, "%s: %d columns of %d rows (at most 65536 columns, 2^31 - 1 rows)", who, columns, page);
+    if (B > 0 && (table == nullptr || len == nullptr)) return fail(YTHIP_EINVAL, "%s: table or len is NULL", who);
+    if (ld < columns) return fail(YTHIP_EINVAL, "%s: a table row of %d entries at a stride of %lld", who, columns, (long long)ld);
+    return 0;
+}
+
+int check_state(const char* who, int B, int columns, int pages, int page, const void* ref, const void* table,
+                int64_t ld, const void* len, const void* ref_out, const void* table_out, int64_t ld_out,
+                const void* len_out) {
+    if (const int st = check_table(who, B, columns, pages, page, table, ld, len)) return st;
+    if (const int st = check_table(who, B, columns, pages, page, table_out, ld_out, len_out)) return st;
+    if (pages > 0 && (ref == nullptr || ref_out == nullptr)) return fail(YTHIP_EINVAL, "%s: ref is NULL", who);
+    if (table == table_out && ld != ld_out) return fail(YTHIP_EINVAL, "%s: one table with two strides", who);
+    return 0;
+}
+
+int make_pools(const char* who, int n_pools, int layers, const ythip_page_pool* pools, PoolSet& ps) {
+    if (n_pools < 0 || n_pools > MAX_POOLS || layers < 0) return fail(YTHIP_EINVAL, "%s: %d pools of %d layers", who, n_pools, layers);
+    if (n_pools > 0 && pools == nullptr) return fail(YTHIP_EINVAL, "%s: pools is NULL", who);
+    ps.n = n_pools;
+    ps.layers = layers;
+    for (int k = 0; k < n_pools; ++k) {
+        const ythip_page_pool& p = pools[k];
+        const int64_t all = (int64_t)(uintptr_t)p.data | p.layer_stride | p.page_stride | p.page_bytes;
+        if (p.data == nullptr || p.page_bytes <= 0 || (all & 3) != 0 || p.page_bytes > ((int64_t)INT_MAX / 2) * COPY_BYTES)
+            return fail(YTHIP_EINVAL, "%s: pool %d (data, strides and bytes: multiples of 4, bytes > 0)", who, k);
+        ps.data[k] = static_cast<char*>(p.data);
+        ps.ls[k] = p.layer_stride;
+        ps.ps[k] = p.page_stride;
+        ps.bytes[k] = p.page_bytes;
+        ps.chunks[k] = (int)((p.page_bytes + COPY_BYTES - 1) / COPY_BYTES);
+        ps.wide[k] = (all & 15) == 0;
+    }
+    return 0;
+}
+
+int64_t units(const PoolSet& ps, int64_t n) {
+    int64_t u = 0;
+    for (int k = 0; k < ps.n; ++k) u += n * ps.layers * ps.chunks[k];
+    return u;
+}
+
+void copy_state(const StateArgs& a, hipStream_t s) {
+    if (a.ref == a.ref_out && a.table == a.table_out && a.len == a.len_out) return;
+    int64_t most = (int64_t)a.B * a.columns;
+    if (a.pages > most) most = a.pages;
+    const int64_t grid = (most + 255) / 256;
+    if (grid > 0) cache_state_copy<<<(int)(grid < 1024 ? grid : 1024), 256, 0, s>>>(a);
+}
+
+}  // namespace
+}  // namespace ythip
+
+using namespace ythip;
+
+extern "C" {
+
+__attribute__((visibility("default"))) int ythip_cache_append(
+    int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn, const int64_t new_str[4],
+    void* Kp, void* Vp, const int64_t pool_str[4], int pages, int page, float* sums, const int64_t sums_str[3],
+    const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len, const int32_t* n_new,
+    const int32_t* path, int64_t ld_path, void* stream) {
+    const char* who = "ythip_cache_append";
+    if (dtype != YTHIP_F32 && dtype != YTHIP_F16 && dtype != YTHIP_BF16) return fail(YTHIP_EINVAL, "%s: invalid dtype %d", who, dtype);
+    if (layers < 0 || B < 0 || Hkv < 0 || T < 0 || d <= 0) return fail(YTHIP_EINVAL, "%s: bad size", who);
+    if (const int st = check_table(who, B, columns, pages, page, table, ld_table, kv_len)) return st;
+    if (!Kn || !Vn || !Kp || !Vp || !new_str || !pool_str || (sums && !sums_str)) return fail(YTHIP_EINVAL, "%s: NULL argument", who);
+    const int es = dtype == YTHIP_F32 ? 4 : 2;
+    if ((int64_t)d * es % 16 != 0 || (int64_t)d * es > 4096)
+        return fail(YTHIP_EUNSUPPORTED, "%s: rows of %lld bytes (a multiple of 16, at most 4096)", who, (long long)d * es);
+    int64_t all = (int64_t)(uintptr_t)Kn | (int64_t)(uintptr_t)Vn | (int64_t)(uintptr_t)Kp | (int64_t)(uintptr_t)Vp;
+    for (int i = 0; i < 4; ++i) all |= new_str[i] * es | pool_str[i] * es;
+    if ((all & 15) != 0) return fail(YTHIP_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
+    if (layers == 0 || B == 0 || Hkv == 0 || T == 0 || pages == 0 || columns == 0) return 0;
+    AppendArgs a;
+    a.layers = layers, a.B = B, a.Hkv = Hkv, a.T = T, a.pages = pages, a.shift = page_shift(page), a.columns = columns;
+    a.slots = (int)(((int64_t)T + page - 2) / page + 1);  // pages that T rows touch at most
+    a.Kn = static_cast<const char*>(Kn), a.Vn = static_cast<const char*>(Vn);
+    a.Kp = static_cast<char*>(Kp), a.Vp = static_cast<char*>(Vp);
+    a.ns0 = new_str[0] * es, a.ns1 = new_str[1] * es, a.ns2 = new_str[2] * es, a.ns3 = new_str[3] * es;
+    a.ps0 = pool_str[0] * es, a.ps1 = pool_str[1] * es, a.ps2 = pool_str[2] * es, a.ps3 = pool_str[3] * es;
+    a.sums = sums;
+    a.ss0 = sums ? sums_str[0] : 0, a.ss1 = sums ? sums_str[1] : 0, a.ss2 = sums ? sums_str[2] : 0;
+    a.table = table, a.kv_len = kv_len, a.n_new = n_new, a.path = path, a.ld_table = ld_table, a.ld_path = ld_path;
+    a.chunks = (int)((int64_t)d * es / 16);
+    const int64_t grid = (int64_t)a.slots * Hkv * B * layers;
+    if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pages to write", who, (long long)grid);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == YTHIP_F32) cache_append_kernel<F32><<<(int)grid, 256, 0, s>>>(a);
+    else if (dtype == YTHIP_F16) cache_append_kernel<F16><<<(int)grid, 256, 0, s>>>(a);
+    else cache_append_kernel<BF16><<<(int)grid, 256, 0, s>>>(a);
+    return status_of(hipGetLastError());
+}
+
+__attribute__((visibility("default"))) int ythip_cache_grow(int B, int columns, int pages, int page, const int32_t* ref,
+                                                            const int32_t* table, int64_t ld_table, const int32_t* len,
+                                                            const int32_t* n_new, int32_t* ref_out, int32_t* table_out,
+                                                            int64_t ld_out, int32_t* len_out, int32_t* status,
+                                                            void* stream) {
+    const char* who = "ythip_cache_grow";
+    if (const int st = check_state(who, B, columns, pages, page, ref, table, ld_table, len, ref_out, table_out, ld_out, len_out)) return st;
+    if (B > MAX_SEQS) return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences (at most %d)", who, B, MAX_SEQS);
+    if (B > 0 && n_new == nullptr) return fail(YTHIP_EINVAL, "%s: n_new is NULL", who);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    copy_state({B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, s);
+    if (B > 0) cache_grow_kernel<<<1, PLAN_THREADS, 0, s>>>({B, columns, pages, page_shift(page), n_new, ref_out, table_out, len_out, ld_out, status});
+    return status_of(hipGetLastError());
+}
+
+__attribute__((visibility("default"))) size_t ythip_cache_fork_workspace_size(int n) {
+    return n > 0 ? (size_t)n * sizeof(int4) : 0;
+}
+
+__attribute__((visibility("default"))) int ythip_cache_fork(int B, int columns, int pages, int page, const int32_t* ref,
+                                                            const int32_t* table, int64_t ld_table, const int32_t* len,
+                                                            int n, const int32_t* src, const int32_t* dst,
+                                                            int32_t* ref_out, int32_t* table_out, int64_t ld_out,
+                                                            int32_t* len_out, int n_pools, int layers,
+                                                            const ythip_page_pool* pools, int32_t* status,
+                                                            void* workspace, size_t ws_bytes, void* stream) {
+    const char* who = "ythip_cache_fork";
+    if (const int st = check_state(who, B, columns, pages, page, ref, table, ld_table, len, ref_out, table_out, ld_out, len_out)) return st;
+    if (n < 0 || (n > 0 && (!src || !dst))) return fail(YTHIP_EINVAL, "%s: %d pairs, or src or dst is NULL", who, n);
+    if (n > MAX_SEQS) return fail(YTHIP_EUNSUPPORTED, "%s: %d pairs (at most %d)", who, n, MAX_SEQS);
+    PoolSet ps;
+    if (const int st = make_pools(who, n_pools, layers, pools, ps)) return st;
+    const size_t need = ythip_cache_fork_workspace_size(n);
+    if (need > 0 && (workspace == nullptr || ws_bytes < need || ((uintptr_t)workspace & 15) != 0))
+        return fail(YTHIP_EINVAL, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, need, ws_bytes);
+    const int64_t grid = n + units(ps, n);
+    if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pieces to copy", who, (long long)grid);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    copy_state({B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, s);
+    if (n > 0) {
+        const ForkArgs a = {B, columns, pages, page_shift(page), n, src, dst, ref_out, table_out, len_out, ld_out, static_cast<int4*>(workspace), status};
+        cache_fork_plan<<<1, PLAN_THREADS, 0, s>>>(a);
+        cache_fork_copy<<<(int)grid, 256, 0, s>>>(a, ps);
+    }
+    return status_of(hipGetLastError());
+}
+
+__attribute__((visibility("default"))) int ythip_cache_free(int B, int columns, int pages, int page, const int32_t* ref,
+                                                            const int32_t* table, int64_t ld_table, const int32_t* len,
+                                                            int n, const int32_t* seqs, int32_t* ref_out,
+                                                            int32_t* table_out, int64_t ld_out, int32_t* len_out,
+                                                            int32_t* status, void* stream) {
+    const char* who = "ythip_cache_free";
+    if (const int st = check_state(who, B, columns, pages, page, ref, table, ld_table, len, ref_out, table_out, ld_out, len_out)) return st;
+    if (n < 0 || (n > 0 && !seqs)) return fail(YTHIP_EINVAL, "%s: %d sequences, or seqs is NULL", who, n);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    copy_state({B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, s);
+    if (n > 0) cache_free_kernel<<<n, 256, 0, s>>>({B, columns, pages, page_shift(page), seqs, ref_out, table_out, len_out, ld_out, status});
+    return status_of(hipGetLastError());
+}
+
+__attribute__((visibility("default"))) size_t ythip_cache_compact_workspace_size(int pages) {
+    return pages > 0 ? (4 + 3 * (size_t)pages) * sizeof(int32_t) : 16;
+}
+
+__attribute__((visibility("default"))) int ythip_cache_compact(int B, int columns, int pages, int page,
+                                                               const int32_t* ref, const int32_t* table,
+                                                               int64_t ld_table, const int32_t* len, int32_t* ref_out,
+                                                               int32_t* table_out, int64_t ld_out, int32_t* live,
+                                                               int n_pools, int layers, const ythip_page_pool* pools,
+                                                               void* workspace, size_t ws_bytes, void* stream) {
+    const char* who = "ythip_cache_compact";
+    if (const int st = check_state(who, B, columns, pages, page, ref, table, ld_table, len, ref_out, table_out, ld_out, len)) return st;
+    if (live == nullptr) return fail(YTHIP_EINVAL, "%s: live is NULL", who);
+    PoolSet ps;
+    if (const int st = make_pools(who, n_pools, layers, pools, ps)) return st;
+    const size_t need = ythip_cache_compact_workspace_size(pages);
+    if (workspace == nullptr || ws_bytes < need || ((uintptr_t)workspace & 3) != 0)
+        return fail(YTHIP_EINVAL, "%s: needs a workspace of %zu bytes, got %zu", who, need, ws_bytes);
+    int32_t* ws = static_cast<int32_t*>(workspace);
+    const CompactArgs a = {B, columns, pages, page_shift(page), ref, table, len, ld_table, ld_out, ref_out, table_out, live,
+                           ws, ws + 4, ws + 4 + pages, ws + 4 + 2 * (int64_t)pages};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    cache_compact_plan<<<1, PLAN_THREADS, 0, s>>>(a);
+    // how many pages move is known on the device alone: enough workgroups to fill the chip
+    // (8 on each of 256 CUs) walk the pieces
+    int64_t grid = units(ps, pages / 2);
+    const int64_t entries = ((int64_t)B * columns + 255) / 256;
+    if (grid < entries) grid = entries;
+    if (grid > 2048) grid = 2048;
+    if (grid > 0) cache_compact_move<<<(int)grid, 256, 0, s>>>(a, ps);
+    return status_of(hipGetLastError());
+}
+
+__attribute__((visibility("default"))) int ythip_cache_copy_pages(int pages, int n, const int32_t* src,
+                                                                  const int32_t* dst, int n_pools, int layers,
+                                                                  const ythip_page_pool* pools, int32_t* status,
+                                                                  void* stream) {
+    const char* who = "ythip_cache_copy_pages";
+    if (pages < 0 || n < 0 || (n > 0 && (!src || !dst))) return fail(YTHIP_EINVAL, "%s: %d pages, or src or dst is NULL", who, n);
+    PoolSet ps;
+    if (const int st = make_pools(who, n_pools, layers, pools, ps)) return st;
+    const int64_t grid = units(ps, n);
+    if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pieces to copy", who, (long long)grid);
+    if (grid == 0) return 0;
+    cache_copy_kernel<<<(int)grid, 256, 0, static_cast<hipStream_t>(stream)>>>(pages, n, src, dst, ps, status);
+    return status_of(hipGetLastError());
+}
+
+}  // extern "C"

@@ -1,0 +1,373 @@
+"""Operators of the paged KV cache over libythip.so (include/ythip.h, "Paged KV cache").
+
+The reference keeps a ring of rows a sequence (KVCache, example/qwen3/src/qwen3.cpp:57-126);
+here sequences hold pages of a shared pool, so that they grow without moving, share a
+prompt's rows and give them back:
+
+    k_pool, v_pool [P, Hkv, page, d]   (layers in front: [L, P, Hkv, page, d])
+    key_sums       [P, Hkv, d] float32 a page's K rows in use added up ([L, P, Hkv, d])
+    table          int32 [B, columns]  row r of sequence b: page table[b, r // page], row r % page
+    kv_len         int32 [B]           rows in use
+    ref            int32 [P]           sequences that hold a page (0: free)
+
+    paged_attention(...)         new tokens (one, a drafted tree, a chunk) over the cache
+    paged_sparse_attention(...)  the same over the pages that a score selects
+    cache_grow / cache_append    pages for new rows; the rows into them
+    cache_fork / cache_free      sequences that share another's pages; their end
+    cache_compact / cache_copy_pages
+
+Everything is read on the device when the kernels run, and no call waits for the host, so a
+step (attend, grow, append) can be captured as one HIP graph. Argument problems raise
+ValueError or YthipError; what only the device can see (no free page, an index out of range)
+sets bits of `status`, an int32 device tensor (CACHE_ERR_*).
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import functools
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .ops import _DT, _code, _stream
+
+CACHE_ERR_INDEX, CACHE_ERR_BUSY, CACHE_ERR_FULL = 1, 2, 4
+
+
+@functools.lru_cache(maxsize=4096)
+def _i64(vals: tuple) -> ctypes.Array:
+    """Strides for the C call, which reads them only."""
+    return _lib.i64array(vals)
+
+
+def _same_device(first: torch.Tensor, *rest) -> contextlib.AbstractContextManager | None:
+    """All on one GPU; a context that makes it the current one where it is not."""
+    if not first.is_cuda:
+        raise ValueError("ytensor_amd operators take device (cuda/hip) tensors")
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+    return None if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+
+
+def _ints(name: str, t: torch.Tensor, *shape) -> torch.Tensor:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return t
+
+
+def _rows(t: torch.Tensor, es: int) -> torch.Tensor:
+    """t with its last dim contiguous and 16-byte aligned rows (a copy where it has neither)."""
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in st[:-1]):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, scale, out,
+               workspace):
+    guard = _same_device(q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, out, workspace)
+    if guard is not None:
+        with guard:
+            return _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len,
+                              scale, out, workspace)
+    if q.dim() != 4 or k_pool.dim() != 4:
+        raise ValueError("q must be [B, Hq, T, d] and the pools [P, Hkv, page, d]")
+    B, Hq, T, d = q.shape
+    P, Hkv, page, dk = k_pool.shape
+    code, dt = _code(q), q.dtype
+    if dk != d or Hkv == 0 or Hq % Hkv != 0:
+        raise ValueError(f"q {list(q.shape)} does not fit pools {list(k_pool.shape)}")
+    if k_pool.dtype != dt or v_pool.dtype != dt:
+        raise ValueError("q and the pools must share a dtype")
+    if v_pool.shape != k_pool.shape or v_pool.stride() != k_pool.stride() or k_pool.stride(3) != 1:
+        raise ValueError("k_pool and v_pool must share a shape and strides, with d contiguous")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    es = q.element_size()
+    q = _rows(q, es)
+    if k_new is not None:
+        if k_new.shape != (B, Hkv, T, d) or v_new.shape != (B, Hkv, T, d) or k_new.dtype != dt or v_new.dtype != dt:
+            raise ValueError(f"k_new and v_new must be {dt} {[B, Hkv, T, d]}")
+        k_new, v_new = _rows(k_new, es), _rows(v_new, es)
+    if table.dim() != 2:
+        raise ValueError("table must be int32 [B, columns]")
+    columns = table.shape[1]
+    _ints("table", table, B, columns)
+    if table.stride(1) != 1 and columns > 1:
+        raise ValueError("table must have contiguous rows")
+    kv_len = _ints("kv_len", kv_len, B).contiguous()
+    if parents is not None:
+        parents = _ints("parents", parents, B, T).contiguous()
+    if tree_len is not None:
+        tree_len = _ints("tree_len", tree_len, B).contiguous()
+    if out is None:
+        out = (torch.empty if tree_len is None else torch.zeros)((B, Hq, T, d), dtype=dt, device=q.device)
+    elif out.shape != (B, Hq, T, d) or out.dtype != dt or out.stride(3) != 1:
+        raise ValueError(f"out must be {dt} {[B, Hq, T, d]} with d contiguous")
+    L = _lib.lib()
+    args = (code, B, Hq, Hkv, T, d, q.data_ptr(), _i64(q.stride()[:3]),
+            None if k_new is None else k_new.data_ptr(), None if k_new is None else _i64(k_new.stride()[:3]),
+            None if v_new is None else v_new.data_ptr(), None if v_new is None else _i64(v_new.stride()[:3]),
+            k_pool.data_ptr(), v_pool.data_ptr(), _i64(k_pool.stride()[:3]), P, page)
+    tail = (table.data_ptr(), max(table.stride(0), columns), columns, kv_len.data_ptr(),
+            None if parents is None else parents.data_ptr(), T, None if tree_len is None else tree_len.data_ptr())
+    need = _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k or 0)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ws = (None, 0) if not need else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    to = (out.data_ptr(), _i64(out.stride()[:3]), float(scale), *ws, _stream())
+    if top_k is None:
+        st = L.ythip_paged_attn(*args, *tail, *to)
+        if st:
+            check(st, "ythip_paged_attn")
+        return out
+    if key_sums.dtype != torch.float32 or key_sums.shape != (P, Hkv, d) or key_sums.stride(2) != 1:
+        raise ValueError(f"key_sums must be float32 {[P, Hkv, d]} with d contiguous")
+    sel = torch.empty((B, Hkv, T, top_k), dtype=torch.int32, device=q.device)
+    st = L.ythip_paged_attn_sparse(*args, key_sums.data_ptr(), _i64(key_sums.stride()[:2]), *tail, top_k,
+                                   sel.data_ptr(), *to)
+    if st:
+        check(st, "ythip_paged_attn_sparse")
+    return out, sel
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k) -> int:
+    if top_k:
+        return int(_lib.lib().ythip_paged_attn_sparse_workspace_size(code, B, Hq, Hkv, T, d, columns, page, top_k))
+    return int(_lib.lib().ythip_paged_attn_workspace_size(code, B, Hq, Hkv, T, d, columns, page))
+
+
+def paged_workspace_bytes(dtype: torch.dtype, B: int, Hq: int, Hkv: int, T: int, d: int, columns: int, page: int,
+                          top_k: int = 0) -> int:
+    """Bytes that paged_attention (top_k 0) or paged_sparse_attention writes."""
+    return _workspace(_DT[dtype], B, Hq, Hkv, T, d, columns, page, top_k)
+
+
+def paged_attention(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None, k_pool: torch.Tensor,
+                    v_pool: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor,
+                    parents: torch.Tensor | None = None, tree_len: torch.Tensor | None = None, scale: float = 0.0,
+                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of T new tokens a sequence, q [B, Hq, T, d], over the kv_len[b] cached rows of
+    a layer's pools and the tokens' own k_new / v_new [B, Hkv, T, d] (None: the cache alone).
+
+    parents int32 [B, T]: the new tokens are a drafted tree, token t sees itself, parents[b, t],
+    that one's parent, ... up to a value outside [0, child) (the cache's last row). None: token t
+    sees the new tokens 0..t (T = 1: a decode step; a chunk of a prompt). tree_len int32 [B]: the
+    new tokens of each sequence; rows behind them in `out` are left as they were (zeros in an
+    `out` made here). Query head h reads KV head h // (Hq // Hkv). A page id outside the pool
+    hides its rows; a row that sees nothing is zero. d 64 or 128, page a power of two >= 16.
+    Returns out [B, Hq, T, d]."""
+    return _attention(None, q, k_new, v_new, k_pool, v_pool, None, table, kv_len, parents, tree_len, scale, out,
+                      workspace)
+
+
+def paged_sparse_attention(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None,
+                           k_pool: torch.Tensor, v_pool: torch.Tensor, key_sums: torch.Tensor, table: torch.Tensor,
+                           kv_len: torch.Tensor, top_k: int, parents: torch.Tensor | None = None,
+                           tree_len: torch.Tensor | None = None, scale: float = 0.0,
+                           out: torch.Tensor | None = None,
+                           workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """paged_attention over top_k of the sequence's pages, chosen for each new token and KV head:
+    the last page, then those with the highest (sum of the token's queries of that KV head) .
+    key_sums[page] (in 64 bits; equal ones and NaN, the lowest, by the lower index). key_sums as
+    cache_append keeps them. Returns (out, sel): sel int32 [B, Hkv, T, top_k] holds the chosen
+    table columns ascending, then -1 (-1 alone for t >= tree_len[b])."""
+    if top_k < 1:
+        raise ValueError(f"top_k = {top_k}: at least one page")
+    return _attention(int(top_k), q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, scale,
+                      out, workspace)
+
+
+# ---------------------------------------------------------------------------
+# The cache's rows and pages
+# ---------------------------------------------------------------------------
+
+def _state(ref, table, kv_len, out, page, status, *rest):
+    """(arguments up to len, arguments of the outputs, the outputs) of a bookkeeping call."""
+    if table.dim() != 2 or ref.dim() != 1:
+        raise ValueError("table must be int32 [B, columns] and ref int32 [P]")
+    B, columns = table.shape
+    out = (ref, table, kv_len) if out is None else tuple(out)
+    for r, t, n in ((ref, table, kv_len), out):
+        _ints("ref", r, ref.shape[0])
+        _ints("table", t, B, columns)
+        _ints("kv_len", n, B)
+        if not r.is_contiguous() or not n.is_contiguous() or (columns > 1 and t.stride(1) != 1):
+            raise ValueError("ref and kv_len must be contiguous, table with contiguous rows")
+    if status is not None:
+        _ints("status", status, 1)
+    ld = lambda t: max(t.stride(0), columns)  # noqa: E731
+    head = (B, columns, ref.shape[0], int(page), ref.data_ptr(), table.data_ptr(), ld(table), kv_len.data_ptr())
+    tail = (out[0].data_ptr(), out[1].data_ptr(), ld(out[1]), out[2].data_ptr())
+    return head, tail, out
+
+
+def _list(name: str, t: torch.Tensor) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1:
+        raise ValueError(f"{name} must be int32 [n]")
+    return t.contiguous()
+
+
+def _pools(pools, pages: int):
+    """ythip_page_pool descriptors of [L, P, ...] tensors whose pages are contiguous."""
+    arr, layers = (_lib.PagePool * max(len(pools), 1))(), 0
+    for i, t in enumerate(pools):
+        if t.dim() < 3 or t.shape[1] != pages or (i and t.shape[0] != layers):
+            raise ValueError(f"pool {i} has shape {list(t.shape)}; needs [layers, {pages}, ...]")
+        layers, inner = t.shape[0], 1
+        for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
+            if size != 1 and stride != inner:
+                raise ValueError(f"pool {i}: a page must be contiguous")
+            inner *= size
+        es = t.element_size()
+        arr[i] = _lib.PagePool(t.data_ptr(), t.stride(0) * es, t.stride(1) * es, inner * es)
+    return len(pools), layers, arr
+
+
+def _guarded(fn):
+    """Runs fn on the GPU of its tensors (they must share one)."""
+    @functools.wraps(fn)
+    def call(*args, **kw):
+        flat = []
+        for v in (*args, *kw.values()):
+            flat += list(v) if isinstance(v, (tuple, list)) else [v]
+        ts = [t for t in flat if isinstance(t, torch.Tensor)]
+        if not ts:
+            raise ValueError("ytensor_amd operators take device (cuda/hip) tensors")
+        guard = _same_device(*ts)
+        if guard is None:
+            return fn(*args, **kw)
+        with guard:
+            return fn(*args, **kw)
+    return call
+
+
+@_guarded
+def cache_grow(ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, n_new: torch.Tensor, page: int,
+               out=None, status: torch.Tensor | None = None):
+    """Pages (lowest free first) for n_new[b] more rows of each sequence, and the new lengths.
+    A sequence that finds too few pages or columns keeps what it has (status). out: (ref,
+    table, kv_len) to write instead of the given ones. Returns those written. cache_append
+    takes the kv_len from before."""
+    head, tail, out = _state(ref, table, kv_len, out, page, status)
+    n_new = _ints("n_new", n_new, table.shape[0]).contiguous()
+    check(_lib.lib().ythip_cache_grow(*head, n_new.data_ptr(), *tail, None if status is None else status.data_ptr(),
+                                      _stream()), "ythip_cache_grow")
+    return out
+
+
+@_guarded
+def cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                 table: torch.Tensor, kv_len: torch.Tensor, n_new: torch.Tensor | None = None,
+                 path: torch.Tensor | None = None, key_sums: torch.Tensor | None = None) -> None:
+    """Cached row kv_len[b] + i of sequence b takes row path[b, i] (None: i) of k_new / v_new
+    [L, B, Hkv, T, d], for i < n_new[b] (None: T) and every layer; pools [L, P, Hkv, page, d].
+    A path entry outside [0, T) writes zeros. table holds the pages already (cache_grow),
+    kv_len is the length before. key_sums [L, P, Hkv, d]: the sums of the pages written to."""
+    if k_new.dim() != 5 or k_pool.dim() != 5:
+        raise ValueError("k_new must be [L, B, Hkv, T, d] and the pools [L, P, Hkv, page, d]")
+    L, B, Hkv, T, d = k_new.shape
+    P, page = k_pool.shape[1], k_pool.shape[3]
+    if tuple(k_pool.shape) != (L, P, Hkv, page, d) or k_pool.shape != v_pool.shape or k_new.shape != v_new.shape:
+        raise ValueError(f"k_new {list(k_new.shape)}, v_new {list(v_new.shape)}, pools {list(k_pool.shape)}, "
+                         f"{list(v_pool.shape)} do not fit")
+    if not (k_new.dtype == v_new.dtype == k_pool.dtype == v_pool.dtype):
+        raise ValueError("k_new, v_new and the pools must share a dtype")
+    if k_pool.stride() != v_pool.stride() or k_pool.stride(4) != 1:
+        raise ValueError("k_pool and v_pool must share strides, with d contiguous")
+    es = k_new.element_size()
+    k_new, v_new = _rows(k_new, es), _rows(v_new, es)
+    if k_new.stride() != v_new.stride():
+        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    if table.dim() != 2:
+        raise ValueError("table must be int32 [B, columns]")
+    columns = table.shape[1]
+    _ints("table", table, B, columns)
+    if table.stride(1) != 1 and columns > 1:
+        raise ValueError("table must have contiguous rows")
+    kv_len = _ints("kv_len", kv_len, B).contiguous()
+    if n_new is not None:
+        n_new = _ints("n_new", n_new, B).contiguous()
+    if path is not None:
+        path = _ints("path", path, B, T).contiguous()
+    if key_sums is not None and (key_sums.dtype != torch.float32 or key_sums.shape != (L, P, Hkv, d)
+                                 or key_sums.stride(3) != 1):
+        raise ValueError(f"key_sums must be float32 {[L, P, Hkv, d]} with d contiguous")
+    check(_lib.lib().ythip_cache_append(
+        _code(k_new), L, B, Hkv, T, d, k_new.data_ptr(), v_new.data_ptr(), _i64(k_new.stride()[:4]),
+        k_pool.data_ptr(), v_pool.data_ptr(), _i64(k_pool.stride()[:4]), P, page,
+        None if key_sums is None else key_sums.data_ptr(), None if key_sums is None else _i64(key_sums.stride()[:3]),
+        table.data_ptr(), max(table.stride(0), columns), columns, kv_len.data_ptr(),
+        None if n_new is None else n_new.data_ptr(), None if path is None else path.data_ptr(), T, _stream()),
+        "ythip_cache_append")
+
+
+@_guarded
+def cache_fork(pools, ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, src: torch.Tensor,
+               dst: torch.Tensor, page: int, out=None, status: torch.Tensor | None = None):
+    """Sequence dst[i] (empty before) becomes a copy of src[i]: it shares the whole pages and
+    gets a copy of the partial last one, in every pool ([L, P, ...] tensors: K, V, key sums).
+    All pairs read the state before the call. A pair that is refused (dst in use or named
+    twice, no free page, an index out of range) leaves dst empty (status). out and the result
+    as for cache_grow."""
+    head, tail, out = _state(ref, table, kv_len, out, page, status)
+    src, dst = _list("src", src), _list("dst", dst)
+    if src.shape != dst.shape:
+        raise ValueError("src and dst must have the same length")
+    n = src.shape[0]
+    n_pools, layers, descr = _pools(pools, ref.shape[0])
+    ws = torch.empty(max(int(_lib.lib().ythip_cache_fork_workspace_size(n)), 16), dtype=torch.uint8, device=ref.device)
+    check(_lib.lib().ythip_cache_fork(*head, n, src.data_ptr(), dst.data_ptr(), *tail, n_pools, layers, descr,
+                                      None if status is None else status.data_ptr(), ws.data_ptr(), ws.numel(),
+                                      _stream()), "ythip_cache_fork")
+    return out
+
+
+@_guarded
+def cache_free(ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, seqs: torch.Tensor, page: int, out=None,
+               status: torch.Tensor | None = None):
+    """The pages of sequences seqs lose a user; their table rows become -1, their lengths 0.
+    An empty sequence and a second mention change nothing. out and the result as for cache_grow."""
+    head, tail, out = _state(ref, table, kv_len, out, page, status)
+    seqs = _list("seqs", seqs)
+    check(_lib.lib().ythip_cache_free(*head, seqs.shape[0], seqs.data_ptr(), *tail,
+                                      None if status is None else status.data_ptr(), _stream()), "ythip_cache_free")
+    return out
+
+
+@_guarded
+def cache_compact(pools, ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, page: int, out=None):
+    """Moves the pages in use to the front of every pool ([L, P, ...] tensors), in order, and
+    has ref and table follow. out: (ref, table) to write instead of the given ones. Returns
+    (ref, table, live): live int32 [1], the pages in use."""
+    out = (ref, table) if out is None else tuple(out)
+    head, tail, out = _state(ref, table, kv_len, (*out, kv_len), page, None)
+    n_pools, layers, descr = _pools(pools, ref.shape[0])
+    live = torch.empty(1, dtype=torch.int32, device=ref.device)
+    ws = torch.empty(int(_lib.lib().ythip_cache_compact_workspace_size(ref.shape[0])), dtype=torch.uint8,
+                     device=ref.device)
+    check(_lib.lib().ythip_cache_compact(*head, *tail[:3], live.data_ptr(), n_pools, layers, descr, ws.data_ptr(),
+                                         ws.numel(), _stream()), "ythip_cache_compact")
+    return out[0], out[1], live
+
+
+@_guarded
+def cache_copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, status: torch.Tensor | None = None) -> None:
+    """Page src[i] over page dst[i] of every pool ([L, P, ...] tensors). No dst may be another
+    pair's src or dst; a pair with an index out of range is left out (status)."""
+    src, dst = _list("src", src), _list("dst", dst)
+    if src.shape != dst.shape:
+        raise ValueError("src and dst must have the same length")
+    if len(pools) == 0:
+        return
+    if status is not None:
+        _ints("status", status, 1)
+    pages = pools[0].shape[1] if pools[0].dim() >= 3 else 0
+    n_pools, layers, descr = _pools(pools, pages)
+    check(_lib.lib().ythip_cache_copy_pages(pages, src.shape[0], src.data_ptr(), dst.data_ptr(), n_pools, layers,
+                                            descr, None if status is None else status.data_ptr(), _stream()),
+          "ythip_cache_copy_pages")
