@@ -24,7 +24,7 @@ struct PagedArgs {
     const float* sums;
     int64_t ss[2];
     double* score;  // sparse: [B][Hkv][T][columns]
-    int target, min_chunk, items, row_tiles;  // the cut: items aimed at (sparse: of a token), tiles an item has at least
+    int target, min_chunk, items, row_tiles;  // the cut: ranges (0: a sequence each; sparse: of a token), tiles one has at least
     float *part, *part_ml;  // partials of items: [items][Hkv][rows][d] and (max, sum)
 };
 
@@ -39,58 +39,77 @@ __device__ __forceinline__ int new_rows(const PagedArgs& a, int b) {
     return a.new_len != nullptr ? min(max(a.new_len[b], 0), a.T) : a.T;
 }
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = uniform((int)(uint64_t)v), hi = uniform((int)((uint64_t)v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ const char* uniform(const char* p) {
+    return reinterpret_cast<const char*>((uintptr_t)uniform((int64_t)(uintptr_t)p));
+}
+
 __device__ __forceinline__ int64_t tiles_of(const PagedArgs& a, int len, int tn, int kt) {
     return ((int64_t)len + kt - 1) / kt + (a.Kn != nullptr ? (tn + kt - 1) / kt : 0);
 }
 
-// The cut of the batch: sequence b's tiles (KT cached rows or new tokens each) are dealt in
-// chunks of the same size to ceil(tiles / chunk) workgroup items (one for none), so that a
-// ragged batch gives every workgroup the same work; the chunk is what makes about
-// a.target items of all the batch's tiles. Every wave works it out for itself from the
-// lengths (one sequence a lane): `first` and `count` of the items of sequence b when `item`
-// is negative, else b, its first item and count for that item (b = -1: past the last).
+// The cut of the batch: the tiles (KT cached rows or new tokens each) of all sequences in a row,
+// at least one a sequence, are dealt in `target` equal ranges, so that a ragged batch gives
+// the workgroups the same work; a range that holds the end of one sequence and the start of
+// another is two items, one a sequence. Item r + b is what range r holds of sequence b: the
+// pairs that occur form a staircase, so the sums are distinct and a sequence's lie side by
+// side. Every wave works the cut out for itself from the lengths, one sequence a lane.
 struct Cut {
-    int b, first, count, chunk;
+    int b, first, count;  // the sequence, its first item and how many it has
+    int chunk;            // tiles a range
+    int64_t start;        // the sequence's first tile
 };
+// b < 0: of the sequence that `item` belongs to (b = -1: to none)
 __device__ __forceinline__ Cut cut_of(const PagedArgs& a, int kt, int item, int b) {
     const int lane = threadIdx.x & 63;
-    auto tiles = [&](int i) { return i < a.B ? tiles_of(a, rows_in_use(a, i), new_rows(a, i), kt) : 0; };
-    int64_t total = 0, n0 = tiles(lane);
+    auto tiles = [&](int i) { return i < a.B ? max(tiles_of(a, rows_in_use(a, i), new_rows(a, i), kt), (int64_t)1) : 0; };
+    const int64_t n0 = tiles(lane);
+    int64_t total = 0;
     for (int base = 0; base < a.B; base += 64) {
         int64_t n = base == 0 ? n0 : tiles(base + lane);
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) n += __shfl_xor(n, off, 64);
         total += n;
     }
-    const int64_t even = (total + a.target - 1) / a.target;
+    total = uniform(total);
+    auto ratio = [&](int64_t x, int64_t y) { return total <= INT_MAX ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y; };
+    const int64_t even = ratio(total + a.target - 1, a.target);
     Cut c;
-    c.chunk = __builtin_amdgcn_readfirstlane((int)(even < a.min_chunk ? a.min_chunk : even));
-    int before = 0;
+    c.chunk = uniform((int)(even < a.min_chunk ? a.min_chunk : even));
+    int64_t before = 0;
     for (int base = 0; base < a.B; base += 64) {
-        const int64_t n = base == 0 ? n0 : tiles(base + lane);
-        const int mine = base + lane < a.B ? max((int)((n + c.chunk - 1) / c.chunk), 1) : 0;
-        int inc = mine;
+        int64_t inc = base == 0 ? n0 : tiles(base + lane);
+        const int64_t mine = inc;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
-            const int x = __shfl_up(inc, off, 64);
+            const int64_t x = __shfl_up(inc, off, 64);
             if (lane >= off) inc += x;
         }
-        const int all = __shfl(inc, 63, 64);
+        const int64_t start = before + inc - mine;
+        const int first = (int)ratio(start, c.chunk) + base + lane, last = (int)ratio(before + inc - 1, c.chunk) + base + lane;
+        const int n = min(a.B - base, 64);
         int at = -1;
-        if (item >= 0) {
-            if (item < before + all) at = __popcll(__ballot(before + inc <= item));
-        } else if (b < base + 64) {
-            at = b - base;
+        if (b >= 0) {
+            if (b < base + 64) at = b - base;
+        } else {
+            const int below = __popcll(__ballot(lane < n && last < item));
+            if (below < n) at = below;
         }
         if (at >= 0) {
-            c.b = __builtin_amdgcn_readfirstlane(base + at);
-            c.count = __builtin_amdgcn_readfirstlane(__shfl(mine, at, 64));
-            c.first = __builtin_amdgcn_readfirstlane(before + __shfl(inc - mine, at, 64));
+            c.b = uniform(base + at);
+            c.first = uniform(__shfl(first, at, 64));
+            c.count = uniform(__shfl(last, at, 64)) - c.first + 1;
+            c.start = uniform(__shfl(start, at, 64));
+            if (b < 0 && item < c.first) c.b = -1;  // a range ended with a sequence: one sum is left out
             return c;
         }
-        before += all;
+        before = uniform(before + __shfl(inc, 63, 64));
     }
-    c.b = -1, c.first = before, c.count = 0;
+    c.b = -1;
     return c;
 }
 
@@ -105,31 +124,39 @@ __device__ __forceinline__ int scalar_word(const int32_t* p) {
 #endif
 }
 
-__device__ __forceinline__ const char* uniform(const char* p) {
-    const uint64_t v = (uint64_t)(uintptr_t)p;
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-    return reinterpret_cast<const char*>((uintptr_t)((uint64_t)hi << 32 | lo));
+// mfma_chunk over 16 keys: lane l holds k = 4 (l / 16) + 0..3.
+__device__ __forceinline__ f32x4 mfma_half(BF16, u32x2 a, u32x2 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4i16, a), __builtin_bit_cast(v4i16, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_half(F16, u32x2 a, u32x2 b, f32x4 c) {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
 }
 
 __device__ __forceinline__ void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
-template <class T, int D, int QT, int WR, int KT>
+// Waves of a workgroup: eight where each streams its own keys and their stages fit LDS (half the
+// partials of four), four where they share a tile (two workgroups a CU fill each other's waits).
+constexpr int waves_of(int row_bytes, int wr) { return wr == 1 && row_bytes <= 256 ? 8 : 4; }
+
+template <class T, int D, int QT, int WR>
 struct Shape {
     static constexpr int ES = sizeof(typename T::raw), ROWB = D * ES, CH = ROWB / 16;
+    static constexpr int NW = waves_of(ROWB, WR), KT = 16 * WR;
     static constexpr int RPI = 1024 / ROWB;  // rows of one DMA instruction
     static constexpr int IPG = 16 / RPI;     // instructions of 16 rows
-    static constexpr int WK = 4 / WR;        // key groups of the workgroup
+    static constexpr int WK = NW / WR;       // key groups of the workgroup
     static constexpr int KG = KT / 16, GPW = KG / WR, NI = GPW * IPG;
     static constexpr int TILE = KT * CH, STG = WK * TILE;  // in 16-byte chunks
     static constexpr int KS = CH / 4, DT = D / 16, RW = 16 * QT * WR;
     static constexpr int OLD = D + 4;  // floats of a row of O in LDS: 16 rows fall in different banks
     static constexpr int EPI = WK == 1 ? 0 : (WK * RW * (OLD + 2) * 4 + 15) / 16;  // the epilogue's use of the stages
     static constexpr int LDS = 4 * STG > EPI ? 4 * STG : EPI;
-    static_assert(KG % WR == 0 && (ES == 4 || KT % 32 == 0), "tile");
+    static_assert(KG % WR == 0, "a wave stages whole groups of 16 rows");
 };
 
 // One workgroup: RW = 16 QT WR query rows of one KV head (row = token * G + head of the group)
-// over a chunk of its sequence's tiles. Its four waves are WR row groups x WK key groups: few
+// over a chunk of its sequence's tiles. Its waves are WR row groups x WK key groups: few
 // rows share out the keys (WR = 1: each wave streams its own tiles, no barrier in the loop),
 // many rows share the staged tile.
 //   S^T = K . Q^T and O^T = V^T . P^T on the matrix cores, lane l holding query l % 16: the
@@ -140,9 +167,10 @@ struct Shape {
 //   query's token once, then cached rows.
 // Numerics: scores, maxima, sums and O in fp32; p is rounded to the inputs' 16-bit type for
 // the second product (2^-9 of each weight in bf16, as the rounding of O).
-template <class T, int D, int QT, int WR, int KT, bool SPARSE>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
-    using S = Shape<T, D, QT, WR, KT>;
+template <class T, int D, int QT, int WR, bool SPARSE>
+__global__ __launch_bounds__((64 * Shape<T, D, QT, WR>::NW), (8 / Shape<T, D, QT, WR>::NW)) void paged_attn_kernel(PagedArgs a) {
+    using S = Shape<T, D, QT, WR>;
+    constexpr int KT = S::KT, THREADS = 64 * S::NW;
     using raw = typename T::raw;
     constexpr bool F = std::is_same_v<T, F32>;
     constexpr int KMASK = S::CH - 1 < 15 ? S::CH - 1 : 15;
@@ -164,21 +192,23 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
     if (gi >= a.items * a.Hkv) return;
     const int h = gi % a.Hkv, item = gi / a.Hkv;
 
-    int b, split, nsplit, chunk, t_one = 0;
-    if constexpr (SPARSE) {
-        split = item % a.target;
-        t_one = item / a.target % a.T;
-        b = item / a.target / a.T;
-    } else {
-        const Cut c = cut_of(a, KT, item, 0);
-        if (c.b < 0) return;
-        b = c.b, split = item - c.first, nsplit = c.count, chunk = c.chunk;
-    }
-    const int len = __builtin_amdgcn_readfirstlane(rows_in_use(a, b)), tn = __builtin_amdgcn_readfirstlane(new_rows(a, b));
     const int R = SPARSE ? a.G : a.T * a.G;
     const int r0 = rt * S::RW;
+    int b, t_one = 0;
+    Cut cut;
+    if constexpr (SPARSE) {
+        t_one = item / a.target % a.T;
+        b = item / a.target / a.T;
+    } else if (a.target == 0) {  // a sequence a workgroup
+        b = item;
+    } else {
+        cut = cut_of(a, KT, item, -1);
+        if (cut.b < 0) return;
+        b = cut.b;
+    }
+    b = uniform(b);
+    const int len = uniform(rows_in_use(a, b)), tn = uniform(new_rows(a, b));
     const int t_first = SPARSE ? t_one : r0 / a.G, t_last = SPARSE ? t_one : min((min(R, r0 + S::RW) - 1) / a.G, tn - 1);
-    if (t_first >= tn) return;
     const int32_t* table = a.table + b * a.ld_table;
     const int32_t* sel = nullptr;
     int nsel = 0, nct, lim = tn;
@@ -191,18 +221,31 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
         nct = (len + KT - 1) / KT;
     }
     const int nt = nct + (a.Kn != nullptr ? (lim + KT - 1) / KT : 0);
+    // this workgroup's tiles of the sequence, and whether they are all
+    int c0 = 0, c1 = nt;
+    bool whole;
     if constexpr (SPARSE) {
-        chunk = max((nt + a.target - 1) / a.target, a.min_chunk);
-        nsplit = max((nt + chunk - 1) / chunk, 1);
-        if (split >= nsplit) return;
+        const int chunk = max((nt + a.target - 1) / a.target, a.min_chunk), split = item % a.target;
+        if (t_one >= tn || (split > 0 && split * chunk >= nt)) return;
+        c0 = split * chunk;
+        c1 = min(nt, c0 + chunk);
+        whole = c0 == 0 && c1 == nt;
+    } else if (a.target == 0) {
+        whole = true;
+    } else {
+        const int64_t at = (int64_t)(item - b) * cut.chunk - cut.start;
+        c0 = (int)max(at, (int64_t)0);
+        c1 = (int)min(at + cut.chunk, (int64_t)nt);
+        whole = cut.count == 1;
     }
-    const int c0 = split * chunk, c1 = min(nt, c0 + chunk);
+    c0 = uniform(c0), c1 = uniform(c1);
+    if (t_first >= tn) return;
     const int nst = (max(c1 - c0, 0) + S::WK - 1) / S::WK;
 
     // for the walks, where the chunk holds new tokens
     const bool walk = a.parents != nullptr && c1 > nct;
     if (walk) {
-        for (int u = tid; u < tn; u += 256) {
+        for (int u = tid; u < tn; u += THREADS) {
             const int p = a.parents[b * a.ld_par + u];
             s_up[u] = (int16_t)(p >= 0 && p < u ? p : -1);
         }
@@ -213,6 +256,8 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
     int tok[QT], cur[QT];
     bool real[QT];
     u32x4 qf[QT][S::KS];
+    constexpr uint32_t SIGN = F ? 0x80000000u : 0x80008000u;
+    const float c = fabsf(a.scale_log2);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         const int r = r0 + wr * 16 * QT + qt * 16 + l16;
@@ -225,45 +270,68 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
         for (int ks = 0; ks < S::KS; ++ks) {
             qf[qt][ks] = u32x4{0u, 0u, 0u, 0u};
             if (real[qt]) qf[qt][ks] = *reinterpret_cast<const u32x4*>(qp + (ks * 4 + g) * (16 / S::ES));
+            if (a.scale_log2 < 0.f) qf[qt][ks] ^= u32x4{SIGN, SIGN, SIGN, SIGN};
         }
     }
 
-    // DMA: lane -> (row of the instruction, chunk), the chunk swizzled by the row in its 16
-    uint32_t kof[S::IPG], vof[S::IPG], kch[S::IPG], vch[S::IPG];
-    const int pool_row = (int)a.ps[2] * S::ES;
-#pragma unroll
-    for (int i = 0; i < S::IPG; ++i) {
-        const int row = i * S::RPI + lane / S::CH, ps = lane % S::CH;
-        kch[i] = (ps ^ (row & KMASK)) * 16;
-        vch[i] = F ? (ps ^ (((row >> 2) & 3) << 2)) * 16 : (((ps >> 1) ^ (row & BMASK)) * 32 + (ps & 1) * 16);
-        kof[i] = row * pool_row + kch[i];
-        vof[i] = row * pool_row + vch[i];
+    // DMA: lane -> (row of the instruction, chunk), the chunk swizzled by the row in its 16: the
+    // first instruction's, which the e-th turns by a constant
+    const int dma_row = lane / S::CH;
+    uint32_t kx, vx;  // bytes in the row
+    {
+        const int ps = lane % S::CH, r = dma_row;
+        kx = (ps ^ (r & KMASK)) * 16;
+        vx = F ? (ps ^ (((r >> 2) & 3) << 2)) * 16 : (((ps >> 1) ^ (r & BMASK)) * 32 + (ps & 1) * 16);
     }
+    auto k_turn = [](int e) { return (uint32_t)((e * S::RPI & KMASK) * 16); };
+    auto v_turn = [](int e) { return (uint32_t)(F ? (((e * S::RPI) >> 2 & 3) << 2) * 16 : (e * S::RPI & BMASK) * 32); };
+    const int pool_row = (int)a.ps[2] * S::ES;
+    const uint32_t lane_row = dma_row * pool_row;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
     const char *Kp = static_cast<const char*>(a.Kp) + h * a.ps[1] * S::ES, *Vp = static_cast<const char*>(a.Vp) + h * a.ps[1] * S::ES;
     const char* Kn = static_cast<const char*>(a.Kn) + (b * a.kns[0] + h * a.kns[1]) * S::ES;
     const char* Vn = static_cast<const char*>(a.Vn) + (b * a.vns[0] + h * a.vns[1]) * S::ES;
 
+    auto tile_at = [&](int s) { return c1 - 1 - (s * S::WK + wk); };
+    // The pages of stage s, looked up ahead: the table's columns, then the ids in the pool.
+    int col[S::KG], id[S::KG];
+    auto columns = [&](int s) {
+        const int row = tile_at(s) * KT;
+#pragma unroll
+        for (int i = 0; i < S::KG; ++i) {
+            const int slot = (row + 16 * i) >> a.shift;
+            if constexpr (SPARSE) {
+                col[i] = -1;
+                if (row >= c0 * KT && slot < nsel) col[i] = scalar_word(sel + slot);
+            } else {
+                col[i] = slot;
+            }
+        }
+    };
+    auto ids = [&](int s) {
+        const int ti = tile_at(s);
+#pragma unroll
+        for (int i = 0; i < S::KG; ++i) {
+            id[i] = -1;
+            if (ti >= c0 && ti < nct && col[i] >= 0 && col[i] << a.shift < len) id[i] = scalar_word(table + col[i]);
+        }
+    };
     // Stage s: the rows in use of each 16 (5 bits a group; 0: nothing was staged, the tile is
     // skipped) and this wave's share of the DMA. Rows that are not in use read zeros.
-    auto tile_at = [&](int s) { return c1 - 1 - (s * S::WK + wk); };
-    auto issue = [&](int s) {
+    int cols[S::KG];  // of the stage that `id` is for
+    auto issue = [&](int s, auto with_new) {
         const int ti = tile_at(s);
         uint32_t pack = 0;
         if (ti < c0) return pack;
         const char *kb[S::KG], *vb[S::KG];
-        const bool cached = ti < nct;
+        const bool cached = !decltype(with_new)::value || ti < nct;
 #pragma unroll
         for (int i = 0; i < S::KG; ++i) {
             int n;
             if (cached) {
-                const int row = ti * KT + 16 * i, slot = row >> a.shift, off = row & ((1 << a.shift) - 1);
-                int lp = slot;
-                if constexpr (SPARSE) lp = slot < nsel ? scalar_word(sel + slot) : -1;
-                n = lp < 0 ? 0 : min(max(len - (lp << a.shift) - off, 0), 16);
-                const int p = n > 0 ? scalar_word(table + lp) : -1;
-                if ((uint32_t)p >= (uint32_t)a.pages) n = 0;
-                const int64_t at = (p * a.ps[0] + off * a.ps[2]) * S::ES;
+                const int off = (ti * KT + 16 * i) & ((1 << a.shift) - 1);
+                n = (uint32_t)id[i] < (uint32_t)a.pages ? min(max(len - (cols[i] << a.shift) - off, 0), 16) : 0;
+                const int64_t at = (id[i] * a.ps[0] + off * a.ps[2]) * S::ES;
                 kb[i] = Kp + at;
                 vb[i] = Vp + at;
             } else {
@@ -288,19 +356,23 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
             const uint32_t lk = lds0 + ((s & 1) * 2 * S::STG + wk * S::TILE + i * 16 * S::CH) * 16, lv = lk + S::STG * 16;
             if (cached && n == 16) {
                 k = uniform(k), v = uniform(v);
+                // the lane offsets anew each time: kept, they would not all fit the registers
+                uint32_t kl = kx, vl = vx;
+                asm volatile("" : "+v"(kl), "+v"(vl));
 #pragma unroll
                 for (int e = 0; e < S::IPG; ++e) {
-                    dma16_soff(k, kof[e], lk + e * 1024);
-                    dma16_soff(v, vof[e], lv + e * 1024);
+                    const int64_t rows = (int64_t)e * S::RPI * pool_row;
+                    dma16_soff(k + rows, lane_row + (kl ^ k_turn(e)), lk + e * 1024);
+                    dma16_soff(v + rows, lane_row + (vl ^ v_turn(e)), lv + e * 1024);
                 }
             } else {
                 const int64_t kr = (cached ? a.ps[2] : a.kns[2]) * S::ES, vr = (cached ? a.ps[2] : a.vns[2]) * S::ES;
 #pragma unroll
                 for (int e = 0; e < S::IPG; ++e) {
-                    const int row = e * S::RPI + lane / S::CH;
+                    const int row = e * S::RPI + dma_row;
                     const char* zero = reinterpret_cast<const char*>(zeros);
-                    const char* ka = row < n ? k + row * kr + kch[e] : zero;
-                    const char* va = row < n ? v + row * vr + vch[e] : zero;
+                    const char* ka = row < n ? k + row * kr + (kx ^ k_turn(e)) : zero;
+                    const char* va = row < n ? v + row * vr + (vx ^ v_turn(e)) : zero;
                     dma16_async(ka, smem + (lk - lds0) / 16 + e * 64);
                     dma16_async(va, smem + (lv - lds0) / 16 + e * 64);
                 }
@@ -319,72 +391,68 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
         for (int t = 0; t < S::DT; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // acc += V^T . P^T over the tile's keys, or those of `keep` alone (the others' V taken as 0)
-    auto pv = [&](const u32x4* cV, const f32x4 (&p)[QT][S::KG], f32x4 (&acc)[QT][S::DT], auto some, uint64_t keep) {
-        constexpr bool SOME = decltype(some)::value;
+    // acc += V^T . P^T for output rows 16 t..16 t + 15 over the tile's keys (CLEAN: elements of V that
+    // are not finite taken as 0); pk: p as the MFMA takes it
+    constexpr uint32_t EXP2 = std::is_same_v<T, BF16> ? 0x7f807f80u : 0x7c007c00u, STEP2 = std::is_same_v<T, BF16> ? 0x00800080u : 0x04000400u;
+    constexpr int PK = F ? S::KG : S::KG >= 2 ? S::KG / 2 : 1;
+    auto pv = [&](const u32x4* cV, int t, const u32x4 (&pk)[QT][PK], f32x4 (&acc)[QT], auto clean) {
+        constexpr bool CLEAN = decltype(clean)::value;
         if constexpr (F) {
             const float* V = reinterpret_cast<const float*>(cV);
 #pragma unroll
             for (int kt = 0; kt < S::KG; ++kt)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int key = kt * 16 + 4 * g + j;
+                    const int key = kt * 16 + 4 * g + j, c = t * 4 + (l16 >> 2);
+                    float v = V[key * D + ((c ^ (((key >> 2) & 3) << 2)) << 2) + (l16 & 3)];
+                    if (CLEAN) v = fabsf(v) < INFINITY ? v : 0.f;
 #pragma unroll
-                    for (int t = 0; t < S::DT; ++t) {
-                        const int c = t * 4 + (l16 >> 2);
-                        float v = V[key * D + ((c ^ (((key >> 2) & 3) << 2)) << 2) + (l16 & 3)];
-                        if (SOME) v = (keep >> key & 1) ? v : 0.f;
-#pragma unroll
-                        for (int qt = 0; qt < QT; ++qt)
-                            acc[qt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[qt][kt][j], acc[qt][t], 0, 0, 0);
-                    }
+                    for (int qt = 0; qt < QT; ++qt)
+                        acc[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, __uint_as_float(pk[qt][kt][j]), acc[qt], 0, 0, 0);
                 }
         } else {
 #pragma unroll
-            for (int kk = 0; kk < S::KG / 2; ++kk) {
-                u32x4 pk[QT], km;
+            for (int kk = 0; kk < PK; ++kk) {
+                u32x4 vf = {0u, 0u, 0u, 0u};
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                    pk[qt] = u32x4{pack2<T>(p[qt][2 * kk][0], p[qt][2 * kk][1]), pack2<T>(p[qt][2 * kk][2], p[qt][2 * kk][3]),
-                                   pack2<T>(p[qt][2 * kk + 1][0], p[qt][2 * kk + 1][1]), pack2<T>(p[qt][2 * kk + 1][2], p[qt][2 * kk + 1][3])};
-                if (SOME) {
+                for (int hh = 0; hh < (S::KG >= 2 ? 2 : 1); ++hh) {
+                    const int key = (2 * kk + hh) * 16 + g * 4 + (l16 >> 2);
+                    const u32x2 w = lds_read_tr16(cV, key * S::ROWB + ((t ^ (key & BMASK)) << 5) + 8 * (l16 & 3));
+                    vf[2 * hh] = w[0];
+                    vf[2 * hh + 1] = w[1];
+                }
+                if (CLEAN) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int key = (2 * kk + (e >> 1)) * 16 + 4 * g + (e & 1) * 2;
-                        km[e] = (keep >> key & 1 ? 0xffffu : 0u) | (keep >> (key + 1) & 1 ? 0xffff0000u : 0u);
+                        // an exponent of ones carries into the bit above it
+                        const uint32_t odd = (((vf[e] & EXP2) + STEP2) >> 15) & 0x00010001u;
+                        vf[e] &= ~(odd * 0xffffu);
                     }
                 }
 #pragma unroll
-                for (int t = 0; t < S::DT; ++t) {
-                    u32x4 vf;
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        const int key = (2 * kk + hh) * 16 + g * 4 + (l16 >> 2);
-                        const u32x2 w = lds_read_tr16(cV, key * S::ROWB + ((t ^ (key & BMASK)) << 5) + 8 * (l16 & 3));
-                        vf[2 * hh] = w[0];
-                        vf[2 * hh + 1] = w[1];
-                    }
-                    if (SOME) vf &= km;
-#pragma unroll
-                    for (int qt = 0; qt < QT; ++qt) acc[qt][t] = mfma_chunk(T{}, vf, pk[qt], acc[qt][t]);
+                for (int qt = 0; qt < QT; ++qt) {
+                    if constexpr (S::KG >= 2) acc[qt] = mfma_chunk(T{}, vf, pk[qt][kk], acc[qt]);
+                    else acc[qt] = mfma_half(T{}, u32x2{vf[0], vf[1]}, u32x2{pk[qt][0][0], pk[qt][0][1]}, acc[qt]);
                 }
             }
         }
     };
 
-    auto compute = [&](int s, uint32_t pack) {
+    auto compute = [&](int s, uint32_t pack, auto with_new) {
+        constexpr bool NEW = decltype(with_new)::value;
         const int ti = tile_at(s);
         const u32x4* cK = smem + (s & 1) * 2 * S::STG + wk * S::TILE;
         const u32x4* cV = cK + S::STG;
-        const bool cached = ti < nct;
+        const bool cached = !NEW || ti < nct;
         uint64_t see[QT];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) see[qt] = 0;
         if (!cached) {
             // the new tokens of this tile on each query's path
             const int u0 = (ti - nct) * KT;
             bool any = false;
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
-                see[qt] = 0;
                 if (walk) {
                     while (cur[qt] >= u0) {
                         if (cur[qt] < u0 + KT) see[qt] |= 1ull << (cur[qt] - u0);
@@ -411,25 +479,27 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
             }
         }
         constexpr uint32_t FULL = S::KG == 1 ? 16u : S::KG == 2 ? 16u | 16u << 5 : 16u | 16u << 5 | 16u << 10 | 16u << 15;
-        const bool whole = cached && pack == FULL;
+        if (!cached || pack != FULL) {
+#pragma unroll
+            for (int kt = 0; kt < S::KG; ++kt) {
+                // the rows in use of the group, and the path's bits, of this lane's four keys
+                const int n = (int)((pack >> (5 * kt)) & 31) - 4 * g;
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    const uint32_t vis = cached ? 15u : (uint32_t)(see[qt] >> (kt * 16 + 4 * g));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[qt][kt][r] = r < n && (vis >> r & 1) ? p[qt][kt][r] : -INFINITY;
+                }
+            }
+        }
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-            float mx = -INFINITY;
+            float mx = -INFINITY;  // of the scores before the scale (it is positive: a negative one went into Q)
 #pragma unroll
             for (int kt = 0; kt < S::KG; ++kt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float x = p[qt][kt][r] * a.scale_log2;
-                    if (!whole) {
-                        const int key = kt * 16 + 4 * g + r;
-                        bool vis = 4 * g + r < (int)((pack >> (5 * kt)) & 31);
-                        if (!cached) vis = vis && (see[qt] >> key & 1);
-                        x = vis ? x : -INFINITY;
-                    }
-                    p[qt][kt][r] = x;
-                    mx = __builtin_elementwise_maximum(mx, x);
-                }
-            const float top = __builtin_elementwise_maximum(m[qt], max_across_rows(mx));
+                for (int r = 0; r < 4; ++r) mx = __builtin_elementwise_maximum(mx, p[qt][kt][r]);
+            const float top = __builtin_elementwise_maximum(m[qt], max_across_rows(mx) * c);
             const float ref = top == -INFINITY ? 0.f : top;  // nothing seen yet: every weight is 0
             const float corr = __builtin_amdgcn_exp2f(m[qt] - ref);
             m[qt] = top;
@@ -438,7 +508,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
             for (int kt = 0; kt < S::KG; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    p[qt][kt][r] = __builtin_amdgcn_exp2f(p[qt][kt][r] - ref);
+                    p[qt][kt][r] = __builtin_amdgcn_exp2f(fmaf(p[qt][kt][r], c, -ref));
                     sum += p[qt][kt][r];
                 }
             l[qt] = l[qt] * corr + sum;
@@ -449,17 +519,16 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
         }
         uint64_t odd = 0;
         if (!cached) {
-            // 0 . V is NaN for a V that is not finite: such rows of the tile are left out and added
-            // for the queries alone that see them
-            constexpr uint32_t EXP = std::is_same_v<T, BF16> ? 0x7f80u : 0x7c00u;
-#pragma unroll
+            // 0 . V is NaN for a V that is not finite: such elements are left out of the product and
+            // added (their weight cannot change what comes of them) for the queries that see the row
+#pragma unroll 1
             for (int i = 0; i < S::TILE / 64; ++i) {
                 const u32x4 v = cV[i * 64 + lane];
                 bool bad = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (F) bad = bad || (v[e] & 0x7f800000u) == 0x7f800000u;
-                    else bad = bad || (v[e] & EXP) == EXP || (v[e] >> 16 & EXP) == EXP;
+                    else bad = bad || (((v[e] & EXP2) + STEP2) & 0x80008000u) != 0;
                 }
                 const uint64_t w = __ballot(bad);
                 if (w != 0) {
@@ -469,39 +538,83 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
                 }
             }
         }
-        if (odd == 0) {
-            pv(cV, p, o, std::false_type{}, 0);
+        u32x4 pk[QT][PK];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int kk = 0; kk < PK; ++kk) {
+                if constexpr (F) {
+                    pk[qt][kk] = __builtin_bit_cast(u32x4, p[qt][kk]);
+                } else {
+                    const f32x4 x = p[qt][S::KG >= 2 ? 2 * kk : 0], y = p[qt][S::KG >= 2 ? 2 * kk + 1 : 0];
+                    pk[qt][kk] = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+                }
+            }
+        auto product = [&](auto clean) {
+#pragma unroll
+            for (int t = 0; t < S::DT; ++t) {
+                f32x4 acc[QT];
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) acc[qt] = o[qt][t];
+                pv(cV, t, pk, acc, clean);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) o[qt][t] = acc[qt];
+            }
+        };
+        if (!NEW || odd == 0) {
+            product(std::false_type{});
             return;
         }
-        pv(cV, p, o, std::true_type{}, ~odd);
+        asm volatile("" ::: "memory");  // or the two products are run both and one result taken
+        product(std::true_type{});
         for (uint64_t left = odd; left != 0; left &= left - 1) {
             const int u = __builtin_ctzll(left);
-            f32x4 one[QT][S::DT];
+            const char* row = reinterpret_cast<const char*>(cV) + u * S::ROWB;
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
+            for (int t = 0; t < S::DT; ++t) {
+                float v[4];
+                if constexpr (F) {
+                    const f32x4 w = *reinterpret_cast<const f32x4*>(row + ((4 * t + g) ^ (((u >> 2) & 3) << 2)) * 16);
+                    for (int i = 0; i < 4; ++i) v[i] = w[i];
+                } else {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(row + (t ^ (u & BMASK)) * 32 + g * 8);
+                    for (int i = 0; i < 2; ++i) v[2 * i] = lo_as_f32(T{}, w[i]), v[2 * i + 1] = hi_as_f32(T{}, w[i]);
+                }
 #pragma unroll
-                for (int t = 0; t < S::DT; ++t) one[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            pv(cV, p, one, std::true_type{}, 1ull << u);
+                for (int i = 0; i < 4; ++i) {
+                    const float add = fabsf(v[i]) < INFINITY ? 0.f : v[i];
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-                for (int t = 0; t < S::DT; ++t)
-                    if (see[qt] >> u & 1) o[qt][t] += one[qt][t];
+                    for (int qt = 0; qt < QT; ++qt) o[qt][t][i] += (see[qt] >> u & 1) ? add : 0.f;
+                }
+            }
         }
     };
 
-    uint32_t here = nst > 0 ? issue(0) : 0, next = nst > 1 ? issue(1) : 0;
-    for (int s = 0; s < nst; ++s) {
-        if (next != 0) wait_vmcnt<2 * S::NI>();  // stage s has landed, s + 1 is in flight
-        else wait_vmcnt<0>();
-        if constexpr (WR > 1) wg_barrier();
-        else asm volatile("" ::: "memory");
-        if (here != 0) compute(s, here);
-        if constexpr (WR > 1) wg_barrier();
-        else asm volatile("" ::: "memory");
+    uint32_t here = 0, next = 0;  // what is staged for s and s + 1
+    auto step = [&](int s, auto with_new) {
+        // the lookups of stage s + 2 run beside the arithmetic of stage s
+        ids(s + 2);
+#pragma unroll
+        for (int i = 0; i < S::KG; ++i) cols[i] = col[i];
+        columns(s + 3);
+        if (s >= 0) {
+            if (next != 0) wait_vmcnt<2 * S::NI>();  // stage s has landed, s + 1 is in flight
+            else wait_vmcnt<0>();
+            if constexpr (WR > 1) wg_barrier();
+            else asm volatile("" ::: "memory");
+            if (here != 0) compute(s, here, with_new);
+            if constexpr (WR > 1) wg_barrier();
+            else asm volatile("" ::: "memory");
+        }
         here = next;
-        next = s + 2 < nst ? issue(s + 2) : 0;
-    }
+        next = s + 2 < nst ? issue(s + 2, with_new) : 0;
+    };
+    // stages with new tokens, then those of cached rows alone: a loop of its own, that holds none of
+    // the paths' state in registers
+    const int s_new = (max(c1 - max(c0, nct), 0) + S::WK - 1) / S::WK;
+    columns(0);
+    for (int s = -2; s < s_new; ++s) step(s, std::true_type{});
+    for (int s = s_new; s < nst; ++s) step(s, std::false_type{});
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         l[qt] += __shfl_xor(l[qt], 16, 64);
@@ -512,7 +625,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
     auto store4 = [&](int r, int d, f32x4 v, float M, float L) {
         const int t = SPARSE ? t_one : r / a.G, gh = SPARSE ? r : r - t * a.G;
         if (r >= R || t >= tn) return;
-        if (nsplit == 1) {
+        if (whole) {
             raw* op = static_cast<raw*>(a.O) + b * a.os[0] + (int64_t)(h * a.G + gh) * a.os[1] + t * a.os[2] + d;
             const float inv = M == -INFINITY ? 0.f : 1.0f / L;
             v = M == -INFINITY ? f32x4{0.f, 0.f, 0.f, 0.f} : v * inv;
@@ -548,7 +661,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedArgs a) {
             }
         }
         __syncthreads();
-        for (int i = tid; i < S::RW * D / 4; i += 256) {
+        for (int i = tid; i < S::RW * D / 4; i += THREADS) {
             const int row = i / (D / 4), d = i % (D / 4) * 4;
             float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -587,7 +700,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, int kt) {
         first = (((int64_t)(b * a.T + t) * a.target) * a.Hkv + h) * a.G + gh;
         step = (int64_t)a.Hkv * a.G;
     } else {
-        const Cut c = cut_of(a, kt, -1, b);
+        const Cut c = cut_of(a, kt, 0, b);
         count = c.count;
         first = ((int64_t)c.first * a.Hkv + h) * a.T * a.G + r;
         step = (int64_t)a.Hkv * a.T * a.G;
@@ -678,59 +791,63 @@ struct Plan {
     size_t part_bytes, ml_bytes, score_bytes;
     size_t bytes() const { return part_bytes + ml_bytes + score_bytes; }
 };
-constexpr int CUS = 256;  // MI355X
+constexpr int WAVES = 2048;  // eight on each CU of an MI355X
+constexpr int WHOLE = 3;     // stages up to which a sequence stays with one workgroup
 Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int page, int top_k) {
-    const bool f32 = dtype == YTHIP_F32;
     const int rows = top_k > 0 ? G : (int)std::min<int64_t>((int64_t)T * G, 1 << 20);
     Plan p;
     // 16 rows or 32 leave the keys to the four waves; more share each staged tile between
     // two or four of them
     p.qt = rows <= 16 ? 1 : 2;
     p.wr = rows <= 32 || top_k > 0 ? 1 : rows <= 64 ? 2 : 4;
-    p.kt = p.wr == 4 ? 64 : p.wr == 1 && f32 ? 16 : 32;
+    p.kt = 16 * p.wr;
     const int64_t all_rows = top_k > 0 ? G : (int64_t)T * G;
     const int rw = 16 * p.qt * p.wr;
     p.row_tiles = (int)((all_rows + rw - 1) / rw);
     const int64_t per = (int64_t)Hkv * p.row_tiles;
-    p.min_chunk = 4 / p.wr;
+    const int nw = waves_of(d * (dtype == YTHIP_F32 ? 4 : 2), p.wr);
+    p.min_chunk = nw / p.wr;
+    const int64_t slots = WAVES / nw;  // workgroups that run at once
     const int64_t new_tiles = ((int64_t)T + p.kt - 1) / p.kt;
+    const int64_t seq_rows = (int64_t)std::min(top_k > 0 ? top_k : columns, columns) * page;
+    const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + new_tiles, most = (tiles + p.min_chunk - 1) / p.min_chunk;
+    int64_t part_items = 0;
     if (top_k > 0) {
-        const int64_t tiles = ((int64_t)std::min(top_k, columns) * page + p.kt - 1) / p.kt + new_tiles;
-        const int64_t most = (tiles + p.min_chunk - 1) / p.min_chunk, want = (CUS + per * B * T - 1) / (per * B * T);
-        p.target = (int)std::max<int64_t>(1, std::min(most, want));
+        p.target = (int)std::max<int64_t>(1, std::min(most, (slots + per * B * T - 1) / (per * B * T)));
         p.items = (int64_t)B * T * p.target;
+        if (p.target > 1) part_items = p.items;
+    } else if (most <= WHOLE) {
+        p.target = 0;
+        p.items = B;
     } else {
-        const int64_t tiles = ((int64_t)columns * page + p.kt - 1) / p.kt + new_tiles;
-        const int64_t most = (tiles + p.min_chunk - 1) / p.min_chunk;
-        p.target = (int)std::max<int64_t>(1, CUS / per);
-        p.items = std::min<int64_t>((int64_t)p.target + B, B * most);
+        p.target = (int)std::min(std::max<int64_t>(1, slots / per), B * most);
+        p.items = part_items = (int64_t)p.target + B - 1;
     }
-    const bool parts = top_k > 0 ? p.target > 1 : p.items > B;
-    const int64_t part_rows = parts ? p.items * Hkv * all_rows : 0;
+    const int64_t part_rows = part_items * Hkv * all_rows;
     p.part_bytes = (size_t)part_rows * d * sizeof(float);
     p.ml_bytes = ((size_t)part_rows * 2 * sizeof(float) + 15) / 16 * 16;
     p.score_bytes = top_k > 0 ? (size_t)B * Hkv * T * columns * sizeof(double) : 0;
     return p;
 }
 
-template <class T, int D, int QT, int WR, int KT, bool SPARSE>
+template <class T, int D, int QT, int WR, bool SPARSE>
 int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
     const int64_t groups = (p.items * a.Hkv + 7) / 8 * 8;
     if (groups * p.row_tiles > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups", (long long)(groups * p.row_tiles));
-    paged_attn_kernel<T, D, QT, WR, KT, SPARSE><<<(int)(groups * p.row_tiles), 256, 0, s>>>(a);
-    if (p.part_bytes > 0) paged_merge_kernel<T, D, SPARSE><<<dim3((a.T * a.G + 3) / 4, a.Hkv, a.B), 256, 0, s>>>(a, KT);
+    using S = Shape<T, D, QT, WR>;
+    paged_attn_kernel<T, D, QT, WR, SPARSE><<<(int)(groups * p.row_tiles), 64 * S::NW, 0, s>>>(a);
+    if (p.part_bytes > 0) paged_merge_kernel<T, D, SPARSE><<<dim3((a.T * a.G + 3) / 4, a.Hkv, a.B), 256, 0, s>>>(a, S::KT);
     return status_of(hipGetLastError());
 }
 template <class T, int D, bool SPARSE>
 int run_typed(const PagedArgs& a, const Plan& p, hipStream_t s) {
-    constexpr int K1 = std::is_same_v<T, F32> ? 16 : 32;
     if constexpr (SPARSE) paged_select_simple<T, D><<<dim3(a.T, a.Hkv, a.B), 256, 0, s>>>(a);
-    if (p.qt == 1) return launch<T, D, 1, 1, K1, SPARSE>(a, p, s);
+    if (p.qt == 1) return launch<T, D, 1, 1, SPARSE>(a, p, s);
     if constexpr (!SPARSE) {
-        if (p.wr == 2) return launch<T, D, 2, 2, 32, SPARSE>(a, p, s);
-        if (p.wr == 4) return launch<T, D, 2, 4, 64, SPARSE>(a, p, s);
+        if (p.wr == 2) return launch<T, D, 2, 2, SPARSE>(a, p, s);
+        if (p.wr == 4) return launch<T, D, 2, 4, SPARSE>(a, p, s);
     }
-    return launch<T, D, 2, 1, K1, SPARSE>(a, p, s);
+    return launch<T, D, 2, 1, SPARSE>(a, p, s);
 }
 template <bool SPARSE>
 int run(int dtype, int d, PagedArgs& a, void* ws, hipStream_t s) {
