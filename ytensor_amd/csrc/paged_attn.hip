@@ -48,8 +48,8 @@ __device__ __forceinline__ const char* uniform(const char* p) {
     return reinterpret_cast<const char*>((uintptr_t)uniform((int64_t)(uintptr_t)p));
 }
 
-__device__ __forceinline__ int64_t tiles_of(const PagedArgs& a, int len, int tn, int kt) {
-    return ((int64_t)len + kt - 1) / kt + (a.Kn != nullptr ? (tn + kt - 1) / kt : 0);
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, int len, int tn, int kt) {
+    return (int)(((int64_t)len + kt - 1) / kt) + (a.Kn != nullptr ? (tn + kt - 1) / kt : 0);
 }
 
 // The cut of the batch: the tiles (KT cached rows or new tokens each) of all sequences in a row,
@@ -60,38 +60,45 @@ __device__ __forceinline__ int64_t tiles_of(const PagedArgs& a, int len, int tn,
 // side. Every wave works the cut out for itself from the lengths, one sequence a lane.
 struct Cut {
     int b, first, count;  // the sequence, its first item and how many it has
-    int chunk;            // tiles a range
-    int64_t start;        // the sequence's first tile
+    int chunk, start;     // tiles a range, the sequence's first tile
+    int len, tn;          // rows_in_use and new_rows of the sequence
 };
+// Sums over the lanes up to this one (DPP: within rows of 16, then across them).
+__device__ __forceinline__ int wave_scan(int v) {
+    auto add = [](int x, auto ctrl, auto rows) {
+        return x + __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    using std::integral_constant;
+    v = add(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
+    v = add(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+    v = add(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+    v = add(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+    v = add(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast 15 into rows 1 and 3
+    v = add(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast 31 into rows 2 and 3
+    return v;
+}
 // b < 0: of the sequence that `item` belongs to (b = -1: to none)
 __device__ __forceinline__ Cut cut_of(const PagedArgs& a, int kt, int item, int b) {
     const int lane = threadIdx.x & 63;
-    auto tiles = [&](int i) { return i < a.B ? max(tiles_of(a, rows_in_use(a, i), new_rows(a, i), kt), (int64_t)1) : 0; };
-    const int64_t n0 = tiles(lane);
-    int64_t total = 0;
-    for (int base = 0; base < a.B; base += 64) {
-        int64_t n = base == 0 ? n0 : tiles(base + lane);
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) n += __shfl_xor(n, off, 64);
-        total += n;
+    int len = 0, tn = 0, mine = 0, inc = 0;
+    auto load = [&](int i) {
+        const bool is = i < a.B;
+        len = is ? rows_in_use(a, i) : 0;
+        tn = is ? new_rows(a, i) : 0;
+        mine = is ? max(tiles_of(a, len, tn, kt), 1) : 0;
+        inc = wave_scan(mine);
+    };
+    int total = 0;
+    for (int base = (a.B - 1) & ~63; base >= 0; base -= 64) {  // the first 64 last: they are kept
+        load(base + lane);
+        total += __builtin_amdgcn_readlane(inc, 63);
     }
-    total = uniform(total);
-    auto ratio = [&](int64_t x, int64_t y) { return total <= INT_MAX ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y; };
-    const int64_t even = ratio(total + a.target - 1, a.target);
     Cut c;
-    c.chunk = uniform((int)(even < a.min_chunk ? a.min_chunk : even));
-    int64_t before = 0;
-    for (int base = 0; base < a.B; base += 64) {
-        int64_t inc = base == 0 ? n0 : tiles(base + lane);
-        const int64_t mine = inc;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int64_t x = __shfl_up(inc, off, 64);
-            if (lane >= off) inc += x;
-        }
-        const int64_t start = before + inc - mine;
-        const int first = (int)ratio(start, c.chunk) + base + lane, last = (int)ratio(before + inc - 1, c.chunk) + base + lane;
-        const int n = min(a.B - base, 64);
+    c.chunk = max((int)(((uint32_t)total + a.target - 1) / (uint32_t)a.target), a.min_chunk);
+    for (int base = 0, before = 0;; ) {
+        const int start = before + inc - mine, n = min(a.B - base, 64);
+        const int first = (int)((uint32_t)start / (uint32_t)c.chunk) + base + lane;
+        const int last = (int)((uint32_t)(before + inc - 1) / (uint32_t)c.chunk) + base + lane;
         int at = -1;
         if (b >= 0) {
             if (b < base + 64) at = b - base;
@@ -100,14 +107,19 @@ __device__ __forceinline__ Cut cut_of(const PagedArgs& a, int kt, int item, int 
             if (below < n) at = below;
         }
         if (at >= 0) {
-            c.b = uniform(base + at);
-            c.first = uniform(__shfl(first, at, 64));
-            c.count = uniform(__shfl(last, at, 64)) - c.first + 1;
-            c.start = uniform(__shfl(start, at, 64));
+            c.b = base + at;
+            c.first = __builtin_amdgcn_readlane(first, at);
+            c.count = __builtin_amdgcn_readlane(last, at) - c.first + 1;
+            c.start = __builtin_amdgcn_readlane(start, at);
+            c.len = __builtin_amdgcn_readlane(len, at);
+            c.tn = __builtin_amdgcn_readlane(tn, at);
             if (b < 0 && item < c.first) c.b = -1;  // a range ended with a sequence: one sum is left out
             return c;
         }
-        before = uniform(before + __shfl(inc, 63, 64));
+        before += __builtin_amdgcn_readlane(inc, 63);
+        base += 64;
+        if (base >= a.B) break;
+        load(base + lane);
     }
     c.b = -1;
     return c;
@@ -124,6 +136,17 @@ __device__ __forceinline__ int scalar_word(const int32_t* p) {
 #endif
 }
 
+// dma16_soff for rows that this launch reads once: kept out of the caches' way (16 x 1 token over
+// 8192 rows 82 -> 73 us, a tree of 64 over 131072 rows 140 -> 125 us).
+__device__ __forceinline__ void dma16_stream(const void* sbase, uint32_t voff, uint32_t lds_wave_base) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(voff), "s"(sbase), "s"(lds_wave_base)
+                 : "memory", "m0");
+#endif
+}
+
 // mfma_chunk over 16 keys: lane l holds k = 4 (l / 16) + 0..3.
 __device__ __forceinline__ f32x4 mfma_half(BF16, u32x2 a, u32x2 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4i16, a), __builtin_bit_cast(v4i16, b), c, 0, 0, 0);
@@ -135,17 +158,13 @@ __device__ __forceinline__ f32x4 mfma_half(F16, u32x2 a, u32x2 b, f32x4 c) {
 
 __device__ __forceinline__ void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
-// Waves of a workgroup: eight where each streams its own keys and their stages fit LDS (half the
-// partials of four), four where they share a tile (two workgroups a CU fill each other's waits).
-constexpr int waves_of(int row_bytes, int wr) { return wr == 1 && row_bytes <= 256 ? 8 : 4; }
-
 template <class T, int D, int QT, int WR>
 struct Shape {
     static constexpr int ES = sizeof(typename T::raw), ROWB = D * ES, CH = ROWB / 16;
-    static constexpr int NW = waves_of(ROWB, WR), KT = 16 * WR;
+    static constexpr int KT = 16 * WR;       // keys of a tile
     static constexpr int RPI = 1024 / ROWB;  // rows of one DMA instruction
     static constexpr int IPG = 16 / RPI;     // instructions of 16 rows
-    static constexpr int WK = NW / WR;       // key groups of the workgroup
+    static constexpr int WK = 4 / WR;        // key groups of the workgroup
     static constexpr int KG = KT / 16, GPW = KG / WR, NI = GPW * IPG;
     static constexpr int TILE = KT * CH, STG = WK * TILE;  // in 16-byte chunks
     static constexpr int KS = CH / 4, DT = D / 16, RW = 16 * QT * WR;
@@ -168,9 +187,9 @@ struct Shape {
 // Numerics: scores, maxima, sums and O in fp32; p is rounded to the inputs' 16-bit type for
 // the second product (2^-9 of each weight in bf16, as the rounding of O).
 template <class T, int D, int QT, int WR, bool SPARSE>
-__global__ __launch_bounds__((64 * Shape<T, D, QT, WR>::NW), (8 / Shape<T, D, QT, WR>::NW)) void paged_attn_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     using S = Shape<T, D, QT, WR>;
-    constexpr int KT = S::KT, THREADS = 64 * S::NW;
+    constexpr int KT = S::KT;
     using raw = typename T::raw;
     constexpr bool F = std::is_same_v<T, F32>;
     constexpr int KMASK = S::CH - 1 < 15 ? S::CH - 1 : 15;
@@ -206,8 +225,10 @@ __global__ __launch_bounds__((64 * Shape<T, D, QT, WR>::NW), (8 / Shape<T, D, QT
         if (cut.b < 0) return;
         b = cut.b;
     }
-    b = uniform(b);
-    const int len = uniform(rows_in_use(a, b)), tn = uniform(new_rows(a, b));
+    int len, tn;
+    if (!SPARSE && a.target > 0) len = cut.len, tn = cut.tn;
+    else len = rows_in_use(a, b), tn = new_rows(a, b);
+    b = uniform(b), len = uniform(len), tn = uniform(tn);
     const int t_first = SPARSE ? t_one : r0 / a.G, t_last = SPARSE ? t_one : min((min(R, r0 + S::RW) - 1) / a.G, tn - 1);
     const int32_t* table = a.table + b * a.ld_table;
     const int32_t* sel = nullptr;
@@ -233,9 +254,9 @@ __global__ __launch_bounds__((64 * Shape<T, D, QT, WR>::NW), (8 / Shape<T, D, QT
     } else if (a.target == 0) {
         whole = true;
     } else {
-        const int64_t at = (int64_t)(item - b) * cut.chunk - cut.start;
-        c0 = (int)max(at, (int64_t)0);
-        c1 = (int)min(at + cut.chunk, (int64_t)nt);
+        const int at = (item - b) * cut.chunk - cut.start;
+        c0 = max(at, 0);
+        c1 = min(at + cut.chunk, nt);
         whole = cut.count == 1;
     }
     c0 = uniform(c0), c1 = uniform(c1);
@@ -245,7 +266,7 @@ __global__ __launch_bounds__((64 * Shape<T, D, QT, WR>::NW), (8 / Shape<T, D, QT
     // for the walks, where the chunk holds new tokens
     const bool walk = a.parents != nullptr && c1 > nct;
     if (walk) {
-        for (int u = tid; u < tn; u += THREADS) {
+        for (int u = tid; u < tn; u += 256) {
             const int p = a.parents[b * a.ld_par + u];
             s_up[u] = (int16_t)(p >= 0 && p < u ? p : -1);
         }
@@ -362,8 +383,8 @@ __global__ __launch_bounds__((64 * Shape<T, D, QT, WR>::NW), (8 / Shape<T, D, QT
 #pragma unroll
                 for (int e = 0; e < S::IPG; ++e) {
                     const int64_t rows = (int64_t)e * S::RPI * pool_row;
-                    dma16_soff(k + rows, lane_row + (kl ^ k_turn(e)), lk + e * 1024);
-                    dma16_soff(v + rows, lane_row + (vl ^ v_turn(e)), lv + e * 1024);
+                    dma16_stream(k + rows, lane_row + (kl ^ k_turn(e)), lk + e * 1024);
+                    dma16_stream(v + rows, lane_row + (vl ^ v_turn(e)), lv + e * 1024);
                 }
             } else {
                 const int64_t kr = (cached ? a.ps[2] : a.kns[2]) * S::ES, vr = (cached ? a.ps[2] : a.vns[2]) * S::ES;
@@ -661,7 +682,7 @@ __global__ __launch_bounds__((64 * Shape<T, D, QT, WR>::NW), (8 / Shape<T, D, QT
             }
         }
         __syncthreads();
-        for (int i = tid; i < S::RW * D / 4; i += THREADS) {
+        for (int i = tid; i < S::RW * D / 4; i += 256) {
             const int row = i / (D / 4), d = i % (D / 4) * 4;
             float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -791,8 +812,8 @@ struct Plan {
     size_t part_bytes, ml_bytes, score_bytes;
     size_t bytes() const { return part_bytes + ml_bytes + score_bytes; }
 };
-constexpr int WAVES = 2048;  // eight on each CU of an MI355X
-constexpr int WHOLE = 3;     // stages up to which a sequence stays with one workgroup
+constexpr int SLOTS = 512, SLOTS1 = 768;
+constexpr int WHOLE = 6;  // stages up to which a sequence stays with one workgroup
 Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int page, int top_k) {
     const int rows = top_k > 0 ? G : (int)std::min<int64_t>((int64_t)T * G, 1 << 20);
     Plan p;
@@ -805,9 +826,11 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     const int rw = 16 * p.qt * p.wr;
     p.row_tiles = (int)((all_rows + rw - 1) / rw);
     const int64_t per = (int64_t)Hkv * p.row_tiles;
-    const int nw = waves_of(d * (dtype == YTHIP_F32 ? 4 : 2), p.wr);
-    p.min_chunk = nw / p.wr;
-    const int64_t slots = WAVES / nw;  // workgroups that run at once
+    p.min_chunk = 4 / p.wr;
+    // Workgroups that the work is dealt to: the 512 that run at once where they share tiles (1024 of
+    // them: a tree of 64 over 131072 rows 126 -> 146 us, more partials); half as many again where
+    // each streams its own rows, so that none waits for the last (16 x 1 token 67 -> 63 us).
+    const int64_t slots = p.wr == 1 ? SLOTS1 : SLOTS;
     const int64_t new_tiles = ((int64_t)T + p.kt - 1) / p.kt;
     const int64_t seq_rows = (int64_t)std::min(top_k > 0 ? top_k : columns, columns) * page;
     const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + new_tiles, most = (tiles + p.min_chunk - 1) / p.min_chunk;
@@ -835,7 +858,7 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
     const int64_t groups = (p.items * a.Hkv + 7) / 8 * 8;
     if (groups * p.row_tiles > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups", (long long)(groups * p.row_tiles));
     using S = Shape<T, D, QT, WR>;
-    paged_attn_kernel<T, D, QT, WR, SPARSE><<<(int)(groups * p.row_tiles), 64 * S::NW, 0, s>>>(a);
+    paged_attn_kernel<T, D, QT, WR, SPARSE><<<(int)(groups * p.row_tiles), 256, 0, s>>>(a);
     if (p.part_bytes > 0) paged_merge_kernel<T, D, SPARSE><<<dim3((a.T * a.G + 3) / 4, a.Hkv, a.B), 256, 0, s>>>(a, S::KT);
     return status_of(hipGetLastError());
 }
@@ -937,6 +960,8 @@ int prepare(const char* who, const Call& c, PagedArgs& a, bool& done) {
     a.ld_table = c.ld_table, a.ld_par = c.ld_par, a.O = c.O;
     a.scale_log2 = (c.scale == 0.f ? 1.0f / sqrtf((float)c.d) : c.scale) * 1.4426950408889634f;
     a.sel = nullptr, a.top_k = 0, a.sums = nullptr, a.score = nullptr;
+    if (((int64_t)c.columns * c.page / 16 + c.T / 16 + 2) * c.B > INT_MAX)
+        return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences of up to %lld rows (2^35 in all)", who, c.B, (long long)c.columns * c.page);
     if (c.B > 65535 || c.Hq > 65535) return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences, %d heads (at most 65535 each)", who, c.B, c.Hq);
     return 0;
 }
