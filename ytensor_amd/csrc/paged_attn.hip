@@ -23,7 +23,7 @@ struct PagedArgs {
     int top_k;
     const float* sums;
     int64_t ss[2];
-    double* score;  // sparse: [B][Hkv][T][columns]
+    uint64_t* rank;  // sparse: [B][Hkv][T][columns], the pages' scores as rank_of has them
     int target, min_chunk, items, row_tiles;  // the cut: ranges (0: a sequence each; sparse: of a token), tiles one has at least
     float *part, *part_ml;  // partials of items: [items][Hkv][rows][d] and (max, sum)
 };
@@ -758,50 +758,174 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, int kt) {
     for (int e = 0; e < E; ++e) store_from_f32<T>(a.O, at + e, M == -INFINITY ? 0.f : acc[e] / L);
 }
 
-// One workgroup per (token, KV head, sequence): every page's score, then the pages that
-// fewer than top_k others beat.
-template <class T, int D>
-__global__ __launch_bounds__(256) void paged_select_simple(PagedArgs a) {
-    __shared__ double s_q[D];
-    const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+// ---------------------------------------------------------------------------
+// The choice of pages
+// ---------------------------------------------------------------------------
+
+// A score as an unsigned number of the same order: NaN lowest (as -inf), both zeros alike.
+__device__ __forceinline__ uint64_t rank_of(double s) {
+    s = s == s ? s + 0.0 : -INFINITY;
+    const uint64_t u = __builtin_bit_cast(uint64_t, s);
+    return (int64_t)u < 0 ? ~u : u | 1ull << 63;
+}
+constexpr uint64_t RANK_TOP = ~0ull;  // the last page's: above every score's
+
+// Scores of 64 pages of one KV head for TB tokens: 16 lanes a page (D / 16 dims each), four
+// pages a wave at a time, all a lane's pages in flight together. The products are of float32 sums
+// and sums of the group's queries, all in 64 bits (the fp64 rate is the fp32 rate here, and the
+// time is that of the sums' bytes): scores that differ in their first 50 bits keep their order,
+// so the choice does not depend on how they were added up.
+template <class T, int D, int TB>
+__global__ __launch_bounds__(256) void paged_score_kernel(PagedArgs a) {
+    constexpr int E = D / 16, V = E / 4, U = 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
+    const int h = blockIdx.y % a.Hkv, t0 = blockIdx.y / a.Hkv * TB, b = blockIdx.z;
+    const int tn = new_rows(a, b), len = rows_in_use(a, b);
+    const int n = (int)(((int64_t)len + (1 << a.shift) - 1) >> a.shift);
+    const int first = (blockIdx.x * 4 + wave) * 16 + (lane >> 4);  // and + 4, + 8, + 12
+    if (t0 >= tn || blockIdx.x * 64 >= n) return;
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        id[u] = first + 4 * u < n ? a.table[b * a.ld_table + first + 4 * u] : -1;
+        if ((uint32_t)id[u] >= (uint32_t)a.pages) id[u] = -1;
+    }
+    f32x4 x[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            x[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+            // 16 lanes read 256 consecutive bytes
+            if (id[u] >= 0) {
+                const float* p = a.sums + id[u] * a.ss[0] + h * a.ss[1] + v * 64 + l16 * 4;
+                x[u][v] = f32x4{p[0], p[1], p[2], p[3]};
+            }
+        }
+#pragma unroll
+    for (int k = 0; k < TB; ++k) {
+        const int t = t0 + k;
+        if (t >= tn) return;
+        double q[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[e] = 0.0;
+        for (int g = 0; g < a.G; ++g) {
+            const int64_t at = b * a.qs[0] + (int64_t)(h * a.G + g) * a.qs[1] + t * a.qs[2] + l16 * 4;
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[e] += (double)load_as_f32<T>(a.Q, at + e / 4 * 64 + e % 4);
+        }
+        uint64_t* out = a.rank + (((int64_t)b * a.Hkv + h) * a.T + t) * a.columns;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            double s = 0.0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) s = fma(q[e], (double)x[u][e / 4][e % 4], s);
+#pragma unroll
+            for (int off = 8; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
+            const int i = first + 4 * u;
+            if (l16 == 0 && i < n) out[i] = i == n - 1 ? RANK_TOP : rank_of(id[u] >= 0 ? s : -INFINITY);
+        }
+    }
+}
+
+// The top_k highest of a row of ranks, ascending by page: the k-th highest rank is found eight
+// bits at a time (a histogram in LDS of the ranks that agree with the bits so far, in 16
+// copies: ranks of like scores fall into few bins), until a bin is taken whole; scores are
+// far apart in their first 24 bits, so that is three rounds mostly. Then a wave takes a run of pages
+// each and writes its share in order.
+constexpr int SEL = 256, SEL_KEEP = 8;  // threads; ranks each keeps in registers (longer rows are read again)
+__global__ __launch_bounds__(SEL) void paged_select_kernel(PagedArgs a) {
+    constexpr int COPIES = 16;
+    __shared__ int s_hist[256 * COPIES], s_bin[256], s_found[3], s_count[SEL / 64][2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     const int64_t row = ((int64_t)b * a.Hkv + h) * a.T + t;
     int32_t* sel = a.sel + row * a.top_k;
-    const int len = rows_in_use(a, b), n = t < new_rows(a, b) ? (int)(((int64_t)len + (1 << a.shift) - 1) >> a.shift) : 0;
-    if (tid < D) {
-        double q = 0.0;
-        for (int g = 0; g < a.G; ++g)
-            q += (double)load_as_f32<T>(a.Q, b * a.qs[0] + (h * a.G + g) * a.qs[1] + t * a.qs[2] + tid);
-        s_q[tid] = q;
+    const int len = rows_in_use(a, b);
+    const int n = t < new_rows(a, b) ? (int)(((int64_t)len + (1 << a.shift) - 1) >> a.shift) : 0;
+    if (n <= a.top_k) {
+        for (int i = tid; i < a.top_k; i += SEL) sel[i] = i < n ? i : -1;
+        return;
     }
-    __syncthreads();
-    double* score = a.score + row * a.columns;
-    for (int i = tid; i < n; i += 256) {
-        const int p = a.table[b * a.ld_table + i];
-        double s = 0.0;
-        if (p >= 0 && p < a.pages)
-            for (int e = 0; e < D; ++e) s = fma(s_q[e], (double)a.sums[p * a.ss[0] + h * a.ss[1] + e], s);
-        else s = -INFINITY;
-        if (s != s) s = -INFINITY;
-        score[i] = s;
-    }
-    for (int i = tid; i < a.top_k; i += 256) sel[i] = -1;
-    __threadfence_block();
-    __syncthreads();
-    for (int i = tid; i < n; i += 256) {
-        const double s = score[i];
-        int above = i < n - 1 ? 1 : 0;  // the last page
-        for (int j = 0; j < n - 1 && i < n - 1; ++j) above += score[j] > s || (score[j] == s && j < i);
-        if (above < a.top_k) sel[above] = i;
-    }
-    __threadfence_block();
-    __syncthreads();
-    if (tid == 0)  // ascending
-        for (int i = 1; i < min(n, a.top_k); ++i) {
-            const int v = sel[i];
-            int j = i;
-            for (; j > 0 && sel[j - 1] > v; --j) sel[j] = sel[j - 1];
-            sel[j] = v;
+    const uint64_t* rank = a.rank + row * a.columns;
+    // wave w has the pages from w * run on, 64 at a time
+    const int run = (n + SEL - 1) / SEL * 64;
+    const bool kept = n <= SEL * SEL_KEEP;
+    uint64_t r[SEL_KEEP];
+    if (kept) {
+#pragma unroll
+        for (int j = 0; j < SEL_KEEP; ++j) {
+            const int i = wave * run + j * 64 + lane;
+            r[j] = j * 64 < run && i < n ? rank[i] : 0;
         }
+    }
+    // f(j-th rank of this lane, whether it exists)
+    auto each = [&](auto f) {
+        if (kept) {
+#pragma unroll
+            for (int j = 0; j < SEL_KEEP; ++j)
+                if (j * 64 < run) f(r[j], wave * run + j * 64 + lane, wave * run + j * 64 + lane < n);
+        } else {
+            for (int j = 0; j * 64 < run; ++j) {
+                const int i = wave * run + j * 64 + lane;
+                f(i < n ? rank[i] : 0, i, i < n);
+            }
+        }
+    };
+    uint64_t prefix = 0;  // of the k-th highest rank, above bit `low`
+    int low = 64, want = a.top_k;  // still to be taken among the ranks with that prefix
+    for (;;) {
+        low -= 8;
+        for (int i = tid; i < 256 * COPIES; i += SEL) s_hist[i] = 0;
+        __syncthreads();
+        each([&](uint64_t x, int, bool is) {
+            if (is && (low == 56 || x >> (low + 8) == prefix)) atomicAdd(&s_hist[(int)(x >> low & 255) * COPIES + (lane & (COPIES - 1))], 1);
+        });
+        __syncthreads();
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) c += s_hist[tid * COPIES + ((i + tid) & (COPIES - 1))];
+        s_bin[tid] = c;
+        __syncthreads();
+        if (wave == 0) {
+            // lane l sums bins 255 - 4 l down; the bin that brings the sum to `want`
+            int v[4], mine = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine += v[i] = s_bin[255 - 4 * lane - i];
+            int before = wave_scan(mine) - mine;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (before < want && before + v[i] >= want) {
+                    s_found[0] = 255 - 4 * lane - i;
+                    s_found[1] = want - before;
+                    s_found[2] = v[i];
+                }
+                before += v[i];
+            }
+        }
+        __syncthreads();
+        prefix = prefix << 8 | (uint64_t)s_found[0];
+        want = s_found[1];
+        if (low == 0 || s_found[2] == want) break;
+    }
+    // above the prefix: taken; with it: the first `want`
+    int over = 0, same = 0;
+    each([&](uint64_t x, int, bool is) {
+        over += __popcll(__ballot(is && x >> low > prefix));
+        same += __popcll(__ballot(is && x >> low == prefix));
+    });
+    if (lane == 0) s_count[wave][0] = over, s_count[wave][1] = same;
+    __syncthreads();
+    over = same = 0;
+    for (int w = 0; w < wave; ++w) over += s_count[w][0], same += s_count[w][1];
+    const uint64_t below = (1ull << lane) - 1;
+    each([&](uint64_t x, int i, bool is) {
+        const uint64_t o = __ballot(is && x >> low > prefix), e = __ballot(is && x >> low == prefix);
+        const int eq = same + __popcll(e & below), at = over + __popcll(o & below) + min(eq, want);
+        if ((o >> lane & 1) || ((e >> lane & 1) && eq < want)) sel[at] = i;
+        over += __popcll(o);
+        same += __popcll(e);
+    });
 }
 
 // How a call is cut. Both the size of the workspace and the launch come from this alone.
@@ -809,8 +933,8 @@ struct Plan {
     int qt, wr, kt;  // the workgroup's shape
     int target, min_chunk, row_tiles;
     int64_t items;
-    size_t part_bytes, ml_bytes, score_bytes;
-    size_t bytes() const { return part_bytes + ml_bytes + score_bytes; }
+    size_t part_bytes, ml_bytes, rank_bytes;
+    size_t bytes() const { return part_bytes + ml_bytes + rank_bytes; }
 };
 constexpr int SLOTS = 512, SLOTS1 = 768;
 constexpr int WHOLE = 6;  // stages up to which a sequence stays with one workgroup
@@ -849,7 +973,7 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     const int64_t part_rows = part_items * Hkv * all_rows;
     p.part_bytes = (size_t)part_rows * d * sizeof(float);
     p.ml_bytes = ((size_t)part_rows * 2 * sizeof(float) + 15) / 16 * 16;
-    p.score_bytes = top_k > 0 ? (size_t)B * Hkv * T * columns * sizeof(double) : 0;
+    p.rank_bytes = top_k > 0 ? (size_t)B * Hkv * T * columns * sizeof(uint64_t) : 0;
     return p;
 }
 
@@ -864,7 +988,12 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
 }
 template <class T, int D, bool SPARSE>
 int run_typed(const PagedArgs& a, const Plan& p, hipStream_t s) {
-    if constexpr (SPARSE) paged_select_simple<T, D><<<dim3(a.T, a.Hkv, a.B), 256, 0, s>>>(a);
+    if constexpr (SPARSE) {
+        constexpr int TB = 4;
+        if (a.columns > 0)
+            paged_score_kernel<T, D, TB><<<dim3((a.columns + 63) / 64, a.Hkv * ((a.T + TB - 1) / TB), a.B), 256, 0, s>>>(a);
+        paged_select_kernel<<<dim3(a.T, a.Hkv, a.B), SEL, 0, s>>>(a);
+    }
     if (p.qt == 1) return launch<T, D, 1, 1, SPARSE>(a, p, s);
     if constexpr (!SPARSE) {
         if (p.wr == 2) return launch<T, D, 2, 2, SPARSE>(a, p, s);
@@ -877,9 +1006,9 @@ int run(int dtype, int d, PagedArgs& a, void* ws, hipStream_t s) {
     const Plan p = plan_of(dtype, a.B, a.Hkv, a.G, a.T, d, a.columns, 1 << a.shift, SPARSE ? a.top_k : 0);
     a.target = p.target, a.min_chunk = p.min_chunk, a.items = (int)p.items, a.row_tiles = p.row_tiles;
     char* w = static_cast<char*>(ws);
-    a.score = reinterpret_cast<double*>(w);
-    a.part = reinterpret_cast<float*>(w + p.score_bytes);
-    a.part_ml = reinterpret_cast<float*>(w + p.score_bytes + p.part_bytes);
+    a.rank = reinterpret_cast<uint64_t*>(w);
+    a.part = reinterpret_cast<float*>(w + p.rank_bytes);
+    a.part_ml = reinterpret_cast<float*>(w + p.rank_bytes + p.part_bytes);
     if (dtype == YTHIP_F32) return d == 64 ? run_typed<F32, 64, SPARSE>(a, p, s) : run_typed<F32, 128, SPARSE>(a, p, s);
     if (dtype == YTHIP_F16) return d == 64 ? run_typed<F16, 64, SPARSE>(a, p, s) : run_typed<F16, 128, SPARSE>(a, p, s);
     return d == 64 ? run_typed<BF16, 64, SPARSE>(a, p, s) : run_typed<BF16, 128, SPARSE>(a, p, s);
@@ -959,7 +1088,7 @@ int prepare(const char* who, const Call& c, PagedArgs& a, bool& done) {
     a.table = c.table, a.kv_len = c.kv_len, a.parents = c.parents, a.new_len = c.new_len;
     a.ld_table = c.ld_table, a.ld_par = c.ld_par, a.O = c.O;
     a.scale_log2 = (c.scale == 0.f ? 1.0f / sqrtf((float)c.d) : c.scale) * 1.4426950408889634f;
-    a.sel = nullptr, a.top_k = 0, a.sums = nullptr, a.score = nullptr;
+    a.sel = nullptr, a.top_k = 0, a.sums = nullptr, a.rank = nullptr;
     if (((int64_t)c.columns * c.page / 16 + c.T / 16 + 2) * c.B > INT_MAX)
         return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences of up to %lld rows (2^35 in all)", who, c.B, (long long)c.columns * c.page);
     if (c.B > 65535 || c.Hq > 65535) return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences, %d heads (at most 65535 each)", who, c.B, c.Hq);
@@ -1015,6 +1144,7 @@ __attribute__((visibility("default"))) int ythip_paged_attn_sparse(
                     table, ld_table, columns, kv_len, parents, ld_parents, new_len, O, o_str, scale};
     const int st = prepare(who, c, a, done);
     if (st || done) return st;
+    if ((int64_t)Hkv * T > 65535) return fail(YTHIP_EUNSUPPORTED, "%s: %d tokens of %d KV heads (at most 65535)", who, T, Hkv);
     if (top_k < 1 || top_k > 4096) return fail(YTHIP_EINVAL, "%s: top_k %d (1 to 4096)", who, top_k);
     if (!sel || !sums_str || (pages > 0 && !sums)) return fail(YTHIP_EINVAL, "%s: sel or sums is NULL", who);
     if (const int e = check_workspace(who, workspace(dtype, B, Hq, Hkv, T, d, columns, page, top_k), workspace_, ws_bytes)) return e;
