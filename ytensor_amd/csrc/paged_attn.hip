@@ -209,7 +209,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         gi = (q / a.row_tiles) * 8 + (w & 7);
     }
     if (gi >= a.items * a.Hkv) return;
-    const int h = gi % a.Hkv, item = gi / a.Hkv;
+    const int h = gi % a.Hkv;
+    // the last items first: those with new tokens, whose tiles cost more, do not end alone
+    const int item = a.items - 1 - gi / a.Hkv;
 
     const int R = SPARSE ? a.G : a.T * a.G;
     const int r0 = rt * S::RW;
@@ -306,8 +308,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     }
     auto k_turn = [](int e) { return (uint32_t)((e * S::RPI & KMASK) * 16); };
     auto v_turn = [](int e) { return (uint32_t)(F ? (((e * S::RPI) >> 2 & 3) << 2) * 16 : (e * S::RPI & BMASK) * 32); };
-    const int pool_row = (int)a.ps[2] * S::ES;
-    const uint32_t lane_row = dma_row * pool_row;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
     const char *Kp = static_cast<const char*>(a.Kp) + h * a.ps[1] * S::ES, *Vp = static_cast<const char*>(a.Vp) + h * a.ps[1] * S::ES;
     const char* Kn = static_cast<const char*>(a.Kn) + (b * a.kns[0] + h * a.kns[1]) * S::ES;
@@ -375,25 +375,24 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             }
             const int i = wr * S::GPW + j, n = (pack >> (5 * i)) & 31;
             const uint32_t lk = lds0 + ((s & 1) * 2 * S::STG + wk * S::TILE + i * 16 * S::CH) * 16, lv = lk + S::STG * 16;
-            if (cached && n == 16) {
+            const int kr = (int)(cached ? a.ps[2] : a.kns[2]) * S::ES, vr = (int)(cached ? a.ps[2] : a.vns[2]) * S::ES;
+            if (n == 16) {
                 k = uniform(k), v = uniform(v);
                 // the lane offsets anew each time: kept, they would not all fit the registers
                 uint32_t kl = kx, vl = vx;
                 asm volatile("" : "+v"(kl), "+v"(vl));
 #pragma unroll
                 for (int e = 0; e < S::IPG; ++e) {
-                    const int64_t rows = (int64_t)e * S::RPI * pool_row;
-                    dma16_stream(k + rows, lane_row + (kl ^ k_turn(e)), lk + e * 1024);
-                    dma16_stream(v + rows, lane_row + (vl ^ v_turn(e)), lv + e * 1024);
+                    dma16_stream(k + (int64_t)e * S::RPI * kr, dma_row * kr + (kl ^ k_turn(e)), lk + e * 1024);
+                    dma16_stream(v + (int64_t)e * S::RPI * vr, dma_row * vr + (vl ^ v_turn(e)), lv + e * 1024);
                 }
             } else {
-                const int64_t kr = (cached ? a.ps[2] : a.kns[2]) * S::ES, vr = (cached ? a.ps[2] : a.vns[2]) * S::ES;
 #pragma unroll
                 for (int e = 0; e < S::IPG; ++e) {
                     const int row = e * S::RPI + dma_row;
                     const char* zero = reinterpret_cast<const char*>(zeros);
-                    const char* ka = row < n ? k + row * kr + (kx ^ k_turn(e)) : zero;
-                    const char* va = row < n ? v + row * vr + (vx ^ v_turn(e)) : zero;
+                    const char* ka = row < n ? k + (int64_t)row * kr + (kx ^ k_turn(e)) : zero;
+                    const char* va = row < n ? v + (int64_t)row * vr + (vx ^ v_turn(e)) : zero;
                     dma16_async(ka, smem + (lk - lds0) / 16 + e * 64);
                     dma16_async(va, smem + (lv - lds0) / 16 + e * 64);
                 }
@@ -468,6 +467,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         uint64_t see[QT];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) see[qt] = 0;
+        bool paths = false;  // some query does not see all of a tile of new tokens
         if (!cached) {
             // the new tokens of this tile on each query's path
             const int u0 = (ti - nct) * KT;
@@ -483,8 +483,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                     see[qt] = tok[qt] - u0 >= 63 ? ~0ull : (2ull << (tok[qt] - u0)) - 1;
                 }
                 any = any || see[qt] != 0;
+                paths = paths || see[qt] != (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
             }
             if (__ballot(any) == 0) return;
+            paths = __ballot(paths) != 0;
         }
         f32x4 p[QT][S::KG];
 #pragma unroll
@@ -500,14 +502,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             }
         }
         constexpr uint32_t FULL = S::KG == 1 ? 16u : S::KG == 2 ? 16u | 16u << 5 : 16u | 16u << 5 | 16u << 10 | 16u << 15;
-        if (!cached || pack != FULL) {
+        if (paths || pack != FULL) {
 #pragma unroll
             for (int kt = 0; kt < S::KG; ++kt) {
                 // the rows in use of the group, and the path's bits, of this lane's four keys
                 const int n = (int)((pack >> (5 * kt)) & 31) - 4 * g;
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt) {
-                    const uint32_t vis = cached ? 15u : (uint32_t)(see[qt] >> (kt * 16 + 4 * g));
+                    const uint32_t vis = !paths ? 15u : (uint32_t)(see[qt] >> (kt * 16 + 4 * g));
 #pragma unroll
                     for (int r = 0; r < 4; ++r) p[qt][kt][r] = r < n && (vis >> r & 1) ? p[qt][kt][r] : -INFINITY;
                 }
@@ -539,10 +541,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             }
         }
         uint64_t odd = 0;
-        if (!cached) {
+        if (paths) {
             // 0 . V is NaN for a V that is not finite: such elements are left out of the product and
             // added (their weight cannot change what comes of them) for the queries that see the row
-#pragma unroll 1
+#pragma unroll 4
             for (int i = 0; i < S::TILE / 64; ++i) {
                 const u32x4 v = cV[i * 64 + lane];
                 bool bad = false;
@@ -967,7 +969,10 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
         p.target = 0;
         p.items = B;
     } else {
-        p.target = (int)std::min(std::max<int64_t>(1, slots / per), B * most);
+        // a few sequences: their boundaries' items among the slots too
+        int64_t ranges = slots / per;
+        if (B - 1 <= ranges / 2) ranges -= B - 1;
+        p.target = (int)std::min(std::max<int64_t>(1, ranges), B * most);
         p.items = part_items = (int64_t)p.target + B - 1;
     }
     const int64_t part_rows = part_items * Hkv * all_rows;
@@ -1078,7 +1083,8 @@ int prepare(const char* who, const Call& c, PagedArgs& a, bool& done) {
         if (c.Kn) all |= (c.kn_str[i] | c.vn_str[i]) * es;
     }
     if ((all & 15) != 0) return fail(YTHIP_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
-    if (c.pool_str[2] < 0 || c.pool_str[2] >= 1 << 24) return fail(YTHIP_EUNSUPPORTED, "%s: pool rows at a stride of %lld (0 to 2^24 - 1)", who, (long long)c.pool_str[2]);
+    for (const int64_t row : {c.pool_str[2], c.Kn ? c.kn_str[2] : 0, c.Kn ? c.vn_str[2] : 0})  // 16 rows within 32-bit offsets
+        if (row < 0 || row >= 1 << 24) return fail(YTHIP_EUNSUPPORTED, "%s: K or V rows at a stride of %lld (0 to 2^24 - 1)", who, (long long)row);
     a.B = c.B, a.Hq = c.Hq, a.Hkv = c.Hkv, a.G = c.Hq / c.Hkv, a.T = c.T, a.pages = c.pages, a.columns = c.columns;
     a.Q = c.Q, a.Kn = c.Kn, a.Vn = c.Vn, a.Kp = c.Kp, a.Vp = c.Vp;
     for (int i = 0; i < 3; ++i) {
