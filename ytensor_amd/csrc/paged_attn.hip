@@ -376,23 +376,25 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             const int i = wr * S::GPW + j, n = (pack >> (5 * i)) & 31;
             const uint32_t lk = lds0 + ((s & 1) * 2 * S::STG + wk * S::TILE + i * 16 * S::CH) * 16, lv = lk + S::STG * 16;
             const int kr = (int)(cached ? a.ps[2] : a.kns[2]) * S::ES, vr = (int)(cached ? a.ps[2] : a.vns[2]) * S::ES;
+            // the lane offsets anew each time: kept, they would not all fit the registers, and a register
+            // read back from memory waits for every row in flight
+            uint32_t kl = kx, vl = vx;
+            int lane_row = dma_row;
+            asm volatile("" : "+v"(kl), "+v"(vl), "+v"(lane_row));
             if (n == 16) {
                 k = uniform(k), v = uniform(v);
-                // the lane offsets anew each time: kept, they would not all fit the registers
-                uint32_t kl = kx, vl = vx;
-                asm volatile("" : "+v"(kl), "+v"(vl));
 #pragma unroll
                 for (int e = 0; e < S::IPG; ++e) {
-                    dma16_stream(k + (int64_t)e * S::RPI * kr, dma_row * kr + (kl ^ k_turn(e)), lk + e * 1024);
-                    dma16_stream(v + (int64_t)e * S::RPI * vr, dma_row * vr + (vl ^ v_turn(e)), lv + e * 1024);
+                    dma16_stream(k + (int64_t)e * S::RPI * kr, lane_row * kr + (kl ^ k_turn(e)), lk + e * 1024);
+                    dma16_stream(v + (int64_t)e * S::RPI * vr, lane_row * vr + (vl ^ v_turn(e)), lv + e * 1024);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < S::IPG; ++e) {
-                    const int row = e * S::RPI + dma_row;
+                    const int row = e * S::RPI + lane_row;
                     const char* zero = reinterpret_cast<const char*>(zeros);
-                    const char* ka = row < n ? k + (int64_t)row * kr + (kx ^ k_turn(e)) : zero;
-                    const char* va = row < n ? v + (int64_t)row * vr + (vx ^ v_turn(e)) : zero;
+                    const char* ka = row < n ? k + (int64_t)row * kr + (kl ^ k_turn(e)) : zero;
+                    const char* va = row < n ? v + (int64_t)row * vr + (vl ^ v_turn(e)) : zero;
                     dma16_async(ka, smem + (lk - lds0) / 16 + e * 64);
                     dma16_async(va, smem + (lv - lds0) / 16 + e * 64);
                 }
@@ -411,20 +413,24 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         for (int t = 0; t < S::DT; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+    const char* lds = reinterpret_cast<const char*>(smem);
+    const int k_frag = l16 * S::ROWB + ((g ^ (l16 & KMASK)) << 4);
+    const int v_key = 4 * g + (l16 >> 2);
+    const int v_frag = F ? 4 * g * S::ROWB + ((l16 >> 2) ^ (g << 2)) * 16 + (l16 & 3) * 4
+                         : v_key * S::ROWB + ((v_key & BMASK) << 5) + 8 * (l16 & 3);
     // acc += V^T . P^T for output rows 16 t..16 t + 15 over the tile's keys (CLEAN: elements of V that
     // are not finite taken as 0); pk: p as the MFMA takes it
     constexpr uint32_t EXP2 = std::is_same_v<T, BF16> ? 0x7f807f80u : 0x7c007c00u, STEP2 = std::is_same_v<T, BF16> ? 0x00800080u : 0x04000400u;
     constexpr int PK = F ? S::KG : S::KG >= 2 ? S::KG / 2 : 1;
-    auto pv = [&](const u32x4* cV, int t, const u32x4 (&pk)[QT][PK], f32x4 (&acc)[QT], auto clean) {
+    auto pv = [&](int v_at, int t, const u32x4 (&pk)[QT][PK], f32x4 (&acc)[QT], auto clean) {
         constexpr bool CLEAN = decltype(clean)::value;
         if constexpr (F) {
-            const float* V = reinterpret_cast<const float*>(cV);
 #pragma unroll
             for (int kt = 0; kt < S::KG; ++kt)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int key = kt * 16 + 4 * g + j, c = t * 4 + (l16 >> 2);
-                    float v = V[key * D + ((c ^ (((key >> 2) & 3) << 2)) << 2) + (l16 & 3)];
+                    // chunk 4 t + l16 / 4 of key 16 kt + 4 g + j, stored at the chunk ^ 4 g
+                    float v = *reinterpret_cast<const float*>(lds + ((v_at ^ (t << 6)) + (kt * 16 + j) * S::ROWB));
                     if (CLEAN) v = fabsf(v) < INFINITY ? v : 0.f;
 #pragma unroll
                     for (int qt = 0; qt < QT; ++qt)
@@ -436,8 +442,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                 u32x4 vf = {0u, 0u, 0u, 0u};
 #pragma unroll
                 for (int hh = 0; hh < (S::KG >= 2 ? 2 : 1); ++hh) {
-                    const int key = (2 * kk + hh) * 16 + g * 4 + (l16 >> 2);
-                    const u32x2 w = lds_read_tr16(cV, key * S::ROWB + ((t ^ (key & BMASK)) << 5) + 8 * (l16 & 3));
+                    // 32-byte block t of key 16 (2 kk + hh) + 4 g + l16 / 4, stored at the block ^ (key & BMASK)
+                    const u32x2 w = lds_read_tr16(smem, (v_at ^ (t << 5)) + (2 * kk + hh) * 16 * S::ROWB);
                     vf[2 * hh] = w[0];
                     vf[2 * hh + 1] = w[1];
                 }
@@ -461,8 +467,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     auto compute = [&](int s, uint32_t pack, auto with_new) {
         constexpr bool NEW = decltype(with_new)::value;
         const int ti = tile_at(s);
-        const u32x4* cK = smem + (s & 1) * 2 * S::STG + wk * S::TILE;
-        const u32x4* cV = cK + S::STG;
+        // LDS bytes of this lane's first K and V fragments; the others are a constant's turn and distance
+        // away (worked out each time: kept, they would not all fit the registers)
+        const int stage = ((s & 1) * 2 * S::STG + wk * S::TILE) * 16;
+        int k_at = stage + k_frag, v_at = stage + S::STG * 16 + v_frag;
+        asm volatile("" : "+v"(k_at), "+v"(v_at));
+        const u32x4* cV = smem + (stage >> 4) + S::STG;
         const bool cached = !NEW || ti < nct;
         uint64_t see[QT];
 #pragma unroll
@@ -493,10 +503,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         for (int kt = 0; kt < S::KG; ++kt) {
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) p[qt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const int key = kt * 16 + l16;
 #pragma unroll
             for (int ks = 0; ks < S::KS; ++ks) {
-                const u32x4 kf = cK[key * S::CH + ((ks * 4 + g) ^ (key & KMASK))];
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(lds + ((k_at ^ (ks << 6)) + kt * 16 * S::ROWB));
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt) p[qt][kt] = mfma_chunk(T{}, kf, qf[qt][ks], p[qt][kt]);
             }
@@ -579,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                 f32x4 acc[QT];
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt) acc[qt] = o[qt][t];
-                pv(cV, t, pk, acc, clean);
+                pv(v_at, t, pk, acc, clean);
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt) o[qt][t] = acc[qt];
             }
