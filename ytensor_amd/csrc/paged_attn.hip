@@ -711,62 +711,86 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     }
 }
 
-// Joins the partials of a sequence that several items worked on: a wave per (token, head), in
-// the order of the items.
-template <class T, int D, bool SPARSE>
+// Joins the partials of a sequence that several items worked on, in the order of the items: D / 4
+// lanes a row of O (token, head), each four elements of every partial, MERGE_AHEAD of them in
+// flight. Bound by the partials' bytes for many rows, by four round trips to memory (lengths,
+// maxima and sums, partials, O) for few, whose partials the four waves of a workgroup share
+// (SHARE).
+constexpr int MERGE_AHEAD = 8;
+template <class T, int D, bool SPARSE, bool SHARE>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, int kt) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int r = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z;
-    const int tn = new_rows(a, b);
-    const int t = r / a.G, gh = r - t * a.G;
-    if (t >= tn) return;
-    int64_t first, step;
-    int count;
+    constexpr int LPR = D / 4, RPW = 64 / LPR;
+    const int lane = threadIdx.x & 63, sub = lane % LPR, group = lane / LPR;
+    const int h = blockIdx.y, b = blockIdx.z;
+    const int wave = uniform((int)threadIdx.x >> 6);
+    const int r = (SHARE ? blockIdx.x : blockIdx.x * 4 + wave) * RPW + group;
+    const int R = SPARSE ? a.G : a.T * a.G;
+    int64_t first;
+    int count, tn, t, gh;
+    const int64_t step = (int64_t)a.Hkv * R;  // rows between an item's partial and the next one's
     if constexpr (SPARSE) {
         const int len = rows_in_use(a, b);
+        tn = new_rows(a, b);
+        t = r / a.G, gh = r - t * a.G;
         const int nsel = min(a.top_k, (int)(((int64_t)len + (1 << a.shift) - 1) >> a.shift));
         const int nt = (int)((((int64_t)nsel << a.shift) + kt - 1) / kt) + (a.Kn != nullptr ? (t + kt) / kt : 0);
         const int chunk = max((nt + a.target - 1) / a.target, a.min_chunk);
         count = max((nt + chunk - 1) / chunk, 1);
         first = (((int64_t)(b * a.T + t) * a.target) * a.Hkv + h) * a.G + gh;
-        step = (int64_t)a.Hkv * a.G;
     } else {
         const Cut c = cut_of(a, kt, 0, b);
-        count = c.count;
-        first = ((int64_t)c.first * a.Hkv + h) * a.T * a.G + r;
-        step = (int64_t)a.Hkv * a.T * a.G;
+        count = c.count, tn = c.tn;
+        if (count == 1) return;
+        t = r / a.G, gh = r - t * a.G;
+        first = ((int64_t)c.first * a.Hkv + h) * R + r;
     }
-    if (count == 1) return;
-    float M = -INFINITY, L = 0.f, acc[E];
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int s = lane; s < count; s += 64) M = __builtin_elementwise_maximum(M, a.part_ml[2 * (first + s * step)]);
+    if (t >= tn || t >= a.T) count = 1;  // nothing to join: it stays for the others' shuffles, on partial 0
+    const bool join = count > 1;
+    if (__ballot(join) == 0) return;
+    if (!join) first = 0;
+    const float* ml = a.part_ml + 2 * first;
+    const float* src = a.part + first * D + sub * 4;
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = sub; s < count; s += LPR) M = __builtin_elementwise_maximum(M, ml[2 * s * step]);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) M = __builtin_elementwise_maximum(M, __shfl_xor(M, off, 64));
+    for (int off = LPR / 2; off >= 1; off >>= 1) M = __builtin_elementwise_maximum(M, __shfl_xor(M, off, 64));
     const float ref = M == -INFINITY ? 0.f : M;
-    for (int s0 = 0; s0 < count; s0 += 64) {
-        const int64_t mine = first + (int64_t)min(s0 + lane, count - 1) * step;
-        const float w = s0 + lane < count ? __builtin_amdgcn_exp2f(a.part_ml[2 * mine] - ref) : 0.f;
-        const float lw = s0 + lane < count ? w * a.part_ml[2 * mine + 1] : 0.f;
-        L += wave_sum(lw);
-        const int n = min(count - s0, 64);
-        const float* src = a.part + (first + (int64_t)s0 * step) * D + lane * E;
-        for (int s = 0; s < n; s += 8) {
-            float v[8][E];
+    int most = count;
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
+    for (int off = 32; off >= LPR; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
+    most = uniform(most);
+    for (int s0 = 0; s0 < most; s0 += LPR) {
+        // loads without a branch around them (past the last partial: the last again, with no weight),
+        // so that they are in flight together
+        const float* mine = ml + 2 * min(s0 + sub, count - 1) * step;
+        const float w = s0 + sub < count ? __builtin_amdgcn_exp2f(mine[0] - ref) : 0.f;
+        L += s0 + sub < count ? w * mine[1] : 0.f;
+        for (int s = SHARE ? wave * MERGE_AHEAD : 0; s < min(most - s0, LPR); s += SHARE ? 4 * MERGE_AHEAD : MERGE_AHEAD) {
+            f32x4 v[MERGE_AHEAD];
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[u][e] = src[(int64_t)min(s + u, n - 1) * step * D + e];
+            for (int u = 0; u < MERGE_AHEAD; ++u)
+                v[u] = *reinterpret_cast<const f32x4*>(src + min(s0 + s + u, count - 1) * step * D);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float ws = s + u < n ? __shfl(w, s + u, 64) : 0.f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] = s + u < n ? fmaf(ws, v[u][e], acc[e]) : acc[e];
-            }
+            for (int u = 0; u < MERGE_AHEAD; ++u)
+                if (s0 + s + u < count) acc += __shfl(w, group * LPR + s + u, 64) * v[u];
         }
     }
-    const int64_t at = b * a.os[0] + (int64_t)(h * a.G + gh) * a.os[1] + t * a.os[2] + lane * E;
-    for (int e = 0; e < E; ++e) store_from_f32<T>(a.O, at + e, M == -INFINITY ? 0.f : acc[e] / L);
+#pragma unroll
+    for (int off = LPR / 2; off >= 1; off >>= 1) L += __shfl_xor(L, off, 64);
+    if constexpr (SHARE) {
+        __shared__ f32x4 s_acc[4][64];
+        s_acc[wave][lane] = acc;
+        __syncthreads();
+        if (wave != 0) return;
+        acc = (s_acc[0][lane] + s_acc[1][lane]) + (s_acc[2][lane] + s_acc[3][lane]);
+    }
+    if (!join) return;
+    const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+    const f32x4 o = M == -INFINITY ? f32x4{0.f, 0.f, 0.f, 0.f} : acc * inv;
+    const int64_t at = b * a.os[0] + (int64_t)(h * a.G + gh) * a.os[1] + t * a.os[2] + sub * 4;
+    if constexpr (std::is_same_v<T, F32>) *reinterpret_cast<f32x4*>(static_cast<float*>(a.O) + at) = o;
+    else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.O) + at) = u32x2{pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
 }
 
 // ---------------------------------------------------------------------------
@@ -997,7 +1021,16 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
     if (groups * p.row_tiles > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups", (long long)(groups * p.row_tiles));
     using S = Shape<T, D, QT, WR>;
     paged_attn_kernel<T, D, QT, WR, SPARSE><<<(int)(groups * p.row_tiles), 256, 0, s>>>(a);
-    if (p.part_bytes > 0) paged_merge_kernel<T, D, SPARSE><<<dim3((a.T * a.G + 3) / 4, a.Hkv, a.B), 256, 0, s>>>(a, S::KT);
+    if (p.part_bytes > 0) {
+        constexpr int ROWS = 256 / D;  // of a wave
+        const int rows = a.T * a.G;
+        // few rows: a workgroup's waves share them (16 rows of 32 partials 6.8 -> 4.9 us; 5000 rows of
+        // about 12 8.3 -> 9.9)
+        if ((int64_t)a.B * a.Hkv * rows <= 512)
+            paged_merge_kernel<T, D, SPARSE, true><<<dim3((rows + ROWS - 1) / ROWS, a.Hkv, a.B), 256, 0, s>>>(a, S::KT);
+        else
+            paged_merge_kernel<T, D, SPARSE, false><<<dim3((rows + 4 * ROWS - 1) / (4 * ROWS), a.Hkv, a.B), 256, 0, s>>>(a, S::KT);
+    }
     return status_of(hipGetLastError());
 }
 template <class T, int D, bool SPARSE>

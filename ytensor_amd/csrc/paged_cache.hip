@@ -177,11 +177,10 @@ __device__ __forceinline__ void copy_piece(const PoolSet& ps, int k, int layer, 
         const int n = bytes >> 4;
         u32x4 v[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i * 256 + (int)threadIdx.x < n) v[i] = s[i * 256 + threadIdx.x];
+        for (int i = 0; i < N; ++i) v[i] = __builtin_nontemporal_load(s + min(i * 256 + (int)threadIdx.x, n - 1));
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (i * 256 + (int)threadIdx.x < n) d[i * 256 + threadIdx.x] = v[i];
+            if (i * 256 + (int)threadIdx.x < n) __builtin_nontemporal_store(v[i], d + i * 256 + threadIdx.x);
     } else {
         const uint32_t* s = reinterpret_cast<const uint32_t*>(src);
         uint32_t* d = reinterpret_cast<uint32_t*>(dst);
@@ -483,21 +482,39 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
             }
         }
     };
-    for (int r = works ? rg : hi; r < hi; r += rows) {
-        if (r < lo) {
-            if (a.sums != nullptr) add(*reinterpret_cast<const u32x4*>(kp + r * a.ps3));
-            continue;
+    // AHEAD rows of a thread at a time, all loads before the first store (loads without a branch
+    // around them: a row that is not there reads the page's first and its value is dropped)
+    constexpr int AHEAD = 4;
+    const int r_first = a.sums != nullptr ? rg : lo + rg;  // without sums the old rows are not read
+    for (int r = works ? r_first : hi; r < hi; r += AHEAD * rows) {
+        u32x4 k[AHEAD], v[AHEAD];
+        int from[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int j = r0 + r + u * rows - len;  // the new row; negative: an old one
+            const bool fresh = j >= 0 && r + u * rows < hi;
+            from[u] = fresh ? j : -1;
+            if (a.path != nullptr && fresh) from[u] = a.path[b * a.ld_path + j];
+            if (from[u] >= a.T) from[u] = -1;
         }
-        const int j = r0 + r - len;
-        const int from = a.path != nullptr ? a.path[b * a.ld_path + j] : j;
-        u32x4 k = {0u, 0u, 0u, 0u}, v = {0u, 0u, 0u, 0u};
-        if (from >= 0 && from < a.T) {
-            k = *reinterpret_cast<const u32x4*>(kn + from * a.ns3);
-            v = *reinterpret_cast<const u32x4*>(vn + from * a.ns3);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int row = r + u * rows;
+            const char* kk = row < lo ? kp + row * a.ps3 : kn + max(from[u], 0) * a.ns3;
+            k[u] = *reinterpret_cast<const u32x4*>(kk);
+            v[u] = *reinterpret_cast<const u32x4*>(vn + max(from[u], 0) * a.ns3);
         }
-        *reinterpret_cast<u32x4*>(kp + r * a.ps3) = k;
-        *reinterpret_cast<u32x4*>(vp + r * a.ps3) = v;
-        if (a.sums != nullptr) add(k);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int row = r + u * rows;
+            if (row >= hi) break;
+            if (row >= lo) {
+                if (from[u] < 0) k[u] = v[u] = u32x4{0u, 0u, 0u, 0u};
+                *reinterpret_cast<u32x4*>(kp + row * a.ps3) = k[u];
+                *reinterpret_cast<u32x4*>(vp + row * a.ps3) = v[u];
+            }
+            if (a.sums != nullptr) add(k[u]);
+        }
     }
     if (a.sums == nullptr) return;
     const int d = a.chunks * VN;
