@@ -868,7 +868,8 @@ __global__ __launch_bounds__(256) void paged_score_kernel(PagedArgs a) {
 // copies: ranks of like scores fall into few bins), until a bin is taken whole; scores are
 // far apart in their first 24 bits, so that is three rounds mostly. Then a wave takes a run of pages
 // each and writes its share in order.
-constexpr int SEL = 256, SEL_KEEP = 8;  // threads; ranks each keeps in registers (longer rows are read again)
+constexpr int SEL_KEEP = 8;  // ranks a thread keeps in registers (longer rows are read again)
+template <int SEL>           // threads
 __global__ __launch_bounds__(SEL) void paged_select_kernel(PagedArgs a) {
     constexpr int COPIES = 16;
     __shared__ int s_hist[256 * COPIES], s_bin[256], s_found[3], s_count[SEL / 64][2];
@@ -917,10 +918,12 @@ __global__ __launch_bounds__(SEL) void paged_select_kernel(PagedArgs a) {
             if (is && (low == 56 || x >> (low + 8) == prefix)) atomicAdd(&s_hist[(int)(x >> low & 255) * COPIES + (lane & (COPIES - 1))], 1);
         });
         __syncthreads();
-        int c = 0;
+        if (tid < 256) {
+            int c = 0;
 #pragma unroll
-        for (int i = 0; i < COPIES; ++i) c += s_hist[tid * COPIES + ((i + tid) & (COPIES - 1))];
-        s_bin[tid] = c;
+            for (int i = 0; i < COPIES; ++i) c += s_hist[tid * COPIES + ((i + tid) & (COPIES - 1))];
+            s_bin[tid] = c;
+        }
         __syncthreads();
         if (wave == 0) {
             // lane l sums bins 255 - 4 l down; the bin that brings the sum to `want`
@@ -1039,7 +1042,8 @@ int run_typed(const PagedArgs& a, const Plan& p, hipStream_t s) {
         constexpr int TB = 4;
         if (a.columns > 0)
             paged_score_kernel<T, D, TB><<<dim3((a.columns + 63) / 64, a.Hkv * ((a.T + TB - 1) / TB), a.B), 256, 0, s>>>(a);
-        paged_select_kernel<<<dim3(a.T, a.Hkv, a.B), SEL, 0, s>>>(a);
+        if (a.columns > 1024) paged_select_kernel<1024><<<dim3(a.T, a.Hkv, a.B), 1024, 0, s>>>(a);
+        else paged_select_kernel<256><<<dim3(a.T, a.Hkv, a.B), 256, 0, s>>>(a);
     }
     if (p.qt == 1) return launch<T, D, 1, 1, SPARSE>(a, p, s);
     if constexpr (!SPARSE) {

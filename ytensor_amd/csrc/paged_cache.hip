@@ -72,15 +72,16 @@ __device__ __forceinline__ int scan_free(const int32_t* ref, int pages, int want
     return met;
 }
 
-// (ref, table, len) into the arrays that a call writes, where those are others.
+// (ref, table, len) into the arrays that a call writes, where those are others; `here`: by the
+// deciding workgroup itself (a few words a thread), else in a launch before it.
 struct StateArgs {
+    bool here;
     int B, columns, pages;
     const int32_t *ref, *table, *len;
     int64_t ld, ld_out;
     int32_t *ref_out, *table_out, *len_out;
 };
-__global__ __launch_bounds__(256) void cache_state_copy(StateArgs a) {
-    const int64_t step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void copy_state_words(const StateArgs& a, int64_t at, int64_t step) {
     if (a.ref_out != a.ref)
         for (int64_t i = at; i < a.pages; i += step) a.ref_out[i] = a.ref[i];
     if (a.len_out != a.len)
@@ -91,6 +92,9 @@ __global__ __launch_bounds__(256) void cache_state_copy(StateArgs a) {
             a.table_out[b * a.ld_out + c] = a.table[b * a.ld + c];
         }
 }
+__global__ __launch_bounds__(256) void cache_state_copy(StateArgs a) {
+    copy_state_words(a, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
 
 struct GrowArgs {
     int B, columns, pages, shift;
@@ -98,12 +102,17 @@ struct GrowArgs {
     int32_t *ref, *table, *len;  // in place
     int64_t ld;
     int32_t* status;
+    StateArgs state;
 };
 // The prefix sum of the pages that the sequences need gives each its ranks among the free
 // pages; a free page's rank then finds its sequence by bisection.
 __global__ __launch_bounds__(PLAN_THREADS) void cache_grow_kernel(GrowArgs a) {
     constexpr int LIST = 4096;  // more pages than that: the free ones are looked up twice
     __shared__ int s_off[MAX_SEQS + 1], s_have[MAX_SEQS], s_list[LIST], s_scan[PLAN_THREADS / 64];
+    if (a.state.here) {
+        copy_state_words(a.state, threadIdx.x, PLAN_THREADS);
+        __syncthreads();
+    }
     const int64_t cap = (int64_t)a.columns << a.shift;
     int want = 0;
     for (int base = 0; base < a.B; base += PLAN_THREADS) {
@@ -214,9 +223,11 @@ struct ForkArgs {
     int64_t ld;
     int4* plan;  // per pair: source, destination (-1: refused), whole pages, the fresh page (-1: none)
     int32_t* status;
+    StateArgs state;
 };
 __global__ __launch_bounds__(PLAN_THREADS) void cache_fork_plan(ForkArgs a) {
     __shared__ int s_dst[MAX_SEQS], s_who[MAX_SEQS], s_page[MAX_SEQS], s_scan[PLAN_THREADS / 64];
+    if (a.state.here) copy_state_words(a.state, threadIdx.x, PLAN_THREADS);
     for (int i = threadIdx.x; i < a.n; i += PLAN_THREADS) s_dst[i] = a.dst[i];
     __syncthreads();
     const int64_t cap = (int64_t)a.columns << a.shift;
@@ -437,14 +448,17 @@ struct AppendArgs {
     int64_t ld_table, ld_path;
     int chunks;  // 16-byte chunks of a row
 };
-// A workgroup takes one page that the new rows of one (layer, sequence, KV head) touch:
-// thread = (row group, 16-byte chunk), so that a row moves as one run of bytes. It writes the
-// new rows and, for the key sums, adds every row in use to fp32 partials in registers, then the
-// row groups in order, so the sum is determined by the page's rows alone.
-template <class T>
-__global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
-    constexpr int VN = Vec<T>::n;
-    __shared__ float s_sum[256 * VN];
+// A workgroup of NW waves takes one page that the new rows of one (layer, sequence, KV head)
+// touch: thread = (row group, 16-byte chunk), so that a row moves as one run of bytes. It adds
+// the rows that are there and the new ones, which it writes, to fp32 partials in registers (row
+// r to group r % groups, ascending), then the groups in order, so the sum is determined by
+// the page's rows alone. Bound by the latency of the lengths, the table and the rows in turn, so
+// a page of up to 64 rows is one wave and all pages of a step are in flight at once
+// (16 sequences, 28 layers: APPEND us).
+template <class T, int NW>
+__global__ __launch_bounds__(64 * NW) void cache_append_kernel(AppendArgs a) {
+    constexpr int VN = Vec<T>::n, AHEAD = 8;
+    __shared__ float s_sum[64 * NW * VN];
     int w = blockIdx.x;
     const int i = w % a.slots;
     w /= a.slots;
@@ -453,18 +467,18 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
     const int b = w % a.B, l = w / a.B;
     const int page = 1 << a.shift;
     const int len = a.kv_len[b];
-    int n = a.n_new != nullptr ? min(a.n_new[b], a.T) : a.T;
+    const int n = a.n_new != nullptr ? min(a.n_new[b], a.T) : a.T;
     if (len < 0 || n <= 0) return;
     const int slot = (len >> a.shift) + i;
     const int64_t end = (int64_t)len + n;  // rows in use afterwards
     if (slot >= a.columns || ((int64_t)slot << a.shift) >= end) return;
     const int p = a.table[b * a.ld_table + slot];
     if (p < 0 || p >= a.pages) return;
-    const int r0 = slot << a.shift;                              // the page's first row
+    const int r0 = slot << a.shift;                                           // the page's first row
     const int lo = max(len - r0, 0), hi = (int)min(end - r0, (int64_t)page);  // its new rows
-    const int rows = 256 / a.chunks;                             // rows at a time
+    const int groups = 64 * NW / a.chunks;                                    // rows at a time
     const int rg = (int)threadIdx.x / a.chunks, ch = (int)threadIdx.x % a.chunks;
-    const bool works = rg < rows;
+    const bool works = rg < groups;
     char* kp = a.Kp + l * a.ps0 + p * a.ps1 + h * a.ps2 + ch * 16;
     char* vp = a.Vp + l * a.ps0 + p * a.ps1 + h * a.ps2 + ch * 16;
     const char* kn = a.Kn + l * a.ns0 + b * a.ns1 + h * a.ns2 + ch * 16;
@@ -482,40 +496,42 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
             }
         }
     };
-    // AHEAD rows of a thread at a time, all loads before the first store (loads without a branch
-    // around them: a row that is not there reads the page's first and its value is dropped)
-    constexpr int AHEAD = 4;
-    const int r_first = a.sums != nullptr ? rg : lo + rg;  // without sums the old rows are not read
-    for (int r = works ? r_first : hi; r < hi; r += AHEAD * rows) {
-        u32x4 k[AHEAD], v[AHEAD];
-        int from[AHEAD];
+    // AHEAD rows of a thread at a time: all their loads before the first use, without a branch around
+    // them (past the end: the last row again, dropped)
+    if (a.sums != nullptr && works && rg < lo)
+        for (int r = rg; r < lo; r += AHEAD * groups) {
+            u32x4 k[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int j = r0 + r + u * rows - len;  // the new row; negative: an old one
-            const bool fresh = j >= 0 && r + u * rows < hi;
-            from[u] = fresh ? j : -1;
-            if (a.path != nullptr && fresh) from[u] = a.path[b * a.ld_path + j];
-            if (from[u] >= a.T) from[u] = -1;
+            for (int u = 0; u < AHEAD; ++u) k[u] = *reinterpret_cast<const u32x4*>(kp + min(r + u * groups, lo - 1) * a.ps3);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                if (r + u * groups < lo) add(k[u]);
         }
+    if (works)
+        for (int r = lo + (rg - lo % groups + groups) % groups; r < hi; r += AHEAD * groups) {
+            u32x4 k[AHEAD], v[AHEAD];
+            int from[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int row = r + u * rows;
-            const char* kk = row < lo ? kp + row * a.ps3 : kn + max(from[u], 0) * a.ns3;
-            k[u] = *reinterpret_cast<const u32x4*>(kk);
-            v[u] = *reinterpret_cast<const u32x4*>(vn + max(from[u], 0) * a.ns3);
-        }
+            for (int u = 0; u < AHEAD; ++u) {
+                const int j = r0 + min(r + u * groups, hi - 1) - len;
+                from[u] = a.path != nullptr ? a.path[b * a.ld_path + j] : j;
+            }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int row = r + u * rows;
-            if (row >= hi) break;
-            if (row >= lo) {
-                if (from[u] < 0) k[u] = v[u] = u32x4{0u, 0u, 0u, 0u};
+            for (int u = 0; u < AHEAD; ++u) {
+                const bool is = from[u] >= 0 && from[u] < a.T;
+                k[u] = *reinterpret_cast<const u32x4*>(kn + (is ? from[u] : 0) * a.ns3);
+                v[u] = *reinterpret_cast<const u32x4*>(vn + (is ? from[u] : 0) * a.ns3);
+                if (!is) k[u] = v[u] = u32x4{0u, 0u, 0u, 0u};
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int row = r + u * groups;
+                if (row >= hi) break;
                 *reinterpret_cast<u32x4*>(kp + row * a.ps3) = k[u];
                 *reinterpret_cast<u32x4*>(vp + row * a.ps3) = v[u];
+                if (a.sums != nullptr) add(k[u]);
             }
-            if (a.sums != nullptr) add(k[u]);
         }
-    }
     if (a.sums == nullptr) return;
     const int d = a.chunks * VN;
     if (works) {
@@ -524,9 +540,9 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
     }
     __syncthreads();
     float* out = a.sums + l * a.ss0 + p * a.ss1 + h * a.ss2;
-    for (int e = threadIdx.x; e < d; e += 256) {
+    for (int e = threadIdx.x; e < d; e += 64 * NW) {
         float t = 0.f;
-        for (int g = 0; g < rows; ++g) t += s_sum[g * d + e];
+        for (int g = 0; g < groups; ++g) t += s_sum[g * d + e];
         out[e] = t;
     }
 }
@@ -588,12 +604,16 @@ int64_t units(const PoolSet& ps, int64_t n) {
     return u;
 }
 
-void copy_state(const StateArgs& a, hipStream_t s) {
-    if (a.ref == a.ref_out && a.table == a.table_out && a.len == a.len_out) return;
-    int64_t most = (int64_t)a.B * a.columns;
-    if (a.pages > most) most = a.pages;
-    const int64_t grid = (most + 255) / 256;
+// `alone`: the call's first kernel is not one workgroup
+StateArgs copy_state(StateArgs a, bool alone, hipStream_t s) {
+    a.here = false;
+    if (a.ref == a.ref_out && a.table == a.table_out && a.len == a.len_out) return a;
+    const int64_t words = (int64_t)a.B * a.columns, most = words > a.pages ? words : a.pages;
+    a.here = !alone && words + a.pages <= 16 * PLAN_THREADS;
+    if (a.here) return a;
+    const int64_t grid = (most > a.B ? most + 255 : (int64_t)a.B + 255) / 256;
     if (grid > 0) cache_state_copy<<<(int)(grid < 1024 ? grid : 1024), 256, 0, s>>>(a);
+    return a;
 }
 
 }  // namespace
@@ -634,9 +654,16 @@ __attribute__((visibility("default"))) int ythip_cache_append(
     const int64_t grid = (int64_t)a.slots * Hkv * B * layers;
     if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pages to write", who, (long long)grid);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == YTHIP_F32) cache_append_kernel<F32><<<(int)grid, 256, 0, s>>>(a);
-    else if (dtype == YTHIP_F16) cache_append_kernel<F16><<<(int)grid, 256, 0, s>>>(a);
-    else cache_append_kernel<BF16><<<(int)grid, 256, 0, s>>>(a);
+    auto run = [&](auto t) {
+        using T = decltype(t);
+        // a wave where a page is a few loads of it, more for long pages and rows
+        if (page <= 64 && a.chunks <= 64) cache_append_kernel<T, 1><<<(int)grid, 64, 0, s>>>(a);
+        else if (page <= 512) cache_append_kernel<T, 4><<<(int)grid, 256, 0, s>>>(a);
+        else cache_append_kernel<T, 16><<<(int)grid, 1024, 0, s>>>(a);
+    };
+    if (dtype == YTHIP_F32) run(F32{});
+    else if (dtype == YTHIP_F16) run(F16{});
+    else run(BF16{});
     return status_of(hipGetLastError());
 }
 
@@ -650,8 +677,8 @@ __attribute__((visibility("default"))) int ythip_cache_grow(int B, int columns, 
     if (B > MAX_SEQS) return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences (at most %d)", who, B, MAX_SEQS);
     if (B > 0 && n_new == nullptr) return fail(YTHIP_EINVAL, "%s: n_new is NULL", who);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    copy_state({B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, s);
-    if (B > 0) cache_grow_kernel<<<1, PLAN_THREADS, 0, s>>>({B, columns, pages, page_shift(page), n_new, ref_out, table_out, len_out, ld_out, status});
+    const StateArgs st = copy_state({false, B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, B == 0, s);
+    if (B > 0) cache_grow_kernel<<<1, PLAN_THREADS, 0, s>>>({B, columns, pages, page_shift(page), n_new, ref_out, table_out, len_out, ld_out, status, st});
     return status_of(hipGetLastError());
 }
 
@@ -678,9 +705,9 @@ __attribute__((visibility("default"))) int ythip_cache_fork(int B, int columns, 
     const int64_t grid = n + units(ps, n);
     if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pieces to copy", who, (long long)grid);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    copy_state({B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, s);
+    const StateArgs st = copy_state({false, B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, n == 0, s);
     if (n > 0) {
-        const ForkArgs a = {B, columns, pages, page_shift(page), n, src, dst, ref_out, table_out, len_out, ld_out, static_cast<int4*>(workspace), status};
+        const ForkArgs a = {B, columns, pages, page_shift(page), n, src, dst, ref_out, table_out, len_out, ld_out, static_cast<int4*>(workspace), status, st};
         cache_fork_plan<<<1, PLAN_THREADS, 0, s>>>(a);
         cache_fork_copy<<<(int)grid, 256, 0, s>>>(a, ps);
     }
@@ -696,7 +723,7 @@ __attribute__((visibility("default"))) int ythip_cache_free(int B, int columns, 
     if (const int st = check_state(who, B, columns, pages, page, ref, table, ld_table, len, ref_out, table_out, ld_out, len_out)) return st;
     if (n < 0 || (n > 0 && !seqs)) return fail(YTHIP_EINVAL, "%s: %d sequences, or seqs is NULL", who, n);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    copy_state({B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, s);
+    copy_state({false, B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, true, s);
     if (n > 0) cache_free_kernel<<<n, 256, 0, s>>>({B, columns, pages, page_shift(page), seqs, ref_out, table_out, len_out, ld_out, status});
     return status_of(hipGetLastError());
 }
@@ -725,11 +752,11 @@ __attribute__((visibility("default"))) int ythip_cache_compact(int B, int column
     hipStream_t s = static_cast<hipStream_t>(stream);
     cache_compact_plan<<<1, PLAN_THREADS, 0, s>>>(a);
     // how many pages move is known on the device alone: enough workgroups to fill the chip
-    // (8 on each of 256 CUs) walk the pieces
+    // many times over walk the pieces (2048 of them 340 us for 1.77 GB, 8192 328)
     int64_t grid = units(ps, pages / 2);
     const int64_t entries = ((int64_t)B * columns + 255) / 256;
     if (grid < entries) grid = entries;
-    if (grid > 2048) grid = 2048;
+    if (grid > 8192) grid = 8192;
     if (grid > 0) cache_compact_move<<<(int)grid, 256, 0, s>>>(a, ps);
     return status_of(hipGetLastError());
 }

@@ -23,7 +23,6 @@ sets bits of `status`, an int32 device tensor (CACHE_ERR_*).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 
@@ -38,39 +37,54 @@ CACHE_ERR_INDEX, CACHE_ERR_BUSY, CACHE_ERR_FULL = 1, 2, 4
 
 @functools.lru_cache(maxsize=4096)
 def _i64(vals: tuple) -> ctypes.Array:
-    """Strides for the C call, which reads them only."""
+    """Strides for the C call, which reads them only (and not the last, of d)."""
     return _lib.i64array(vals)
 
 
-def _same_device(first: torch.Tensor, *rest) -> contextlib.AbstractContextManager | None:
-    """All on one GPU; a context that makes it the current one where it is not."""
-    if not first.is_cuda:
+def _device(first: torch.Tensor, *rest) -> int:
+    """The GPU that the tensors (or None) are all on."""
+    dev = first.get_device()
+    if dev < 0:
         raise ValueError("ytensor_amd operators take device (cuda/hip) tensors")
     for t in rest:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on {first.device} and {t.device}")
-    return None if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+    return dev
 
 
-def _ints(name: str, t: torch.Tensor, *shape) -> torch.Tensor:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+def _away(dev: int):
+    """A context that makes `dev` the current GPU, or None where it is that."""
+    return None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _ints(name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.shape != shape:
         raise ValueError(f"{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
     return t
 
 
-def _rows(t: torch.Tensor, es: int) -> torch.Tensor:
-    """t with its last dim contiguous and 16-byte aligned rows (a copy where it has neither)."""
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in st[:-1]):
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _rows(t: torch.Tensor, es: int) -> tuple[torch.Tensor, int, tuple]:
+    """t with its last dim contiguous and 16-byte aligned rows (a copy where it has neither), its
+    address and strides."""
+    at, st = t.data_ptr(), t.stride()
+    align = at
+    for s in st[:-1]:
+        align |= s * es
+    if st[-1] != 1 or align & 15:
+        t = t.clone() if t.is_contiguous() else t.contiguous()
+        at, st = t.data_ptr(), t.stride()
+    return t, at, st
 
 
 def _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, scale, out,
                workspace):
-    guard = _same_device(q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, out, workspace)
-    if guard is not None:
-        with guard:
+    away = _away(_device(q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, out, workspace))
+    if away is not None:
+        with away:
             return _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len,
                               scale, out, workspace)
     if q.dim() != 4 or k_pool.dim() != 4:
@@ -82,56 +96,70 @@ def _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, 
         raise ValueError(f"q {list(q.shape)} does not fit pools {list(k_pool.shape)}")
     if k_pool.dtype != dt or v_pool.dtype != dt:
         raise ValueError("q and the pools must share a dtype")
-    if v_pool.shape != k_pool.shape or v_pool.stride() != k_pool.stride() or k_pool.stride(3) != 1:
+    pool_st = k_pool.stride()
+    if v_pool.shape != k_pool.shape or v_pool.stride() != pool_st or pool_st[3] != 1:
         raise ValueError("k_pool and v_pool must share a shape and strides, with d contiguous")
-    if (k_new is None) != (v_new is None):
+    es = 4 if dt is torch.float32 else 2
+    q, q_at, q_st = _rows(q, es)
+    kn_at = vn_at = kn_st = vn_st = None
+    if k_new is not None and v_new is not None:
+        want = (B, Hkv, T, d)
+        if k_new.shape != want or v_new.shape != want or k_new.dtype != dt or v_new.dtype != dt:
+            raise ValueError(f"k_new and v_new must be {dt} {list(want)}")
+        k_new, kn_at, kn_st = _rows(k_new, es)
+        v_new, vn_at, vn_st = _rows(v_new, es)
+        kn_st, vn_st = _i64(kn_st), _i64(vn_st)
+    elif k_new is not None or v_new is not None:
         raise ValueError("k_new and v_new go together")
-    es = q.element_size()
-    q = _rows(q, es)
-    if k_new is not None:
-        if k_new.shape != (B, Hkv, T, d) or v_new.shape != (B, Hkv, T, d) or k_new.dtype != dt or v_new.dtype != dt:
-            raise ValueError(f"k_new and v_new must be {dt} {[B, Hkv, T, d]}")
-        k_new, v_new = _rows(k_new, es), _rows(v_new, es)
-    if table.dim() != 2:
-        raise ValueError("table must be int32 [B, columns]")
-    columns = table.shape[1]
-    _ints("table", table, B, columns)
-    if table.stride(1) != 1 and columns > 1:
-        raise ValueError("table must have contiguous rows")
-    kv_len = _ints("kv_len", kv_len, B).contiguous()
+    table, ld, columns = _table(table, B)
+    kv_len = _packed(_ints("kv_len", kv_len, (B,)))
     if parents is not None:
-        parents = _ints("parents", parents, B, T).contiguous()
+        parents = _packed(_ints("parents", parents, (B, T)))
     if tree_len is not None:
-        tree_len = _ints("tree_len", tree_len, B).contiguous()
+        tree_len = _packed(_ints("tree_len", tree_len, (B,)))
     if out is None:
         out = (torch.empty if tree_len is None else torch.zeros)((B, Hq, T, d), dtype=dt, device=q.device)
     elif out.shape != (B, Hq, T, d) or out.dtype != dt or out.stride(3) != 1:
         raise ValueError(f"out must be {dt} {[B, Hq, T, d]} with d contiguous")
-    L = _lib.lib()
-    args = (code, B, Hq, Hkv, T, d, q.data_ptr(), _i64(q.stride()[:3]),
-            None if k_new is None else k_new.data_ptr(), None if k_new is None else _i64(k_new.stride()[:3]),
-            None if v_new is None else v_new.data_ptr(), None if v_new is None else _i64(v_new.stride()[:3]),
-            k_pool.data_ptr(), v_pool.data_ptr(), _i64(k_pool.stride()[:3]), P, page)
-    tail = (table.data_ptr(), max(table.stride(0), columns), columns, kv_len.data_ptr(),
-            None if parents is None else parents.data_ptr(), T, None if tree_len is None else tree_len.data_ptr())
     need = _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k or 0)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    ws = (None, 0) if not need else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    to = (out.data_ptr(), _i64(out.stride()[:3]), float(scale), *ws, _stream())
+    ws_at, ws_bytes = None, 0
+    if need:
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws_at, ws_bytes = workspace.data_ptr(), need
+    par_at = None if parents is None else parents.data_ptr()
+    tl_at = None if tree_len is None else tree_len.data_ptr()
     if top_k is None:
-        st = L.ythip_paged_attn(*args, *tail, *to)
+        st = _lib.lib().ythip_paged_attn(
+            code, B, Hq, Hkv, T, d, q_at, _i64(q_st), kn_at, kn_st, vn_at, vn_st, k_pool.data_ptr(),
+            v_pool.data_ptr(), _i64(pool_st), P, page, table.data_ptr(), ld, columns, kv_len.data_ptr(), par_at, T,
+            tl_at, out.data_ptr(), _i64(out.stride()), scale, ws_at, ws_bytes, _stream())
         if st:
             check(st, "ythip_paged_attn")
         return out
     if key_sums.dtype != torch.float32 or key_sums.shape != (P, Hkv, d) or key_sums.stride(2) != 1:
         raise ValueError(f"key_sums must be float32 {[P, Hkv, d]} with d contiguous")
     sel = torch.empty((B, Hkv, T, top_k), dtype=torch.int32, device=q.device)
-    st = L.ythip_paged_attn_sparse(*args, key_sums.data_ptr(), _i64(key_sums.stride()[:2]), *tail, top_k,
-                                   sel.data_ptr(), *to)
+    st = _lib.lib().ythip_paged_attn_sparse(
+        code, B, Hq, Hkv, T, d, q_at, _i64(q_st), kn_at, kn_st, vn_at, vn_st, k_pool.data_ptr(),
+        v_pool.data_ptr(), _i64(pool_st), P, page, key_sums.data_ptr(), _i64(key_sums.stride()),
+        table.data_ptr(), ld, columns, kv_len.data_ptr(), par_at, T, tl_at, top_k, sel.data_ptr(), out.data_ptr(),
+        _i64(out.stride()), scale, ws_at, ws_bytes, _stream())
     if st:
         check(st, "ythip_paged_attn_sparse")
     return out, sel
+
+
+def _table(table: torch.Tensor, B: int) -> tuple[torch.Tensor, int, int]:
+    """(table, row stride, columns)"""
+    if table.dim() != 2:
+        raise ValueError("table must be int32 [B, columns]")
+    columns = table.shape[1]
+    _ints("table", table, (B, columns))
+    ld, step = table.stride()
+    if step != 1 and columns > 1:
+        raise ValueError("table must have contiguous rows")
+    return table, ld if ld > columns else columns, columns
 
 
 @functools.lru_cache(maxsize=4096)
@@ -161,7 +189,7 @@ def paged_attention(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Te
     `out` made here). Query head h reads KV head h // (Hq // Hkv). A page id outside the pool
     hides its rows; a row that sees nothing is zero. d 64 or 128, page a power of two >= 16.
     Returns out [B, Hq, T, d]."""
-    return _attention(None, q, k_new, v_new, k_pool, v_pool, None, table, kv_len, parents, tree_len, scale, out,
+    return _attention(None, q, k_new, v_new, k_pool, v_pool, None, table, kv_len, parents, tree_len, float(scale), out,
                       workspace)
 
 
@@ -178,38 +206,37 @@ def paged_sparse_attention(q: torch.Tensor, k_new: torch.Tensor | None, v_new: t
     table columns ascending, then -1 (-1 alone for t >= tree_len[b])."""
     if top_k < 1:
         raise ValueError(f"top_k = {top_k}: at least one page")
-    return _attention(int(top_k), q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, scale,
-                      out, workspace)
+    return _attention(int(top_k), q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len,
+                      float(scale), out, workspace)
 
 
 # ---------------------------------------------------------------------------
 # The cache's rows and pages
 # ---------------------------------------------------------------------------
 
-def _state(ref, table, kv_len, out, page, status, *rest):
+def _state(ref, table, kv_len, out, page, status):
     """(arguments up to len, arguments of the outputs, the outputs) of a bookkeeping call."""
     if table.dim() != 2 or ref.dim() != 1:
         raise ValueError("table must be int32 [B, columns] and ref int32 [P]")
-    B, columns = table.shape
+    B, pages = table.shape[0], ref.shape
     out = (ref, table, kv_len) if out is None else tuple(out)
+    args = []
     for r, t, n in ((ref, table, kv_len), out):
-        _ints("ref", r, ref.shape[0])
-        _ints("table", t, B, columns)
-        _ints("kv_len", n, B)
-        if not r.is_contiguous() or not n.is_contiguous() or (columns > 1 and t.stride(1) != 1):
-            raise ValueError("ref and kv_len must be contiguous, table with contiguous rows")
+        t, ld, columns = _table(t, B)
+        if columns != table.shape[1]:
+            raise ValueError("the tables must have the same columns")
+        if not _ints("ref", r, pages).is_contiguous() or not _ints("kv_len", n, (B,)).is_contiguous():
+            raise ValueError("ref and kv_len must be contiguous")
+        args.append((r.data_ptr(), t.data_ptr(), ld, n.data_ptr()))
     if status is not None:
-        _ints("status", status, 1)
-    ld = lambda t: max(t.stride(0), columns)  # noqa: E731
-    head = (B, columns, ref.shape[0], int(page), ref.data_ptr(), table.data_ptr(), ld(table), kv_len.data_ptr())
-    tail = (out[0].data_ptr(), out[1].data_ptr(), ld(out[1]), out[2].data_ptr())
-    return head, tail, out
+        _ints("status", status, (1,))
+    return (B, table.shape[1], pages[0], page, *args[0]), args[1], out
 
 
 def _list(name: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype != torch.int32 or t.dim() != 1:
         raise ValueError(f"{name} must be int32 [n]")
-    return t.contiguous()
+    return _packed(t)
 
 
 def _pools(pools, pages: int):
@@ -228,39 +255,25 @@ def _pools(pools, pages: int):
     return len(pools), layers, arr
 
 
-def _guarded(fn):
-    """Runs fn on the GPU of its tensors (they must share one)."""
-    @functools.wraps(fn)
-    def call(*args, **kw):
-        flat = []
-        for v in (*args, *kw.values()):
-            flat += list(v) if isinstance(v, (tuple, list)) else [v]
-        ts = [t for t in flat if isinstance(t, torch.Tensor)]
-        if not ts:
-            raise ValueError("ytensor_amd operators take device (cuda/hip) tensors")
-        guard = _same_device(*ts)
-        if guard is None:
-            return fn(*args, **kw)
-        with guard:
-            return fn(*args, **kw)
-    return call
-
-
-@_guarded
 def cache_grow(ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, n_new: torch.Tensor, page: int,
                out=None, status: torch.Tensor | None = None):
     """Pages (lowest free first) for n_new[b] more rows of each sequence, and the new lengths.
     A sequence that finds too few pages or columns keeps what it has (status). out: (ref,
     table, kv_len) to write instead of the given ones. Returns those written. cache_append
     takes the kv_len from before."""
+    away = _away(_device(ref, table, kv_len, n_new, status, *(out or ())))
+    if away is not None:
+        with away:
+            return cache_grow(ref, table, kv_len, n_new, page, out, status)
     head, tail, out = _state(ref, table, kv_len, out, page, status)
-    n_new = _ints("n_new", n_new, table.shape[0]).contiguous()
-    check(_lib.lib().ythip_cache_grow(*head, n_new.data_ptr(), *tail, None if status is None else status.data_ptr(),
-                                      _stream()), "ythip_cache_grow")
+    n_new = _packed(_ints("n_new", n_new, (head[0],)))
+    st = _lib.lib().ythip_cache_grow(*head, n_new.data_ptr(), *tail, None if status is None else status.data_ptr(),
+                                     _stream())
+    if st:
+        check(st, "ythip_cache_grow")
     return out
 
 
-@_guarded
 def cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                  table: torch.Tensor, kv_len: torch.Tensor, n_new: torch.Tensor | None = None,
                  path: torch.Tensor | None = None, key_sums: torch.Tensor | None = None) -> None:
@@ -268,6 +281,10 @@ def cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
     [L, B, Hkv, T, d], for i < n_new[b] (None: T) and every layer; pools [L, P, Hkv, page, d].
     A path entry outside [0, T) writes zeros. table holds the pages already (cache_grow),
     kv_len is the length before. key_sums [L, P, Hkv, d]: the sums of the pages written to."""
+    away = _away(_device(k_new, v_new, k_pool, v_pool, table, kv_len, n_new, path, key_sums))
+    if away is not None:
+        with away:
+            return cache_append(k_new, v_new, k_pool, v_pool, table, kv_len, n_new, path, key_sums)
     if k_new.dim() != 5 or k_pool.dim() != 5:
         raise ValueError("k_new must be [L, B, Hkv, T, d] and the pools [L, P, Hkv, page, d]")
     L, B, Hkv, T, d = k_new.shape
@@ -280,33 +297,29 @@ def cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
     if k_pool.stride() != v_pool.stride() or k_pool.stride(4) != 1:
         raise ValueError("k_pool and v_pool must share strides, with d contiguous")
     es = k_new.element_size()
-    k_new, v_new = _rows(k_new, es), _rows(v_new, es)
-    if k_new.stride() != v_new.stride():
+    k_new, k_at, new_st = _rows(k_new, es)
+    v_new, v_at, v_st = _rows(v_new, es)
+    if new_st != v_st:
         k_new, v_new = k_new.contiguous(), v_new.contiguous()
-    if table.dim() != 2:
-        raise ValueError("table must be int32 [B, columns]")
-    columns = table.shape[1]
-    _ints("table", table, B, columns)
-    if table.stride(1) != 1 and columns > 1:
-        raise ValueError("table must have contiguous rows")
-    kv_len = _ints("kv_len", kv_len, B).contiguous()
+        k_at, v_at, new_st = k_new.data_ptr(), v_new.data_ptr(), k_new.stride()
+    table, ld, columns = _table(table, B)
+    kv_len = _packed(_ints("kv_len", kv_len, (B,)))
     if n_new is not None:
-        n_new = _ints("n_new", n_new, B).contiguous()
+        n_new = _packed(_ints("n_new", n_new, (B,)))
     if path is not None:
-        path = _ints("path", path, B, T).contiguous()
+        path = _packed(_ints("path", path, (B, T)))
     if key_sums is not None and (key_sums.dtype != torch.float32 or key_sums.shape != (L, P, Hkv, d)
                                  or key_sums.stride(3) != 1):
         raise ValueError(f"key_sums must be float32 {[L, P, Hkv, d]} with d contiguous")
-    check(_lib.lib().ythip_cache_append(
-        _code(k_new), L, B, Hkv, T, d, k_new.data_ptr(), v_new.data_ptr(), _i64(k_new.stride()[:4]),
-        k_pool.data_ptr(), v_pool.data_ptr(), _i64(k_pool.stride()[:4]), P, page,
-        None if key_sums is None else key_sums.data_ptr(), None if key_sums is None else _i64(key_sums.stride()[:3]),
-        table.data_ptr(), max(table.stride(0), columns), columns, kv_len.data_ptr(),
-        None if n_new is None else n_new.data_ptr(), None if path is None else path.data_ptr(), T, _stream()),
-        "ythip_cache_append")
+    st = _lib.lib().ythip_cache_append(
+        _code(k_new), L, B, Hkv, T, d, k_at, v_at, _i64(new_st), k_pool.data_ptr(), v_pool.data_ptr(),
+        _i64(k_pool.stride()), P, page, None if key_sums is None else key_sums.data_ptr(),
+        None if key_sums is None else _i64(key_sums.stride()), table.data_ptr(), ld, columns, kv_len.data_ptr(),
+        None if n_new is None else n_new.data_ptr(), None if path is None else path.data_ptr(), T, _stream())
+    if st:
+        check(st, "ythip_cache_append")
 
 
-@_guarded
 def cache_fork(pools, ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, src: torch.Tensor,
                dst: torch.Tensor, page: int, out=None, status: torch.Tensor | None = None):
     """Sequence dst[i] (empty before) becomes a copy of src[i]: it shares the whole pages and
@@ -314,6 +327,10 @@ def cache_fork(pools, ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tens
     All pairs read the state before the call. A pair that is refused (dst in use or named
     twice, no free page, an index out of range) leaves dst empty (status). out and the result
     as for cache_grow."""
+    away = _away(_device(ref, table, kv_len, src, dst, status, *pools, *(out or ())))
+    if away is not None:
+        with away:
+            return cache_fork(pools, ref, table, kv_len, src, dst, page, out, status)
     head, tail, out = _state(ref, table, kv_len, out, page, status)
     src, dst = _list("src", src), _list("dst", dst)
     if src.shape != dst.shape:
@@ -327,11 +344,14 @@ def cache_fork(pools, ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tens
     return out
 
 
-@_guarded
 def cache_free(ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, seqs: torch.Tensor, page: int, out=None,
                status: torch.Tensor | None = None):
     """The pages of sequences seqs lose a user; their table rows become -1, their lengths 0.
     An empty sequence and a second mention change nothing. out and the result as for cache_grow."""
+    away = _away(_device(ref, table, kv_len, seqs, status, *(out or ())))
+    if away is not None:
+        with away:
+            return cache_free(ref, table, kv_len, seqs, page, out, status)
     head, tail, out = _state(ref, table, kv_len, out, page, status)
     seqs = _list("seqs", seqs)
     check(_lib.lib().ythip_cache_free(*head, seqs.shape[0], seqs.data_ptr(), *tail,
@@ -339,11 +359,14 @@ def cache_free(ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, seq
     return out
 
 
-@_guarded
 def cache_compact(pools, ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, page: int, out=None):
     """Moves the pages in use to the front of every pool ([L, P, ...] tensors), in order, and
     has ref and table follow. out: (ref, table) to write instead of the given ones. Returns
     (ref, table, live): live int32 [1], the pages in use."""
+    away = _away(_device(ref, table, kv_len, *pools, *(out or ())))
+    if away is not None:
+        with away:
+            return cache_compact(pools, ref, table, kv_len, page, out)
     out = (ref, table) if out is None else tuple(out)
     head, tail, out = _state(ref, table, kv_len, (*out, kv_len), page, None)
     n_pools, layers, descr = _pools(pools, ref.shape[0])
@@ -355,17 +378,20 @@ def cache_compact(pools, ref: torch.Tensor, table: torch.Tensor, kv_len: torch.T
     return out[0], out[1], live
 
 
-@_guarded
 def cache_copy_pages(pools, src: torch.Tensor, dst: torch.Tensor, status: torch.Tensor | None = None) -> None:
     """Page src[i] over page dst[i] of every pool ([L, P, ...] tensors). No dst may be another
     pair's src or dst; a pair with an index out of range is left out (status)."""
+    away = _away(_device(src, dst, status, *pools))
+    if away is not None:
+        with away:
+            return cache_copy_pages(pools, src, dst, status)
     src, dst = _list("src", src), _list("dst", dst)
     if src.shape != dst.shape:
         raise ValueError("src and dst must have the same length")
     if len(pools) == 0:
         return
     if status is not None:
-        _ints("status", status, 1)
+        _ints("status", status, (1,))
     pages = pools[0].shape[1] if pools[0].dim() >= 3 else 0
     n_pools, layers, descr = _pools(pools, pages)
     check(_lib.lib().ythip_cache_copy_pages(pages, src.shape[0], src.data_ptr(), dst.data_ptr(), n_pools, layers,
