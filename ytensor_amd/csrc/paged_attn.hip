@@ -277,24 +277,19 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
 
     // this lane's query rows
     int tok[QT], cur[QT];
-    bool real[QT];
     u32x4 qf[QT][S::KS];
     constexpr uint32_t SIGN = F ? 0x80000000u : 0x80008000u;
     const float c = fabsf(a.scale_log2);
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         const int r = r0 + wr * 16 * QT + qt * 16 + l16;
-        const int t = SPARSE ? t_one : r / a.G, gh = SPARSE ? r : r - t * a.G;
-        real[qt] = r < R && t < tn;
-        tok[qt] = real[qt] ? t : -1;
+        // a row past the last reads the last's query, and what comes of it is not stored
+        const int rq = min(r, R - 1), t = SPARSE ? t_one : rq / a.G, gh = SPARSE ? rq : rq - t * a.G;
+        tok[qt] = r < R && t < tn ? t : -1;
         cur[qt] = tok[qt];
         const raw* qp = static_cast<const raw*>(a.Q) + b * a.qs[0] + (int64_t)(h * a.G + gh) * a.qs[1] + t * a.qs[2];
 #pragma unroll
-        for (int ks = 0; ks < S::KS; ++ks) {
-            qf[qt][ks] = u32x4{0u, 0u, 0u, 0u};
-            if (real[qt]) qf[qt][ks] = *reinterpret_cast<const u32x4*>(qp + (ks * 4 + g) * (16 / S::ES));
-            if (a.scale_log2 < 0.f) qf[qt][ks] ^= u32x4{SIGN, SIGN, SIGN, SIGN};
-        }
+        for (int ks = 0; ks < S::KS; ++ks) qf[qt][ks] = *reinterpret_cast<const u32x4*>(qp + (ks * 4 + g) * (16 / S::ES));
     }
 
     // DMA: lane -> (row of the instruction, chunk), the chunk swizzled by the row in its 16: the
@@ -629,23 +624,50 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
         for (int i = 0; i < S::KG; ++i) cols[i] = col[i];
         columns(s + 3);
-        if (s >= 0) {
-            if (next != 0) wait_vmcnt<2 * S::NI>();  // stage s has landed, s + 1 is in flight
-            else wait_vmcnt<0>();
-            if constexpr (WR > 1) wg_barrier();
-            else asm volatile("" ::: "memory");
-            if (here != 0) compute(s, here, with_new);
-            if constexpr (WR > 1) wg_barrier();
-            else asm volatile("" ::: "memory");
-        }
+        if (next != 0) wait_vmcnt<2 * S::NI>();  // stage s has landed, s + 1 is in flight
+        else wait_vmcnt<0>();
+        if constexpr (WR > 1) wg_barrier();
+        else asm volatile("" ::: "memory");
+        if (here != 0) compute(s, here, with_new);
+        if constexpr (WR > 1) wg_barrier();
+        else asm volatile("" ::: "memory");
         here = next;
         next = s + 2 < nst ? issue(s + 2, with_new) : 0;
     };
     // stages with new tokens, then those of cached rows alone: a loop of its own, that holds none of
     // the paths' state in registers
     const int s_new = (max(c1 - max(c0, nct), 0) + S::WK - 1) / S::WK;
-    columns(0);
-    for (int s = -2; s < s_new; ++s) step(s, std::true_type{});
+    {
+        // the first two stages: both lookups and the queries' latency side by side
+        int ids0[S::KG], col0[S::KG];
+        columns(0);
+        ids(0);
+#pragma unroll
+        for (int i = 0; i < S::KG; ++i) ids0[i] = id[i], col0[i] = col[i];
+        columns(1);
+        ids(1);
+        int ids1[S::KG], col1[S::KG];
+#pragma unroll
+        for (int i = 0; i < S::KG; ++i) ids1[i] = id[i], col1[i] = col[i];
+        columns(2);
+        // the queries are there before the first DMA: waited for in the loop they would have every
+        // row in flight waited for
+        const uint32_t flip = a.scale_log2 < 0.f ? SIGN : 0u;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int ks = 0; ks < S::KS; ++ks) {
+                qf[qt][ks] ^= u32x4{flip, flip, flip, flip};
+                asm volatile("" : "+v"(qf[qt][ks]));
+            }
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int i = 0; i < S::KG; ++i) id[i] = s == 0 ? ids0[i] : ids1[i], cols[i] = s == 0 ? col0[i] : col1[i];
+            here = next;
+            next = s < nst ? issue(s, std::true_type{}) : 0;
+        }
+    }
+    for (int s = 0; s < s_new; ++s) step(s, std::true_type{});
     for (int s = s_new; s < nst; ++s) step(s, std::false_type{});
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
