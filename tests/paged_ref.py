@@ -23,8 +23,9 @@ def attention(q, k_new, v_new, k_pool, v_pool, table, kv_len, parents=None, tree
     """(out, tol) in float64 on the CPU; rows behind tree_len are NaN in out. tol bounds a kernel that
     rounds the weights p and the result to q's type and else works in float32:
       result      half a step of |o|
-      weights     half a step of sum p |v| (and in float16, where a weight below 2^-24 of the largest is lost,
-                  2^-25 max |v| a key)
+      weights     each half a step off, in the product and in their sum alike: sum (w' - w) v / sum w' is
+                  sum (w' - w) (v - o) / sum w', at most half a step of sum p |v - o| <= sum p |v| + |o|
+                  (and in float16, where a weight below 2^-24 of the largest is lost, 2^-25 max |v| a key)
       float32     a score of d products is off by (d + 3) 2^-24 S, S = scale sum |q k| its largest, and an exponential
                   by 2^-22 more; the sums over n keys by n 2^-24: each against sum p |v|, numerator and denominator
     """
@@ -68,7 +69,7 @@ def attention(q, k_new, v_new, k_pool, v_pool, table, kv_len, parents=None, tree
                 av = p @ v.abs()
                 S = (abs(scale) * (qd[b, rows, t].abs() @ k.abs().T)).amax(-1, keepdim=True)
                 f32 = 2.0 ** -24 * (2 * (d + 3) * S + 8 + 2 * len(k))
-                tol[b, rows, t] = 1.01 * (u * o.abs() + u * av + f32 * av)
+                tol[b, rows, t] = 1.01 * (2 * u * o.abs() + u * av + f32 * av)
                 if q.dtype == torch.float16:
                     tol[b, rows, t] += 2.0 ** -25 * len(k) * v.abs().max()
     return out, tol

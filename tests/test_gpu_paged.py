@@ -97,6 +97,45 @@ def test_attention_over_long_caches(dtype, B, Hkv, G, d, T, n, page):
     compare(out, want, tol)
 
 
+@pytest.mark.parametrize("dtype,B,T,columns", [("bf16", 150, 1, 40), ("f16", 70, 2, 20), ("f32", 129, 1, 9)])
+def test_attention_of_many_sequences(dtype, B, T, columns):
+    """More sequences than lanes of a wave, empty and full ones side by side, ranges that begin and end
+    with a sequence."""
+    dt, Hkv, page, d = DT[dtype], 1, 16, 64
+    lens = [(0, 16 * columns, 64, 1, 128, 5)[b % 6] if b % 7 else 64 * (b % 3) for b in range(B)]
+    lens = [min(n, 16 * columns) for n in lens]
+    g, kp, vp, table, kv_len = cache(B, lens, Hkv, page, d, dt, columns=columns)
+    q, kn, vn = tokens(g, B, 2, Hkv, T, d, dt)
+    for new in ((kn, vn), (None, None)):
+        want, tol = attention(q, *new, kp, vp, table, kv_len)
+        compare(yt.paged_attention(q, *new, kp, vp, table, kv_len), want, tol)
+
+
+@pytest.mark.parametrize("dtype,T,kind", [("bf16", 700, "tree"), ("f16", 1100, "chain"), ("f32", 300, "tree"),
+                                          ("bf16", 4096, "tree")])
+def test_attention_of_many_tokens(dtype, T, kind):
+    """Long trees and chunks over several row tiles, with and without cached rows."""
+    dt, B, Hkv, G, page, d = DT[dtype], 2, 1, 2, 32, 64
+    g, kp, vp, table, kv_len = cache(T, [0, 333], Hkv, page, d, dt)
+    q, kn, vn = tokens(g, B, Hkv * G, Hkv, T, d, dt)
+    parents = tree(g, B, T) if kind == "tree" else None
+    tree_len = ints([T - 3, T])
+    out = yt.paged_attention(q, kn, vn, kp, vp, table, kv_len, parents=parents, tree_len=tree_len)
+    want, tol = attention(q, kn, vn, kp, vp, table, kv_len, parents, tree_len)
+    compare(out, want, tol, torch.zeros_like(out))
+
+
+def test_attention_path_values():
+    """A parent outside [0, child) ends the path, whatever it is."""
+    dt, T, d = torch.float32, 9, 64
+    g, kp, vp, table, kv_len = cache(8, [20], 1, 16, d, dt)
+    q, kn, vn = tokens(g, 1, 2, 1, T, d, dt)
+    parents = ints([[5, 0, 2, 7, -2 ** 31, 2 ** 31 - 1, 1, 6, 100]])
+    out = yt.paged_attention(q, kn, vn, kp, vp, table, kv_len, parents=parents)
+    want, tol = attention(q, kn, vn, kp, vp, table, kv_len, parents)
+    compare(out, want, tol)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attention_strides_and_layouts(dtype):
     """Rows of a fused projection, pools [P, page, Hkv, d], a table with a longer row stride, out
@@ -247,6 +286,20 @@ def test_sparse_ties_nan_and_bad_pages():
         _, sel = yt.paged_sparse_attention(q, kn, vn, kp, vp, sums, table, kv_len, top)
         want = select(q, sums, table, kv_len, page, top)
         assert torch.equal(sel.cpu(), want), top
+
+
+@pytest.mark.parametrize("n,columns", [(1500, 1500), (900, 1000), (9000, 9001)])
+def test_sparse_choice_of_few_of_many(n, columns):
+    """Both sizes of the choosing workgroup, ranks kept and read again, scores alike in their first bits."""
+    page, d = 16, 64
+    g = torch.Generator().manual_seed(n)
+    kp = torch.randn(64, 1, page, d, generator=g).bfloat16().cuda()
+    table = torch.randint(0, 64, (1, columns), generator=g).int().cuda()
+    sums = 1 + 1e-6 * torch.randn(64, 1, d, generator=g).cuda()
+    q = torch.rand(1, 2, 3, d, generator=g).bfloat16().cuda()
+    for top in (1, 7, 100, min(n - 1, 4096)):
+        out, sel = yt.paged_sparse_attention(q, None, None, kp, kp, sums, table, ints([n * page]), top)
+        assert torch.equal(sel.cpu(), select(q, sums, table, ints([n * page]), page, top))
 
 
 def test_sparse_many_columns():

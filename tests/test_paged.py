@@ -43,8 +43,12 @@ EINVAL, EUNSUP = _lib.YTHIP_EINVAL, _lib.YTHIP_EUNSUPPORTED
     (dict(Hq=5), EINVAL, b"heads"),
     (dict(Hkv=0), EINVAL, b"heads"),
     (dict(columns=70000, ld=70000), EUNSUP, b"columns"),
-    (dict(columns=65536, ld=65536, page=32768), EUNSUP, b"2^31"),
+    (dict(columns=65536, ld=65536, page=32768), EUNSUP, b"2^30"),
     (dict(parents=FAKE, T=4097, ldp=4097), EUNSUP, b"tree"),
+    (dict(T=1 << 29), EUNSUP, b"new tokens"),
+    (dict(kn=_lib.i64array([128, 128, 1 << 24])), EUNSUP, b"stride"),
+    (dict(p=_lib.i64array([128, 128, -128])), EUNSUP, b"stride"),
+    (dict(B=65536), EUNSUP, b"65535"),
     (dict(parents=FAKE, ldp=2), EINVAL, b"parents"),
     (dict(Q=None), EINVAL, b"NULL"),
     (dict(O=None), EINVAL, b"NULL"),
@@ -175,3 +179,17 @@ def test_model_of_the_pages():
     sums = torch.tensor([[[1.0] * 64], [[3.0] * 64], [[3.0] * 64], [[0.0] * 64]])
     s = select(torch.ones(1, 1, 1, 64), sums, torch.tensor([[0, 1, 2, 3]]), torch.tensor([50]), 16, 2)
     assert s.tolist() == [[[[1, 3]]]]
+
+
+def test_attention_workspace():
+    """None where a sequence stays with one workgroup; else room for every partial, whatever the lengths."""
+    lib = yt.load()
+    size = lambda B, T, columns, page=64, G=2, d=128: int(lib.ythip_paged_attn_workspace_size(_lib.BF16, B, 8 * G, 8, T, d, columns, page))  # noqa: E731
+    assert size(1, 1, 5) == 0 and size(64, 1, 5) == 0 and size(1, 1, 0) == 0 and size(0, 1, 5) == 0
+    big = size(1, 1, 2048)
+    assert big > 0 and big % (8 * 2 * 130 * 4) == 0
+    st = attn(lib, Hq=16, Hkv=8, T=1, B=1, columns=2048, ld=2048, page=64, bytes=big - 1)
+    assert st == EINVAL and b"workspace of" in lib.ythip_last_error()
+    assert attn(lib, Hq=16, Hkv=8, T=1, B=1, columns=2048, ld=2048, page=64, ws=None) == EINVAL
+    sparse = int(lib.ythip_paged_attn_sparse_workspace_size(_lib.BF16, 2, 16, 8, 3, 128, 100, 64, 4))
+    assert sparse >= 2 * 8 * 3 * 100 * 8

@@ -398,12 +398,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         return pack;
     };
 
-    float m[QT], l[QT];
+    float m[QT];
+    f32x4 l[QT];  // ones . P^T: the sum of the weights as the product takes them, from the matrix cores
     f32x4 o[QT][S::DT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         m[qt] = -INFINITY;
-        l[qt] = 0.f;
+        l[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < S::DT; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -493,6 +494,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             if (__ballot(any) == 0) return;
             paths = __ballot(paths) != 0;
         }
+        __builtin_amdgcn_s_setprio(1);  // the matrix cores' turns first: the other wave has its softmax to go on with
         f32x4 p[QT][S::KG];
 #pragma unroll
         for (int kt = 0; kt < S::KG; ++kt) {
@@ -506,6 +508,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             }
         }
         constexpr uint32_t FULL = S::KG == 1 ? 16u : S::KG == 2 ? 16u | 16u << 5 : 16u | 16u << 5 | 16u << 10 | 16u << 15;
+        __builtin_amdgcn_s_setprio(0);
         if (paths || pack != FULL) {
 #pragma unroll
             for (int kt = 0; kt < S::KG; ++kt) {
@@ -530,15 +533,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             const float ref = top == -INFINITY ? 0.f : top;  // nothing seen yet: every weight is 0
             const float corr = __builtin_amdgcn_exp2f(m[qt] - ref);
             m[qt] = top;
-            float sum = 0.f;
 #pragma unroll
             for (int kt = 0; kt < S::KG; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     p[qt][kt][r] = __builtin_amdgcn_exp2f(fmaf(p[qt][kt][r], c, -ref));
-                    sum += p[qt][kt][r];
                 }
-            l[qt] = l[qt] * corr + sum;
+            l[qt] *= corr;
             if (__ballot(corr != 1.0f) != 0) {
 #pragma unroll
                 for (int t = 0; t < S::DT; ++t) o[qt][t] *= corr;
@@ -577,6 +578,21 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                     pk[qt][kk] = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
                 }
             }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int kk = 0; kk < PK; ++kk) {
+                constexpr uint32_t ONE2 = std::is_same_v<T, BF16> ? 0x3F803F80u : 0x3C003C00u;
+                if constexpr (F) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        l[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, __uint_as_float(pk[qt][kk][j]), l[qt], 0, 0, 0);
+                } else if constexpr (S::KG >= 2) {
+                    l[qt] = mfma_chunk(T{}, u32x4{ONE2, ONE2, ONE2, ONE2}, pk[qt][kk], l[qt]);
+                } else {
+                    l[qt] = mfma_half(T{}, u32x2{ONE2, ONE2}, u32x2{pk[qt][0][0], pk[qt][0][1]}, l[qt]);
+                }
+            }
         auto product = [&](auto clean) {
 #pragma unroll
             for (int t = 0; t < S::DT; ++t) {
@@ -589,7 +605,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             }
         };
         if (!NEW || odd == 0) {
+            __builtin_amdgcn_s_setprio(1);
             product(std::false_type{});
+            __builtin_amdgcn_s_setprio(0);
             return;
         }
         asm volatile("" ::: "memory");  // or the two products are run both and one result taken
@@ -669,12 +687,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     }
     for (int s = 0; s < s_new; ++s) step(s, std::true_type{});
     for (int s = s_new; s < nst; ++s) step(s, std::false_type{});
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        l[qt] += __shfl_xor(l[qt], 16, 64);
-        l[qt] += __shfl_xor(l[qt], 32, 64);
-    }
-
     // the place of row r's result: O itself, or this item's partial
     auto store4 = [&](int r, int d, f32x4 v, float M, float L) {
         const int t = SPARSE ? t_one : r / a.G, gh = SPARSE ? r : r - t * a.G;
@@ -698,7 +710,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-            for (int t = 0; t < S::DT; ++t) store4(r0 + wr * 16 * QT + qt * 16 + l16, 16 * t + 4 * g, o[qt][t], m[qt], l[qt]);
+            for (int t = 0; t < S::DT; ++t) store4(r0 + wr * 16 * QT + qt * 16 + l16, 16 * t + 4 * g, o[qt][t], m[qt], l[qt][0]);
     } else {
         // the key groups' results side by side in LDS, then joined
         float* so = reinterpret_cast<float*>(smem);
@@ -711,7 +723,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             for (int t = 0; t < S::DT; ++t) *reinterpret_cast<f32x4*>(so + row * S::OLD + 16 * t + 4 * g) = o[qt][t];
             if (g == 0) {
                 sm[2 * row] = m[qt];
-                sm[2 * row + 1] = l[qt];
+                sm[2 * row + 1] = l[qt][0];
             }
         }
         __syncthreads();
@@ -1043,7 +1055,6 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
 template <class T, int D, int QT, int WR, bool SPARSE>
 int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
     const int64_t groups = (p.items * a.Hkv + 7) / 8 * 8;
-    if (groups * p.row_tiles > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups", (long long)(groups * p.row_tiles));
     using S = Shape<T, D, QT, WR>;
     paged_attn_kernel<T, D, QT, WR, SPARSE><<<(int)(groups * p.row_tiles), 256, 0, s>>>(a);
     if (p.part_bytes > 0) {
@@ -1077,6 +1088,8 @@ int run_typed(const PagedArgs& a, const Plan& p, hipStream_t s) {
 template <bool SPARSE>
 int run(int dtype, int d, PagedArgs& a, void* ws, hipStream_t s) {
     const Plan p = plan_of(dtype, a.B, a.Hkv, a.G, a.T, d, a.columns, 1 << a.shift, SPARSE ? a.top_k : 0);
+    if ((p.items * a.Hkv + 8) * p.row_tiles > INT_MAX)
+        return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups", (long long)(p.items * a.Hkv * p.row_tiles));
     a.target = p.target, a.min_chunk = p.min_chunk, a.items = (int)p.items, a.row_tiles = p.row_tiles;
     char* w = static_cast<char*>(ws);
     a.rank = reinterpret_cast<uint64_t*>(w);
@@ -1135,8 +1148,9 @@ int prepare(const char* who, const Call& c, PagedArgs& a, bool& done) {
         return 0;
     }
     if (c.Hkv == 0 || c.Hq % c.Hkv != 0) return fail(YTHIP_EINVAL, "%s: %d query heads over %d KV heads", who, c.Hq, c.Hkv);
-    if (c.columns > 65536 || (int64_t)c.columns * c.page > INT_MAX)
-        return fail(YTHIP_EUNSUPPORTED, "%s: %d columns of %d rows (at most 65536 columns, 2^31 - 1 rows)", who, c.columns, c.page);
+    if (c.columns > 65536 || (int64_t)c.columns * c.page > 1 << 30)
+        return fail(YTHIP_EUNSUPPORTED, "%s: %d columns of %d rows (at most 65536 columns, 2^30 rows)", who, c.columns, c.page);
+    if ((int64_t)c.T * c.Hq > 1 << 30) return fail(YTHIP_EUNSUPPORTED, "%s: %d new tokens of %d heads (2^30 in all)", who, c.T, c.Hq);
     if (c.parents != nullptr && c.T > MAX_TREE) return fail(YTHIP_EUNSUPPORTED, "%s: a tree of %d tokens (at most %d)", who, c.T, MAX_TREE);
     if (!c.Q || !c.O || !c.kv_len || !c.q_str || !c.o_str || !c.pool_str) return fail(YTHIP_EINVAL, "%s: NULL argument", who);
     if ((c.Kn == nullptr) != (c.Vn == nullptr) || (c.Kn && (!c.kn_str || !c.vn_str))) return fail(YTHIP_EINVAL, "%s: Kn and Vn go together, with their strides", who);

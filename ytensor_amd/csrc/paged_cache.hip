@@ -561,8 +561,8 @@ int check_table(const char* who, int B, int columns, int pages, int page, const 
                 const void* len) {
     if (B < 0 || columns < 0 || pages < 0) return fail(YTHIP_EINVAL, "%s: negative size", who);
     if (page_shift(page) < 0) return fail(YTHIP_EINVAL, "%s: a page of %d rows (a power of two from 16 to 32768)", who, page);
-    if (columns > MAX_COLUMNS || (int64_t)columns * page > INT_MAX)
-        return fail(YTHIP_EUNSUPPORTED, "%s: %d columns of %d rows (at most 65536 columns, 2^31 - 1 rows)", who, columns, page);
+    if (columns > MAX_COLUMNS || (int64_t)columns * page > 1 << 30)
+        return fail(YTHIP_EUNSUPPORTED, "%s: %d columns of %d rows (at most 65536 columns, 2^30 rows)", who, columns, page);
     if (B > 0 && (table == nullptr || len == nullptr)) return fail(YTHIP_EINVAL, "%s: table or len is NULL", who);
     if (ld < columns) return fail(YTHIP_EINVAL, "%s: a table row of %d entries at a stride of %lld", who, columns, (long long)ld);
     return 0;
