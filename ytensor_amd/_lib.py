@@ -46,7 +46,6 @@ class PagePool(ctypes.Structure):
 
 
 _U64 = ctypes.c_uint64
-_PP = ctypes.POINTER(PagePool)
 
 # Every symbol include/ythip.h declares, with its ctypes signature.
 SIGNATURES = {
@@ -105,12 +104,12 @@ SIGNATURES = {
                                 _P, _L, _P]),
     "ythip_cache_grow": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _P, _P, _P, _L, _P, _P, _P]),
     "ythip_cache_fork_workspace_size": (ctypes.c_size_t, [_I]),
-    "ythip_cache_fork": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _I, _P, _P, _P, _P, _L, _P, _I, _I, _PP, _P, _P,
+    "ythip_cache_fork": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _I, _P, _P, _P, _P, _L, _P, _I, _I, _P, _P, _P,
                               ctypes.c_size_t, _P]),
     "ythip_cache_free": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _I, _P, _P, _P, _L, _P, _P, _P]),
     "ythip_cache_compact_workspace_size": (ctypes.c_size_t, [_I]),
-    "ythip_cache_compact": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _P, _P, _L, _P, _I, _I, _PP, _P, ctypes.c_size_t, _P]),
-    "ythip_cache_copy_pages": (_I, [_I, _I, _P, _P, _I, _I, _PP, _P, _P]),
+    "ythip_cache_compact": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _P, _P, _L, _P, _I, _I, _P, _P, ctypes.c_size_t, _P]),
+    "ythip_cache_copy_pages": (_I, [_I, _I, _P, _P, _I, _I, _P, _P, _P]),
     "ythip_yt_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "ythip_yt_close": (_I, [_P]),
     "ythip_yt_count": (_I, [_P]),

@@ -239,20 +239,29 @@ def _list(name: str, t: torch.Tensor) -> torch.Tensor:
     return _packed(t)
 
 
+@functools.lru_cache(maxsize=4096)
+def _pool_layout(shape: tuple, stride: tuple, es: int) -> tuple:
+    """(layers, pages, layer stride, page stride, page bytes) of a [L, P, ...] tensor, in bytes."""
+    if len(shape) < 3:
+        raise ValueError(f"a pool of shape {list(shape)}; needs [layers, pages, ...]")
+    inner = 1
+    for size, step in zip(reversed(shape[2:]), reversed(stride[2:])):
+        if size != 1 and step != inner:
+            raise ValueError(f"a pool of shape {list(shape)} and strides {list(stride)}: a page must be contiguous")
+        inner *= size
+    return shape[0], shape[1], stride[0] * es, stride[1] * es, inner * es
+
+
 def _pools(pools, pages: int):
-    """ythip_page_pool descriptors of [L, P, ...] tensors whose pages are contiguous."""
-    arr, layers = (_lib.PagePool * max(len(pools), 1))(), 0
-    for i, t in enumerate(pools):
-        if t.dim() < 3 or t.shape[1] != pages or (i and t.shape[0] != layers):
-            raise ValueError(f"pool {i} has shape {list(t.shape)}; needs [layers, {pages}, ...]")
-        layers, inner = t.shape[0], 1
-        for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
-            if size != 1 and stride != inner:
-                raise ValueError(f"pool {i}: a page must be contiguous")
-            inner *= size
-        es = t.element_size()
-        arr[i] = _lib.PagePool(t.data_ptr(), t.stride(0) * es, t.stride(1) * es, inner * es)
-    return len(pools), layers, arr
+    """(pools, layers, their ythip_page_pool descriptors)"""
+    layers, words = None, []
+    for t in pools:
+        n, p, ls, ps, size = _pool_layout(t.shape, t.stride(), t.element_size())
+        if p != pages or (layers is not None and n != layers):
+            raise ValueError(f"a pool of shape {list(t.shape)}; needs [{'layers' if layers is None else layers}, {pages}, ...]")
+        layers = n
+        words += (t.data_ptr(), ls, ps, size)
+    return len(pools), layers or 0, (ctypes.c_int64 * len(words))(*words)
 
 
 def cache_grow(ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, n_new: torch.Tensor, page: int,
