@@ -24,7 +24,8 @@ struct PagedArgs {
     const float* sums;
     int64_t ss[2];
     uint64_t* rank;  // sparse: [B][Hkv][T][columns], the pages' scores as rank_of has them
-    int target, min_chunk, items, row_tiles;  // the cut: ranges (0: a sequence each; sparse: of a token), tiles one has at least
+    int target, min_chunk, items, row_tiles;  // the cut: ranges (0: a sequence each; sparse: of a token), tiles of a stage
+    bool even;  // the cut of a few sequences: each by itself
     float *part, *part_ml;  // partials of items: [items][Hkv][rows][d] and (max, sum)
 };
 
@@ -57,10 +58,13 @@ __device__ __forceinline__ int tiles_of(const PagedArgs& a, int len, int tn, int
 // the workgroups the same work; a range that holds the end of one sequence and the start of
 // another is two items, one a sequence. Item r + b is what range r holds of sequence b: the
 // pairs that occur form a staircase, so the sums are distinct and a sequence's lie side by
-// side. Every wave works the cut out for itself from the lengths, one sequence a lane.
+// side. Where there are few ranges a sequence (`even`) that would leave the longest range well above
+// the average, so each sequence is cut by itself: into equal items of at most the fewest stages
+// with which all items number no more than `target` (two chunks of 512 over 2048 and 8192 rows,
+// 8 items 82.5 -> 79 us; three trees of 7, 96 items 14.4 -> 14.9, left as they were). Every wave works the cut out for itself from the lengths, one sequence a lane.
 struct Cut {
     int b, first, count;  // the sequence, its first item and how many it has
-    int chunk, start;     // tiles a range, the sequence's first tile
+    int chunk, at;        // tiles of an item, the item's first tile (before the sequence's start: negative)
     int len, tn;          // rows_in_use and new_rows of the sequence
 };
 // Sums over the lanes up to this one (DPP: within rows of 16, then across them).
@@ -88,12 +92,34 @@ __device__ __forceinline__ Cut cut_of(const PagedArgs& a, int kt, int item, int 
         mine = is ? max(tiles_of(a, len, tn, kt), 1) : 0;
         inc = wave_scan(mine);
     };
+    Cut c;
+    if (a.even) {
+        auto over = [](int x, int y) { return (int)(((uint32_t)x + y - 1) / (uint32_t)y); };
+        load(lane);
+        const int stages = over(mine, a.min_chunk), all = __builtin_amdgcn_readlane(wave_scan(stages), 63);
+        // of 64 lengths of an item, a lane each, the shortest that will do; the last one does: of a
+        // sequence's items all but one are full
+        const int low = over(all, a.target), most = over(all, a.target - a.B + 1), by = max(over(most - low, 63), 1);
+        int sum = 0;
+        for (int i = 0; i < a.B; ++i) sum += over(__builtin_amdgcn_readlane(stages, i), low + lane * by);
+        const int longest = low + by * __builtin_ctzll(__ballot(sum <= a.target));
+        const int n = over(stages, longest), end = wave_scan(n);
+        if (b < 0) b = __popcll(__ballot(lane < a.B && end <= item));
+        c.b = b < a.B ? b : -1;
+        b = min(b, a.B - 1);
+        c.count = __builtin_amdgcn_readlane(n, b);
+        c.first = __builtin_amdgcn_readlane(end, b) - c.count;
+        c.chunk = over(__builtin_amdgcn_readlane(stages, b), c.count) * a.min_chunk;
+        c.at = (item - c.first) * c.chunk;
+        c.len = __builtin_amdgcn_readlane(len, b);
+        c.tn = __builtin_amdgcn_readlane(tn, b);
+        return c;
+    }
     int total = 0;
     for (int base = (a.B - 1) & ~63; base >= 0; base -= 64) {  // the first 64 last: they are kept
         load(base + lane);
         total += __builtin_amdgcn_readlane(inc, 63);
     }
-    Cut c;
     c.chunk = max((int)(((uint32_t)total + a.target - 1) / (uint32_t)a.target), a.min_chunk);
     for (int base = 0, before = 0;; ) {
         const int start = before + inc - mine, n = min(a.B - base, 64);
@@ -110,7 +136,7 @@ __device__ __forceinline__ Cut cut_of(const PagedArgs& a, int kt, int item, int 
             c.b = base + at;
             c.first = __builtin_amdgcn_readlane(first, at);
             c.count = __builtin_amdgcn_readlane(last, at) - c.first + 1;
-            c.start = __builtin_amdgcn_readlane(start, at);
+            c.at = (item - c.b) * c.chunk - __builtin_amdgcn_readlane(start, at);
             c.len = __builtin_amdgcn_readlane(len, at);
             c.tn = __builtin_amdgcn_readlane(tn, at);
             if (b < 0 && item < c.first) c.b = -1;  // a range ended with a sequence: one sum is left out
@@ -157,6 +183,22 @@ __device__ __forceinline__ f32x4 mfma_half(F16, u32x2 a, u32x2 b, f32x4 c) {
 }
 
 __device__ __forceinline__ void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+// The order of a product's instructions: AHEAD of its READS reads from LDS first, then MF MFMAs and
+// PER reads in turn; left to itself each read is waited for right away (a tree of 64 over
+// 131072 rows 126 -> 122 us, two chunks of 512 85 -> 83).
+template <int READS, int PER, int MF, int AHEAD>
+__device__ __forceinline__ void interleave() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD < READS ? AHEAD : READS, 0);
+#pragma unroll
+    for (int i = AHEAD; i < READS; i += PER) {
+        __builtin_amdgcn_sched_group_barrier(0x008, MF, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, (AHEAD < READS ? AHEAD : READS) / PER * MF, 0);
+#endif
+}
 
 template <class T, int D, int QT, int WR>
 struct Shape {
@@ -261,9 +303,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     } else if (a.target == 0) {
         whole = true;
     } else {
-        const int at = (item - b) * cut.chunk - cut.start;
-        c0 = max(at, 0);
-        c1 = min(at + cut.chunk, nt);
+        c0 = max(cut.at, 0);
+        c1 = min(cut.at + cut.chunk, nt);
         whole = cut.count == 1;
     }
     c0 = uniform(c0), c1 = uniform(c1);
@@ -512,6 +553,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                 for (int qt = 0; qt < QT; ++qt) p[qt][kt] = mfma_chunk(T{}, kf, qf[qt][ks], p[qt][kt]);
             }
         }
+        if constexpr (!F) interleave<S::KG * S::KS, 1, QT, 6>();
         constexpr uint32_t FULL = S::KG == 1 ? 16u : S::KG == 2 ? 16u | 16u << 5 : 16u | 16u << 5 | 16u << 10 | 16u << 15;
         __builtin_amdgcn_s_setprio(0);
         if (paths || pack != FULL) {
@@ -608,6 +650,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt) o[qt][t] = acc[qt];
             }
+            if constexpr (!F && !decltype(clean)::value) interleave<S::DT * S::KG, S::KG, QT * PK, 3 * S::KG>();
         };
         if (!NEW || odd == 0) {
             __builtin_amdgcn_s_setprio(1);
@@ -1009,11 +1052,13 @@ __global__ __launch_bounds__(SEL) void paged_select_kernel(PagedArgs a) {
 struct Plan {
     int qt, wr, kt;  // the workgroup's shape
     int target, min_chunk, row_tiles;
+    bool even = false;
     int64_t items;
     size_t part_bytes, ml_bytes, rank_bytes;
     size_t bytes() const { return part_bytes + ml_bytes + rank_bytes; }
 };
 constexpr int SLOTS = 512, SLOTS1 = 768;
+constexpr int EVEN_SEQS = 8;  // sequences whose cut is one by one at most: its search asks each in turn
 constexpr int WHOLE = 6;  // stages up to which a sequence stays with one workgroup
 Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int page, int top_k) {
     const int rows = top_k > 0 ? G : (int)std::min<int64_t>((int64_t)T * G, 1 << 20);
@@ -1044,11 +1089,12 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
         p.target = 0;
         p.items = B;
     } else {
-        // a few sequences: their boundaries' items among the slots too
         int64_t ranges = slots / per;
-        if (B - 1 <= ranges / 2) ranges -= B - 1;
+        p.even = B <= EVEN_SEQS && B <= ranges && ranges <= 8 * B;
+        // the items at the ends of a few sequences count among the slots too
+        if (!p.even && B - 1 <= ranges / 2) ranges -= B - 1;
         p.target = (int)std::min(std::max<int64_t>(1, ranges), B * most);
-        p.items = part_items = (int64_t)p.target + B - 1;
+        p.items = part_items = (int64_t)p.target + (p.even ? 0 : B - 1);
     }
     const int64_t part_rows = part_items * Hkv * all_rows;
     p.part_bytes = (size_t)part_rows * d * sizeof(float);
@@ -1095,7 +1141,7 @@ int run(int dtype, int d, PagedArgs& a, void* ws, hipStream_t s) {
     const Plan p = plan_of(dtype, a.B, a.Hkv, a.G, a.T, d, a.columns, 1 << a.shift, SPARSE ? a.top_k : 0);
     if ((p.items * a.Hkv + 8) * p.row_tiles > INT_MAX)
         return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups", (long long)(p.items * a.Hkv * p.row_tiles));
-    a.target = p.target, a.min_chunk = p.min_chunk, a.items = (int)p.items, a.row_tiles = p.row_tiles;
+    a.target = p.target, a.min_chunk = p.min_chunk, a.items = (int)p.items, a.row_tiles = p.row_tiles, a.even = p.even;
     char* w = static_cast<char*>(ws);
     a.rank = reinterpret_cast<uint64_t*>(w);
     a.part = reinterpret_cast<float*>(w + p.rank_bytes);
