@@ -125,6 +125,20 @@ def test_attention_of_many_tokens(dtype, T, kind):
     compare(out, want, tol, torch.zeros_like(out))
 
 
+@pytest.mark.parametrize("dtype,lens,new", [
+    ("bf16", [1500], [260]), ("bf16", [40, 2100], [260, 260]), ("f16", [0, 1900, 3], [7, 260, 0]),
+    ("f32", [700, 0, 16, 900, 65], [1, 260, 64, 65, 0]), ("bf16", [0] * 7 + [1700], [0, 1, 260, 0, 3, 0, 0, 129]),
+    ("f16", [400] * 9, [260] * 9)])
+def test_attention_of_few_sequences_of_many_rows(dtype, lens, new):
+    dt, B, T, Hkv, G = DT[dtype], len(lens), 260, 8, 4
+    g, k, v, table, kv_len = cache(38, lens, Hkv, 16, 64, dt, columns=160)
+    q, kn, vn = tokens(g, B, Hkv * G, Hkv, T, 64, dt)
+    parents, tree_len = tree(g, B, T), ints(new)
+    before = torch.full_like(q, 7.0)
+    out = yt.paged_attention(q, kn, vn, k, v, table, kv_len, parents=parents, tree_len=tree_len, out=before.clone())
+    compare(out, *attention(q, kn, vn, k, v, table, kv_len, parents, tree_len), before)
+
+
 def test_attention_path_values():
     """A parent outside [0, child) ends the path, whatever it is."""
     dt, T, d = torch.float32, 9, 64
