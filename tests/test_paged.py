@@ -44,6 +44,7 @@ EINVAL, EUNSUP = _lib.YTHIP_EINVAL, _lib.YTHIP_EUNSUPPORTED
     (dict(Hkv=0), EINVAL, b"heads"),
     (dict(columns=70000, ld=70000), EUNSUP, b"columns"),
     (dict(columns=65536, ld=65536, page=32768), EUNSUP, b"2^30"),
+    (dict(columns=65536, ld=65536, page=16384, B=17), EUNSUP, b"2^34"),
     (dict(parents=FAKE, T=4097, ldp=4097), EUNSUP, b"tree"),
     (dict(T=1 << 29), EUNSUP, b"new tokens"),
     (dict(kn=_lib.i64array([128, 128, 1 << 24])), EUNSUP, b"stride"),

@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "launch.hpp"
 
@@ -24,8 +25,9 @@ struct PagedArgs {
     const float* sums;
     int64_t ss[2];
     uint64_t* rank;  // sparse: [B][Hkv][T][columns], the pages' scores as rank_of has them
-    int target, min_chunk, items, row_tiles;  // the cut: ranges (0: a sequence each; sparse: of a token), tiles of a stage
-    bool even;  // the cut of a few sequences: each by itself
+    int target, stage, items, row_tiles;  // the cut: ranges (0: a sequence each; sparse: of a token), tiles of a stage
+    bool even;      // the cut of a few sequences: each by itself
+    int short_run;  // stages up to which half as many ranges are better
     float *part, *part_ml;  // partials of items: [items][Hkv][rows][d] and (max, sum)
 };
 
@@ -61,16 +63,20 @@ __device__ __forceinline__ int tiles_of(const PagedArgs& a, int len, int tn, int
 // side. Where there are few ranges a sequence (`even`) that would leave the longest range well above
 // the average, so each sequence is cut by itself: into equal items of at most the fewest stages
 // with which all items number no more than `target` (two chunks of 512 over 2048 and 8192 rows,
-// 8 items 82.5 -> 79 us; three trees of 7, 96 items 14.4 -> 14.9, left as they were). Every wave works the cut out for itself from the lengths, one sequence a lane.
+// 8 items 82.5 -> 79 us; three trees of 7, 96 items 14.4 -> 14.9, left as they were).
+// A range has at least `least_stages`: the more ranges, the longer the merge of their partials.
+// Every wave works the cut out for itself from the lengths, one sequence a lane.
 struct Cut {
     int b, first, count;  // the sequence, its first item and how many it has
     int chunk, at;        // tiles of an item, the item's first tile (before the sequence's start: negative)
     int len, tn;          // rows_in_use and new_rows of the sequence
 };
-// Sums over the lanes up to this one (DPP: within rows of 16, then across them).
-__device__ __forceinline__ int wave_scan(int v) {
-    auto add = [](int x, auto ctrl, auto rows) {
-        return x + __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+// Sums (or the maxima of numbers that are not negative) over the lanes up to this one (DPP:
+// within rows of 16, then across them).
+template <class Op>
+__device__ __forceinline__ int wave_scan(int v, Op op) {
+    auto add = [&](int x, auto ctrl, auto rows) {
+        return op(x, __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
     };
     using std::integral_constant;
     v = add(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
@@ -80,6 +86,20 @@ __device__ __forceinline__ int wave_scan(int v) {
     v = add(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast 15 into rows 1 and 3
     v = add(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast 31 into rows 2 and 3
     return v;
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    return wave_scan(v, [](int x, int y) { return x + y; });
+}
+__device__ __forceinline__ int over(int x, int y) { return (int)(((uint32_t)x + y - 1) / (uint32_t)y); }
+
+// The fewest stages a range has, of `all` in the batch and `longest` in a sequence. The merge takes about
+// 1/20 of a stage's time a partial, so n ranges of s = longest / n stages cost the least at
+// s = sqrt(longest / 20) (1 token, 1 KV head, 30000 rows: 512 ranges 34 us, 256 22, 128 17.4, 64 16.6).
+// And where a tile's rows are shared, half of the ranges are better than fewer than four stages each:
+// one workgroup a CU (5 trees of 16, 4 heads a group, over up to 4097 rows: 64 ranges 31 us, 32 27).
+__device__ __forceinline__ int least_stages(const PagedArgs& a, int all, int longest) {
+    const int root = (int)ceilf(__builtin_amdgcn_sqrtf((float)longest * 0.05f));
+    return max(max(root, 1), over(all, a.target) < a.short_run ? over(all, (a.target + 1) / 2) : 1);
 }
 // b < 0: of the sequence that `item` belongs to (b = -1: to none)
 __device__ __forceinline__ Cut cut_of(const PagedArgs& a, int kt, int item, int b) {
@@ -94,12 +114,12 @@ __device__ __forceinline__ Cut cut_of(const PagedArgs& a, int kt, int item, int 
     };
     Cut c;
     if (a.even) {
-        auto over = [](int x, int y) { return (int)(((uint32_t)x + y - 1) / (uint32_t)y); };
         load(lane);
-        const int stages = over(mine, a.min_chunk), all = __builtin_amdgcn_readlane(wave_scan(stages), 63);
+        const int stages = over(mine, a.stage), all = __builtin_amdgcn_readlane(wave_scan(stages), 63);
         // of 64 lengths of an item, a lane each, the shortest that will do; the last one does: of a
         // sequence's items all but one are full
-        const int low = over(all, a.target), most = over(all, a.target - a.B + 1), by = max(over(most - low, 63), 1);
+        const int least = least_stages(a, all, __builtin_amdgcn_readlane(wave_scan(stages, [](int x, int y) { return max(x, y); }), 63));
+        const int low = max(over(all, a.target), least), most = max(over(all, a.target - a.B + 1), low), by = max(over(most - low, 63), 1);
         int sum = 0;
         for (int i = 0; i < a.B; ++i) sum += over(__builtin_amdgcn_readlane(stages, i), low + lane * by);
         const int longest = low + by * __builtin_ctzll(__ballot(sum <= a.target));
@@ -109,18 +129,20 @@ __device__ __forceinline__ Cut cut_of(const PagedArgs& a, int kt, int item, int 
         b = min(b, a.B - 1);
         c.count = __builtin_amdgcn_readlane(n, b);
         c.first = __builtin_amdgcn_readlane(end, b) - c.count;
-        c.chunk = over(__builtin_amdgcn_readlane(stages, b), c.count) * a.min_chunk;
+        c.chunk = over(__builtin_amdgcn_readlane(stages, b), c.count) * a.stage;
         c.at = (item - c.first) * c.chunk;
         c.len = __builtin_amdgcn_readlane(len, b);
         c.tn = __builtin_amdgcn_readlane(tn, b);
         return c;
     }
-    int total = 0;
+    int total = 0, longest = 0;
     for (int base = (a.B - 1) & ~63; base >= 0; base -= 64) {  // the first 64 last: they are kept
         load(base + lane);
         total += __builtin_amdgcn_readlane(inc, 63);
+        longest = max(longest, __builtin_amdgcn_readlane(wave_scan(mine, [](int x, int y) { return max(x, y); }), 63));
     }
-    c.chunk = max((int)(((uint32_t)total + a.target - 1) / (uint32_t)a.target), a.min_chunk);
+    total = over(total, a.stage);
+    c.chunk = max(over(total, a.target), least_stages(a, total, over(longest, a.stage))) * a.stage;
     for (int base = 0, before = 0;; ) {
         const int start = before + inc - mine, n = min(a.B - base, 64);
         const int first = (int)((uint32_t)start / (uint32_t)c.chunk) + base + lane;
@@ -295,7 +317,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     int c0 = 0, c1 = nt;
     bool whole;
     if constexpr (SPARSE) {
-        const int chunk = max((nt + a.target - 1) / a.target, a.min_chunk), split = item % a.target;
+        const int chunk = max((nt + a.target - 1) / a.target, a.stage), split = item % a.target;
         if (t_one >= tn || (split > 0 && split * chunk >= nt)) return;
         c0 = split * chunk;
         c1 = min(nt, c0 + chunk);
@@ -816,7 +838,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, int kt) {
         t = r / a.G, gh = r - t * a.G;
         const int nsel = min(a.top_k, (int)(((int64_t)len + (1 << a.shift) - 1) >> a.shift));
         const int nt = (int)((((int64_t)nsel << a.shift) + kt - 1) / kt) + (a.Kn != nullptr ? (t + kt) / kt : 0);
-        const int chunk = max((nt + a.target - 1) / a.target, a.min_chunk);
+        const int chunk = max((nt + a.target - 1) / a.target, a.stage);
         count = max((nt + chunk - 1) / chunk, 1);
         first = (((int64_t)(b * a.T + t) * a.target) * a.Hkv + h) * a.G + gh;
     } else {
@@ -1051,13 +1073,14 @@ __global__ __launch_bounds__(SEL) void paged_select_kernel(PagedArgs a) {
 // How a call is cut. Both the size of the workspace and the launch come from this alone.
 struct Plan {
     int qt, wr, kt;  // the workgroup's shape
-    int target, min_chunk, row_tiles;
+    int target, stage, row_tiles;
     bool even = false;
+    int short_run;
     int64_t items;
     size_t part_bytes, ml_bytes, rank_bytes;
     size_t bytes() const { return part_bytes + ml_bytes + rank_bytes; }
 };
-constexpr int SLOTS = 512, SLOTS1 = 768;
+constexpr int SLOTS = 512;
 constexpr int EVEN_SEQS = 8;  // sequences whose cut is one by one at most: its search asks each in turn
 constexpr int WHOLE = 6;  // stages up to which a sequence stays with one workgroup
 Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int page, int top_k) {
@@ -1072,17 +1095,28 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     const int rw = 16 * p.qt * p.wr;
     p.row_tiles = (int)((all_rows + rw - 1) / rw);
     const int64_t per = (int64_t)Hkv * p.row_tiles;
-    p.min_chunk = 4 / p.wr;
-    // Workgroups that the work is dealt to: the 512 that run at once where they share tiles (1024 of
-    // them: a tree of 64 over 131072 rows 126 -> 146 us, more partials); half as many again where
-    // each streams its own rows, so that none waits for the last (16 x 1 token 67 -> 63 us).
-    const int64_t slots = p.wr == 1 ? SLOTS1 : SLOTS;
+    p.stage = 4 / p.wr;
+    // Workgroups that the work is dealt to: the 512 that run at once (of 768 that stream their own rows
+    // a third waits: 16 sequences, 1 token, up to 8192 rows 60 -> 63 us; 1024 that share tiles: a tree of 64 over
+    // 131072 rows 126 -> 146 us).
+    // Half of them where a workgroup has a CU to itself (128 rows of fp32, d 128: 136 KB of LDS) and the
+    // sequences are few, whose items are alike (a tree of 64 over 32768 rows 219 -> 198 us; 16 ragged
+    // sequences 152 -> 188 us, left as they were).
+    const bool alone = dtype == YTHIP_F32 && d == 128 && p.wr > 1 && B <= EVEN_SEQS;
+    // And half where rows are streamed and a sequence has many ranges, which are alike then and whose
+    // partials cost more than the second workgroup of a CU brings (1 token, 4 KV heads, 60000 rows 32 ->
+    // 29 us; 16 sequences, 8 heads, 4 ranges each 60 -> 67 us, left as they were).
+    const bool many = p.wr == 1 && SLOTS / per >= 8 * (int64_t)B * (top_k > 0 ? T : 1);
+    const int64_t slots = alone || many ? SLOTS / 2 : SLOTS;
+    p.short_run = p.wr > 1 ? 4 : 0;
     const int64_t new_tiles = ((int64_t)T + p.kt - 1) / p.kt;
     const int64_t seq_rows = (int64_t)std::min(top_k > 0 ? top_k : columns, columns) * page;
-    const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + new_tiles, most = (tiles + p.min_chunk - 1) / p.min_chunk;
+    const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + new_tiles, most = (tiles + p.stage - 1) / p.stage;
     int64_t part_items = 0;
     if (top_k > 0) {
-        p.target = (int)std::max<int64_t>(1, std::min(most, (slots + per * B * T - 1) / (per * B * T)));
+        // (a token's pages in ranges of at least the stages that least_stages explains)
+        const int64_t root = std::max<int64_t>(1, (int64_t)std::ceil(std::sqrt((double)most / 20)));
+        p.target = (int)std::max<int64_t>(1, std::min((most + root - 1) / root, (slots + per * B * T - 1) / (per * B * T)));
         p.items = (int64_t)B * T * p.target;
         if (p.target > 1) part_items = p.items;
     } else if (most <= WHOLE) {
@@ -1141,7 +1175,7 @@ int run(int dtype, int d, PagedArgs& a, void* ws, hipStream_t s) {
     const Plan p = plan_of(dtype, a.B, a.Hkv, a.G, a.T, d, a.columns, 1 << a.shift, SPARSE ? a.top_k : 0);
     if ((p.items * a.Hkv + 8) * p.row_tiles > INT_MAX)
         return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups", (long long)(p.items * a.Hkv * p.row_tiles));
-    a.target = p.target, a.min_chunk = p.min_chunk, a.items = (int)p.items, a.row_tiles = p.row_tiles, a.even = p.even;
+    a.target = p.target, a.stage = p.stage, a.items = (int)p.items, a.row_tiles = p.row_tiles, a.even = p.even, a.short_run = p.short_run;
     char* w = static_cast<char*>(ws);
     a.rank = reinterpret_cast<uint64_t*>(w);
     a.part = reinterpret_cast<float*>(w + p.rank_bytes);
@@ -1201,6 +1235,8 @@ int prepare(const char* who, const Call& c, PagedArgs& a, bool& done) {
     if (c.Hkv == 0 || c.Hq % c.Hkv != 0) return fail(YTHIP_EINVAL, "%s: %d query heads over %d KV heads", who, c.Hq, c.Hkv);
     if (c.columns > 65536 || (int64_t)c.columns * c.page > 1 << 30)
         return fail(YTHIP_EUNSUPPORTED, "%s: %d columns of %d rows (at most 65536 columns, 2^30 rows)", who, c.columns, c.page);
+    if ((int64_t)c.B * c.columns * c.page > (int64_t)1 << 34)
+        return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences of %d columns of %d rows (2^34 rows in all)", who, c.B, c.columns, c.page);
     if ((int64_t)c.T * c.Hq > 1 << 30) return fail(YTHIP_EUNSUPPORTED, "%s: %d new tokens of %d heads (2^30 in all)", who, c.T, c.Hq);
     if (c.parents != nullptr && c.T > MAX_TREE) return fail(YTHIP_EUNSUPPORTED, "%s: a tree of %d tokens (at most %d)", who, c.T, MAX_TREE);
     if (!c.Q || !c.O || !c.kv_len || !c.q_str || !c.o_str || !c.pool_str) return fail(YTHIP_EINVAL, "%s: NULL argument", who);
