@@ -105,7 +105,8 @@ struct GrowArgs {
     StateArgs state;
 };
 // The prefix sum of the pages that the sequences need gives each its ranks among the free
-// pages; a free page's rank then finds its sequence by bisection.
+// pages; a free page's rank then finds its sequence by bisection. One workgroup: the counts' sums
+// need all of them, and its round trips (counts, users, table) are the time (16 sequences 3.4 us).
 __global__ __launch_bounds__(PLAN_THREADS) void cache_grow_kernel(GrowArgs a) {
     constexpr int LIST = 4096;  // more pages than that: the free ones are looked up twice
     __shared__ int s_off[MAX_SEQS + 1], s_have[MAX_SEQS], s_list[LIST], s_scan[PLAN_THREADS / 64];
@@ -288,6 +289,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void cache_fork_plan(ForkArgs a) {
 }
 
 // Workgroups [0, n): pair i's row and page counts; the others its partial page, in every pool.
+// Bound by the copies' bytes (8 pairs, 28 layers, 119 MB read and written 21.4 us, 5.5 TB/s).
 __global__ __launch_bounds__(256) void cache_fork_copy(ForkArgs a, PoolSet ps) {
     const int w = blockIdx.x;
     if (w < a.n) {
@@ -324,7 +326,8 @@ struct FreeArgs {
     int32_t* status;
     StateArgs state;
 };
-// One wave a mention; the one that finds rows takes them all (an exchange of the length).
+// One wave a mention; the one that finds rows takes them all (an exchange of the length). Bound by
+// its round trips (length, table, users): 32 sequences of up to 41 pages 6 us.
 __global__ __launch_bounds__(PLAN_THREADS) void cache_free_kernel(FreeArgs a) {
     if (a.state.here) {  // one workgroup then, whose barrier orders its own memory
         copy_state_words(a.state, threadIdx.x, PLAN_THREADS);
@@ -359,6 +362,8 @@ __global__ __launch_bounds__(PLAN_THREADS) void cache_free_kernel(FreeArgs a) {
     }
 }
 
+// The plan: one workgroup gives the holes below the live count the live pages above it, both
+// ascending (4.7 us for 2048 pages). The move: bound by its bytes (1.77 GB read and written 289-321 us, 5.5-6.1 TB/s).
 struct CompactArgs {
     int B, columns, pages, shift;
     const int32_t *ref, *table, *len;
