@@ -537,6 +537,19 @@ def test_refusals_of_the_python_layer():
 
 # ------------------------------------------------------------------- together
 
+def test_refusals_of_expanded_arguments():
+    """A table whose rows are one row (stride 0), and a workspace of fewer bytes than elements."""
+    g, k, v, table, kv_len = cache(5, [900, 900], 2, 16, 64, torch.bfloat16, columns=57)
+    q, kn, vn = tokens(g, 2, 4, 2, 1, 64, torch.bfloat16)
+    with pytest.raises(yt.YthipError, match="stride"):
+        yt.paged_attention(q, kn, vn, k, v, table[:1].expand(2, 57), kv_len)
+    with pytest.raises(yt.YthipError, match="stride"):
+        yt.cache_free(torch.ones(8, dtype=torch.int32, device="cuda"), table[:1].expand(2, 57), kv_len, ints([0]), 16)
+    space = torch.empty(1, dtype=torch.uint8, device="cuda").expand(1 << 26)
+    with pytest.raises(ValueError, match="contiguous"):
+        yt.paged_attention(q, kn, vn, k, v, table, kv_len, workspace=space)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_a_generation_with_drafts(dtype):
     """Prompt, fork, drafted trees verified and committed, sparse attention, an end and a packing:

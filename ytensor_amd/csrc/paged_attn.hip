@@ -1269,7 +1269,7 @@ int prepare(const char* who, const Call& c, PagedArgs& a, bool& done) {
     a.scale_log2 = (c.scale == 0.f ? 1.0f / sqrtf((float)c.d) : c.scale) * 1.4426950408889634f;
     a.sel = nullptr, a.top_k = 0, a.sums = nullptr, a.rank = nullptr;
     if (((int64_t)c.columns * c.page / 16 + c.T / 16 + 2) * c.B > INT_MAX)
-        return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences of up to %lld rows (2^35 in all)", who, c.B, (long long)c.columns * c.page);
+        return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences of %d new tokens over up to %lld rows (2^35 in all)", who, c.B, c.T, (long long)c.columns * c.page);
     if (c.B > 65535 || c.Hq > 65535) return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences, %d heads (at most 65535 each)", who, c.B, c.Hq);
     return 0;
 }

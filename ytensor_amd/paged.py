@@ -124,6 +124,8 @@ def _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, 
     need = _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k or 0)
     ws_at, ws_bytes = None, 0
     if need:
+        if workspace is not None and not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
         if workspace is None or workspace.numel() * workspace.element_size() < need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         ws_at, ws_bytes = workspace.data_ptr(), need
@@ -159,7 +161,7 @@ def _table(table: torch.Tensor, B: int) -> tuple[torch.Tensor, int, int]:
     ld, step = table.stride()
     if step != 1 and columns > 1:
         raise ValueError("table must have contiguous rows")
-    return table, ld if ld > columns else columns, columns
+    return table, ld if B > 1 else max(ld, columns), columns  # a single row has no stride
 
 
 @functools.lru_cache(maxsize=4096)
