@@ -911,52 +911,43 @@ __device__ __forceinline__ uint64_t rank_of(double s) {
 }
 constexpr uint64_t RANK_TOP = ~0ull;  // the last page's: above every score's
 
-// Scores of 64 pages of one KV head for TB tokens: 16 lanes a page (D / 16 dims each), four
-// pages a wave at a time, all a lane's pages in flight together. The products are of float32 sums
-// and sums of the group's queries, all in 64 bits (the fp64 rate is the fp32 rate here, and the
-// time is that of the sums' bytes): scores that differ in their first 50 bits keep their order,
-// so the choice does not depend on how they were added up.
-// 8 MB of sums, 1 token 5.3 us; 16 sequences, 4 tokens, 21 MB 14 us.
-template <class T, int D, int TB>
-__global__ __launch_bounds__(256) void paged_score_kernel(PagedArgs a) {
-    constexpr int E = D / 16, V = E / 4, U = 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
-    const int h = blockIdx.y % a.Hkv, t0 = blockIdx.y / a.Hkv * TB, b = blockIdx.z;
-    const int tn = new_rows(a, b), len = rows_in_use(a, b);
-    const int n = (int)(((int64_t)len + (1 << a.shift) - 1) >> a.shift);
-    const int first = (blockIdx.x * 4 + wave) * 16 + (lane >> 4);  // and + 4, + 8, + 12
-    if (t0 >= tn || blockIdx.x * 64 >= n) return;
-    int id[U];
+// The sum of a token's queries of one KV head, lane l16's D / 16 of it (dims 64 v + 4 l16 + 0..3).
+template <class T, int D>
+__device__ __forceinline__ void query_sum(const PagedArgs& a, int b, int h, int t, int l16, double (&q)[D / 16]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        id[u] = first + 4 * u < n ? a.table[b * a.ld_table + first + 4 * u] : -1;
-        if ((uint32_t)id[u] >= (uint32_t)a.pages) id[u] = -1;
+    for (int e = 0; e < D / 16; ++e) q[e] = 0.0;
+    for (int g = 0; g < a.G; ++g) {
+        const int64_t at = b * a.qs[0] + (int64_t)(h * a.G + g) * a.qs[1] + t * a.qs[2] + l16 * 4;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) q[e] += (double)load_as_f32<T>(a.Q, at + e / 4 * 64 + e % 4);
     }
+}
+// Key sums of U pages of a sequence (first, first + 4, ...): 16 lanes a page, all in flight together.
+template <int D, int U>
+struct PageSums {
+    static constexpr int E = D / 16, V = E / 4;
+    int id[U];
     f32x4 x[U][V];
+    __device__ __forceinline__ void load(const PagedArgs& a, int b, int h, int first, int n, int l16) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            id[u] = first + 4 * u < n ? a.table[b * a.ld_table + first + 4 * u] : -1;
+            if ((uint32_t)id[u] >= (uint32_t)a.pages) id[u] = -1;
+        }
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            x[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
-            // 16 lanes read 256 consecutive bytes
-            if (id[u] >= 0) {
-                const float* p = a.sums + id[u] * a.ss[0] + h * a.ss[1] + v * 64 + l16 * 4;
-                x[u][v] = f32x4{p[0], p[1], p[2], p[3]};
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                x[u][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+                // 16 lanes read 256 consecutive bytes
+                if (id[u] >= 0) {
+                    const float* p = a.sums + id[u] * a.ss[0] + h * a.ss[1] + v * 64 + l16 * 4;
+                    x[u][v] = f32x4{p[0], p[1], p[2], p[3]};
+                }
             }
-        }
-#pragma unroll
-    for (int k = 0; k < TB; ++k) {
-        const int t = t0 + k;
-        if (t >= tn) return;
-        double q[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) q[e] = 0.0;
-        for (int g = 0; g < a.G; ++g) {
-            const int64_t at = b * a.qs[0] + (int64_t)(h * a.G + g) * a.qs[1] + t * a.qs[2] + l16 * 4;
-#pragma unroll
-            for (int e = 0; e < E; ++e) q[e] += (double)load_as_f32<T>(a.Q, at + e / 4 * 64 + e % 4);
-        }
-        uint64_t* out = a.rank + (((int64_t)b * a.Hkv + h) * a.T + t) * a.columns;
+    }
+    // out[i]: page i's rank, the last page's above all
+    __device__ __forceinline__ void ranks(const double (&q)[E], int first, int n, int l16, uint64_t* out) const {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             double s = 0.0;
@@ -968,6 +959,32 @@ __global__ __launch_bounds__(256) void paged_score_kernel(PagedArgs a) {
             if (l16 == 0 && i < n) out[i] = i == n - 1 ? RANK_TOP : rank_of(id[u] >= 0 ? s : -INFINITY);
         }
     }
+};
+
+// Scores of 64 pages of one KV head for TB tokens: 16 lanes a page (D / 16 dims each), four
+// pages a wave at a time, all a lane's pages in flight together. The products are of float32 sums
+// and sums of the group's queries, all in 64 bits (the fp64 rate is the fp32 rate here, and the
+// time is that of the sums' bytes): scores that differ in their first 50 bits keep their order,
+// so the choice does not depend on how they were added up.
+// 8 MB of sums, 1 token 5.3 us; 16 sequences, 4 tokens, 21 MB 14 us.
+template <class T, int D, int TB>
+__global__ __launch_bounds__(256) void paged_score_kernel(PagedArgs a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
+    const int h = blockIdx.y % a.Hkv, t0 = blockIdx.y / a.Hkv * TB, b = blockIdx.z;
+    const int tn = new_rows(a, b), len = rows_in_use(a, b);
+    const int n = (int)(((int64_t)len + (1 << a.shift) - 1) >> a.shift);
+    const int first = (blockIdx.x * 4 + wave) * 16 + (lane >> 4);  // and + 4, + 8, + 12
+    if (t0 >= tn || blockIdx.x * 64 >= n) return;
+    PageSums<D, 4> sums;
+    sums.load(a, b, h, first, n, l16);
+#pragma unroll
+    for (int k = 0; k < TB; ++k) {
+        const int t = t0 + k;
+        if (t >= tn) return;
+        double q[D / 16];
+        query_sum<T, D>(a, b, h, t, l16, q);
+        sums.ranks(q, first, n, l16, a.rank + (((int64_t)b * a.Hkv + h) * a.T + t) * a.columns);
+    }
 }
 
 // The top_k highest of a row of ranks, ascending by page: the k-th highest rank is found eight
@@ -975,11 +992,16 @@ __global__ __launch_bounds__(256) void paged_score_kernel(PagedArgs a) {
 // copies: ranks of like scores fall into few bins), until a bin is taken whole; scores are
 // far apart in their first 24 bits, so that is three rounds mostly. Then a wave takes a run of pages
 // each and writes its share in order. Bound by the rounds' barriers: 8 rows of 2048 ranks and 512 rows
-// of up to 512 both 7.8 us.
+// of up to 512 both 7.8 us. Where SCORE, the workgroup scores its row's pages itself, a launch less:
+// at most SCORED, what its waves have in flight at once (4 sequences, 5 tokens, 88 pages 23.7 -> 19.5 us in all;
+// 250 pages in two turns 18.3 -> 20.8).
+constexpr int SCORED = 128;
 constexpr int SEL_KEEP = 8;  // ranks a thread keeps in registers (longer rows are read again)
-template <int SEL>           // threads
+template <class T, int D, int SEL, bool SCORE>  // SEL threads
 __global__ __launch_bounds__(SEL) void paged_select_kernel(PagedArgs a) {
+    static_assert(!SCORE || SCORED == SEL / 64 * 32);
     constexpr int COPIES = 16;
+    __shared__ uint64_t s_rank[SCORE ? SCORED : 1];
     __shared__ int s_hist[256 * COPIES], s_bin[256], s_found[3], s_count[SEL / 64][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
@@ -991,7 +1013,16 @@ __global__ __launch_bounds__(SEL) void paged_select_kernel(PagedArgs a) {
         for (int i = tid; i < a.top_k; i += SEL) sel[i] = i < n ? i : -1;
         return;
     }
-    const uint64_t* rank = a.rank + row * a.columns;
+    const uint64_t* rank = SCORE ? s_rank : a.rank + row * a.columns;
+    if constexpr (SCORE) {
+        double q[D / 16];
+        query_sum<T, D>(a, b, h, t, lane & 15, q);
+        const int first = wave * 32 + (lane >> 4);
+        PageSums<D, 8> sums;
+        sums.load(a, b, h, first, n, lane & 15);
+        sums.ranks(q, first, n, lane & 15, s_rank);
+        __syncthreads();
+    }
     // wave w has the pages from w * run on, 64 at a time
     const int run = (n + SEL - 1) / SEL * 64;
     const bool kept = n <= SEL * SEL_KEEP;
@@ -1162,10 +1193,15 @@ template <class T, int D, bool SPARSE>
 int run_typed(const PagedArgs& a, const Plan& p, hipStream_t s) {
     if constexpr (SPARSE) {
         constexpr int TB = 4;
-        if (a.columns > 0)
-            paged_score_kernel<T, D, TB><<<dim3((a.columns + 63) / 64, a.Hkv * ((a.T + TB - 1) / TB), a.B), 256, 0, s>>>(a);
-        if (a.columns > 1024) paged_select_kernel<1024><<<dim3(a.T, a.Hkv, a.B), 1024, 0, s>>>(a);
-        else paged_select_kernel<256><<<dim3(a.T, a.Hkv, a.B), 256, 0, s>>>(a);
+        const dim3 rows(a.T, a.Hkv, a.B);
+        if (a.columns <= SCORED) {
+            paged_select_kernel<T, D, 256, true><<<rows, 256, 0, s>>>(a);
+        } else {
+            if (a.columns > 0)
+                paged_score_kernel<T, D, TB><<<dim3((a.columns + 63) / 64, a.Hkv * ((a.T + TB - 1) / TB), a.B), 256, 0, s>>>(a);
+            if (a.columns > 1024) paged_select_kernel<T, D, 1024, false><<<rows, 1024, 0, s>>>(a);
+            else paged_select_kernel<T, D, 256, false><<<rows, 256, 0, s>>>(a);
+        }
     }
     if (p.qt == 1) return launch<T, D, 1, 1, SPARSE>(a, p, s);
     if constexpr (!SPARSE) {
