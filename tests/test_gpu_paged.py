@@ -550,6 +550,25 @@ def test_refusals_of_expanded_arguments():
         yt.paged_attention(q, kn, vn, k, v, table, kv_len, workspace=space)
 
 
+@pytest.mark.parametrize("apart", range(8))
+@pytest.mark.parametrize("columns", [12, 700])
+def test_some_outputs_in_place(columns, apart):
+    """Any of ref, table and kv_len written in place and the others elsewhere: the same state."""
+    _, ref, table, kv_len = state(61, 40, columns, 600, 16, [(7 * b) % 150 for b in range(30)] + [0] * 10)
+    n_new = [b % 20 for b in range(38)] + [0, 0]
+    want, got = [], []
+    for outs, bits in ((want, 0), (got, apart)):
+        st = [x.clone() for x in (ref, table, kv_len)]
+        for call in (lambda o: yt.cache_grow(*st, ints(n_new), 16, out=o),
+                     lambda o: yt.cache_fork((), *st, ints([3, 4]), ints([39, 38]), 16, out=o),
+                     lambda o: yt.cache_free(*st, ints([0, 5, 39]), 16, out=o)):
+            o = tuple(torch.full_like(x, 77) if bits >> i & 1 else x for i, x in enumerate(st))
+            call(o)
+            st = list(o)
+            outs += [x.cpu() for x in st]
+    assert all(torch.equal(x, y) for x, y in zip(want, got)) and want[5][39] == want[2][3] > 0
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_a_generation_with_drafts(dtype):
     """Prompt, fork, drafted trees verified and committed, sparse attention, an end and a packing:
