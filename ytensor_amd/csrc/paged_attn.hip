@@ -204,6 +204,21 @@ __device__ __forceinline__ f32x4 mfma_half(F16, u32x2 a, u32x2 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
 }
 
+// Two weights as two pairs of 16-bit numbers that the matrix cores take one after the other: `hi` their first bits
+// (truncated, 8 or 11 of them), `rest` what is left. The weights taken are w (1 + 2^-23) (bf16) and w (1 + 2^-10)
+// (fp16), of all keys alike, so that their sum has the factor too and it cancels; it keeps `rest` above 0 for any weight
+// that is, and an infinite V times the two never makes inf - inf or 0 . inf. Of a weight 2^-16 (bf16) or 2^-21 (fp16)
+// is lost at most.
+template <class T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& rest) {
+    constexpr float ABOVE = std::is_same_v<T, BF16> ? 1.0f + 0x1p-23f : 1.0f + 0x1p-10f;
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (std::is_same_v<T, BF16>) hi = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302);
+    else hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+#endif
+    rest = pack2<T>(fmaf(x, ABOVE, -lo_as_f32(T{}, hi)), fmaf(y, ABOVE, -hi_as_f32(T{}, hi)));
+}
+
 __device__ __forceinline__ void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // The order of a product's instructions: AHEAD of its READS reads from LDS first, then MF MFMAs and
@@ -248,10 +263,11 @@ struct Shape {
 //   XOR-swizzled by key, V 32-byte blocks likewise and read transposed.
 //   Tiles run from the last to the first: new tokens, whose path is walked down from each
 //   query's token once, then cached rows.
-// Numerics: scores, maxima, sums and O in fp32; p is rounded to the inputs' 16-bit type for the
-//   second product (at most 2^-9 of each weight in bf16, as O's own rounding). In two pieces it
-//   would cost 0.4 of 7.9 us at 1 token over 300 rows, and an infinite V would meet a second
-//   piece of 0 or of the other sign.
+// Numerics: scores, maxima, sums and O in fp32; the weights of 16-bit inputs enter the second product
+//   (and their sum) as two 16-bit numbers each (split2), a 256th or less of O's own rounding away
+//   from fp32's. As one number each, half a step of O's type off, they would make O's error a third
+//   larger and the kernel faster (1 token over 300 rows 8.2 -> 7.8 us, a tree of 64 over 131072 rows
+//   140 -> 119, two chunks of 512 90 -> 78).
 // Measured (MI355X): 16 sequences, 1 token, 335 MB of rows 56 us (6.0 TB/s) and 5 us for the merge; a tree
 //   of 64 over 131072 rows, 537 MB 104-112 us (4.8-5.1 TB/s) and 13; two chunks of 512 over up to 8192
 //   rows, 45 GFLOP 75 us (600 TFLOP/s, the matrix cores busy 26%, no LDS conflicts: a stage's loads,
@@ -485,10 +501,16 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     const int v_frag = F ? 4 * g * S::ROWB + ((l16 >> 2) ^ (g << 2)) * 16 + (l16 & 3) * 4
                          : v_key * S::ROWB + ((v_key & BMASK) << 5) + 8 * (l16 & 3);
     // acc += V^T . P^T for output rows 16 t..16 t + 15 over the tile's keys (CLEAN: elements of V that
-    // are not finite taken as 0); pk: p as the MFMA takes it
+    // are not finite taken as 0); pk: p as the MFMA takes it, in 16 bits with what is left of it in `rest`
     constexpr uint32_t EXP2 = std::is_same_v<T, BF16> ? 0x7f807f80u : 0x7c007c00u, STEP2 = std::is_same_v<T, BF16> ? 0x00800080u : 0x04000400u;
     constexpr int PK = F ? S::KG : S::KG >= 2 ? S::KG / 2 : 1;
-    auto pv = [&](int v_at, int t, const u32x4 (&pk)[QT][PK], f32x4 (&acc)[QT], auto clean) {
+    // over 32 keys, or the 16 that a tile has
+    auto mfma_keys = [](u32x4 a, u32x4 b, f32x4 acc) {
+        if constexpr (F) return acc;
+        else if constexpr (S::KG >= 2) return mfma_chunk(T{}, a, b, acc);
+        else return mfma_half(T{}, u32x2{a[0], a[1]}, u32x2{b[0], b[1]}, acc);
+    };
+    auto pv = [&](int v_at, int t, const u32x4 (&pk)[QT][PK], const u32x4 (&rest)[QT][PK], f32x4 (&acc)[QT], auto clean) {
         constexpr bool CLEAN = decltype(clean)::value;
         if constexpr (F) {
 #pragma unroll
@@ -522,10 +544,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                     }
                 }
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt) {
-                    if constexpr (S::KG >= 2) acc[qt] = mfma_chunk(T{}, vf, pk[qt][kk], acc[qt]);
-                    else acc[qt] = mfma_half(T{}, u32x2{vf[0], vf[1]}, u32x2{pk[qt][0][0], pk[qt][0][1]}, acc[qt]);
-                }
+                for (int qt = 0; qt < QT; ++qt) acc[qt] = mfma_keys(vf, pk[qt][kk], acc[qt]);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) acc[qt] = mfma_keys(vf, rest[qt][kk], acc[qt]);
             }
         }
     };
@@ -637,7 +658,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                 }
             }
         }
-        u32x4 pk[QT][PK];
+        u32x4 pk[QT][PK], rest[QT][PK];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
@@ -645,8 +666,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                 if constexpr (F) {
                     pk[qt][kk] = __builtin_bit_cast(u32x4, p[qt][kk]);
                 } else {
-                    const f32x4 x = p[qt][S::KG >= 2 ? 2 * kk : 0], y = p[qt][S::KG >= 2 ? 2 * kk + 1 : 0];
-                    pk[qt][kk] = u32x4{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3])};
+#pragma unroll
+                    for (int i = 0; i < (S::KG >= 2 ? 4 : 2); ++i) {
+                        const f32x4 x = p[qt][S::KG >= 2 ? 2 * kk + i / 2 : 0];
+                        uint32_t hi, left;
+                        split2<T>(x[2 * (i & 1)], x[2 * (i & 1) + 1], hi, left);
+                        pk[qt][kk][i] = hi;
+                        rest[qt][kk][i] = left;
+                    }
                 }
             }
 #pragma unroll
@@ -658,10 +685,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         l[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, __uint_as_float(pk[qt][kk][j]), l[qt], 0, 0, 0);
-                } else if constexpr (S::KG >= 2) {
-                    l[qt] = mfma_chunk(T{}, u32x4{ONE2, ONE2, ONE2, ONE2}, pk[qt][kk], l[qt]);
                 } else {
-                    l[qt] = mfma_half(T{}, u32x2{ONE2, ONE2}, u32x2{pk[qt][0][0], pk[qt][0][1]}, l[qt]);
+                    const u32x4 ones = {ONE2, ONE2, ONE2, ONE2};
+                    l[qt] = mfma_keys(ones, rest[qt][kk], mfma_keys(ones, pk[qt][kk], l[qt]));
                 }
             }
         auto product = [&](auto clean) {
@@ -670,11 +696,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                 f32x4 acc[QT];
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt) acc[qt] = o[qt][t];
-                pv(v_at, t, pk, acc, clean);
+                pv(v_at, t, pk, rest, acc, clean);
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt) o[qt][t] = acc[qt];
             }
-            if constexpr (!F && !decltype(clean)::value) interleave<S::DT * S::KG, S::KG, QT * PK, 3 * S::KG>();
+            if constexpr (!F && !decltype(clean)::value) interleave<S::DT * S::KG, S::KG, 2 * QT * PK, 3 * S::KG>();
         };
         if (!NEW || odd == 0) {
             __builtin_amdgcn_s_setprio(1);
