@@ -1,5 +1,5 @@
-"""The numbers of the paged attention on the GPU: the weights' bits and values that are not finite, for every number of
-rows that a workgroup holds."""
+"""The numbers of the paged attention on the GPU: the weights' bits, their tail and values that are not
+finite, each for every number of rows that a workgroup holds."""
 from __future__ import annotations
 
 import math
@@ -22,10 +22,10 @@ WEIGHT = {torch.float32: 0.0, torch.float16: 2.0 ** -21, torch.bfloat16: 2.0 ** 
 def bound(o, av, S, d, n, v_max, dt):
     """The result rounded once, the weights off by WEIGHT each in the product and in their sum, fp32 for the rest:
     a score of d products off by (d + 3) 2^-24 S, an exponential by 2^-22, the sums over n keys by n 2^-24, each in
-    numerator and denominator; and a weight in float16 by 2^-25."""
+    numerator and denominator; and a weight in float16, held 2^14 times as large, by 2^-25 of that unit."""
     tol = HALF_STEP[dt] * o.abs() + WEIGHT[dt] * (av + o.abs()) + 2.0 ** -24 * (2 * (d + 3) * S + 8 + 2 * n) * av
     if dt == torch.float16:
-        tol = tol + 2.0 ** -24 * n * v_max
+        tol = tol + 2.0 ** -25 + 2.0 ** -38 * n * v_max  # (the first: a result among float16's subnormals)
     return 1.01 * tol
 
 
@@ -69,6 +69,27 @@ def test_weights_keep_their_bits(dtype, d, G, T, n):
     sums = torch.nan_to_num(kp.float()).sum(2)
     out, _ = yt.paged_sparse_attention(q, kn, vn, kp, vp, sums, table, kv_len, -(-n // page), parents=parents)
     compare(out[0], want, tol)
+
+
+@pytest.mark.parametrize("n", [200, 6000])
+@pytest.mark.parametrize("G,T", SHAPES)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_the_tail_behind_a_large_weight(dtype, G, T, n):
+    """A key whose score is 17.5 nats above all others', and has no value: what the others bring is not lost,
+    wherever the sequence is cut."""
+    dt, Hkv, page, d = DT[dtype], 1, 16, 64
+    g, kp, vp, table, kv_len = cache(n, [n], Hkv, page, d, dt)
+    q, kn, vn = tokens(g, 1, G, Hkv, T, d, dt)
+    q[:], kn[:], vn[:] = 0.0, 0.0, 0.0
+    q[..., 0] = 10.0
+    kp[:], vp[:] = 0.0, (4096 * (1 + torch.rand(vp.shape, generator=g))).to(dt).cuda()
+    for row in (0, n // 2, n - 1):
+        k, v = kp.clone(), vp.clone()
+        k[table[0, row // page].long(), :, row % page, 0] = 14.0  # 10 * 14 / 8
+        v[table[0, row // page].long(), :, row % page] = 0.0
+        out = yt.paged_attention(q, kn, vn, k, v, table, kv_len)[0]
+        want, tol = formula(q[0], rows_of(k, table[0], n), rows_of(v, table[0], n), kn[0], vn[0], None)
+        compare(out, want, tol)
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])

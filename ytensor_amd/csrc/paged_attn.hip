@@ -484,7 +484,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         return pack;
     };
 
-    float m[QT];
+    // The largest weight in the running reference's unit is 2^UNIT: float16 has no number between 0 and 2^-24, so weights
+    // against a largest of 1 would be lost below 2^-25 of it (and in the ranges that hold it alone); 2^14, the unit that
+    // leaves room above, takes that to 2^-39. L and O have the same unit, so it cancels.
+    constexpr float UNIT = std::is_same_v<T, F16> ? 14.f : 0.f;
+    float m[QT];  // the reference, UNIT below the largest score so far
     f32x4 l[QT];  // ones . P^T: the sum of the weights as the product takes them, from the matrix cores
     f32x4 o[QT][S::DT];
 #pragma unroll
@@ -621,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             for (int kt = 0; kt < S::KG; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = __builtin_elementwise_maximum(mx, p[qt][kt][r]);
-            const float top = __builtin_elementwise_maximum(m[qt], max_across_rows(mx) * c);
+            const float top = __builtin_elementwise_maximum(m[qt], fmaf(max_across_rows(mx), c, -UNIT));
             const float ref = top == -INFINITY ? 0.f : top;  // nothing seen yet: every weight is 0
             const float corr = __builtin_amdgcn_exp2f(m[qt] - ref);
             m[qt] = top;
