@@ -1,5 +1,5 @@
-"""The numbers of the paged attention on the GPU: the weights' bits, their tail and values that are not
-finite, each for every number of rows that a workgroup holds."""
+"""The numbers of the paged attention on the GPU: the weights' bits, their tail, scores far from 0 and
+values that are not finite, each for every number of rows that a workgroup holds."""
 from __future__ import annotations
 
 import math
@@ -90,6 +90,32 @@ def test_the_tail_behind_a_large_weight(dtype, G, T, n):
         out = yt.paged_attention(q, kn, vn, k, v, table, kv_len)[0]
         want, tol = formula(q[0], rows_of(k, table[0], n), rows_of(v, table[0], n), kn[0], vn[0], None)
         compare(out, want, tol)
+
+
+@pytest.mark.parametrize("n", [30, 2500])
+@pytest.mark.parametrize("G,T", SHAPES)
+@pytest.mark.parametrize("dtype,size", [("bf16", 3e4), ("f16", 2e4), ("f32", 1e12)])
+def test_scores_far_from_zero(dtype, size, G, T, n):
+    """Scores whose last bit is worth more than an exponential can hold: equal ones weigh the same, the largest
+    takes all."""
+    dt, Hkv, page, d = DT[dtype], 1, 16, 64
+    g, kp, vp, table, kv_len = cache(n, [n], Hkv, page, d, dt)
+    q, kn, vn = tokens(g, 1, G, Hkv, T, d, dt)
+    side = size * (1 + torch.arange(d) / 100.0)  # no power of two, so that the scaled score is rounded
+    q[:], kn[:], kp[:] = side.to(dt).cuda(), side.to(dt).cuda(), side.to(dt).cuda()
+    for sign in (1.0, -1.0):
+        out = yt.paged_attention(q, kn, vn, kp, vp, table, kv_len, scale=sign / 8)[0].cpu().double()
+        v = rows_of(vp, table[0], n)[0].cpu().double()
+        for t in range(T):
+            all_v = torch.cat([v, vn[0, 0, : t + 1].cpu().double()])
+            mean = all_v.mean(0)
+            tol = bound(mean, all_v.abs().mean(0), 0.0, d, len(all_v), all_v.abs().max(), dt)
+            assert ((out[:, t] - mean).abs() <= tol).all(), (sign, t)
+    row = n // 3
+    kp[table[0, row // page].long(), :, row % page] *= 1.25
+    out = yt.paged_attention(q, kn, vn, kp, vp, table, kv_len)[0]
+    one = rows_of(vp, table[0], n)[0, row]
+    assert (out == one).all()
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])

@@ -488,7 +488,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     // against a largest of 1 would be lost below 2^-25 of it (and in the ranges that hold it alone); 2^14, the unit that
     // leaves room above, takes that to 2^-39. L and O have the same unit, so it cancels.
     constexpr float UNIT = std::is_same_v<T, F16> ? 14.f : 0.f;
-    float m[QT];  // the reference, UNIT below the largest score so far
+    float m[QT];  // the largest score so far, before the scale
     f32x4 l[QT];  // ones . P^T: the sum of the weights as the product takes them, from the matrix cores
     f32x4 o[QT][S::DT];
 #pragma unroll
@@ -625,15 +625,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             for (int kt = 0; kt < S::KG; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = __builtin_elementwise_maximum(mx, p[qt][kt][r]);
-            const float top = __builtin_elementwise_maximum(m[qt], fmaf(max_across_rows(mx), c, -UNIT));
+            const float top = __builtin_elementwise_maximum(m[qt], max_across_rows(mx));
             const float ref = top == -INFINITY ? 0.f : top;  // nothing seen yet: every weight is 0
-            const float corr = __builtin_amdgcn_exp2f(m[qt] - ref);
+            const float corr = __builtin_amdgcn_exp2f((m[qt] - ref) * c);
             m[qt] = top;
 #pragma unroll
             for (int kt = 0; kt < S::KG; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    p[qt][kt][r] = __builtin_amdgcn_exp2f(fmaf(p[qt][kt][r], c, -ref));
+                    // the difference first: scaled, the largest score is rounded, by more than an exponent can hold
+                    // where it is beyond 2^31
+                    p[qt][kt][r] = __builtin_amdgcn_exp2f(fmaf(p[qt][kt][r] - ref, c, UNIT));
                 }
             l[qt] *= corr;
             if (__ballot(corr != 1.0f) != 0) {
@@ -789,6 +791,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     }
     for (int s = 0; s < s_new; ++s) step(s, std::true_type{});
     for (int s = s_new; s < nst; ++s) step(s, std::false_type{});
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) m[qt] *= c;
     // the place of row r's result: O itself, or this item's partial
     auto store4 = [&](int r, int d, f32x4 v, float M, float L) {
         const int t = SPARSE ? t_one : r / a.G, gh = SPARSE ? r : r - t * a.G;
