@@ -502,7 +502,7 @@ int ythip_rope_tables(int dim, int max_len, float theta, float* cosv, float* sin
  *            from 16 to 32768. Several layers: [layers][pages]...
  *   key sums fp32 [pages][Hkv][d], a page's K rows in use added up (sparse attention's scores)
  *   table    int32 [B][columns], row stride ld_table: row r of sequence b lies in page
- *            table[b][r / page] at r % page. An id outside [0, pages) is never an address: its
+ *            table[b][r / page] at r % page; behind the pages of its rows it may hold anything. An id outside [0, pages) is never an address: its
  *            rows are hidden (attention) or not written (append)
  *            At most 65536 columns, 2^30 rows a sequence and 2^34 rows (B * columns * page)
  *   kv_len   int32 [B], rows in use (clamped to [0, columns * page])
@@ -566,12 +566,23 @@ int ythip_paged_attn_sparse(int dtype, int B, int Hq, int Hkv, int T, int d, con
  * rows in use, anew. Strides: new_str of both Kn and Vn (layer, batch, head, token), pool_str
  * (layer, page, head, row). d * element size a multiple of 16, at most 4096. No two sequences
  * may write one page (ythip_cache_fork sees to that).
+ * The rows go where the table says: after a grow that may refuse a sequence (no free page) take
+ * ythip_cache_append_to, which is given the lengths that the grow wrote, new_len (device
+ * int32[B]), in place of n_new: sequence b takes rows kv_len[b] up to new_len[b], none where
+ * it was refused, whatever the table holds behind its pages. Rows past the T that are given are
+ * zeros. `status` (NULL: none) gets YTHIP_CACHE_ERR_INDEX for a length that is negative, past
+ * the table, below kv_len or more than T above it, and for a page id outside the pool.
  */
 int ythip_cache_append(int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn,
                        const int64_t new_str[4], void* Kp, void* Vp, const int64_t pool_str[4], int pages, int page,
                        float* sums, const int64_t sums_str[3], const int32_t* table, int64_t ld_table, int columns,
                        const int32_t* kv_len, const int32_t* n_new, const int32_t* path, int64_t ld_path,
                        void* stream);
+int ythip_cache_append_to(int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn,
+                          const int64_t new_str[4], void* Kp, void* Vp, const int64_t pool_str[4], int pages, int page,
+                          float* sums, const int64_t sums_str[3], const int32_t* table, int64_t ld_table, int columns,
+                          const int32_t* kv_len, const int32_t* new_len, const int32_t* path, int64_t ld_path,
+                          int32_t* status, void* stream);
 
 /*
  * The page bookkeeping: each call reads (ref, table, len) and writes (ref_out, table_out,

@@ -1,0 +1,122 @@
+"""The paged cache's calls as a server makes them, on the GPU: a pool that runs full."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import ytensor_amd as yt
+from paged_ref import Pages
+from test_gpu_paged import DT, ints
+
+pytestmark = pytest.mark.gpu
+
+
+def pools_of(g, L, P, Hkv, page, d, dt):
+    k, v = (torch.randn(L, P, Hkv, page, d, generator=g).to(dt).cuda() for _ in range(2))
+    return k, v, torch.randn(L, P, Hkv, d, generator=g).cuda()
+
+
+def expect(pools, kn, vn, table, old, new, path=None):
+    """What the append has to leave: the pools and, of each page written to, the sums (others as they were)."""
+    k, v, sums = (x.cpu().clone() for x in pools)
+    page, T, tol = k.shape[3], kn.shape[3], torch.zeros_like(sums, dtype=torch.float64)
+    sums, table = sums.double(), torch.as_tensor(table)
+    for b, (lo, hi) in enumerate(zip(old, new)):
+        for i in range(hi - lo):
+            f = -1 if i >= T else i if path is None else int(path[b, i])
+            p, r = int(table[b, (lo + i) // page]), (lo + i) % page
+            for pool, rows in ((k, kn), (v, vn)):
+                pool[:, p, :, r] = rows[:, b, :, f].cpu() if 0 <= f < T else 0.0
+        for c in range(lo // page, -(-hi // page) if hi > lo else 0):
+            p, r = int(table[b, c]), min(page, hi - c * page)
+            sums[:, p] = k[:, p, :, :r].double().sum(2)
+            tol[:, p] = r * 2.0 ** -24 * k[:, p, :, :r].double().abs().sum(2)
+    return k, v, sums, tol
+
+
+def same(pools, want):
+    assert torch.equal(pools[0].cpu(), want[0]) and torch.equal(pools[1].cpu(), want[1])
+    assert ((pools[2].cpu().double() - want[2]).abs() <= want[3]).all()
+
+
+@pytest.mark.parametrize("why", ["pool", "columns", "count"])
+@pytest.mark.parametrize("dtype,page,d", [("bf16", 16, 64), ("f32", 64, 128), ("f16", 1024, 64)])
+def test_append_after_a_refused_grow(dtype, page, d, why):
+    """A sequence that the grow refuses keeps its rows, its pages' sums and its length, and no other sequence's page is
+    touched, whatever ids stand behind its pages in the table."""
+    dt, L, Hkv, T, columns = DT[dtype], 2, 2, page + 3, 4
+    lens = [page + 5, 2 * page - 1, 3, 3 * page + 1, 0]
+    n_new = [T, 1, T, page + 2 if why == "columns" else 2, 0]
+    if why == "count":
+        n_new[0] = -1
+    need = [-(-n // page) for n in lens]
+    P = sum(need) + (1 if why == "pool" else 9)
+    g = torch.Generator().manual_seed(page)
+    perm = torch.randperm(P, generator=g).tolist()
+    used = perm[: sum(need)]
+    table = torch.tensor(used)[torch.randint(0, len(used), (5, columns), generator=g)].int()  # live ids everywhere
+    ref, at = torch.zeros(P, dtype=torch.int32), 0
+    for b, n in enumerate(need):
+        for c in range(n):
+            table[b, c], ref[used[at]] = used[at], 1
+            at += 1
+    m = Pages(ref, table, torch.tensor(lens), page)
+    m.grow(n_new)
+    assert m.status == (yt.CACHE_ERR_INDEX if why == "count" else yt.CACHE_ERR_FULL)
+    pools = pools_of(g, L, P, Hkv, page, d, dt)
+    kn, vn = (torch.randn(L, 5, Hkv, T, d, generator=g).to(dt).cuda() for _ in range(2))
+    want = expect(pools, kn, vn, m.table, lens, m.len)
+    ref, table, old, status = ref.cuda(), table.cuda(), ints(lens), ints([0])
+    new = torch.empty_like(old)
+    yt.cache_grow(ref, table, old, ints(n_new), page, out=(ref, table, new), status=status)
+    assert new.tolist() == m.len and table.tolist() == m.table
+    yt.cache_append(kn, vn, *pools[:2], table, old, key_sums=pools[2], new_len=new, status=status)
+    same(pools, want)
+    assert status.item() == m.status
+
+
+@pytest.mark.parametrize("page,T", [(16, 5), (16, 40), (128, 3)])
+def test_append_of_more_rows_than_there_are(page, T):
+    """Lengths that grew by more than the rows at hand: the rest are zeros, no row comes into use unwritten."""
+    L, Hkv, d, lens = 2, 1, 64, [0, 7, page, 2 * page - 1]
+    new = [T + 1, 7 + T + 3 * page, page + T, 2 * page - 1 + 4 * page]
+    g = torch.Generator().manual_seed(T)
+    columns = max(-(-n // page) for n in new)
+    P = 4 * columns
+    table = torch.randperm(P, generator=g).view(4, columns).int()
+    pools = pools_of(g, L, P, Hkv, page, d, torch.bfloat16)
+    kn, vn = (torch.randn(L, 4, Hkv, T, d, generator=g).bfloat16().cuda() for _ in range(2))
+    path = torch.stack([torch.randperm(T, generator=g) for _ in lens]).int()
+    path[2, 0] = T + 3
+    want = expect(pools, kn, vn, table, lens, new, path)
+    status = ints([0])
+    yt.cache_append(kn, vn, *pools[:2], table.cuda(), ints(lens), path=path.cuda(), key_sums=pools[2], new_len=ints(new),
+                    status=status)
+    same(pools, want)
+    assert status.item() == yt.CACHE_ERR_INDEX
+
+
+def test_append_flags_what_it_leaves_out():
+    """Lengths that shrank, pages outside the pool and rows past the table are left out and flagged; nothing else is."""
+    g = torch.Generator().manual_seed(0)
+    kn, vn = (torch.randn(1, 2, 1, 20, 64, generator=g).cuda() for _ in range(2))
+    for table, old, new, bits, pages in (
+            ([[0, 1], [2, 3]], [3, 0], [5, 4], 0, [0, 2]), ([[0, 1], [2, 3]], [3, 0], [2, 0], 1, []),
+            ([[0, -1], [2, 3]], [10, 0], [20, 0], 1, [0]), ([[0, 1], [4, 3]], [0, 10], [0, 20], 1, [3]),
+            ([[0, 1], [2, 3]], [30, 0], [33, 0], 1, [1]), ([[0, 1], [2, 3]], [-4, 0], [-4, 2], 0, [2]),
+            ([[0, 1], [2, 3]], [-4, 0], [3, 2], 1, [2])):
+        k, v = torch.zeros(1, 4, 1, 16, 64, device="cuda"), torch.zeros(1, 4, 1, 16, 64, device="cuda")
+        status = ints([0])
+        yt.cache_append(kn, vn, k, v, ints(table), ints(old), new_len=ints(new), status=status)
+        assert status.item() == bits, (table, old, new)
+        for pool in (k, v):
+            assert (pool[0] != 0).flatten(1).any(1).nonzero().flatten().tolist() == pages, (table, old, new)
+
+
+def test_append_takes_one_count():
+    kn, kp = torch.zeros(1, 1, 1, 2, 64, device="cuda"), torch.zeros(1, 2, 1, 16, 64, device="cuda")
+    args = (kn, kn, kp, kp.clone(), ints([[0]]), ints([0]))
+    for bad in (dict(n_new=ints([1]), new_len=ints([1])), dict(n_new=ints([1]), status=ints([0])),
+                dict(new_len=ints([1, 2])), dict(new_len=ints([1]).long()), dict(new_len=ints([1]), status=ints([0, 0]))):
+        with pytest.raises(ValueError):
+            yt.cache_append(*args, **bad)

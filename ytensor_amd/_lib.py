@@ -102,6 +102,8 @@ SIGNATURES = {
                                      _P, _L, _I, _P, _P, _L, _P, _I, _P, _P, _LP, _F, _P, ctypes.c_size_t, _P]),
     "ythip_cache_append": (_I, [_I, _I, _I, _I, _I, _I, _P, _P, _LP, _P, _P, _LP, _I, _I, _P, _LP, _P, _L, _I, _P, _P,
                                 _P, _L, _P]),
+    "ythip_cache_append_to": (_I, [_I, _I, _I, _I, _I, _I, _P, _P, _LP, _P, _P, _LP, _I, _I, _P, _LP, _P, _L, _I, _P,
+                                   _P, _P, _L, _P, _P]),
     "ythip_cache_grow": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _P, _P, _P, _L, _P, _P, _P]),
     "ythip_cache_fork_workspace_size": (ctypes.c_size_t, [_I]),
     "ythip_cache_fork": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _I, _P, _P, _P, _P, _L, _P, _I, _I, _P, _P, _P,

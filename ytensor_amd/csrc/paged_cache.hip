@@ -454,9 +454,11 @@ struct AppendArgs {
     int64_t ps0, ps1, ps2, ps3;
     float* sums;
     int64_t ss0, ss1, ss2;  // elements
-    const int32_t *table, *kv_len, *n_new, *path;
+    const int32_t *table, *kv_len, *count, *path;
     int64_t ld_table, ld_path;
     int chunks;  // 16-byte chunks of a row
+    bool to;     // count: the lengths afterwards, not the new rows
+    int32_t* status;
 };
 // A workgroup of NW waves takes one page that the new rows of one (layer, sequence, KV head)
 // touch: thread = (row group, 16-byte chunk), so that a row moves as one run of bytes. It adds
@@ -465,6 +467,8 @@ struct AppendArgs {
 // the page's rows alone. Bound by the latency of the lengths, the table and the rows in turn, so
 // a page of up to 64 rows is one wave and all pages of a step are in flight at once
 // (16 sequences, 28 layers, 45 MB: 18.3 us; with four waves a page 20.8).
+// Where the lengths afterwards are given, a sequence that its grow refused has none to write, and rows that are in
+// use but not among the T given are zeros (a workgroup then takes every slots-th page: the grid counts T rows).
 template <class T, int NW>
 __global__ __launch_bounds__(64 * NW) void cache_append_kernel(AppendArgs a) {
     constexpr int VN = Vec<T>::n, AHEAD = 8;
@@ -476,84 +480,94 @@ __global__ __launch_bounds__(64 * NW) void cache_append_kernel(AppendArgs a) {
     w /= a.Hkv;
     const int b = w % a.B, l = w / a.B;
     const int page = 1 << a.shift;
-    const int len = a.kv_len[b];
-    const int n = a.n_new != nullptr ? min(a.n_new[b], a.T) : a.T;
-    if (len < 0 || n <= 0) return;
-    const int slot = (len >> a.shift) + i;
-    const int64_t end = (int64_t)len + n;  // rows in use afterwards
-    if (slot >= a.columns || ((int64_t)slot << a.shift) >= end) return;
-    const int p = a.table[b * a.ld_table + slot];
-    if (p < 0 || p >= a.pages) return;
-    const int r0 = slot << a.shift;                                           // the page's first row
-    const int lo = max(len - r0, 0), hi = (int)min(end - r0, (int64_t)page);  // its new rows
-    const int groups = 64 * NW / a.chunks;                                    // rows at a time
+    const int len = a.kv_len[b], count = a.count != nullptr ? a.count[b] : a.T;
+    const int64_t end = a.to ? count : (int64_t)len + min(count, a.T);  // rows in use afterwards
+    const bool tells = a.to && l == 0 && h == 0 && threadIdx.x == 0;
+    if (tells && i == 0 && end != len && (len < 0 || end < len || end - len > a.T || end > (int64_t)a.columns << a.shift))
+        flag(a.status, YTHIP_CACHE_ERR_INDEX);
+    if (len < 0 || end <= len) return;
+    const int groups = 64 * NW / a.chunks;  // rows at a time
     const int rg = (int)threadIdx.x / a.chunks, ch = (int)threadIdx.x % a.chunks;
     const bool works = rg < groups;
-    char* kp = a.Kp + l * a.ps0 + p * a.ps1 + h * a.ps2 + ch * 16;
-    char* vp = a.Vp + l * a.ps0 + p * a.ps1 + h * a.ps2 + ch * 16;
     const char* kn = a.Kn + l * a.ns0 + b * a.ns1 + h * a.ns2 + ch * 16;
     const char* vn = a.Vn + l * a.ns0 + b * a.ns1 + h * a.ns2 + ch * 16;
-    float acc[VN];
-#pragma unroll
-    for (int e = 0; e < VN; ++e) acc[e] = 0.f;
-    auto add = [&](u32x4 v) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (VN == 4) acc[e] += __uint_as_float(v[e]);
-            else {
-                acc[2 * e] += lo_as_f32(T{}, v[e]);
-                acc[2 * e + 1] += hi_as_f32(T{}, v[e]);
-            }
+    for (int slot = (len >> a.shift) + i; slot < a.columns && ((int64_t)slot << a.shift) < end; slot += a.slots) {
+        const int p = a.table[b * a.ld_table + slot];
+        if (p < 0 || p >= a.pages) {
+            if (tells) flag(a.status, YTHIP_CACHE_ERR_INDEX);
+            continue;
         }
-    };
-    // AHEAD rows of a thread at a time: all their loads before the first use, without a branch around
-    // them (past the end: the last row again, dropped)
-    if (a.sums != nullptr && works && rg < lo)
-        for (int r = rg; r < lo; r += AHEAD * groups) {
-            u32x4 k[AHEAD];
+        const int r0 = slot << a.shift;                                           // the page's first row
+        const int lo = max(len - r0, 0), all = (int)min(end - r0, (int64_t)page);  // its new rows
+        const int hi = (int)min((int64_t)len + a.T - r0, (int64_t)all);            // those that are given
+        char* kp = a.Kp + l * a.ps0 + p * a.ps1 + h * a.ps2 + ch * 16;
+        char* vp = a.Vp + l * a.ps0 + p * a.ps1 + h * a.ps2 + ch * 16;
+        float acc[VN];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) k[u] = *reinterpret_cast<const u32x4*>(kp + min(r + u * groups, lo - 1) * a.ps3);
+        for (int e = 0; e < VN; ++e) acc[e] = 0.f;
+        auto add = [&](u32x4 v) {
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
-                if (r + u * groups < lo) add(k[u]);
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (VN == 4) acc[e] += __uint_as_float(v[e]);
+                else {
+                    acc[2 * e] += lo_as_f32(T{}, v[e]);
+                    acc[2 * e + 1] += hi_as_f32(T{}, v[e]);
+                }
+            }
+        };
+        // AHEAD rows of a thread at a time: all their loads before the first use, without a branch around
+        // them (past the end: the last row again, dropped)
+        if (a.sums != nullptr && works && rg < lo)
+            for (int r = rg; r < lo; r += AHEAD * groups) {
+                u32x4 k[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) k[u] = *reinterpret_cast<const u32x4*>(kp + min(r + u * groups, lo - 1) * a.ps3);
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+                    if (r + u * groups < lo) add(k[u]);
+            }
+        if (works)
+            for (int r = lo + (rg - lo % groups + groups) % groups; r < hi; r += AHEAD * groups) {
+                u32x4 k[AHEAD], v[AHEAD];
+                int from[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int j = r0 + min(r + u * groups, hi - 1) - len;
+                    from[u] = a.path != nullptr ? a.path[b * a.ld_path + j] : j;
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const bool is = from[u] >= 0 && from[u] < a.T;
+                    k[u] = *reinterpret_cast<const u32x4*>(kn + (is ? from[u] : 0) * a.ns3);
+                    v[u] = *reinterpret_cast<const u32x4*>(vn + (is ? from[u] : 0) * a.ns3);
+                    if (!is) k[u] = v[u] = u32x4{0u, 0u, 0u, 0u};
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int row = r + u * groups;
+                    if (row >= hi) break;
+                    *reinterpret_cast<u32x4*>(kp + row * a.ps3) = k[u];
+                    *reinterpret_cast<u32x4*>(vp + row * a.ps3) = v[u];
+                    if (a.sums != nullptr) add(k[u]);
+                }
+            }
+        if (works && hi < all)
+            for (int r = max(lo, hi) + rg; r < all; r += groups)
+                *reinterpret_cast<u32x4*>(kp + r * a.ps3) = *reinterpret_cast<u32x4*>(vp + r * a.ps3) = u32x4{0u, 0u, 0u, 0u};
+        if (a.sums == nullptr) continue;
+        const int d = a.chunks * VN;
+        __syncthreads();  // the last page's sums are read
+        if (works) {
+#pragma unroll
+            for (int e = 0; e < VN; ++e) s_sum[rg * d + ch * VN + e] = acc[e];
         }
-    if (works)
-        for (int r = lo + (rg - lo % groups + groups) % groups; r < hi; r += AHEAD * groups) {
-            u32x4 k[AHEAD], v[AHEAD];
-            int from[AHEAD];
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int j = r0 + min(r + u * groups, hi - 1) - len;
-                from[u] = a.path != nullptr ? a.path[b * a.ld_path + j] : j;
-            }
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const bool is = from[u] >= 0 && from[u] < a.T;
-                k[u] = *reinterpret_cast<const u32x4*>(kn + (is ? from[u] : 0) * a.ns3);
-                v[u] = *reinterpret_cast<const u32x4*>(vn + (is ? from[u] : 0) * a.ns3);
-                if (!is) k[u] = v[u] = u32x4{0u, 0u, 0u, 0u};
-            }
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int row = r + u * groups;
-                if (row >= hi) break;
-                *reinterpret_cast<u32x4*>(kp + row * a.ps3) = k[u];
-                *reinterpret_cast<u32x4*>(vp + row * a.ps3) = v[u];
-                if (a.sums != nullptr) add(k[u]);
-            }
+        __syncthreads();
+        float* out = a.sums + l * a.ss0 + p * a.ss1 + h * a.ss2;
+        for (int e = threadIdx.x; e < d; e += 64 * NW) {
+            float t = 0.f;
+            for (int g = 0; g < groups; ++g) t += s_sum[g * d + e];
+            out[e] = t;
         }
-    if (a.sums == nullptr) return;
-    const int d = a.chunks * VN;
-    if (works) {
-#pragma unroll
-        for (int e = 0; e < VN; ++e) s_sum[rg * d + ch * VN + e] = acc[e];
-    }
-    __syncthreads();
-    float* out = a.sums + l * a.ss0 + p * a.ss1 + h * a.ss2;
-    for (int e = threadIdx.x; e < d; e += 64 * NW) {
-        float t = 0.f;
-        for (int g = 0; g < groups; ++g) t += s_sum[g * d + e];
-        out[e] = t;
     }
 }
 
@@ -626,19 +640,10 @@ StateArgs copy_state(StateArgs a, bool alone, hipStream_t s) {
     return a;
 }
 
-}  // namespace
-}  // namespace ythip
-
-using namespace ythip;
-
-extern "C" {
-
-__attribute__((visibility("default"))) int ythip_cache_append(
-    int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn, const int64_t new_str[4],
-    void* Kp, void* Vp, const int64_t pool_str[4], int pages, int page, float* sums, const int64_t sums_str[3],
-    const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len, const int32_t* n_new,
-    const int32_t* path, int64_t ld_path, void* stream) {
-    const char* who = "ythip_cache_append";
+int append(const char* who, int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn,
+           const int64_t* new_str, void* Kp, void* Vp, const int64_t* pool_str, int pages, int page, float* sums,
+           const int64_t* sums_str, const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len,
+           const int32_t* count, bool to, const int32_t* path, int64_t ld_path, int32_t* status, void* stream) {
     if (dtype != YTHIP_F32 && dtype != YTHIP_F16 && dtype != YTHIP_BF16) return fail(YTHIP_EINVAL, "%s: invalid dtype %d", who, dtype);
     if (layers < 0 || B < 0 || Hkv < 0 || T < 0 || d <= 0) return fail(YTHIP_EINVAL, "%s: bad size", who);
     if (const int st = check_table(who, B, columns, pages, page, table, ld_table, kv_len)) return st;
@@ -659,7 +664,8 @@ __attribute__((visibility("default"))) int ythip_cache_append(
     a.ps0 = pool_str[0] * es, a.ps1 = pool_str[1] * es, a.ps2 = pool_str[2] * es, a.ps3 = pool_str[3] * es;
     a.sums = sums;
     a.ss0 = sums ? sums_str[0] : 0, a.ss1 = sums ? sums_str[1] : 0, a.ss2 = sums ? sums_str[2] : 0;
-    a.table = table, a.kv_len = kv_len, a.n_new = n_new, a.path = path, a.ld_table = ld_table, a.ld_path = ld_path;
+    a.table = table, a.kv_len = kv_len, a.count = count, a.path = path, a.ld_table = ld_table, a.ld_path = ld_path;
+    a.to = to, a.status = status;
     a.chunks = (int)((int64_t)d * es / 16);
     const int64_t grid = (int64_t)a.slots * Hkv * B * layers;
     if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pages to write", who, (long long)grid);
@@ -675,6 +681,32 @@ __attribute__((visibility("default"))) int ythip_cache_append(
     else if (dtype == YTHIP_F16) run(F16{});
     else run(BF16{});
     return status_of(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace ythip
+
+using namespace ythip;
+
+extern "C" {
+
+__attribute__((visibility("default"))) int ythip_cache_append(
+    int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn, const int64_t new_str[4],
+    void* Kp, void* Vp, const int64_t pool_str[4], int pages, int page, float* sums, const int64_t sums_str[3],
+    const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len, const int32_t* n_new,
+    const int32_t* path, int64_t ld_path, void* stream) {
+    return append("ythip_cache_append", dtype, layers, B, Hkv, T, d, Kn, Vn, new_str, Kp, Vp, pool_str, pages, page, sums,
+                  sums_str, table, ld_table, columns, kv_len, n_new, false, path, ld_path, nullptr, stream);
+}
+
+__attribute__((visibility("default"))) int ythip_cache_append_to(
+    int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn, const int64_t new_str[4],
+    void* Kp, void* Vp, const int64_t pool_str[4], int pages, int page, float* sums, const int64_t sums_str[3],
+    const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len, const int32_t* new_len,
+    const int32_t* path, int64_t ld_path, int32_t* status, void* stream) {
+    if (B > 0 && new_len == nullptr) return fail(YTHIP_EINVAL, "ythip_cache_append_to: new_len is NULL");
+    return append("ythip_cache_append_to", dtype, layers, B, Hkv, T, d, Kn, Vn, new_str, Kp, Vp, pool_str, pages, page, sums,
+                  sums_str, table, ld_table, columns, kv_len, new_len, true, path, ld_path, status, stream);
 }
 
 __attribute__((visibility("default"))) int ythip_cache_grow(int B, int columns, int pages, int page, const int32_t* ref,

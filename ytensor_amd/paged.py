@@ -271,7 +271,7 @@ def cache_grow(ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, n_n
     """Pages (lowest free first) for n_new[b] more rows of each sequence, and the new lengths.
     A sequence that finds too few pages or columns keeps what it has (status). out: (ref,
     table, kv_len) to write instead of the given ones. Returns those written. cache_append
-    takes the kv_len from before."""
+    takes the kv_len from before and these new ones."""
     away = _away(_device(ref, table, kv_len, n_new, status, *(out or ())))
     if away is not None:
         with away:
@@ -287,15 +287,24 @@ def cache_grow(ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, n_n
 
 def cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                  table: torch.Tensor, kv_len: torch.Tensor, n_new: torch.Tensor | None = None,
-                 path: torch.Tensor | None = None, key_sums: torch.Tensor | None = None) -> None:
+                 path: torch.Tensor | None = None, key_sums: torch.Tensor | None = None,
+                 new_len: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
     """Cached row kv_len[b] + i of sequence b takes row path[b, i] (None: i) of k_new / v_new
-    [L, B, Hkv, T, d], for i < n_new[b] (None: T) and every layer; pools [L, P, Hkv, page, d].
-    A path entry outside [0, T) writes zeros. table holds the pages already (cache_grow),
-    kv_len is the length before. key_sums [L, P, Hkv, d]: the sums of the pages written to."""
-    away = _away(_device(k_new, v_new, k_pool, v_pool, table, kv_len, n_new, path, key_sums))
+    [L, B, Hkv, T, d], for every layer; pools [L, P, Hkv, page, d]. A path entry outside [0, T)
+    writes zeros. key_sums [L, P, Hkv, d]: the sums of the pages written to.
+
+    kv_len is the length before, table holds the pages already (cache_grow). new_len: the
+    lengths that cache_grow wrote; a sequence that it refused gets no row, rows past the T given
+    are zeros, and lengths or page ids that cannot be set CACHE_ERR_INDEX in `status`. Without
+    new_len i < n_new[b] (None: T), each of which must have its page in the table."""
+    away = _away(_device(k_new, v_new, k_pool, v_pool, table, kv_len, n_new, path, key_sums, new_len, status))
     if away is not None:
         with away:
-            return cache_append(k_new, v_new, k_pool, v_pool, table, kv_len, n_new, path, key_sums)
+            return cache_append(k_new, v_new, k_pool, v_pool, table, kv_len, n_new, path, key_sums, new_len, status)
+    if new_len is None and status is not None:
+        raise ValueError("status goes with new_len")
+    if new_len is not None and n_new is not None:
+        raise ValueError("n_new and new_len both say how many rows there are: give one")
     if k_new.dim() != 5 or k_pool.dim() != 5:
         raise ValueError("k_new must be [L, B, Hkv, T, d] and the pools [L, P, Hkv, page, d]")
     L, B, Hkv, T, d = k_new.shape
@@ -317,18 +326,28 @@ def cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
     kv_len = _packed(_ints("kv_len", kv_len, (B,)))
     if n_new is not None:
         n_new = _packed(_ints("n_new", n_new, (B,)))
+    if new_len is not None:
+        new_len = _packed(_ints("new_len", new_len, (B,)))
+    if status is not None:
+        _ints("status", status, (1,))
     if path is not None:
         path = _packed(_ints("path", path, (B, T)))
     if key_sums is not None and (key_sums.dtype != torch.float32 or key_sums.shape != (L, P, Hkv, d)
                                  or key_sums.stride(3) != 1):
         raise ValueError(f"key_sums must be float32 {[L, P, Hkv, d]} with d contiguous")
-    st = _lib.lib().ythip_cache_append(
-        _code(k_new), L, B, Hkv, T, d, k_at, v_at, _i64(new_st), k_pool.data_ptr(), v_pool.data_ptr(),
-        _i64(k_pool.stride()), P, page, None if key_sums is None else key_sums.data_ptr(),
-        None if key_sums is None else _i64(key_sums.stride()), table.data_ptr(), ld, columns, kv_len.data_ptr(),
-        None if n_new is None else n_new.data_ptr(), None if path is None else path.data_ptr(), T, _stream())
+    head = (_code(k_new), L, B, Hkv, T, d, k_at, v_at, _i64(new_st), k_pool.data_ptr(), v_pool.data_ptr(),
+            _i64(k_pool.stride()), P, page, None if key_sums is None else key_sums.data_ptr(),
+            None if key_sums is None else _i64(key_sums.stride()), table.data_ptr(), ld, columns, kv_len.data_ptr())
+    path_at = None if path is None else path.data_ptr()
+    if new_len is None:
+        st = _lib.lib().ythip_cache_append(*head, None if n_new is None else n_new.data_ptr(), path_at, T, _stream())
+        if st:
+            check(st, "ythip_cache_append")
+        return
+    st = _lib.lib().ythip_cache_append_to(*head, new_len.data_ptr(), path_at, T,
+                                          None if status is None else status.data_ptr(), _stream())
     if st:
-        check(st, "ythip_cache_append")
+        check(st, "ythip_cache_append_to")
 
 
 def cache_fork(pools, ref: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor, src: torch.Tensor,
