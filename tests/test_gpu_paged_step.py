@@ -1,12 +1,13 @@
-"""The paged cache's calls as a server makes them, on the GPU: a pool that runs full."""
+"""The paged cache's calls as a server makes them, on the GPU: a pool that runs full, the documented step captured and
+replayed."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 import ytensor_amd as yt
-from paged_ref import Pages
-from test_gpu_paged import DT, ints
+from paged_ref import Pages, attention
+from test_gpu_paged import DT, compare, ints, tree
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +121,81 @@ def test_append_takes_one_count():
                 dict(new_len=ints([1, 2])), dict(new_len=ints([1]).long()), dict(new_len=ints([1]), status=ints([0, 0]))):
         with pytest.raises(ValueError):
             yt.cache_append(*args, **bad)
+
+
+@pytest.mark.parametrize("full", [False, True])
+def test_the_documented_step_replayed(full):
+    """The step as the integration notes give it, captured once: every replay adds its rows behind those of the one
+    before, no page is lost, and a pool that runs full leaves the sequences as they were."""
+    dt, L, B, Hq, Hkv, d, page, columns, T = torch.bfloat16, 2, 3, 4, 2, 64, 16, 8, 6
+    P = 7 if full else 40
+    g = torch.Generator().manual_seed(3)
+    k_pool, v_pool, key_sums = pools_of(g, L, P, Hkv, page, d, dt)
+    ref, status = torch.zeros(P, dtype=torch.int32, device="cuda"), ints([0])
+    table, kv_len = torch.randint(0, P, (B, columns), generator=g).int().cuda(), ints([0] * B)
+    old = torch.empty_like(kv_len)
+    q = torch.empty(B, Hq, T, d, dtype=dt, device="cuda")
+    k_all, v_all = (torch.empty(L, B, Hkv, T, d, dtype=dt, device="cuda") for _ in range(2))
+    parents, path = torch.empty(B, T, dtype=torch.int32, device="cuda"), torch.empty(B, T, dtype=torch.int32, device="cuda")
+    n_new, tree_len = ints([0] * B), ints([T] * B)
+    rows = [[torch.zeros(L, Hkv, 0, d, dtype=dt) for _ in range(2)] for _ in range(B)]
+    held = {}
+
+    def fill(i):
+        for t in (q, k_all, v_all):
+            t.copy_(torch.randn(t.shape, generator=g).to(dt))
+        parents.copy_(tree(g, B, T))
+        path.copy_(torch.stack([torch.randperm(T, generator=g) for _ in range(B)]).int())
+        n_new.copy_(torch.tensor([1 + (i + b) % T for b in range(B)], dtype=torch.int32))
+
+    def step():
+        held["o"] = [yt.paged_attention(q, k_all[l], v_all[l], k_pool[l], v_pool[l], table, kv_len, parents=parents,
+                                        tree_len=tree_len) for l in range(L)]
+        old.copy_(kv_len)
+        yt.cache_grow(ref, table, kv_len, n_new, page, status=status)
+        yt.cache_append(k_all, v_all, k_pool, v_pool, table, old, new_len=kv_len, path=path, key_sums=key_sums,
+                        status=status)
+
+    fill(0)
+    keep = [x.clone() for x in (k_pool, v_pool, key_sums, ref, table, kv_len)]
+    step()  # what the first calls set up is there before the capture
+    for x, was in zip((k_pool, v_pool, key_sums, ref, table, kv_len), keep):
+        x.copy_(was)
+    status.zero_()
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    m = Pages(ref, table, kv_len, page)
+    for i in range(12):
+        fill(i)
+        before = list(m.len)
+        torch.randn(1 << 20, device="cuda").sum().item()
+        graph.replay()
+        torch.cuda.synchronize()
+        longest = max(max(before), 1)
+        flat = [torch.zeros(B, Hkv, 256, d, dtype=dt) for _ in range(2)]
+        for l in range(L):
+            for b in range(B):
+                for x in range(2):
+                    flat[x][b, :, : before[b]] = rows[b][x][l]
+            want, tol = attention(q, k_all[l], v_all[l], *flat, ints([[b] for b in range(B)]), ints(before), parents)
+            compare(held["o"][l], want, tol)
+        assert longest <= 256
+        m.grow(n_new.tolist())
+        for b in range(B):
+            at = path[b, : m.len[b] - before[b]].tolist()
+            for x, new in enumerate((k_all, v_all)):
+                rows[b][x] = torch.cat([rows[b][x], new[:, b, :, at].cpu()], 2)
+        assert kv_len.tolist() == m.len and ref.tolist() == m.ref and table.tolist() == m.table
+        assert status.item() == m.status and sum(m.ref) == sum(m.pages(n) for n in m.len)
+        for b in range(B):
+            for c in range(m.pages(m.len[b])):
+                p, r = m.table[b][c], min(page, m.len[b] - c * page)
+                mine = rows[b][0][:, :, c * page: c * page + r]
+                assert torch.equal(k_pool[:, p, :, :r].cpu(), mine)
+                assert ((key_sums[:, p].cpu().double() - mine.double().sum(2)).abs()
+                        <= r * 2.0 ** -24 * mine.double().abs().sum(2)).all()
+    assert (m.status == yt.CACHE_ERR_FULL) == full

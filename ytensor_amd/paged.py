@@ -17,7 +17,7 @@ prompt's rows and give them back:
     cache_compact / cache_copy_pages
 
 Everything is read on the device when the kernels run, and no call waits for the host, so a
-step (attend, grow, append) can be captured as one HIP graph. Argument problems raise
+step (attend, keep the lengths, grow in place, append) can be captured as one HIP graph. Argument problems raise
 ValueError or YthipError; what only the device can see (no free page, an index out of range)
 sets bits of `status`, an int32 device tensor (CACHE_ERR_*).
 """
