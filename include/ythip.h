@@ -505,6 +505,7 @@ int ythip_rope_tables(int dim, int max_len, float theta, float* cosv, float* sin
  *            table[b][r / page] at r % page; behind the pages of its rows it may hold anything. An id outside [0, pages) is never an address: its
  *            rows are hidden (attention) or not written (append)
  *            At most 65536 columns, 2^30 rows a sequence and 2^34 rows (B * columns * page)
+ *            Strides of dims of one element (one sequence, layer, token, ...) may hold anything
  *   kv_len   int32 [B], rows in use (clamped to [0, columns * page])
  *   ref      int32 [pages], the sequences that hold a page; 0: free
  * All of it lives on the device and is read when the kernels run, so captured HIP graphs

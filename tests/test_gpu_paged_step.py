@@ -1,5 +1,5 @@
 """The paged cache's calls as a server makes them, on the GPU: a pool that runs full, the documented step captured and
-replayed."""
+replayed, the views that a step has in hand."""
 from __future__ import annotations
 
 import pytest
@@ -7,7 +7,7 @@ import torch
 
 import ytensor_amd as yt
 from paged_ref import Pages, attention
-from test_gpu_paged import DT, compare, ints, tree
+from test_gpu_paged import DT, cache, compare, ints, tokens, tree
 
 pytestmark = pytest.mark.gpu
 
@@ -199,3 +199,41 @@ def test_the_documented_step_replayed(full):
                 assert ((key_sums[:, p].cpu().double() - mine.double().sum(2)).abs()
                         <= r * 2.0 ** -24 * mine.double().abs().sum(2)).all()
     assert (m.status == yt.CACHE_ERR_FULL) == full
+
+
+def test_views_with_one_sequence_or_token():
+    """A dim of one element has no stride that matters, whatever the view says: slices of wider buffers whose width is
+    no multiple of 16 bytes are taken, and written to, as they are."""
+    dt, Hq, Hkv, d, page = torch.bfloat16, 4, 2, 64, 16
+    g, kp, vp, table, kv_len = cache(2, [20], Hkv, page, d, dt)
+    q, kn, vn = tokens(g, 1, Hq, Hkv, 1, d, dt)
+
+    def odd(t):
+        """t with strides of 1001 in its dims of one element"""
+        st = [1001 if n == 1 else s for n, s in zip(t.shape, t.contiguous().stride())]
+        return torch.empty_strided(t.shape, st, dtype=t.dtype, device="cuda").copy_(t)
+
+    want, tol = attention(q, kn, vn, kp, vp, table, kv_len)
+    out = odd(torch.zeros_like(q))
+    yt.paged_attention(odd(q), odd(kn), odd(vn), kp, vp, table, kv_len, out=out)
+    compare(out, want, tol)
+    wide = torch.randn(1, (Hq + 2 * Hkv) * d + 3, generator=g).to(dt).cuda()  # a projection's row of odd width
+    q, kn, vn = (x.unflatten(1, (-1, d))[:, :, None] for x in wide[:, :-3].split([Hq * d, Hkv * d, Hkv * d], 1))
+    want, tol = attention(q, kn, vn, kp, vp, table, kv_len)
+    compare(yt.paged_attention(q, kn, vn, kp, vp, table, kv_len), want, tol)
+    # one KV head, one layer: pools and rows with such strides
+    g, kp, vp, table, kv_len = cache(2, [20], 1, page, d, dt)
+    q, kn, vn = tokens(g, 1, 2, 1, 1, d, dt)
+    want, tol = attention(q, kn, vn, kp, vp, table, kv_len)
+    sums = torch.nan_to_num(kp.float()).sum(2)
+    compare(yt.paged_attention(q, kn, vn, odd(kp), vp, table, kv_len), want, tol)
+    out, _ = yt.paged_sparse_attention(q, kn, vn, kp, odd(vp), odd(sums), table, kv_len, 4)
+    compare(out, want, tol)
+    k2, v2, s2 = odd(kp[None]), vp[None].clone(), odd(sums[None])
+    yt.cache_append(odd(kn[None]), vn[None], k2, v2, table, kv_len, key_sums=s2)
+    assert torch.equal(k2[0, table[0, 1].long(), 0, 4], kn[0, 0, 0])
+    assert torch.equal(v2[0, table[0, 1].long(), 0, 4], vn[0, 0, 0])
+    held = k2[0, table[0, 1].long(), 0, :5].float()
+    assert torch.allclose(s2[0, table[0, 1].long(), 0], held.sum(0), rtol=0, atol=5 * 2.0 ** -24 * held.abs().sum(0).max().item())
+    pool = odd(torch.randn(1, 1, 3, 32, 64, generator=g).to(dt).cuda())  # one layer and one page, 2-byte elements
+    yt.cache_copy_pages([pool], ints([0]), ints([0]))

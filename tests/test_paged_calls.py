@@ -4,9 +4,10 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
 import ytensor_amd as yt
-from ytensor_amd import _lib
+from ytensor_amd import _lib, paged
 
 FAKE = ctypes.c_void_p(4096)
 EINVAL, EUNSUP = _lib.YTHIP_EINVAL, _lib.YTHIP_EUNSUPPORTED
@@ -30,3 +31,25 @@ def test_append_to_given_lengths_refuses(change, status, text):
     lib = yt.load()
     assert append(lib, True, **change) == status
     assert b"ythip_cache_append_to" in lib.ythip_last_error() and text in lib.ythip_last_error()
+
+
+def test_dims_of_one_element_have_no_stride():
+    """A view whose only odd strides are those of dims of one element is taken as it is; others are copied, to
+    strides of their own."""
+    odd = torch.empty_strided((1, 2, 1, 64), (1001, 64, 7, 1), dtype=torch.bfloat16)
+    t, at, st = paged._rows(odd, 2)
+    assert t is odd and at == odd.data_ptr() and st == (1001, 64, 7, 1) and paged._real(odd) == (0, 64, 0, 1)
+    for stride in ((72, 65, 7, 1), (128, 1, 1, 2)):
+        t, at, st = paged._rows(torch.empty_strided((1, 2, 1, 64), stride, dtype=torch.bfloat16), 2)
+        assert st == (128, 64, 64, 1) and at == t.data_ptr() and at % 16 == 0
+    assert paged._pool_layout((1, 1, 3, 16), (7, 5, 16, 1), 2) == (1, 1, 0, 0, 96)
+    assert paged._pool_layout((2, 4, 3, 16), (200, 50, 16, 1), 2) == (2, 4, 400, 100, 96)
+
+
+def test_strides_that_matter_are_still_refused():
+    lib, odd = yt.load(), _lib.i64array([100, 128, 128, 128])
+    assert append(lib, False, ns=odd) == EUNSUP and append(lib, False, ps=odd) == EUNSUP
+    assert b"aligned" in lib.ythip_last_error()
+    for axis in range(4):
+        ns = _lib.i64array([100 if i == axis else 128 for i in range(4)])
+        assert append(lib, False, ns=ns) == EUNSUP

@@ -1321,19 +1321,19 @@ int prepare(const char* who, const Call& c, PagedArgs& a, bool& done) {
     const int es = c.dtype == YTHIP_F32 ? 4 : 2;
     int64_t all = (int64_t)(uintptr_t)c.Q | (int64_t)(uintptr_t)c.O | (int64_t)(uintptr_t)c.Kn | (int64_t)(uintptr_t)c.Vn |
                   (int64_t)(uintptr_t)c.Kp | (int64_t)(uintptr_t)c.Vp;
+    // the stride of a dim of one element may be anything, and is taken as 0
+    const int q_dims[3] = {c.B, c.Hq, c.T}, new_dims[3] = {c.B, c.Hkv, c.T}, pool_dims[3] = {c.pages, c.Hkv, c.page};
+    auto real = [](const int64_t* str, const int* dims, int i) { return dims[i] > 1 ? str[i] : 0; };
     for (int i = 0; i < 3; ++i) {
-        all |= (c.q_str[i] | c.o_str[i] | c.pool_str[i]) * es;
-        if (c.Kn) all |= (c.kn_str[i] | c.vn_str[i]) * es;
+        a.qs[i] = real(c.q_str, q_dims, i), a.os[i] = real(c.o_str, q_dims, i), a.ps[i] = real(c.pool_str, pool_dims, i);
+        a.kns[i] = c.Kn ? real(c.kn_str, new_dims, i) : 0, a.vns[i] = c.Kn ? real(c.vn_str, new_dims, i) : 0;
+        all |= (a.qs[i] | a.os[i] | a.ps[i] | a.kns[i] | a.vns[i]) * es;
     }
     if ((all & 15) != 0) return fail(YTHIP_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
-    for (const int64_t row : {c.pool_str[2], c.Kn ? c.kn_str[2] : 0, c.Kn ? c.vn_str[2] : 0})  // 16 rows within 32-bit offsets
+    for (const int64_t row : {a.ps[2], a.kns[2], a.vns[2]})  // 16 rows within 32-bit offsets
         if (row < 0 || row >= 1 << 24) return fail(YTHIP_EUNSUPPORTED, "%s: K or V rows at a stride of %lld (0 to 2^24 - 1)", who, (long long)row);
     a.B = c.B, a.Hq = c.Hq, a.Hkv = c.Hkv, a.G = c.Hq / c.Hkv, a.T = c.T, a.pages = c.pages, a.columns = c.columns;
     a.Q = c.Q, a.Kn = c.Kn, a.Vn = c.Vn, a.Kp = c.Kp, a.Vp = c.Vp;
-    for (int i = 0; i < 3; ++i) {
-        a.qs[i] = c.q_str[i], a.os[i] = c.o_str[i], a.ps[i] = c.pool_str[i];
-        a.kns[i] = c.Kn ? c.kn_str[i] : 0, a.vns[i] = c.Kn ? c.vn_str[i] : 0;
-    }
     a.table = c.table, a.kv_len = c.kv_len, a.parents = c.parents, a.new_len = c.new_len;
     a.ld_table = c.ld_table, a.ld_par = c.ld_par, a.O = c.O;
     a.scale_log2 = (c.scale == 0.f ? 1.0f / sqrtf((float)c.d) : c.scale) * 1.4426950408889634f;

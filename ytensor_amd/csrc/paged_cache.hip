@@ -609,7 +609,7 @@ int make_pools(const char* who, int n_pools, int layers, const ythip_page_pool* 
     ps.layers = layers;
     for (int k = 0; k < n_pools; ++k) {
         const ythip_page_pool& p = pools[k];
-        const int64_t all = (int64_t)(uintptr_t)p.data | p.layer_stride | p.page_stride | p.page_bytes;
+        const int64_t all = (int64_t)(uintptr_t)p.data | (layers > 1 ? p.layer_stride : 0) | p.page_stride | p.page_bytes;
         if (p.data == nullptr || p.page_bytes <= 0 || (all & 3) != 0 || p.page_bytes > ((int64_t)INT_MAX / 2) * COPY_BYTES)
             return fail(YTHIP_EINVAL, "%s: pool %d (data, strides and bytes: multiples of 4, bytes > 0)", who, k);
         ps.data[k] = static_cast<char*>(p.data);
@@ -652,7 +652,8 @@ int append(const char* who, int dtype, int layers, int B, int Hkv, int T, int d,
     if ((int64_t)d * es % 16 != 0 || (int64_t)d * es > 4096)
         return fail(YTHIP_EUNSUPPORTED, "%s: rows of %lld bytes (a multiple of 16, at most 4096)", who, (long long)d * es);
     int64_t all = (int64_t)(uintptr_t)Kn | (int64_t)(uintptr_t)Vn | (int64_t)(uintptr_t)Kp | (int64_t)(uintptr_t)Vp;
-    for (int i = 0; i < 4; ++i) all |= new_str[i] * es | pool_str[i] * es;
+    const int new_dims[4] = {layers, B, Hkv, T}, pool_dims[4] = {layers, pages, Hkv, page};
+    for (int i = 0; i < 4; ++i) all |= (new_dims[i] > 1 ? new_str[i] * es : 0) | (pool_dims[i] > 1 ? pool_str[i] * es : 0);
     if ((all & 15) != 0) return fail(YTHIP_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
     if (layers == 0 || B == 0 || Hkv == 0 || T == 0 || pages == 0 || columns == 0) return 0;
     AppendArgs a;

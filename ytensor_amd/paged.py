@@ -37,8 +37,13 @@ CACHE_ERR_INDEX, CACHE_ERR_BUSY, CACHE_ERR_FULL = 1, 2, 4
 
 @functools.lru_cache(maxsize=4096)
 def _i64(vals: tuple) -> ctypes.Array:
-    """Strides for the C call, which reads them only (and not the last, of d)."""
+    """Strides for the C call, which reads them only (and not the last, of d, nor those of dims of one element)."""
     return _lib.i64array(vals)
+
+
+def _real(t: torch.Tensor) -> tuple:
+    """t's strides, 0 for dims of one element: those may hold anything."""
+    return tuple(0 if n == 1 else s for n, s in zip(t.shape, t.stride()))
 
 
 def _device(first: torch.Tensor, *rest) -> int:
@@ -75,8 +80,12 @@ def _rows(t: torch.Tensor, es: int) -> tuple[torch.Tensor, int, tuple]:
     for s in st[:-1]:
         align |= s * es
     if st[-1] != 1 or align & 15:
-        t = t.clone() if t.is_contiguous() else t.contiguous()
-        at, st = t.data_ptr(), t.stride()
+        align = at
+        for s in _real(t)[:-1]:
+            align |= s * es
+        if st[-1] != 1 or align & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+            at, st = t.data_ptr(), t.stride()
     return t, at, st
 
 
@@ -97,7 +106,7 @@ def _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, 
     if k_pool.dtype != dt or v_pool.dtype != dt:
         raise ValueError("q and the pools must share a dtype")
     pool_st = k_pool.stride()
-    if v_pool.shape != k_pool.shape or v_pool.stride() != pool_st or pool_st[3] != 1:
+    if v_pool.shape != k_pool.shape or pool_st[3] != 1 or (v_pool.stride() != pool_st and _real(v_pool) != _real(k_pool)):
         raise ValueError("k_pool and v_pool must share a shape and strides, with d contiguous")
     es = 4 if dt is torch.float32 else 2
     q, q_at, q_st = _rows(q, es)
@@ -251,7 +260,8 @@ def _pool_layout(shape: tuple, stride: tuple, es: int) -> tuple:
         if size != 1 and step != inner:
             raise ValueError(f"a pool of shape {list(shape)} and strides {list(stride)}: a page must be contiguous")
         inner *= size
-    return shape[0], shape[1], stride[0] * es, stride[1] * es, inner * es
+    layer, page = (0 if n == 1 else step * es for n, step in zip(shape[:2], stride[:2]))
+    return shape[0], shape[1], layer, page, inner * es
 
 
 def _pools(pools, pages: int):
@@ -314,13 +324,13 @@ def cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
                          f"{list(v_pool.shape)} do not fit")
     if not (k_new.dtype == v_new.dtype == k_pool.dtype == v_pool.dtype):
         raise ValueError("k_new, v_new and the pools must share a dtype")
-    if k_pool.stride() != v_pool.stride() or k_pool.stride(4) != 1:
+    if k_pool.stride(4) != 1 or (k_pool.stride() != v_pool.stride() and _real(k_pool) != _real(v_pool)):
         raise ValueError("k_pool and v_pool must share strides, with d contiguous")
     es = k_new.element_size()
     k_new, k_at, new_st = _rows(k_new, es)
     v_new, v_at, v_st = _rows(v_new, es)
-    if new_st != v_st:
-        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    if new_st != v_st and _real(k_new) != _real(v_new):
+        k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
         k_at, v_at, new_st = k_new.data_ptr(), v_new.data_ptr(), k_new.stride()
     table, ld, columns = _table(table, B)
     kv_len = _packed(_ints("kv_len", kv_len, (B,)))
