@@ -237,3 +237,24 @@ def test_views_with_one_sequence_or_token():
     assert torch.allclose(s2[0, table[0, 1].long(), 0], held.sum(0), rtol=0, atol=5 * 2.0 ** -24 * held.abs().sum(0).max().item())
     pool = odd(torch.randn(1, 1, 3, 32, 64, generator=g).to(dt).cuda())  # one layer and one page, 2-byte elements
     yt.cache_copy_pages([pool], ints([0]), ints([0]))
+
+
+def test_calls_with_nothing_to_do():
+    """No tokens, no sequences, no columns, no pages."""
+    kp = torch.zeros(1, 4, 1, 16, 64, device="cuda")
+    for B, T, columns in ((0, 3, 2), (2, 0, 2), (2, 3, 0), (0, 0, 0)):
+        kn = torch.zeros(1, B, 1, T, 64, device="cuda")
+        table, lens = torch.zeros(B, columns, dtype=torch.int32, device="cuda"), ints([0] * B)
+        yt.cache_append(kn, kn, kp, kp.clone(), table, lens)
+        yt.cache_append(kn, kn, kp, kp.clone(), table, lens, new_len=lens)
+        assert (kp == 0).all()
+        ref = ints([1, 0, 1, 1])
+        r, t, n = yt.cache_grow(ref, table, lens, ints([0] * B), 16)
+        assert r.tolist() == [1, 0, 1, 1] and n.tolist() == [0] * B
+        yt.cache_free(ref, table, lens, ints([]), 16)
+        yt.cache_fork([kp], ref, table, lens, ints([]), ints([]), 16)
+        _, _, live = yt.cache_compact([kp], ref, table, lens, 16)
+        assert live.item() == 3 and ref.tolist() == [1, 1, 1, 0]
+    q, empty = torch.zeros(2, 2, 3, 64, device="cuda"), torch.zeros(0, 1, 16, 64, device="cuda")
+    none = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
+    assert (yt.paged_attention(q, None, None, empty, empty, none, ints([5, 0])) == 0).all()

@@ -53,3 +53,21 @@ def test_strides_that_matter_are_still_refused():
     for axis in range(4):
         ns = _lib.i64array([100 if i == axis else 128 for i in range(4)])
         assert append(lib, False, ns=ns) == EUNSUP
+
+
+@pytest.mark.parametrize("empty", ["L", "B", "Hkv", "T", "pages", "columns"])
+def test_appends_of_nothing_take_no_pointers(empty):
+    """An empty tensor has no address."""
+    lib = yt.load()
+    none = dict(Kn=None, Vn=None, Kp=None, Vp=None, sums=None, table=None) if empty != "columns" else dict(table=None)
+    if empty not in ("B", "columns"):
+        del none["table"]
+    for to in (False, True):
+        assert append(lib, to, **{empty: 0, **none}) == 0
+
+
+def test_bookkeeping_without_columns_takes_no_table():
+    lib = yt.load()
+    # (not 0 here, where asking for the last launch's error finds no GPU)
+    assert lib.ythip_cache_free(2, 0, 8, 16, FAKE, None, 0, FAKE, 0, None, FAKE, None, 0, FAKE, None, None) != EINVAL
+    assert lib.ythip_cache_free(2, 1, 8, 16, FAKE, None, 1, FAKE, 0, None, FAKE, None, 1, FAKE, None, None) == EINVAL

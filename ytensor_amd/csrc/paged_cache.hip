@@ -587,7 +587,7 @@ int check_table(const char* who, int B, int columns, int pages, int page, const 
     if (page_shift(page) < 0) return fail(YTHIP_EINVAL, "%s: a page of %d rows (a power of two from 16 to 32768)", who, page);
     if (columns > MAX_COLUMNS || (int64_t)columns * page > 1 << 30)
         return fail(YTHIP_EUNSUPPORTED, "%s: %d columns of %d rows (at most 65536 columns, 2^30 rows)", who, columns, page);
-    if (B > 0 && (table == nullptr || len == nullptr)) return fail(YTHIP_EINVAL, "%s: table or len is NULL", who);
+    if (B > 0 && (len == nullptr || (columns > 0 && table == nullptr))) return fail(YTHIP_EINVAL, "%s: table or len is NULL", who);
     if (ld < columns) return fail(YTHIP_EINVAL, "%s: a table row of %d entries at a stride of %lld", who, columns, (long long)ld);
     return 0;
 }
@@ -647,6 +647,7 @@ int append(const char* who, int dtype, int layers, int B, int Hkv, int T, int d,
     if (dtype != YTHIP_F32 && dtype != YTHIP_F16 && dtype != YTHIP_BF16) return fail(YTHIP_EINVAL, "%s: invalid dtype %d", who, dtype);
     if (layers < 0 || B < 0 || Hkv < 0 || T < 0 || d <= 0) return fail(YTHIP_EINVAL, "%s: bad size", who);
     if (const int st = check_table(who, B, columns, pages, page, table, ld_table, kv_len)) return st;
+    if (layers == 0 || B == 0 || Hkv == 0 || T == 0 || pages == 0 || columns == 0) return 0;
     if (!Kn || !Vn || !Kp || !Vp || !new_str || !pool_str || (sums && !sums_str)) return fail(YTHIP_EINVAL, "%s: NULL argument", who);
     const int es = dtype == YTHIP_F32 ? 4 : 2;
     if ((int64_t)d * es % 16 != 0 || (int64_t)d * es > 4096)
@@ -655,7 +656,6 @@ int append(const char* who, int dtype, int layers, int B, int Hkv, int T, int d,
     const int new_dims[4] = {layers, B, Hkv, T}, pool_dims[4] = {layers, pages, Hkv, page};
     for (int i = 0; i < 4; ++i) all |= (new_dims[i] > 1 ? new_str[i] * es : 0) | (pool_dims[i] > 1 ? pool_str[i] * es : 0);
     if ((all & 15) != 0) return fail(YTHIP_EUNSUPPORTED, "%s: rows must be 16-byte aligned", who);
-    if (layers == 0 || B == 0 || Hkv == 0 || T == 0 || pages == 0 || columns == 0) return 0;
     AppendArgs a;
     a.layers = layers, a.B = B, a.Hkv = Hkv, a.T = T, a.pages = pages, a.shift = page_shift(page), a.columns = columns;
     a.slots = (int)(((int64_t)T + page - 2) / page + 1);  // pages that T rows touch at most
