@@ -258,3 +258,24 @@ def test_calls_with_nothing_to_do():
     q, empty = torch.zeros(2, 2, 3, 64, device="cuda"), torch.zeros(0, 1, 16, 64, device="cuda")
     none = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
     assert (yt.paged_attention(q, None, None, empty, empty, none, ints([5, 0])) == 0).all()
+
+
+def test_more_pieces_than_a_launch_holds():
+    """4096 pairs in 4100 layers, each a workgroup's piece: all of them are copied."""
+    L, n = 4100, 4096
+    g = torch.Generator().manual_seed(12)
+    pool = torch.randint(0, 2 ** 31 - 1, (L, 2 * n, 1), generator=g, dtype=torch.int32).cuda()
+    order = torch.randperm(2 * n, generator=g).int().cuda()
+    src, dst, was = order[:n], order[n:], pool.clone()
+    yt.cache_copy_pages([pool], src, dst)
+    assert torch.equal(pool[:, dst.long()], was[:, src.long()]) and torch.equal(pool[:, src.long()], was[:, src.long()])
+    # the same as forks: each source has one row of its page, each gets the lowest free page
+    pool.copy_(was)
+    ref = torch.cat([torch.ones(n, dtype=torch.int32), torch.zeros(n, dtype=torch.int32)]).cuda()
+    table = torch.full((2 * n, 1), -1, dtype=torch.int32, device="cuda")
+    table[:n, 0] = order[:n].argsort().int()  # page i of the first n, in some order
+    kv_len = torch.cat([torch.ones(n, dtype=torch.int32), torch.zeros(n, dtype=torch.int32)]).cuda()
+    seqs = torch.arange(n, dtype=torch.int32, device="cuda")
+    yt.cache_fork([pool], ref, table, kv_len, seqs, seqs + n, 16)
+    assert (ref == 1).all() and (kv_len == 1).all() and torch.equal(table[n:, 0], seqs + n)
+    assert torch.equal(pool[:, n:], was[:, table[:n, 0].long()]) and torch.equal(pool[:, :n], was[:, :n])

@@ -71,3 +71,20 @@ def test_bookkeeping_without_columns_takes_no_table():
     # (not 0 here, where asking for the last launch's error finds no GPU)
     assert lib.ythip_cache_free(2, 0, 8, 16, FAKE, None, 0, FAKE, 0, None, FAKE, None, 0, FAKE, None, None) != EINVAL
     assert lib.ythip_cache_free(2, 1, 8, 16, FAKE, None, 1, FAKE, 0, None, FAKE, None, 1, FAKE, None, None) == EINVAL
+
+
+def test_more_workgroups_than_a_launch_holds():
+    """A grid's dimension has fewer than 2^32 threads: refused before anything runs."""
+    lib = yt.load()
+    for change in (dict(L=1 << 10, B=1 << 10, Hkv=64), dict(L=1 << 8, B=1 << 8, Hkv=256, page=512),
+                   dict(L=1 << 7, B=1 << 7, Hkv=256, page=1024)):
+        for to in (False, True):
+            assert append(lib, to, **change) == EUNSUP and b"pages to write" in lib.ythip_last_error()
+    i3 = _lib.i64array([128] * 3)
+
+    def attention(B, Hq, Hkv, T, columns):
+        return lib.ythip_paged_attn(_lib.BF16, B, Hq, Hkv, T, 128, FAKE, i3, FAKE, i3, FAKE, i3, FAKE, FAKE, i3, 8, 16, FAKE,
+                                    columns, columns, FAKE, None, 0, None, FAKE, i3, 0.0, FAKE, 1 << 62, None)
+
+    assert attention(65535, 512, 512, 1, 4) == EUNSUP and b"workgroups" in lib.ythip_last_error()
+    assert attention(2, 256, 1, 1 << 21, 64) == EUNSUP and b"workgroups" in lib.ythip_last_error()

@@ -18,6 +18,9 @@ int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 // (positive) hipError_t value.
 int status_of(hipError_t e);
 
+// Whether one launch can hold so many workgroups: a dimension of a grid has fewer than 2^32 threads.
+inline bool launchable(int64_t workgroups, int threads) { return workgroups < (1ll << 32) / threads; }
+
 // Kernel dispatchers (one per translation unit).
 int gemm_dispatch(int dtype_in, int dtype_out, int batch, int m, int n, int k, const void* A, int64_t sa_b,
                   int64_t rsa, int64_t csa, const void* B, int64_t sb_b, int64_t rsb, int64_t csb, void* C,

@@ -1247,8 +1247,8 @@ int run_typed(const PagedArgs& a, const Plan& p, hipStream_t s) {
 template <bool SPARSE>
 int run(int dtype, int d, PagedArgs& a, void* ws, hipStream_t s) {
     const Plan p = plan_of(dtype, a.B, a.Hkv, a.G, a.T, d, a.columns, 1 << a.shift, SPARSE ? a.top_k : 0);
-    if ((p.items * a.Hkv + 8) * p.row_tiles > INT_MAX)
-        return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups", (long long)(p.items * a.Hkv * p.row_tiles));
+    if (!launchable((p.items * a.Hkv + 8) * p.row_tiles, 256))
+        return fail(YTHIP_EUNSUPPORTED, "paged attention: %lld workgroups (2^24 - 1 at most)", (long long)(p.items * a.Hkv * p.row_tiles));
     a.target = p.target, a.stage = p.stage, a.items = (int)p.items, a.row_tiles = p.row_tiles, a.even = p.even, a.short_run = p.short_run;
     char* w = static_cast<char*>(ws);
     a.rank = reinterpret_cast<uint64_t*>(w);

@@ -6,6 +6,7 @@
 // the page counts, done by one workgroup; what it moves (whole pages of every layer, rows) is
 // a second launch over all CUs, bound by HBM (a page is read once and written once).
 
+#include <algorithm>
 #include <climits>
 
 #include "launch.hpp"
@@ -18,6 +19,7 @@ constexpr int PLAN_ROWS = 4;        // pages a thread looks at per step
 constexpr int MAX_SEQS = 4096;      // sequences of a grow, pairs of a fork: their prefix sums lie in LDS
 constexpr int MAX_COLUMNS = 65536;
 constexpr int MAX_POOLS = 4;
+constexpr int64_t MOST_COPIES = 1 << 23;  // pieces a launch
 constexpr int COPY_BYTES = 16384;  // of a page, a workgroup of 256 threads: four 16-byte loads in flight each
 
 __device__ __forceinline__ int pages_of(int rows, int shift) { return (int)(((int64_t)rows + (1ll << shift) - 1) >> shift); }
@@ -290,8 +292,8 @@ __global__ __launch_bounds__(PLAN_THREADS) void cache_fork_plan(ForkArgs a) {
 
 // Workgroups [0, n): pair i's row and page counts; the others its partial page, in every pool.
 // Bound by the copies' bytes (8 pairs, 28 layers, 119 MB read and written 21.4 us, 5.5 TB/s).
-__global__ __launch_bounds__(256) void cache_fork_copy(ForkArgs a, PoolSet ps) {
-    const int w = blockIdx.x;
+__global__ __launch_bounds__(256) void cache_fork_copy(ForkArgs a, PoolSet ps, int64_t first) {
+    const int64_t w = first + blockIdx.x;
     if (w < a.n) {
         const int4 pl = a.plan[w];
         if (pl.y < 0) return;
@@ -435,9 +437,9 @@ __global__ __launch_bounds__(256) void cache_compact_move(CompactArgs a, PoolSet
 }
 
 __global__ __launch_bounds__(256) void cache_copy_kernel(int pages, int n, const int32_t* src, const int32_t* dst,
-                                                         PoolSet ps, int32_t* status) {
+                                                         PoolSet ps, int32_t* status, int64_t first) {
     Unit u;
-    if (!unit_of(ps, n, blockIdx.x, u)) return;
+    if (!unit_of(ps, n, first + blockIdx.x, u)) return;
     const int from = src[u.i], to = dst[u.i];
     if (from < 0 || from >= pages || to < 0 || to >= pages) {
         if (threadIdx.x == 0) flag(status, YTHIP_CACHE_ERR_INDEX);
@@ -669,13 +671,14 @@ int append(const char* who, int dtype, int layers, int B, int Hkv, int T, int d,
     a.to = to, a.status = status;
     a.chunks = (int)((int64_t)d * es / 16);
     const int64_t grid = (int64_t)a.slots * Hkv * B * layers;
-    if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pages to write", who, (long long)grid);
+    // a wave where a page is a few loads of it, more for long pages and rows
+    const int waves = page <= 64 && a.chunks <= 64 ? 1 : page <= 512 ? 4 : 16;
+    if (!launchable(grid, 64 * waves)) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pages to write", who, (long long)grid);
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto t) {
         using T = decltype(t);
-        // a wave where a page is a few loads of it, more for long pages and rows
-        if (page <= 64 && a.chunks <= 64) cache_append_kernel<T, 1><<<(int)grid, 64, 0, s>>>(a);
-        else if (page <= 512) cache_append_kernel<T, 4><<<(int)grid, 256, 0, s>>>(a);
+        if (waves == 1) cache_append_kernel<T, 1><<<(int)grid, 64, 0, s>>>(a);
+        else if (waves == 4) cache_append_kernel<T, 4><<<(int)grid, 256, 0, s>>>(a);
         else cache_append_kernel<T, 16><<<(int)grid, 1024, 0, s>>>(a);
     };
     if (dtype == YTHIP_F32) run(F32{});
@@ -745,14 +748,13 @@ __attribute__((visibility("default"))) int ythip_cache_fork(int B, int columns, 
     const size_t need = ythip_cache_fork_workspace_size(n);
     if (need > 0 && (workspace == nullptr || ws_bytes < need || ((uintptr_t)workspace & 15) != 0))
         return fail(YTHIP_EINVAL, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, need, ws_bytes);
-    const int64_t grid = n + units(ps, n);
-    if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pieces to copy", who, (long long)grid);
+    const int64_t all = n + units(ps, n);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const StateArgs st = copy_state({false, B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, n == 0, s);
     if (n > 0) {
         const ForkArgs a = {B, columns, pages, page_shift(page), n, src, dst, ref_out, table_out, len_out, ld_out, static_cast<int4*>(workspace), status, st};
         cache_fork_plan<<<1, PLAN_THREADS, 0, s>>>(a);
-        cache_fork_copy<<<(int)grid, 256, 0, s>>>(a, ps);
+        for (int64_t w = 0; w < all; w += MOST_COPIES) cache_fork_copy<<<(int)std::min(all - w, MOST_COPIES), 256, 0, s>>>(a, ps, w);
     }
     return status_of(hipGetLastError());
 }
@@ -814,10 +816,10 @@ __attribute__((visibility("default"))) int ythip_cache_copy_pages(int pages, int
     if (pages < 0 || n < 0 || (n > 0 && (!src || !dst))) return fail(YTHIP_EINVAL, "%s: %d pages, or src or dst is NULL", who, n);
     PoolSet ps;
     if (const int st = make_pools(who, n_pools, layers, pools, ps)) return st;
-    const int64_t grid = units(ps, n);
-    if (grid > INT_MAX) return fail(YTHIP_EUNSUPPORTED, "%s: %lld pieces to copy", who, (long long)grid);
-    if (grid == 0) return 0;
-    cache_copy_kernel<<<(int)grid, 256, 0, static_cast<hipStream_t>(stream)>>>(pages, n, src, dst, ps, status);
+    const int64_t all = units(ps, n);
+    if (all == 0) return 0;
+    for (int64_t w = 0; w < all; w += MOST_COPIES)
+        cache_copy_kernel<<<(int)std::min(all - w, MOST_COPIES), 256, 0, static_cast<hipStream_t>(stream)>>>(pages, n, src, dst, ps, status, w);
     return status_of(hipGetLastError());
 }
 
