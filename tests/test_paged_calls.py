@@ -88,3 +88,10 @@ def test_more_workgroups_than_a_launch_holds():
 
     assert attention(65535, 512, 512, 1, 4) == EUNSUP and b"workgroups" in lib.ythip_last_error()
     assert attention(2, 256, 1, 1 << 21, 64) == EUNSUP and b"workgroups" in lib.ythip_last_error()
+
+
+@pytest.mark.parametrize("to", [False, True])
+@pytest.mark.parametrize("stride", [2, 0, -3])
+def test_append_refuses_paths_that_overlap(to, stride):
+    lib = yt.load()
+    assert append(lib, to, path=FAKE, ldp=stride) == EINVAL and b"path" in lib.ythip_last_error()

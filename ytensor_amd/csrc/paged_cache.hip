@@ -651,6 +651,7 @@ int append(const char* who, int dtype, int layers, int B, int Hkv, int T, int d,
     if (const int st = check_table(who, B, columns, pages, page, table, ld_table, kv_len)) return st;
     if (layers == 0 || B == 0 || Hkv == 0 || T == 0 || pages == 0 || columns == 0) return 0;
     if (!Kn || !Vn || !Kp || !Vp || !new_str || !pool_str || (sums && !sums_str)) return fail(YTHIP_EINVAL, "%s: NULL argument", who);
+    if (path && ld_path < T) return fail(YTHIP_EINVAL, "%s: a path of %d entries at a stride of %lld", who, T, (long long)ld_path);
     const int es = dtype == YTHIP_F32 ? 4 : 2;
     if ((int64_t)d * es % 16 != 0 || (int64_t)d * es > 4096)
         return fail(YTHIP_EUNSUPPORTED, "%s: rows of %lld bytes (a multiple of 16, at most 4096)", who, (long long)d * es);
