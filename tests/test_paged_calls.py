@@ -95,3 +95,12 @@ def test_more_workgroups_than_a_launch_holds():
 def test_append_refuses_paths_that_overlap(to, stride):
     lib = yt.load()
     assert append(lib, to, path=FAKE, ldp=stride) == EINVAL and b"path" in lib.ythip_last_error()
+
+
+def test_sparse_workspace_parts_are_aligned():
+    """The ranks lie in front of the partials, which are read 16 bytes at a time."""
+    lib = yt.load()
+    size = lambda B, Hkv, T, columns: int(lib.ythip_paged_attn_sparse_workspace_size(_lib.BF16, B, 2 * Hkv, Hkv, T, 64, columns, 16, 5))  # noqa: E731
+    for B, Hkv, T, columns in ((1, 1, 1, 1251), (1, 1, 1, 129), (3, 1, 5, 1001), (1, 7, 1, 131)):
+        assert B * Hkv * T * columns % 2 == 1 and size(B, Hkv, T, columns) % 16 == 0
+        assert size(B, Hkv, T, columns) >= 8 * B * Hkv * T * columns

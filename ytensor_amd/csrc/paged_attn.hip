@@ -1146,7 +1146,7 @@ struct Plan {
     bool even = false;
     int short_run;
     int64_t items;
-    size_t part_bytes, ml_bytes, rank_bytes;
+    size_t part_bytes, ml_bytes, rank_bytes;  // multiples of 16
     size_t bytes() const { return part_bytes + ml_bytes + rank_bytes; }
 };
 constexpr int SLOTS = 512;
@@ -1202,7 +1202,8 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     const int64_t part_rows = part_items * Hkv * all_rows;
     p.part_bytes = (size_t)part_rows * d * sizeof(float);
     p.ml_bytes = ((size_t)part_rows * 2 * sizeof(float) + 15) / 16 * 16;
-    p.rank_bytes = top_k > 0 ? (size_t)B * Hkv * T * columns * sizeof(uint64_t) : 0;
+    // (the partials behind them are read 16 bytes at a time)
+    p.rank_bytes = top_k > 0 ? ((size_t)B * Hkv * T * columns * sizeof(uint64_t) + 15) / 16 * 16 : 0;
     return p;
 }
 
