@@ -279,3 +279,16 @@ def test_more_pieces_than_a_launch_holds():
     yt.cache_fork([pool], ref, table, kv_len, seqs, seqs + n, 16)
     assert (ref == 1).all() and (kv_len == 1).all() and torch.equal(table[n:, 0], seqs + n)
     assert torch.equal(pool[:, n:], was[:, table[:n, 0].long()]) and torch.equal(pool[:, :n], was[:, :n])
+
+
+@pytest.mark.parametrize("lens,new", [([700], [130]), ([0, 900, 16], [130, 7, 0])])
+def test_chunks_that_no_range_cuts(lens, new):
+    """So many rows that every sequence stays whole: no workspace is asked for."""
+    dt, B, T, Hkv, G, d = torch.bfloat16, len(lens), 130, 32, 8, 64
+    g, k, v, table, kv_len = cache(7, lens, Hkv, 16, d, dt, columns=60)
+    q, kn, vn = tokens(g, B, Hkv * G, Hkv, T, d, dt)
+    assert yt.paged_workspace_bytes(dt, B, Hkv * G, Hkv, T, d, 60, 16) == 0
+    parents, tree_len = tree(g, B, T), ints(new)
+    before = torch.full_like(q, 7.0)
+    out = yt.paged_attention(q, kn, vn, k, v, table, kv_len, parents=parents, tree_len=tree_len, out=before.clone())
+    compare(out, *attention(q, kn, vn, k, v, table, kv_len, parents, tree_len), before)

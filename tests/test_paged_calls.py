@@ -104,3 +104,11 @@ def test_sparse_workspace_parts_are_aligned():
     for B, Hkv, T, columns in ((1, 1, 1, 1251), (1, 1, 1, 129), (3, 1, 5, 1001), (1, 7, 1, 131)):
         assert B * Hkv * T * columns % 2 == 1 and size(B, Hkv, T, columns) % 16 == 0
         assert size(B, Hkv, T, columns) >= 8 * B * Hkv * T * columns
+
+
+def test_one_range_takes_no_workspace():
+    """Where the row tiles alone fill the GPU no sequence is cut, and there are no partials to hold."""
+    lib = yt.load()
+    size = lambda B, Hkv, T, columns: int(lib.ythip_paged_attn_workspace_size(_lib.BF16, B, 2 * Hkv, Hkv, T, 128, columns, 64))  # noqa: E731
+    assert size(1, 8, 4096, 64) == 0 and size(3, 8, 4096, 2048) == 0 and size(2, 8, 2100, 300) == 0
+    assert size(1, 8, 1024, 64) > 0 and size(16, 8, 2048, 100) > 0

@@ -1197,7 +1197,8 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
         // the items at the ends of a few sequences count among the slots too
         if (!p.even && B - 1 <= ranges / 2) ranges -= B - 1;
         p.target = (int)std::min(std::max<int64_t>(1, ranges), B * most);
-        p.items = part_items = (int64_t)p.target + (p.even ? 0 : B - 1);
+        p.items = (int64_t)p.target + (p.even ? 0 : B - 1);
+        if (p.target > 1) part_items = p.items;  // one range holds every sequence whole
     }
     const int64_t part_rows = part_items * Hkv * all_rows;
     p.part_bytes = (size_t)part_rows * d * sizeof(float);
