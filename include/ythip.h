@@ -569,7 +569,7 @@ int ythip_paged_attn_sparse(int dtype, int B, int Hq, int Hkv, int T, int d, con
  * may write one page (ythip_cache_fork sees to that).
  * The rows go where the table says: after a grow that may refuse a sequence (no free page) take
  * ythip_cache_append_to, which is given the lengths that the grow wrote, new_len (device
- * int32[B]), in place of n_new: sequence b takes rows kv_len[b] up to new_len[b], none where
+ * int32[B], another array than kv_len), in place of n_new: sequence b takes rows kv_len[b] up to new_len[b], none where
  * it was refused, whatever the table holds behind its pages. Rows past the T that are given are
  * zeros. `status` (NULL: none) gets YTHIP_CACHE_ERR_INDEX for a length that is negative, past
  * the table, below kv_len or more than T above it, and for a page id outside the pool.

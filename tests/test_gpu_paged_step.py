@@ -246,7 +246,7 @@ def test_calls_with_nothing_to_do():
         kn = torch.zeros(1, B, 1, T, 64, device="cuda")
         table, lens = torch.zeros(B, columns, dtype=torch.int32, device="cuda"), ints([0] * B)
         yt.cache_append(kn, kn, kp, kp.clone(), table, lens)
-        yt.cache_append(kn, kn, kp, kp.clone(), table, lens, new_len=lens)
+        yt.cache_append(kn, kn, kp, kp.clone(), table, lens, new_len=lens.clone())
         assert (kp == 0).all()
         ref = ints([1, 0, 1, 1])
         r, t, n = yt.cache_grow(ref, table, lens, ints([0] * B), 16)

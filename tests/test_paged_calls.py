@@ -9,14 +9,14 @@ import torch
 import ytensor_amd as yt
 from ytensor_amd import _lib, paged
 
-FAKE = ctypes.c_void_p(4096)
+FAKE, OTHER = ctypes.c_void_p(4096), ctypes.c_void_p(8192)
 EINVAL, EUNSUP = _lib.YTHIP_EINVAL, _lib.YTHIP_EUNSUPPORTED
 
 
 def append(lib, to, **kw):
     i4 = _lib.i64array([128] * 4)
     a = dict(dtype=_lib.BF16, L=2, B=2, Hkv=2, T=3, d=128, Kn=FAKE, Vn=FAKE, ns=i4, Kp=FAKE, Vp=FAKE, ps=i4, pages=8,
-             page=16, sums=FAKE, ss=_lib.i64array([1, 1, 1]), table=FAKE, ld=4, columns=4, kv_len=FAKE, count=FAKE,
+             page=16, sums=FAKE, ss=_lib.i64array([1, 1, 1]), table=FAKE, ld=4, columns=4, kv_len=FAKE, count=OTHER,
              path=None, ldp=3)
     a.update(kw)
     return (lib.ythip_cache_append_to(*a.values(), None, None) if to else lib.ythip_cache_append(*a.values(), None))
@@ -112,3 +112,9 @@ def test_one_range_takes_no_workspace():
     size = lambda B, Hkv, T, columns: int(lib.ythip_paged_attn_workspace_size(_lib.BF16, B, 2 * Hkv, Hkv, T, 128, columns, 64))  # noqa: E731
     assert size(1, 8, 4096, 64) == 0 and size(3, 8, 4096, 2048) == 0 and size(2, 8, 2100, 300) == 0
     assert size(1, 8, 1024, 64) > 0 and size(16, 8, 2048, 100) > 0
+
+
+def test_append_refuses_one_array_of_lengths():
+    """A grow in place and an append that is given its lengths as both: no row would be written."""
+    lib = yt.load()
+    assert append(lib, True, kv_len=FAKE, count=FAKE) == EINVAL and b"one array" in lib.ythip_last_error()

@@ -710,6 +710,7 @@ __attribute__((visibility("default"))) int ythip_cache_append_to(
     const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len, const int32_t* new_len,
     const int32_t* path, int64_t ld_path, int32_t* status, void* stream) {
     if (B > 0 && new_len == nullptr) return fail(YTHIP_EINVAL, "ythip_cache_append_to: new_len is NULL");
+    if (B > 0 && new_len == kv_len) return fail(YTHIP_EINVAL, "ythip_cache_append_to: kv_len and new_len are one array, so no row is new");
     return append("ythip_cache_append_to", dtype, layers, B, Hkv, T, d, Kn, Vn, new_str, Kp, Vp, pool_str, pages, page, sums,
                   sums_str, table, ld_table, columns, kv_len, new_len, true, path, ld_path, status, stream);
 }

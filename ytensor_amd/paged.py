@@ -304,7 +304,7 @@ def cache_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
     writes zeros. key_sums [L, P, Hkv, d]: the sums of the pages written to.
 
     kv_len is the length before, table holds the pages already (cache_grow). new_len: the
-    lengths that cache_grow wrote; a sequence that it refused gets no row, rows past the T given
+    lengths that cache_grow wrote, in a tensor of their own; a sequence that it refused gets no row, rows past the T given
     are zeros, and lengths or page ids that cannot be set CACHE_ERR_INDEX in `status`. Without
     new_len i < n_new[b] (None: T), each of which must have its page in the table."""
     away = _away(_device(k_new, v_new, k_pool, v_pool, table, kv_len, n_new, path, key_sums, new_len, status))
