@@ -504,8 +504,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     const int v_key = 4 * g + (l16 >> 2);
     const int v_frag = F ? 4 * g * S::ROWB + ((l16 >> 2) ^ (g << 2)) * 16 + (l16 & 3) * 4
                          : v_key * S::ROWB + ((v_key & BMASK) << 5) + 8 * (l16 & 3);
-    // acc += V^T . P^T for output rows 16 t..16 t + 15 over the tile's keys (CLEAN: elements of V that
-    // are not finite taken as 0); pk: p as the MFMA takes it, in 16 bits with what is left of it in `rest`
     constexpr uint32_t EXP2 = std::is_same_v<T, BF16> ? 0x7f807f80u : 0x7c007c00u, STEP2 = std::is_same_v<T, BF16> ? 0x00800080u : 0x04000400u;
     constexpr int PK = F ? S::KG : S::KG >= 2 ? S::KG / 2 : 1;
     // over 32 keys, or the 16 that a tile has
@@ -514,44 +512,41 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         else if constexpr (S::KG >= 2) return mfma_chunk(T{}, a, b, acc);
         else return mfma_half(T{}, u32x2{a[0], a[1]}, u32x2{b[0], b[1]}, acc);
     };
-    auto pv = [&](int v_at, int t, const u32x4 (&pk)[QT][PK], const u32x4 (&rest)[QT][PK], f32x4 (&acc)[QT], auto clean) {
+    // o += V^T . P^T for output rows 16 t..16 t + 15 over the kk-th keys of the tile (CLEAN: elements of V that are
+    // not finite taken as 0); pk: p as the MFMA takes it, in 16 bits with what is left of it in `rest`
+    auto pv = [&](int v_at, int t, int kk, const u32x4 (&pk)[QT][PK], const u32x4 (&rest)[QT][PK], auto clean) {
         constexpr bool CLEAN = decltype(clean)::value;
         if constexpr (F) {
 #pragma unroll
-            for (int kt = 0; kt < S::KG; ++kt)
+            for (int j = 0; j < 4; ++j) {
+                // chunk 4 t + l16 / 4 of key 16 kk + 4 g + j, stored at the chunk ^ 4 g
+                float v = *reinterpret_cast<const float*>(lds + ((v_at ^ (t << 6)) + (kk * 16 + j) * S::ROWB));
+                if (CLEAN) v = fabsf(v) < INFINITY ? v : 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // chunk 4 t + l16 / 4 of key 16 kt + 4 g + j, stored at the chunk ^ 4 g
-                    float v = *reinterpret_cast<const float*>(lds + ((v_at ^ (t << 6)) + (kt * 16 + j) * S::ROWB));
-                    if (CLEAN) v = fabsf(v) < INFINITY ? v : 0.f;
-#pragma unroll
-                    for (int qt = 0; qt < QT; ++qt)
-                        acc[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, __uint_as_float(pk[qt][kt][j]), acc[qt], 0, 0, 0);
-                }
-        } else {
-#pragma unroll
-            for (int kk = 0; kk < PK; ++kk) {
-                u32x4 vf = {0u, 0u, 0u, 0u};
-#pragma unroll
-                for (int hh = 0; hh < (S::KG >= 2 ? 2 : 1); ++hh) {
-                    // 32-byte block t of key 16 (2 kk + hh) + 4 g + l16 / 4, stored at the block ^ (key & BMASK)
-                    const u32x2 w = lds_read_tr16(smem, (v_at ^ (t << 5)) + (2 * kk + hh) * 16 * S::ROWB);
-                    vf[2 * hh] = w[0];
-                    vf[2 * hh + 1] = w[1];
-                }
-                if (CLEAN) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        // an exponent of ones carries into the bit above it
-                        const uint32_t odd = (((vf[e] & EXP2) + STEP2) >> 15) & 0x00010001u;
-                        vf[e] &= ~(odd * 0xffffu);
-                    }
-                }
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) acc[qt] = mfma_keys(vf, pk[qt][kk], acc[qt]);
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) acc[qt] = mfma_keys(vf, rest[qt][kk], acc[qt]);
+                for (int qt = 0; qt < QT; ++qt)
+                    o[qt][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, __uint_as_float(pk[qt][kk][j]), o[qt][t], 0, 0, 0);
             }
+        } else {
+            u32x4 vf = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int hh = 0; hh < (S::KG >= 2 ? 2 : 1); ++hh) {
+                // 32-byte block t of key 16 (2 kk + hh) + 4 g + l16 / 4, stored at the block ^ (key & BMASK)
+                const u32x2 w = lds_read_tr16(smem, (v_at ^ (t << 5)) + (2 * kk + hh) * 16 * S::ROWB);
+                vf[2 * hh] = w[0];
+                vf[2 * hh + 1] = w[1];
+            }
+            if (CLEAN) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // an exponent of ones carries into the bit above it
+                    const uint32_t odd = (((vf[e] & EXP2) + STEP2) >> 15) & 0x00010001u;
+                    vf[e] &= ~(odd * 0xffffu);
+                }
+            }
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) o[qt][t] = mfma_keys(vf, pk[qt][kk], o[qt][t]);
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) o[qt][t] = mfma_keys(vf, rest[qt][kk], o[qt][t]);
         }
     };
 
@@ -665,12 +660,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             }
         }
         u32x4 pk[QT][PK], rest[QT][PK];
+        // the kk-th keys' weights as the product takes them, and their sum
+        auto weigh = [&](int kk) {
+            constexpr uint32_t ONE2 = std::is_same_v<T, BF16> ? 0x3F803F80u : 0x3C003C00u;
+            constexpr u32x4 ones = {ONE2, ONE2, ONE2, ONE2};
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int kk = 0; kk < PK; ++kk) {
+            for (int qt = 0; qt < QT; ++qt) {
                 if constexpr (F) {
                     pk[qt][kk] = __builtin_bit_cast(u32x4, p[qt][kk]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        l[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, __uint_as_float(pk[qt][kk][j]), l[qt], 0, 0, 0);
                 } else {
 #pragma unroll
                     for (int i = 0; i < (S::KG >= 2 ? 4 : 2); ++i) {
@@ -682,31 +682,28 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                     }
                 }
             }
+            if constexpr (!F) {
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
+                for (int qt = 0; qt < QT; ++qt) l[qt] = mfma_keys(ones, pk[qt][kk], l[qt]);
 #pragma unroll
-            for (int kk = 0; kk < PK; ++kk) {
-                constexpr uint32_t ONE2 = std::is_same_v<T, BF16> ? 0x3F803F80u : 0x3C003C00u;
-                if constexpr (F) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        l[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, __uint_as_float(pk[qt][kk][j]), l[qt], 0, 0, 0);
-                } else {
-                    const u32x4 ones = {ONE2, ONE2, ONE2, ONE2};
-                    l[qt] = mfma_keys(ones, rest[qt][kk], mfma_keys(ones, pk[qt][kk], l[qt]));
-                }
+                for (int qt = 0; qt < QT; ++qt) l[qt] = mfma_keys(ones, rest[qt][kk], l[qt]);
             }
+        };
+        // in 16 bits over cached rows the weights of later keys are split while the matrix cores have those of earlier
+        // ones (a tree of 64 over 131072 rows 147 -> 140 us); with new tokens the registers do not reach for that
+        constexpr bool AS_IT_GOES = !NEW && !F;
+        if constexpr (!AS_IT_GOES) {
+#pragma unroll
+            for (int kk = 0; kk < PK; ++kk) weigh(kk);
+        }
         auto product = [&](auto clean) {
 #pragma unroll
-            for (int t = 0; t < S::DT; ++t) {
-                f32x4 acc[QT];
+            for (int kk = 0; kk < PK; ++kk) {
+                if constexpr (AS_IT_GOES) weigh(kk);
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt) acc[qt] = o[qt][t];
-                pv(v_at, t, pk, rest, acc, clean);
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) o[qt][t] = acc[qt];
+                for (int t = 0; t < S::DT; ++t) pv(v_at, t, kk, pk, rest, clean);
             }
-            if constexpr (!F && !decltype(clean)::value) interleave<S::DT * S::KG, S::KG, 2 * QT * PK, 3 * S::KG>();
+            if constexpr (!F && !decltype(clean)::value) interleave<S::DT * S::KG, S::KG >= 2 ? 2 : 1, 2 * QT, 10>();
         };
         if (!NEW || odd == 0) {
             __builtin_amdgcn_s_setprio(1);
