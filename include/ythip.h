@@ -529,7 +529,9 @@ enum ythip_cache_status {
  * tokens of each sequence: rows t >= new_len[b] of O are left as they were. A row that sees
  * nothing, or only scores of -inf, is zero; K and V of what a row does not see never reach
  * it, NaN and infinities included. scale == 0: 1 / sqrt(d). d in {64, 128}; strides (batch,
- * head, token), d contiguous, 16-byte aligned rows. Any of Q's type. Workspace:
+ * head, token), d contiguous, 16-byte aligned rows. Any of Q's type. The weights p of 16-bit
+ * inputs keep 16 bits (bf16) or 21 (fp16), the rest is fp32. At most 65535 sequences and query
+ * heads, T * Hq <= 2^30, fewer than 2^24 workgroups. Workspace:
  * ythip_paged_attn_workspace_size bytes (0: NULL is accepted).
  */
 size_t ythip_paged_attn_workspace_size(int dtype, int B, int Hq, int Hkv, int T, int d, int columns, int page);
@@ -546,7 +548,7 @@ int ythip_paged_attn(int dtype, int B, int Hq, int Hkv, int T, int d, const void
  * over i < ceil(kv_len[b] / page): the last of them always, then the highest scores, equal
  * ones (and NaN, the lowest) by the lower i. The new tokens are visible as above. sel
  * (contiguous int32 [B][Hkv][T][top_k]) receives the chosen i ascending, then -1 (-1 alone
- * for t >= new_len[b]). sums: strides (page, head). top_k <= 4096, columns <= 65536.
+ * for t >= new_len[b]). sums: strides (page, head). top_k <= 4096, columns <= 65536, Hkv * T <= 65535.
  */
 size_t ythip_paged_attn_sparse_workspace_size(int dtype, int B, int Hq, int Hkv, int T, int d, int columns, int page,
                                               int top_k);

@@ -118,3 +118,14 @@ def test_append_refuses_one_array_of_lengths():
     """A grow in place and an append that is given its lengths as both: no row would be written."""
     lib = yt.load()
     assert append(lib, True, kv_len=FAKE, count=FAKE) == EINVAL and b"one array" in lib.ythip_last_error()
+
+
+def test_sparse_attention_refuses_more_tokens_than_its_grid_holds():
+    lib, i3 = yt.load(), _lib.i64array([128] * 3)
+
+    def sparse(Hkv, T):
+        return lib.ythip_paged_attn_sparse(_lib.BF16, 1, Hkv, Hkv, T, 128, FAKE, i3, None, None, None, None, FAKE, FAKE, i3, 8, 16,
+                                           FAKE, i3, FAKE, 4, 4, FAKE, None, 0, None, 2, FAKE, FAKE, i3, 0.0, FAKE, 0, None)
+
+    assert sparse(8, 8192) == EUNSUP and b"65535" in lib.ythip_last_error()
+    assert sparse(5, 13107) == EINVAL and b"workspace" in lib.ythip_last_error()  # 65535: taken, and stopped further on

@@ -267,12 +267,14 @@ struct Shape {
 //   (and their sum) as two 16-bit numbers each (split2), a 256th or less of O's own rounding away
 //   from fp32's. As one number each, half a step of O's type off, they would make O's error a third
 //   larger and the kernel faster (1 token over 300 rows 8.2 -> 7.8 us, a tree of 64 over 131072 rows
-//   140 -> 119, two chunks of 512 90 -> 78).
-// Measured (MI355X): 16 sequences, 1 token, 335 MB of rows 56 us (6.0 TB/s) and 5 us for the merge; a tree
-//   of 64 over 131072 rows, 537 MB 104-112 us (4.8-5.1 TB/s) and 13; two chunks of 512 over up to 8192
-//   rows, 45 GFLOP 75 us (600 TFLOP/s, the matrix cores busy 26%, no LDS conflicts: a stage's loads,
+//   137 -> 119, two chunks of 512 93 -> 78, a first chunk of 8192 665 -> 588). The comparisons by which the
+//   cut and the loads were chosen, here and below, were made with one number.
+// Measured (MI355X): 16 sequences, 1 token, 335 MB of rows 57 us (5.9 TB/s) and 5 us for the merge; a tree
+//   of 64 over 131072 rows, 537 MB 131 us (4.1 TB/s, the matrix cores busy 41%) and 14; two chunks of 512 over up to 8192
+//   rows, 45 GFLOP 91 us (500 TFLOP/s, the matrix cores busy 35%, no LDS conflicts: a stage's loads,
 //   two products and softmax overlap only as far as two workgroups a CU let them) and 10; 1 token over
-//   300 rows 7.8 us, four round trips to memory (lengths, pages, rows, O).
+//   300 rows 8.2 us, trips to memory one after the other (lengths, pages, five stages of rows of which two are
+//   in flight, O).
 template <class T, int D, int QT, int WR, bool SPARSE>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     using S = Shape<T, D, QT, WR>;
