@@ -129,3 +129,10 @@ def test_sparse_attention_refuses_more_tokens_than_its_grid_holds():
 
     assert sparse(8, 8192) == EUNSUP and b"65535" in lib.ythip_last_error()
     assert sparse(5, 13107) == EINVAL and b"workspace" in lib.ythip_last_error()  # 65535: taken, and stopped further on
+
+
+def test_grow_refuses_its_counts_as_the_lengths_to_write():
+    lib = yt.load()
+    grow = lambda n, out: lib.ythip_cache_grow(2, 4, 8, 16, FAKE, FAKE, 4, FAKE, n, FAKE, FAKE, 4, out, None, None)  # noqa: E731
+    assert grow(OTHER, OTHER) == EINVAL and b"one array" in lib.ythip_last_error()
+    assert grow(None, OTHER) == EINVAL and b"NULL" in lib.ythip_last_error()

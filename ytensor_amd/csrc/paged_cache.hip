@@ -724,6 +724,8 @@ __attribute__((visibility("default"))) int ythip_cache_grow(int B, int columns, 
     if (const int st = check_state(who, B, columns, pages, page, ref, table, ld_table, len, ref_out, table_out, ld_out, len_out)) return st;
     if (B > MAX_SEQS) return fail(YTHIP_EUNSUPPORTED, "%s: %d sequences (at most %d)", who, B, MAX_SEQS);
     if (B > 0 && n_new == nullptr) return fail(YTHIP_EINVAL, "%s: n_new is NULL", who);
+    // (the lengths are copied there before the counts are read)
+    if (B > 0 && n_new == len_out && len != len_out) return fail(YTHIP_EINVAL, "%s: n_new and the lengths to write are one array", who);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const StateArgs st = copy_state({false, B, columns, pages, ref, table, len, ld_table, ld_out, ref_out, table_out, len_out}, B == 0, s);
     if (B > 0) cache_grow_kernel<<<1, PLAN_THREADS, 0, s>>>({B, columns, pages, page_shift(page), n_new, ref_out, table_out, len_out, ld_out, status, st});
