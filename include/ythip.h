@@ -630,6 +630,50 @@ int ythip_cache_copy_pages(int pages, int n, const int32_t* src, const int32_t* 
                            const ythip_page_pool* pools, int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Drafted tokens. No counterpart in the reference, whose step ends with the greedy token
+ * (ythip_argmax_step): the end of a step whose new tokens were drafted (ythip_paged_attn's
+ * `parents`), which gives the path and the counts that ythip_cache_grow and
+ * ythip_cache_append take.
+ * ---------------------------------------------------------------------- */
+
+/*
+ * probs[r] = softmax(logits[r] / temperature) over n columns, in fp32, of rows at strides
+ * ld and ld_out (>= n; any alignment of an element). -inf has probability 0, a row of them
+ * zeros; NaN or +inf makes its row NaN. temperature > 0. rows < 2^22. Workspace:
+ * ythip_token_probs_workspace_size bytes, 8-byte aligned (0: NULL is accepted).
+ */
+size_t ythip_token_probs_workspace_size(int rows, int n);
+int ythip_token_probs(int dtype, int rows, int n, const void* logits, int64_t ld, float temperature, float* probs,
+                      int64_t ld_out, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Which of a sequence's T new tokens are kept, and the token that comes next, drawn by given
+ * random numbers in [0, 1) such that both are distributed as the target's.
+ *   target   [B][T][V] probabilities after each new token, strides (batch, token)
+ *   tokens   int32 [B][T]; token 0 is known and always kept. parents as in ythip_paged_attn
+ *            (NULL: a chain); tree_len (NULL: T): the new tokens of each sequence
+ *   draft    NULL: from token n on, u[b][n] falls into one of the intervals that the
+ *            probabilities of n's children take of [0, 1) in their order (of siblings with one
+ *            token the first has it), and that child is kept, or into none. next is drawn from
+ *            n's row without its children's tokens
+ *   draft    [B][T][V], parents NULL: what token t was drawn from. t is kept while
+ *            u[b][t] draft[b][t][token] < target[b][t - 1][token]. next is drawn from the last
+ *            kept token's row less draft's row of the refused one, where that is positive
+ * After the last token of a path nothing is taken off; where nothing is left the row counts
+ * as it is. The draw: the first entry at which the sum of the weights passes u_next[b] times
+ * all of them. What is not a positive number has no weight; a token outside [0, V) is never
+ * kept. All of it in 64 bits. path int32 [B][T]: the kept tokens' numbers, then -1; kept
+ * int32 [B]; next int32 [B], -1 where tree_len is 0 or the row has no weight. T <= 1024,
+ * V <= 2^22, B <= 65535. Workspace: ythip_verify_drafts_workspace_size bytes, 8-byte aligned.
+ */
+size_t ythip_verify_drafts_workspace_size(int B, int V);
+int ythip_verify_drafts(int dtype, int B, int T, int V, const void* target, const int64_t target_str[2],
+                        const void* draft, const int64_t draft_str[2], const int32_t* tokens, int64_t ld_tokens,
+                        const int32_t* parents, int64_t ld_parents, const int32_t* tree_len, const float* u,
+                        int64_t ld_u, const float* u_next, int32_t* path, int64_t ld_path, int32_t* kept,
+                        int32_t* next, void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * .yt checkpoint files (yt::io::YTensorIO, include/ytensor_io.hpp:81-180,
  * src/ytensor_io.inl) read straight into device memory and written from it.
  * Host-side calls: paths and the info/tensor descriptors are HOST memory,

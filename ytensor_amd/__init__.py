@@ -39,6 +39,7 @@ from .paged import (  # noqa: F401
     paged_sparse_attention,
     paged_workspace_bytes,
 )
+from .sampling import token_probs, verify_drafts  # noqa: F401
 
 
 def load():
@@ -53,4 +54,5 @@ __all__ = [
     "gemv_fused", "gemv_swiglu", "gemv_attn_merge", "argmax_finish", "io", "masked_matmul", "gemm_masked",
     "paged_attention", "paged_sparse_attention", "paged_workspace_bytes", "cache_grow", "cache_append", "cache_fork",
     "cache_free", "cache_compact", "cache_copy_pages", "CACHE_ERR_INDEX", "CACHE_ERR_BUSY", "CACHE_ERR_FULL",
+    "token_probs", "verify_drafts",
 ]

@@ -112,6 +112,11 @@ SIGNATURES = {
     "ythip_cache_compact_workspace_size": (ctypes.c_size_t, [_I]),
     "ythip_cache_compact": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _P, _P, _L, _P, _I, _I, _P, _P, ctypes.c_size_t, _P]),
     "ythip_cache_copy_pages": (_I, [_I, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "ythip_token_probs_workspace_size": (ctypes.c_size_t, [_I, _I]),
+    "ythip_token_probs": (_I, [_I, _I, _I, _P, _L, _F, _P, _L, _P, ctypes.c_size_t, _P]),
+    "ythip_verify_drafts_workspace_size": (ctypes.c_size_t, [_I, _I]),
+    "ythip_verify_drafts": (_I, [_I, _I, _I, _I, _P, _LP, _P, _LP, _P, _L, _P, _L, _P, _P, _L, _P, _P, _L, _P, _P, _P,
+                                 ctypes.c_size_t, _P]),
     "ythip_yt_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "ythip_yt_close": (_I, [_P]),
     "ythip_yt_count": (_I, [_P]),
