@@ -543,6 +543,24 @@ int ythip_paged_attn(int dtype, int B, int Hq, int Hkv, int T, int d, const void
                      const int64_t o_str[3], float scale, void* workspace, size_t ws_bytes, void* stream);
 
 /*
+ * ythip_paged_attn with a sliding window: of what token t sees there, what lies less than
+ * `window` positions before it (t itself is 0 before) or among the first `sinks` positions.
+ * Cached row r is at position r, new token t at kv_len[b] + the tokens above it on its path
+ * (parents NULL: kv_len[b] + t). Rows that no new token sees are not read. window 0: no
+ * window; a Kn that is NULL changes nothing about the positions. Workspace:
+ * ythip_paged_attn_window_workspace_size bytes.
+ */
+size_t ythip_paged_attn_window_workspace_size(int dtype, int B, int Hq, int Hkv, int T, int d, int columns, int page,
+                                              int window, int sinks);
+int ythip_paged_attn_window(int dtype, int B, int Hq, int Hkv, int T, int d, const void* Q, const int64_t q_str[3],
+                            const void* Kn, const int64_t kn_str[3], const void* Vn, const int64_t vn_str[3],
+                            const void* Kp, const void* Vp, const int64_t pool_str[3], int pages, int page,
+                            const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len,
+                            const int32_t* parents, int64_t ld_parents, const int32_t* new_len, int window, int sinks,
+                            void* O, const int64_t o_str[3], float scale, void* workspace, size_t ws_bytes,
+                            void* stream);
+
+/*
  * ythip_paged_attn over the cached rows of top_k pages, chosen for each new token t and KV
  * head h by score(i) = (sum of Q[b, h's query heads, t]) . sums[table[b][i]][h] in 64 bits,
  * over i < ceil(kv_len[b] / page): the last of them always, then the highest scores, equal

@@ -97,6 +97,9 @@ SIGNATURES = {
     "ythip_paged_attn_workspace_size": (ctypes.c_size_t, [_I] * 8),
     "ythip_paged_attn": (_I, [_I, _I, _I, _I, _I, _I, _P, _LP, _P, _LP, _P, _LP, _P, _P, _LP, _I, _I, _P, _L, _I, _P,
                               _P, _L, _P, _P, _LP, _F, _P, ctypes.c_size_t, _P]),
+    "ythip_paged_attn_window_workspace_size": (ctypes.c_size_t, [_I] * 10),
+    "ythip_paged_attn_window": (_I, [_I, _I, _I, _I, _I, _I, _P, _LP, _P, _LP, _P, _LP, _P, _P, _LP, _I, _I, _P, _L, _I,
+                                     _P, _P, _L, _P, _I, _I, _P, _LP, _F, _P, ctypes.c_size_t, _P]),
     "ythip_paged_attn_sparse_workspace_size": (ctypes.c_size_t, [_I] * 9),
     "ythip_paged_attn_sparse": (_I, [_I, _I, _I, _I, _I, _I, _P, _LP, _P, _LP, _P, _LP, _P, _P, _LP, _I, _I, _P, _LP,
                                      _P, _L, _I, _P, _P, _L, _P, _I, _P, _P, _LP, _F, _P, ctypes.c_size_t, _P]),

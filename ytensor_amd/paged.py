@@ -90,12 +90,12 @@ def _rows(t: torch.Tensor, es: int) -> tuple[torch.Tensor, int, tuple]:
 
 
 def _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, scale, out,
-               workspace):
+               workspace, window=0, sinks=0):
     away = _away(_device(q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len, out, workspace))
     if away is not None:
         with away:
             return _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, parents, tree_len,
-                              scale, out, workspace)
+                              scale, out, workspace, window, sinks)
     if q.dim() != 4 or k_pool.dim() != 4:
         raise ValueError("q must be [B, Hq, T, d] and the pools [P, Hkv, page, d]")
     B, Hq, T, d = q.shape
@@ -130,7 +130,7 @@ def _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, 
         out = (torch.empty if tree_len is None else torch.zeros)((B, Hq, T, d), dtype=dt, device=q.device)
     elif out.shape != (B, Hq, T, d) or out.dtype != dt or out.stride(3) != 1:
         raise ValueError(f"out must be {dt} {[B, Hq, T, d]} with d contiguous")
-    need = _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k or 0)
+    need = _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k or 0, window, sinks)
     ws_at, ws_bytes = None, 0
     if need:
         if workspace is not None and not workspace.is_contiguous():
@@ -140,6 +140,14 @@ def _attention(top_k, q, k_new, v_new, k_pool, v_pool, key_sums, table, kv_len, 
         ws_at, ws_bytes = workspace.data_ptr(), need
     par_at = None if parents is None else parents.data_ptr()
     tl_at = None if tree_len is None else tree_len.data_ptr()
+    if top_k is None and window:
+        st = _lib.lib().ythip_paged_attn_window(
+            code, B, Hq, Hkv, T, d, q_at, _i64(q_st), kn_at, kn_st, vn_at, vn_st, k_pool.data_ptr(),
+            v_pool.data_ptr(), _i64(pool_st), P, page, table.data_ptr(), ld, columns, kv_len.data_ptr(), par_at, T,
+            tl_at, window, sinks, out.data_ptr(), _i64(out.stride()), scale, ws_at, ws_bytes, _stream())
+        if st:
+            check(st, "ythip_paged_attn_window")
+        return out
     if top_k is None:
         st = _lib.lib().ythip_paged_attn(
             code, B, Hq, Hkv, T, d, q_at, _i64(q_st), kn_at, kn_st, vn_at, vn_st, k_pool.data_ptr(),
@@ -174,22 +182,32 @@ def _table(table: torch.Tensor, B: int) -> tuple[torch.Tensor, int, int]:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k) -> int:
+def _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k, window=0, sinks=0) -> int:
+    if window:
+        return int(_lib.lib().ythip_paged_attn_window_workspace_size(code, B, Hq, Hkv, T, d, columns, page, window, sinks))
     if top_k:
         return int(_lib.lib().ythip_paged_attn_sparse_workspace_size(code, B, Hq, Hkv, T, d, columns, page, top_k))
     return int(_lib.lib().ythip_paged_attn_workspace_size(code, B, Hq, Hkv, T, d, columns, page))
 
 
 def paged_workspace_bytes(dtype: torch.dtype, B: int, Hq: int, Hkv: int, T: int, d: int, columns: int, page: int,
-                          top_k: int = 0) -> int:
+                          top_k: int = 0, window: int = 0, sinks: int = 0) -> int:
     """Bytes that paged_attention (top_k 0) or paged_sparse_attention writes."""
-    return _workspace(_DT[dtype], B, Hq, Hkv, T, d, columns, page, top_k)
+    return _workspace(_DT[dtype], B, Hq, Hkv, T, d, columns, page, top_k, *_window(window, sinks))
+
+
+def _window(window, sinks) -> tuple[int, int]:
+    """The window as the C calls take it: at most 2^30, which no row lies further behind."""
+    if window < 0 or sinks < 0:
+        raise ValueError(f"a window of {window} and {sinks} sinks")
+    return (min(int(window), 1 << 30), min(int(sinks), 1 << 30)) if window else (0, 0)
 
 
 def paged_attention(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None, k_pool: torch.Tensor,
                     v_pool: torch.Tensor, table: torch.Tensor, kv_len: torch.Tensor,
                     parents: torch.Tensor | None = None, tree_len: torch.Tensor | None = None, scale: float = 0.0,
-                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, window: int = 0,
+                    sinks: int = 0) -> torch.Tensor:
     """Attention of T new tokens a sequence, q [B, Hq, T, d], over the kv_len[b] cached rows of
     a layer's pools and the tokens' own k_new / v_new [B, Hkv, T, d] (None: the cache alone).
 
@@ -199,9 +217,11 @@ def paged_attention(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Te
     new tokens of each sequence; rows behind them in `out` are left as they were (zeros in an
     `out` made here). Query head h reads KV head h // (Hq // Hkv). A page id outside the pool
     hides its rows; a row that sees nothing is zero. d 64 or 128, page a power of two >= 16.
+    window > 0: of these, a token sees what lies less than `window` positions before it (itself the first), and the
+    first `sinks` positions. Cached row r is at position r, new token t at kv_len[b] + the tokens above it.
     Returns out [B, Hq, T, d]."""
     return _attention(None, q, k_new, v_new, k_pool, v_pool, None, table, kv_len, parents, tree_len, float(scale), out,
-                      workspace)
+                      workspace, *_window(window, sinks))
 
 
 def paged_sparse_attention(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None,
