@@ -648,6 +648,55 @@ int ythip_cache_copy_pages(int pages, int n, const int32_t* src, const int32_t* 
                            const ythip_page_pool* pools, int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------
+ * 4-bit pages: the paged cache's K and V in 4 bits and a little for scales. Pools are bytes,
+ * [pages][Hkv] blocks of page (d / 2 + d / 32) bytes at strides pool_str (page, head; with
+ * layers in front of them where a call takes them), in bytes, 16-byte aligned; d in {64, 128}.
+ * Groups of 32 neighbouring channels of a row share a scale 2^e (a byte, e + 127; 255: the
+ * group is NaN); a code is a sign (8) and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (0 to 7), channel
+ * 2 i in the low half of its byte:
+ *   K  codes [page][d / 2], scales [page][d / 32]
+ *   V  codes [page / 8][16][8][d / 32] (entry i of 16: channels i d / 16 and on of 8 rows),
+ *      scales [page / 8][d / 32][8]
+ * Table, lengths and bookkeeping are the paged cache's: the blocks of a page are a
+ * ythip_page_pool.
+ * ---------------------------------------------------------------------- */
+
+/* Bytes of a page and KV head; 0 for a page or head dim that there is not. */
+int64_t ythip_cache_q4_bytes(int page, int d);
+
+/*
+ * ythip_cache_append (n_new; NULL: T) or, where new_len is given, ythip_cache_append_to, into
+ * 4-bit pages. A group's scale is the smallest power of two with which its largest magnitude is
+ * at most 7, within [2^-125, 2^125] (float16: 2^13), a value's code the nearest (of two as near
+ * the even one), the largest for what lies beyond; a group with a NaN or an infinity gets
+ * scale byte 255. new_str in elements (layer, batch, head, token), pool_str in bytes (layer,
+ * page, head). No two sequences may write one page.
+ */
+int ythip_cache_append_q4(int dtype, int layers, int B, int Hkv, int T, int d, const void* Kn, const void* Vn,
+                          const int64_t new_str[4], void* Kp, void* Vp, const int64_t pool_str[3], int pages, int page,
+                          const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len,
+                          const int32_t* n_new, const int32_t* new_len, const int32_t* path, int64_t ld_path,
+                          int32_t* status, void* stream);
+
+/* The values of whole pools, in dtype: K and V contiguous [layers][pages][Hkv][page][d]. */
+int ythip_cache_unpack_q4(int dtype, int layers, int pages, int Hkv, int page, int d, const void* Kp, const void* Vp,
+                          const int64_t pool_str[3], void* K, void* V, void* stream);
+
+/*
+ * ythip_paged_attn_window (window 0: ythip_paged_attn) over 4-bit pages. Q, Kn, Vn and O are of
+ * dtype; the cached values take part as they are. Weights keep 16 bits (fp32: 24), queries all
+ * of theirs, the rest is fp32.
+ */
+size_t ythip_paged_attn_q4_workspace_size(int dtype, int B, int Hq, int Hkv, int T, int d, int columns, int page,
+                                          int window, int sinks);
+int ythip_paged_attn_q4(int dtype, int B, int Hq, int Hkv, int T, int d, const void* Q, const int64_t q_str[3],
+                        const void* Kn, const int64_t kn_str[3], const void* Vn, const int64_t vn_str[3],
+                        const void* Kp, const void* Vp, const int64_t pool_str[2], int pages, int page,
+                        const int32_t* table, int64_t ld_table, int columns, const int32_t* kv_len,
+                        const int32_t* parents, int64_t ld_parents, const int32_t* new_len, int window, int sinks,
+                        void* O, const int64_t o_str[3], float scale, void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Drafted tokens. No counterpart in the reference, whose step ends with the greedy token
  * (ythip_argmax_step): the end of a step whose new tokens were drafted (ythip_paged_attn's
  * `parents`), which gives the path and the counts that ythip_cache_grow and

@@ -69,7 +69,9 @@ def attention(q, k_new, v_new, cached, kv_len, parents=None, tree_len=None, wind
                 av = p @ vt.abs()
                 S = (abs(scale) * (qd[b, rows, t].abs() @ kt.abs().T)).amax(-1, keepdim=True)
                 f32 = 2.0 ** -24 * (2 * (d + 3) * S + 8 + 2 * len(kt))
-                tol[b, rows, t] = 1.01 * (2 * u * o.abs() + u * av + f32 * av)
+                # (a weight below 2^-126 of the largest is no normal float32 and may be lost, in the product and in the
+                # sum: 2^-126 (|v| + |o|) a key, which counts where the others' V is exactly 0)
+                tol[b, rows, t] = 1.01 * (2 * u * o.abs() + u * av + f32 * av) + 2.0 ** -125 * len(kt) * vt.abs().max()
                 if q.dtype == torch.float16:
                     tol[b, rows, t] += 2.0 ** -25 * len(kt) * vt.abs().max()
     return out, tol

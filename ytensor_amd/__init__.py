@@ -39,6 +39,13 @@ from .paged import (  # noqa: F401
     paged_sparse_attention,
     paged_workspace_bytes,
 )
+from .paged_q4 import (  # noqa: F401
+    cache_append_q4,
+    cache_q4_bytes,
+    cache_unpack_q4,
+    paged_attention_q4,
+    paged_q4_workspace_bytes,
+)
 from .sampling import token_probs, verify_drafts  # noqa: F401
 
 
@@ -54,5 +61,6 @@ __all__ = [
     "gemv_fused", "gemv_swiglu", "gemv_attn_merge", "argmax_finish", "io", "masked_matmul", "gemm_masked",
     "paged_attention", "paged_sparse_attention", "paged_workspace_bytes", "cache_grow", "cache_append", "cache_fork",
     "cache_free", "cache_compact", "cache_copy_pages", "CACHE_ERR_INDEX", "CACHE_ERR_BUSY", "CACHE_ERR_FULL",
+    "cache_q4_bytes", "cache_append_q4", "cache_unpack_q4", "paged_attention_q4", "paged_q4_workspace_bytes",
     "token_probs", "verify_drafts",
 ]

@@ -115,6 +115,13 @@ SIGNATURES = {
     "ythip_cache_compact_workspace_size": (ctypes.c_size_t, [_I]),
     "ythip_cache_compact": (_I, [_I, _I, _I, _I, _P, _P, _L, _P, _P, _P, _L, _P, _I, _I, _P, _P, ctypes.c_size_t, _P]),
     "ythip_cache_copy_pages": (_I, [_I, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "ythip_cache_q4_bytes": (_L, [_I, _I]),
+    "ythip_cache_append_q4": (_I, [_I, _I, _I, _I, _I, _I, _P, _P, _LP, _P, _P, _LP, _I, _I, _P, _L, _I, _P, _P, _P, _P, _L,
+                                   _P, _P]),
+    "ythip_cache_unpack_q4": (_I, [_I, _I, _I, _I, _I, _I, _P, _P, _LP, _P, _P, _P]),
+    "ythip_paged_attn_q4_workspace_size": (ctypes.c_size_t, [_I] * 10),
+    "ythip_paged_attn_q4": (_I, [_I, _I, _I, _I, _I, _I, _P, _LP, _P, _LP, _P, _LP, _P, _P, _LP, _I, _I, _P, _L, _I, _P, _P,
+                                 _L, _P, _I, _I, _P, _LP, _F, _P, ctypes.c_size_t, _P]),
     "ythip_token_probs_workspace_size": (ctypes.c_size_t, [_I, _I]),
     "ythip_token_probs": (_I, [_I, _I, _I, _P, _L, _F, _P, _L, _P, ctypes.c_size_t, _P]),
     "ythip_verify_drafts_workspace_size": (ctypes.c_size_t, [_I, _I]),

@@ -33,9 +33,6 @@ __device__ __forceinline__ f32x4 mfma_half(F16, u32x2 a, u32x2 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
 }
 
-// The bits from i on (i < 0: all; i > 63: none).
-__device__ __forceinline__ uint64_t from_bit(int i) { return i <= 0 ? ~0ull : i > 63 ? 0 : ~0ull << i; }
-
 __device__ __forceinline__ void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // The order of a product's instructions: AHEAD of its READS reads from LDS first, then MF MFMAs and
@@ -209,7 +206,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
                 for (int u = tok[qt]; u >= 0; u = s_up[u]) ++deep[qt];
             }
             up[qt] = 0;
-            lo[qt] = max(len + deep[qt] + 1 - a.window, 0);
+            lo[qt] = (int)max((int64_t)len + deep[qt] + 1 - a.window, (int64_t)0);
         }
         const raw* qp = static_cast<const raw*>(a.Q) + b * a.qs[0] + (int64_t)(h * a.G + gh) * a.qs[1] + t * a.qs[2];
 #pragma unroll
@@ -410,14 +407,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             for (int qt = 0; qt < QT; ++qt) {
                 if (walk) {
                     while (cur[qt] >= u0) {
-                        const bool in = !WIN || up[qt] < a.window || len + deep[qt] - up[qt] < a.sinks;
+                        const bool in = !WIN || up[qt] < a.window || deep[qt] - up[qt] < a.sinks - len;
                         if (in && cur[qt] < u0 + KT) see[qt] |= 1ull << (cur[qt] - u0);
                         cur[qt] = s_up[cur[qt]];
                         if constexpr (WIN) ++up[qt];
                     }
                 } else if (tok[qt] >= u0) {
                     see[qt] = tok[qt] - u0 >= 63 ? ~0ull : (2ull << (tok[qt] - u0)) - 1;
-                    if constexpr (WIN) see[qt] &= from_bit(tok[qt] + 1 - a.window - u0) | ~from_bit(a.sinks - len - u0);
+                    if constexpr (WIN) see[qt] &= from_bit((int64_t)tok[qt] + 1 - a.window - u0) | ~from_bit((int64_t)a.sinks - len - u0);
                 }
                 any = any || see[qt] != 0;
                 paths = paths || see[qt] != (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
@@ -916,16 +913,7 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
     const int64_t groups = (p.items * a.Hkv + 7) / 8 * 8;
     using S = Shape<T, D, QT, WR>;
     paged_attn_kernel<T, D, QT, WR, SPARSE, WIN><<<(int)(groups * p.row_tiles), 256, 0, s>>>(a);
-    if (p.part_bytes > 0) {
-        constexpr int ROWS = 256 / D;  // of a wave
-        const int rows = a.T * a.G;
-        // few rows: a workgroup's waves share them (16 rows of 32 partials 6.8 -> 4.9 us; 5000 rows of
-        // about 12 8.3 -> 9.9)
-        if ((int64_t)a.B * a.Hkv * rows <= 512)
-            paged_merge_kernel<T, D, SPARSE, true><<<dim3((rows + ROWS - 1) / ROWS, a.Hkv, a.B), 256, 0, s>>>(a, S::KT);
-        else
-            paged_merge_kernel<T, D, SPARSE, false><<<dim3((rows + 4 * ROWS - 1) / (4 * ROWS), a.Hkv, a.B), 256, 0, s>>>(a, S::KT);
-    }
+    if (p.part_bytes > 0) merge_partials<T, D, SPARSE>(a, S::KT, s);
     return status_of(hipGetLastError());
 }
 template <class T, int D, bool SPARSE, bool WIN>
@@ -966,6 +954,7 @@ int run(int dtype, int d, PagedArgs& a, void* ws, hipStream_t s) {
 
 size_t workspace(int dtype, int B, int Hq, int Hkv, int T, int d, int columns, int page, int top_k, int window = 0, int sinks = 0) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || d <= 0 || columns < 0 || page <= 0 || top_k < 0 || Hq % Hkv != 0 || window < 0 || sinks < 0) return 0;
+    trim_window(T, columns, page, window, sinks);
     return plan_of(dtype, B, Hkv, Hq / Hkv, T, d, columns, page, top_k, window, sinks).bytes();
 }
 
@@ -1019,6 +1008,7 @@ __attribute__((visibility("default"))) int ythip_paged_attn_window(
     const int st = prepare(who, c, a, done);
     if (st || done) return st;
     if (const int e = check_workspace(who, workspace(dtype, B, Hq, Hkv, T, d, columns, page, 0, window, sinks), workspace_, ws_bytes)) return e;
+    trim_window(T, columns, page, window, sinks);
     a.window = window, a.sinks = sinks;
     if (window == 0) return run<false, false>(dtype, d, a, workspace_, static_cast<hipStream_t>(stream));
     return run<false, true>(dtype, d, a, workspace_, static_cast<hipStream_t>(stream));

@@ -197,10 +197,10 @@ def paged_workspace_bytes(dtype: torch.dtype, B: int, Hq: int, Hkv: int, T: int,
 
 
 def _window(window, sinks) -> tuple[int, int]:
-    """The window as the C calls take it: at most 2^30, which no row lies further behind."""
+    """The window as the C calls take it."""
     if window < 0 or sinks < 0:
         raise ValueError(f"a window of {window} and {sinks} sinks")
-    return (min(int(window), 1 << 30), min(int(sinks), 1 << 30)) if window else (0, 0)
+    return (min(int(window), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1)) if window else (0, 0)
 
 
 def paged_attention(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch.Tensor | None, k_pool: torch.Tensor,
