@@ -350,6 +350,27 @@ def test_large_and_close_scores(dtype):
     compare(yt.paged_attention_q4(q, kn, vn, k, v, table, kv_len, page), want, tol)
 
 
+@pytest.mark.parametrize("dtype,d", [("f16", 64), ("f32", 128), ("bf16", 128), ("bf16", 64), ("f16", 128), ("f32", 64)])
+def test_queries_of_all_sizes(dtype, d):
+    """Channels of a query far apart in size, tiny and zero queries; one that is not finite is NaN and no other is."""
+    dt, page, n, T = DT[dtype], 16, 150, 5
+    g, k, v, table, kv_len = cache4(3, [n], 1, page, d, dt)
+    q, kn, vn = tokens(g, 1, 4, 1, T, d, dt)
+    size = torch.exp2(torch.randint(-14, 4, q.shape, generator=g).float()).cuda()
+    q = (q.float() * size).to(dt)
+    q[0, 0, 0], q[0, 1, 1] = 0.0, q[0, 1, 1] * torch.finfo(dt).tiny
+    q[0, 2, 2, 32:] = 0.0
+    want, tol = attention(q, kn, vn, rows4(k, v, table, kv_len, page, d), kv_len)
+    compare(yt.paged_attention_q4(q, kn, vn, k, v, table, kv_len, page), want, tol)
+    bad = q.clone()
+    bad[0, 3, 4, 7], bad[0, 1, 0, 40], bad[0, 2, 1, d - 1] = math.inf, math.nan, -math.inf
+    out = yt.paged_attention_q4(bad, kn, vn, k, v, table, kv_len, page).cpu()
+    hit = torch.zeros(1, 4, T, dtype=torch.bool)
+    hit[0, 3, 4] = hit[0, 1, 0] = hit[0, 2, 1] = True
+    assert out[hit].isnan().all()
+    compare(out[~hit], want[~hit], tol[~hit])
+
+
 # ------------------------------------------------------------------ used together
 
 def test_a_served_step():

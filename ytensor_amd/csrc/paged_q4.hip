@@ -259,35 +259,52 @@ __device__ __forceinline__ float sum_across_rows(float v) {
     return __uint_as_float(p32[0]) + __uint_as_float(p32[1]);
 }
 
+// What stands in for a pool that has no pages: a tile's loads go there.
+static __device__ const u32x4 no_pages[2 * 64 * 64 / 16] = {};
+
+// (a lambda that is not inlined has its arrays in memory)
+#define INLINE __attribute__((always_inline))
+
 template <int D, int QT, int WR>
 struct Q4Shape {
-    static constexpr int KT = 32, WK = 4 / WR, RW = 16 * QT * WR;
-    static constexpr int KS = D / 32, DT = D / 16, OLD = D + 4;
-    static constexpr int EPI = WK == 1 ? 1 : WK * RW * (OLD + 2);  // floats
+    static constexpr bool SHARED = WR == 4;
+    static constexpr int KT = SHARED ? 64 : 32, WK = 4 / WR, RW = 16 * QT * WR;
+    // Workgroups of a CU: three where 168 registers hold the queries' pieces, else two. Three load the next tile while one is
+    // converted, two the next but one (16 sequences, 1 token, up to 32768 rows: 3 and 1 82 us, 2 and 2 88, 2 and 1 98, 3 and
+    // 2 85).
+    static constexpr int waves(bool bf16) { return QT == 1 && WR == 1 && (bf16 || D == 64) ? 3 : 2; }
+    static constexpr int KS = D / 32, DT = D / 16, GROUPS = D / 32, OLD = D + 4;
+    static constexpr int KF = 4 * KS, VF = 2 * DT;  // fragments of a tile (a register quadruple of each lane): of 16 rows, of 32
+    // (in 16-byte chunks) two converted tiles, or the key groups' results
+    static constexpr int LDS = SHARED ? 2 * 64 * (KF + VF) : (WK * RW * (OLD + 2) * 4 + 15) / 16;
 };
 
 // One workgroup: RW = 16 QT WR query rows of one KV head (row = token * G + head of the group) over a chunk of its
-// sequence's tiles of 32 rows; its waves are WR row groups x WK key groups, and nothing is shared between them but the
-// result: every wave loads codes straight into registers, AHEAD tiles early, and has them as the matrix cores take them
-// after one conversion a pair.
-//   S^T = K . Q^T: lane (l16, g) has row 8 (l16 / 4) + l16 % 4 (and + 4) of the tile, channels g D / 4 and on (the
-//     products' order over channels is free: Q is laid out alike), which is 16 (8) bytes of codes and one scale. Of S^T it
-//     has query l16 and rows 8 g .. 8 g + 7, in the order in which the second product takes its weights.
+// sequence's tiles of 32 or 64 rows; its four waves have all its rows and a tile each in turn (WR 1), or its rows by fourths
+// and every tile (WR 4). Codes go straight into registers, a tile or two early, and are bfloat16 after one conversion a
+// pair; few rows: each wave converts its own tiles, many: each a fourth of every tile, which all read from LDS.
+//   S^T = K . Q^T: of 16 rows (subtile j) lane (l16, g) has row 32 (j / 2) + 8 (l16 / 4) + l16 % 4 + 4 (j % 2) of the
+//     tile, channels g D / 4 and on (the products' order over channels is free: Q is laid out alike), which is 16 (8) bytes
+//     of codes and one scale. Of S^T it has query l16 and of each 32 rows rows 8 g .. 8 g + 7, in the order in which the
+//     second product takes its weights.
 //   O^T = V^T . P^T: the lane has rows 8 g .. 8 g + 7 of channels l16 D / 16 and on, 32 (16) consecutive bytes of a V block
 //     and 8 scales; converted row by row, then paired by row (v_perm), it has each of its channels over 8 rows, which is
 //     row l16 of channel tile t. So tile t's row i is channel i D / 16 + t.
 //   New tokens are of the queries' type: their scores on its own matrix instruction, their V as bfloat16 pieces.
 // Numerics: queries and weights as bfloat16 pieces (split) that hold all bits of the queries and 16 (24 for fp32) of the
-//   weights; scores, maxima, sums and O in fp32.
+//   weights; scores, maxima, sums and O in fp32. (The matrix cores' scaled product would take K's codes as they are, with
+//   the queries as e4m3 pieces, but of every 8 products it drops what is 2^13 below the largest: fp32 scores were off by
+//   2^-15 of their terms.)
 template <class T, int D, int QT, int WR, bool WIN>
-__global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, BF16>))) void paged_q4_kernel(PagedArgs a) {
     using S = Q4Shape<D, QT, WR>;
     using raw = typename T::raw;
-    constexpr bool F = std::is_same_v<T, F32>;
-    constexpr int KT = S::KT, KS = S::KS, DT = S::DT, NQ = pieces<T>(), NW = F ? 3 : 2, AHEAD = 3;
+    constexpr bool F = std::is_same_v<T, F32>, SHARED = S::SHARED;
+    constexpr int KT = S::KT, SUB = KT / 16, KG = KT / 32, KS = S::KS, DT = S::DT, NQ = pieces<T>(), NW = F ? 3 : 2, GROUPS = S::GROUPS;
     constexpr int ES = sizeof(raw);
-    __shared__ float s_epi[S::EPI];
+    __shared__ u32x4 smem[S::LDS];
     __shared__ int16_t s_up[MAX_TREE];
+    __shared__ uint32_t s_odd[SHARED ? 2 * 4 * 2 : 1];  // of a converted tile: bits of rows without a value, by channel group
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR;
     const int l16 = lane & 15, g = lane >> 4;
@@ -342,6 +359,79 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
         __syncthreads();
     }
 
+    // ---- tiles of cached rows: lookups and loads
+    const int page = 1 << a.shift;
+    const uint8_t *Kp = static_cast<const uint8_t*>(a.Kp) + h * a.ps[1], *Vp = static_cast<const uint8_t*>(a.Vp) + h * a.ps[1];
+    auto tile_at = [&](int s) { return WIN ? win.at(s * S::WK + wk) : win.high - 1 - (s * S::WK + wk); };
+    struct Ids {
+        int id[SUB];  // of the tile's 16 rows each
+    };
+    auto ids = [&](int s) INLINE {
+        Ids x;
+#pragma unroll
+        for (int i = 0; i < SUB; ++i) x.id[i] = -1;
+        const int ti = tile_at(s);
+        if (ti < c0 || ti >= nct) return x;
+        const int row = seen.row(ti, KT);
+#pragma unroll
+        for (int i = 0; i < SUB; ++i)
+            if (row + 16 * i < len) x.id[i] = scalar_word(table + ((row + 16 * i) >> a.shift));
+        return x;
+    };
+    // What a wave loads of a tile: K of its subtiles, V of its 32 rows
+    constexpr int NK = SHARED ? 1 : SUB, NV = SHARED ? 1 : KG, VW = D / 64;
+    struct Raw {
+        u32x4 k[NK], v[NV][VW];  // (d 64: the first 8 bytes of k)
+        uint32_t ks[NK];
+        u32x2 vs[NV];
+    };
+    const int k_row = 8 * (l16 >> 2) + (l16 & 3), k_group = g * (D / 4) / 32, v_group = l16 * (D / 16) / 32;
+    const uint32_t k_at = k_row * (D / 2) + g * (D / 8), ks_at = k_row * (D / 32) + k_group;
+    const uint32_t v_at = (g * 16 + l16) * (8 * (D / 32)), vs_at = (g * (D / 32) + v_group) * 8;
+    // (rows that a launch reads once stay out of the caches' way; those that row tiles share do not)
+    auto fetch = [](auto* p) INLINE {
+        if constexpr (SHARED) return *p;
+        else return __builtin_nontemporal_load(p);
+    };
+    // Starts the loads of stage s; the rows of the tile that are in use. The loads are the same in number whatever the tile
+    // is (one that is not there, or 16 rows that have no page, read another page and are hidden), so that the wait for one
+    // tile's lets the next ones' go on: with a branch around them each waits for all in flight.
+    auto load = [&](int s, const Ids& x, Raw& w) INLINE {
+        const int ti = tile_at(s), row = seen.row(ti, KT);
+        uint64_t use = 0;
+        int any = 0;
+#pragma unroll
+        for (int i = 0; i < SUB; ++i)
+            if ((uint32_t)x.id[i] < (uint32_t)a.pages) use |= 0xffffull << (16 * i), any = x.id[i];
+        if (len - row < KT) use &= (1ull << max(len - row, 0)) - 1;
+        auto page_of = [&](int i) { return (uint32_t)x.id[i] < (uint32_t)a.pages ? x.id[i] : any; };
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int q = SHARED ? wave >> 1 : i;
+            // where the 32 rows begin in a block, as their two halves have it: with pages of 16 rows those lie in two
+            const int first = row + 32 * q, low = first & (page - 1), high = ((first + 16) & (page - 1)) - 16;
+            const int64_t p0 = page_of(SHARED ? (wave >> 1 ? 2 : 0) : 2 * i) * a.ps[0], p1 = page_of(SHARED ? (wave >> 1 ? 3 : 1) : 2 * i + 1) * a.ps[0];
+            const int64_t codes[2] = {p0 + low * (D / 2), p1 + high * (D / 2)};
+            const int64_t scales[2] = {p0 + page * (D / 2) + low * (D / 32), p1 + page * (D / 2) + high * (D / 32)};
+            const uint8_t *kc = Kp + (l16 >> 3 ? codes[1] : codes[0]) + k_at, *kx = Kp + (l16 >> 3 ? scales[1] : scales[0]) + ks_at;
+            const uint8_t *vc = Vp + (g >> 1 ? codes[1] : codes[0]) + v_at, *vx = Vp + (g >> 1 ? scales[1] : scales[0]) + vs_at;
+#pragma unroll
+            for (int j = 0; j < NK / NV; ++j) {
+                const int sub = SHARED ? wave & 1 : j;
+                if constexpr (D == 128) w.k[i * (NK / NV) + j] = fetch(reinterpret_cast<const u32x4*>(kc + sub * 4 * (D / 2)));
+                else {
+                    const u32x2 y = fetch(reinterpret_cast<const u32x2*>(kc + sub * 4 * (D / 2)));
+                    w.k[i * (NK / NV) + j] = u32x4{y[0], y[1], 0u, 0u};
+                }
+                w.ks[i * (NK / NV) + j] = kx[sub * 4 * (D / 32)];
+            }
+#pragma unroll
+            for (int v = 0; v < VW; ++v) w.v[i][v] = fetch(reinterpret_cast<const u32x4*>(vc + 16 * v));
+            w.vs[i] = *reinterpret_cast<const u32x2*>(vx);
+        }
+        return use;
+    };
+
     // this lane's query rows
     int tok[QT], cur[QT], deep[QT], up[QT], lo[QT];
     const raw* qp[QT];
@@ -394,51 +484,52 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
         for (int t = 0; t < DT; ++t) o[qt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // The scores p of a tile into weights, m and l anew; o is in the new maximum's unit then. `hide`: bits of the rows that a
-    // query sees count.
-    auto weigh = [&](f32x4 (&p)[QT][2], bool hide, const uint32_t (&see)[QT], u32x4 (&pw)[QT][NW]) {
+    // The scores p of N 16 rows into weights, m and l anew; o is in the new maximum's unit then.
+    auto weigh = [&](auto& p, int qt) INLINE {
+        constexpr int N = sizeof(p) / sizeof(f32x4);
+        float mx = -INFINITY;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            if (hide) {
-                const uint32_t mine = see[qt] >> (8 * g);
+        for (int j = 0; j < N; ++j)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+            for (int r = 0; r < 4; ++r) mx = __builtin_elementwise_maximum(mx, p[j][r]);
+        const float top = __builtin_elementwise_maximum(m[qt], max_across_rows(mx));
+        const float ref = top == -INFINITY ? 0.f : top;  // nothing seen yet: every weight is 0
+        const float corr = __builtin_amdgcn_exp2f((m[qt] - ref) * c);
+        m[qt] = top;
+        float sum = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) p[qt][j][r] = mine >> (4 * j + r) & 1 ? p[qt][j][r] : -INFINITY;
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[j][r] = __builtin_amdgcn_exp2f((p[j][r] - ref) * c);
+                sum += p[j][r];
             }
-            float mx = -INFINITY;
+        l[qt] = fmaf(l[qt], corr, sum);
+        if (__ballot(corr != 1.0f) != 0) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mx = __builtin_elementwise_maximum(mx, p[qt][j][r]);
-            const float top = __builtin_elementwise_maximum(m[qt], max_across_rows(mx));
-            const float ref = top == -INFINITY ? 0.f : top;  // nothing seen yet: every weight is 0
-            const float corr = __builtin_amdgcn_exp2f((m[qt] - ref) * c);
-            m[qt] = top;
-            l[qt] *= corr;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    p[qt][j][r] = __builtin_amdgcn_exp2f((p[qt][j][r] - ref) * c);
-                    l[qt] += p[qt][j][r];
-                }
-            if (__ballot(corr != 1.0f) != 0) {
-#pragma unroll
-                for (int t = 0; t < DT; ++t) o[qt][t] *= corr;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t w[NW];
-                split<NW>(p[qt][i / 2][2 * (i & 1)], p[qt][i / 2][2 * (i & 1) + 1], w);
-#pragma unroll
-                for (int n = 0; n < NW; ++n) pw[qt][n][i] = w[n];
-            }
+            for (int t = 0; t < DT; ++t) o[qt][t] *= corr;
         }
     };
-    // Channel pair q (of D / 32) of this lane's 8 rows, v[row], as rows of channel tiles 2 q and 2 q + 1.
-    auto add_pair = [&](int q, const uint32_t (&v)[8], const u32x4 (&pw)[QT][NW]) {
-        u32x4 even, odd;
+    // The weights of 32 rows as the matrix cores take them
+    auto split_weights = [&](const f32x4& p0, const f32x4& p1, u32x4 (&pw)[NW]) INLINE {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4& p = i < 2 ? p0 : p1;
+            uint32_t w[NW];
+            split<NW>(p[2 * (i & 1)], p[2 * (i & 1) + 1], w);
+#pragma unroll
+            for (int n = 0; n < NW; ++n) pw[n][i] = w[n];
+        }
+    };
+    auto hide_rows = [&](f32x4 (&p)[2], uint32_t see) INLINE {
+        const uint32_t mine = see >> (8 * g);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[j][r] = mine >> (4 * j + r) & 1 ? p[j][r] : -INFINITY;
+    };
+    // A channel pair of this lane's 8 rows, v[row], as row l16 of two channel tiles
+    auto pair_rows = [](const uint32_t (&v)[8], u32x4& even, u32x4& odd) INLINE {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -446,31 +537,24 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
             odd[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x07060302);
 #endif
         }
-#pragma unroll
-        for (int n = 0; n < NW; ++n)
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-                o[qt][2 * q] = mfma_chunk(BF16{}, even, pw[qt][n], o[qt][2 * q]);
-                o[qt][2 * q + 1] = mfma_chunk(BF16{}, odd, pw[qt][n], o[qt][2 * q + 1]);
-            }
     };
 
-    // ---- tiles of new tokens
+    // ---- tiles of new tokens, by halves of 32
     const char* Kn = static_cast<const char*>(a.Kn) + (b * a.kns[0] + h * a.kns[1]) * ES;
     const char* Vn = static_cast<const char*>(a.Vn) + (b * a.vns[0] + h * a.vns[1]) * ES;
-    auto new_tile = [&](int ti) {
-        const int u0 = (ti - nct) * KT;
+    auto new_rows_at = [&](int u0) INLINE {
         uint32_t see[QT];
         bool any = false;
-        const int n = min(tn - u0, KT);
-        const uint32_t there = n >= KT ? ~0u : (1u << n) - 1;
+        const int n = min(tn - u0, 32);
+        if (n <= 0) return;
+        const uint32_t there = n >= 32 ? ~0u : (1u << n) - 1;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
             see[qt] = 0;
             if (walk) {
                 while (cur[qt] >= u0) {
                     const bool in = !WIN || up[qt] < a.window || deep[qt] - up[qt] < a.sinks - len;
-                    if (in && cur[qt] < u0 + KT) see[qt] |= 1u << (cur[qt] - u0);
+                    if (in && cur[qt] < u0 + 32) see[qt] |= 1u << (cur[qt] - u0);
                     cur[qt] = s_up[cur[qt]];
                     ++up[qt];
                 }
@@ -482,10 +566,26 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
             any = any || see[qt] != 0;
         }
         if (__ballot(any) == 0) return;
+        // channels l16 D / 16 and on of rows 8 g .. 8 g + 7, a pair at a time
+        const char* v = Vn + l16 * (D / 16) * ES;
+        int64_t at[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) at[e] = min(u0 + 8 * g + e, tn - 1) * a.vns[2] * ES;
+        using Pair = std::conditional_t<F, u32x2, uint32_t>;
+        auto pair_at = [&](int e, int q) INLINE { return *reinterpret_cast<const Pair*>(v + at[e] + q * (int)sizeof(Pair)); };
+        // (in flight beside K where the registers reach for it: all at once, or a pair at a time)
+        constexpr bool EARLY = QT == 1 && !SHARED && (std::is_same_v<T, BF16> || D == 64);
+        Pair ahead[EARLY ? 8 : 1][EARLY ? DT / 2 : 1];
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int q = 0; q < DT / 2; ++q) ahead[e][q] = pair_at(e, q);
+        }
         f32x4 p[QT][2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int u = min(u0 + 8 * (l16 >> 2) + (l16 & 3) + 4 * j, tn - 1);
+            const int u = min(u0 + k_row + 4 * j, tn - 1);
             const char* k = Kn + u * a.kns[2] * ES + g * (D / 4) * ES;
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) p[qt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -500,35 +600,45 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
             for (int qt = 0; qt < QT; ++qt) p[qt][j] *= flip;
         }
         u32x4 pw[QT][NW];
-        weigh(p, true, see, pw);
-        // channels l16 D / 16 and on of rows 8 g .. 8 g + 7, a pair at a time
-        const char* v = Vn + l16 * (D / 16) * ES;
-        int64_t at[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) at[e] = min(u0 + 8 * g + e, tn - 1) * a.vns[2] * ES;
+        for (int qt = 0; qt < QT; ++qt) {
+            hide_rows(p[qt], see[qt]);
+            weigh(p[qt], qt);
+            split_weights(p[qt][0], p[qt][1], pw[qt]);
+        }
         bool bad = false;  // 0 . V is NaN for a V that is not finite: such elements are left out and added to those that see them
 #pragma unroll
         for (int q = 0; q < DT / 2; ++q) {
-            uint32_t part[pieces<T>()][8];
+            constexpr int NP = pieces<T>();
+            uint32_t part[NP][8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+                Pair in;
+                if constexpr (EARLY) in = ahead[e][q];
+                else in = pair_at(e, q);
                 float x, y;
-                if constexpr (F) {
-                    const f32x2 w = *reinterpret_cast<const f32x2*>(v + at[e] + q * 8);
-                    x = w[0], y = w[1];
-                } else {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(v + at[e] + q * 4);
-                    x = lo_as_f32(T{}, w), y = hi_as_f32(T{}, w);
-                }
+                if constexpr (F) x = __uint_as_float(in[0]), y = __uint_as_float(in[1]);
+                else x = lo_as_f32(T{}, in), y = hi_as_f32(T{}, in);
                 const bool fx = fabsf(x) < INFINITY, fy = fabsf(y) < INFINITY;
                 bad = bad || !fx || !fy;
-                uint32_t w[pieces<T>()];
-                split<pieces<T>()>(fx ? x : 0.f, fy ? y : 0.f, w);
+                uint32_t w[NP];
+                split<NP>(fx ? x : 0.f, fy ? y : 0.f, w);
 #pragma unroll
-                for (int i = 0; i < pieces<T>(); ++i) part[i][e] = w[i];
+                for (int i = 0; i < NP; ++i) part[i][e] = w[i];
             }
 #pragma unroll
-            for (int i = 0; i < pieces<T>(); ++i) add_pair(q, part[i], pw);
+            for (int i = 0; i < NP; ++i) {
+                u32x4 even, odd;
+                pair_rows(part[i], even, odd);
+#pragma unroll
+                for (int n = 0; n < NW; ++n)
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt) {
+                        o[qt][2 * q] = mfma_chunk(BF16{}, even, pw[qt][n], o[qt][2 * q]);
+                        o[qt][2 * q + 1] = mfma_chunk(BF16{}, odd, pw[qt][n], o[qt][2 * q + 1]);
+                    }
+            }
+            if constexpr (!EARLY) __builtin_amdgcn_sched_barrier(0);
         }
         if (__ballot(bad) == 0) return;
         for (int u = 0; u < n; ++u) {
@@ -545,75 +655,80 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
         }
     };
 
-    // ---- tiles of cached rows
-    struct Raw {
-        u32x4 k[2], v[2];  // (d 64: 8 and 16 bytes)
-        uint32_t ks[2];
-        u32x2 vs;
+    // ---- tiles of cached rows: values
+    constexpr uint64_t FULL = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
+    auto k_frag = [&](const Raw& w, int i, int ks) INLINE {
+        const float scale = scale_of(w.ks[i]);
+        const uint32_t y = w.k[i][ks];
+        return u32x4{to_bf16<0>(y, scale), to_bf16<1>(y, scale), to_bf16<2>(y, scale), to_bf16<3>(y, scale)};
     };
-    const int page = 1 << a.shift;
-    const uint8_t *Kp = static_cast<const uint8_t*>(a.Kp) + h * a.ps[1], *Vp = static_cast<const uint8_t*>(a.Vp) + h * a.ps[1];
-    const int k_row = 8 * (l16 >> 2) + (l16 & 3), group = g * (D / 4) / 32, v_group = l16 * (D / 16) / 32;
-    auto tile_at = [&](int s) { return WIN ? win.at(s * S::WK + wk) : win.high - 1 - (s * S::WK + wk); };
-    struct Ids {
-        int id[2];  // of the tile's halves
-    };
-    auto ids = [&](int s) {
-        Ids x = {{-1, -1}};
-        const int ti = tile_at(s);
-        if (ti < c0 || ti >= nct) return x;
-        const int row = seen.row(ti, KT);
+    // Rows of 32 that are not in use may hold any scale: 1 in its place. `some`: rows that not every query sees are among
+    // them, so that a row without a value gets 1 too; its bit is in the result, a word for the lane's channel group c.
+    auto clean_scales = [&](u32x2& vs, uint32_t use, bool some, int c) INLINE {
+        const uint32_t mine = use >> (8 * g);
+        uint32_t odd = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (row + 16 * i < len) x.id[i] = scalar_word(table + ((row + 16 * i) >> a.shift));
-        return x;
-    };
-    // Starts the loads of stage s; the rows of the tile that are in use (0: nothing was loaded)
-    auto load = [&](int s, const Ids& x, Raw& w) {
-        const int ti = tile_at(s);
-        uint32_t use = 0;
-        if (ti < c0 || ti >= nct) return use;
-        const int row = seen.row(ti, KT);
-        const bool is0 = (uint32_t)x.id[0] < (uint32_t)a.pages, is1 = (uint32_t)x.id[1] < (uint32_t)a.pages;
-        const int n = len - row;
-        use = (is0 ? 0xffffu : 0u) | (is1 ? 0xffff0000u : 0u);
-        if (n < KT) use &= (1u << n) - 1;
-        if (use == 0) return use;
-        // a half that has no page reads the other's, and is hidden
-        const int id0 = is0 ? x.id[0] : x.id[1], id1 = is1 ? x.id[1] : x.id[0];
-        const int off0 = row & (page - 1), off1 = (row + 16) & (page - 1);
-        const int kh = l16 >> 3, vh = g >> 1;  // the half that this lane's rows lie in
-        const int64_t k_page = (kh ? id1 : id0) * a.ps[0], v_page = (vh ? id1 : id0) * a.ps[0];
-        const int kr = (kh ? off1 - 16 : off0) + k_row, vr = (vh ? off1 - 16 : off0) + 8 * g;
-        const uint8_t* kb = Kp + k_page;
-        const uint8_t* vb = Vp + v_page;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint8_t* at = kb + (kr + 4 * j) * (D / 2) + g * (D / 8);
-            if constexpr (D == 128) w.k[j] = *reinterpret_cast<const u32x4*>(at);
-            else {
-                const u32x2 y = *reinterpret_cast<const u32x2*>(at);
-                w.k[j] = u32x4{y[0], y[1], 0u, 0u};
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t byte = vs[e / 4] >> (8 * (e % 4)) & 255;
+            const bool in = mine >> e & 1;
+            if (some) {
+                // lane 16 i + l16 has rows 8 i .. of channel group v_group(l16)
+                const uint64_t bad = __ballot(in && byte == 255);
+                for (int i = 0; i < 4; ++i) odd |= (uint32_t)(bad >> (16 * i + c * (512 / D)) & 1) << (8 * i + e);
             }
-            w.ks[j] = kb[page * (D / 2) + (kr + 4 * j) * (D / 32) + group];
+            if (!in || (some && byte == 255)) vs[e / 4] = (vs[e / 4] & ~(255u << (8 * (e % 4)))) | 127u << (8 * (e % 4));
         }
-        const uint8_t* at = vb + v_code(vr, l16, D);
-        w.v[0] = *reinterpret_cast<const u32x4*>(at);
-        if constexpr (D == 128) w.v[1] = *reinterpret_cast<const u32x4*>(at + 16);
-        w.vs = *reinterpret_cast<const u32x2*>(vb + v_scale(page, vr, v_group, D));
-        return use;
+        return odd;
     };
-    auto compute = [&](int s, uint32_t use, Raw& w, auto masked) {
-        uint32_t see[QT];
-        bool hide = use != ~0u, some = false;  // some: a query sees rows of it that another does not
+    // V fragments of channel tiles 2 q and 2 q + 1 over 32 rows
+    auto v_frags = [&](const Raw& w, int i, auto q, u32x4& even, u32x4& odd) INLINE {
+        constexpr int Q = decltype(q)::value;
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float scale = scale_of(w.vs[i][e / 4] >> (8 * (e % 4)) & 255);
+            // (d 128: a dword a row; d 64: two rows a dword)
+            if constexpr (D == 128) v[e] = to_bf16<Q>(w.v[i][e / 4][e % 4], scale);
+            else v[e] = e & 1 ? to_bf16<Q + 2>(w.v[i][0][e / 2], scale) : to_bf16<Q>(w.v[i][0][e / 2], scale);
+        }
+        pair_rows(v, even, odd);
+    };
+    // A wave's share of a tile into LDS (SHARED): K's subtile `wave`, and every second channel pair of V's 32 rows
+    auto convert = [&](int s, uint64_t use, Raw& w) INLINE {
+        if (use == 0) return;
+        u32x4* to = smem + (s & 1) * 64 * (S::KF + S::VF) + lane;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) to[(wave * KS + ks) * 64] = k_frag(w, 0, ks);
+        const int half = wave >> 1;
+        if (WIN || use != FULL) {
+            const uint32_t odd = clean_scales(w.vs[0], (uint32_t)(use >> (32 * half)), WIN, lane & (GROUPS - 1));
+            if (WIN && lane < GROUPS && (wave & 1) == 0) s_odd[((s & 1) * 4 + lane) * 2 + half] = odd;
+        }
+        to += (S::KF + half * DT) * 64;
+        static_for<0, DT / 4>([&](auto i) {
+            u32x4 even, odd;
+            if (wave & 1) {
+                v_frags(w, 0, std::integral_constant<int, 2 * decltype(i)::value + 1>{}, even, odd);
+                to[(4 * decltype(i)::value + 2) * 64] = even, to[(4 * decltype(i)::value + 3) * 64] = odd;
+            } else {
+                v_frags(w, 0, std::integral_constant<int, 2 * decltype(i)::value>{}, even, odd);
+                to[(4 * decltype(i)::value) * 64] = even, to[(4 * decltype(i)::value + 1) * 64] = odd;
+            }
+        });
+    };
+
+    auto compute = [&](int s, uint64_t use, Raw& w, auto masked) INLINE {
+        constexpr bool MASKED = decltype(masked)::value;
+        uint64_t see[QT];
+        bool hide = use != FULL, some = false;  // some: a query sees rows of it that another does not
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) see[qt] = use;
-        if constexpr (decltype(masked)::value) {
+        if constexpr (MASKED) {
             const int j0 = seen.row(tile_at(s), KT);
             bool any = false;
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
-                see[qt] &= from_bit(lo[qt] - j0) | ~from_bit(a.sinks - j0);
+                see[qt] &= from_bit((int64_t)lo[qt] - j0) | ~from_bit((int64_t)a.sinks - j0);
                 any = any || see[qt] != 0;
                 some = some || see[qt] != use;
             }
@@ -621,99 +736,148 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
             some = __ballot(some) != 0;
             hide = hide || some;
         }
-        f32x4 p[QT][2];
+        const u32x4* from = smem + (s & 1) * 64 * (S::KF + S::VF) + lane;
+        f32x4 p[QT][SUB];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float scale = scale_of(w.ks[j]);
+        for (int j = 0; j < SUB; ++j) {
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) p[qt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const uint32_t y = w.k[j][ks];
-                const u32x4 kf = {to_bf16<0>(y, scale), to_bf16<1>(y, scale), to_bf16<2>(y, scale), to_bf16<3>(y, scale)};
+                u32x4 kf;
+                if constexpr (SHARED) kf = from[(j * KS + ks) * 64];
+                else kf = k_frag(w, j, ks);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
                     for (int qt = 0; qt < QT; ++qt) p[qt][j] = mfma_chunk(BF16{}, kf, qf[qt][n][ks], p[qt][j]);
             }
         }
-        u32x4 pw[QT][NW];
-        weigh(p, hide, see, pw);
-        uint32_t odd = 0;  // rows without a value in this lane's channels that not every query sees
+        uint32_t odd[KG] = {};  // rows without a value in this lane's channels that not every query sees
         if (hide) {
-            // rows that are not in use may hold any scale: 1 in its place
-            const uint32_t mine = use >> (8 * g);
+            // (few tiles come here: what is worked out stays behind the branch)
+            uint32_t mine[2] = {(uint32_t)use, (uint32_t)(use >> 32)};
+            asm volatile("" : "+s"(mine[0]), "+s"(mine[1]));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t byte = w.vs[e / 4] >> (8 * (e % 4)) & 255;
-                const bool in = mine >> e & 1;
-                if (some) {
-                    // lane 16 g' + l16' has rows 8 g' .. of channel group v_group(l16'): those that this lane's channels
-                    // 4 g D / 16 and on are of
-                    const uint64_t bad = __ballot(in && byte == 255);
-                    const int of = (g * (D / 4) / 32) * (512 / D);
-                    for (int i = 0; i < 4; ++i) odd |= (uint32_t)(bad >> (16 * i + of) & 1) << (8 * i + e);
+            for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+                for (int kk = 0; kk < KG; ++kk) {
+                    f32x4 y[2] = {p[qt][2 * kk], p[qt][2 * kk + 1]};
+                    hide_rows(y, MASKED ? (uint32_t)(see[qt] >> (32 * kk)) & mine[kk] : mine[kk]);
+                    p[qt][2 * kk] = y[0], p[qt][2 * kk + 1] = y[1];
                 }
-                if (!in || (some && byte == 255)) w.vs[e / 4] = (w.vs[e / 4] & ~(255u << (8 * (e % 4)))) | 127u << (8 * (e % 4));
+            }
+            if constexpr (!SHARED) {
+#pragma unroll
+                for (int kk = 0; kk < KG; ++kk) odd[kk] = clean_scales(w.vs[kk], mine[kk], some, g * (D / 4) / 32);
             }
         }
-        float sc[8];
+        if constexpr (SHARED && WIN) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sc[e] = scale_of(w.vs[e / 4] >> (8 * (e % 4)) & 255);
-        static_for<0, DT / 2>([&](auto q) {
-            uint32_t v[8];
-            // (d 128: a dword a row; d 64: two rows a dword)
+            for (int kk = 0; kk < KG; ++kk) odd[kk] = s_odd[((s & 1) * 4 + g * (D / 4) / 32) * 2 + kk];
+        }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (D == 128) v[e] = to_bf16<decltype(q)::value>(w.v[e / 4][e % 4], sc[e]);
-                else v[e] = e & 1 ? to_bf16<decltype(q)::value + 2>(w.v[0][e / 2], sc[e]) : to_bf16<decltype(q)::value>(w.v[0][e / 2], sc[e]);
+        for (int qt = 0; qt < QT; ++qt) weigh(p[qt], qt);
+#pragma unroll
+        for (int kk = 0; kk < KG; ++kk) {
+            u32x4 pw[QT][NW];
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) split_weights(p[qt][2 * kk], p[qt][2 * kk + 1], pw[qt]);
+            static_for<0, DT / 2>([&](auto q) {
+                constexpr int Q = decltype(q)::value;
+                u32x4 even, odd_;
+                if constexpr (SHARED) even = from[(S::KF + kk * DT + 2 * Q) * 64], odd_ = from[(S::KF + kk * DT + 2 * Q + 1) * 64];
+                else v_frags(w, kk, q, even, odd_);
+#pragma unroll
+                for (int n = 0; n < NW; ++n)
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt) {
+                        o[qt][2 * Q] = mfma_chunk(BF16{}, even, pw[qt][n], o[qt][2 * Q]);
+                        o[qt][2 * Q + 1] = mfma_chunk(BF16{}, odd_, pw[qt][n], o[qt][2 * Q + 1]);
+                    }
+            });
+        }
+        if constexpr (SHARED ? WIN : MASKED) {
+            const uint64_t none = odd[0] | (KG == 2 ? (uint64_t)odd[KG - 1] << 32 : 0);
+            if (__ballot(none != 0) != 0) {
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                    if (none & see[qt]) {
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) o[qt][t] = f32x4{NAN, NAN, NAN, NAN};
+                    }
             }
-            add_pair(decltype(q)::value, v, pw);
-        });
-        if (decltype(masked)::value && __ballot(odd != 0) != 0) {
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-                if (odd & see[qt]) {
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) o[qt][t] = f32x4{NAN, NAN, NAN, NAN};
-                }
         }
     };
 
     // new tokens first, from the last: their paths are walked down once
     const int new_tiles = WIN ? max(win.high - max(win.low, nct), 0) + max(win.sink_end - max(c0, nct), 0) : max(win.high - max(c0, nct), 0);
     const int s_first = new_tiles / S::WK;  // the first stage with a tile of cached rows (for some wave)
-    Raw w[AHEAD];
-    uint32_t use[AHEAD];
-    Ids x[AHEAD + 1];
-#pragma unroll
-    for (int i = 0; i <= AHEAD; ++i) x[i] = ids(s_first + i);
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) use[i] = load(s_first + i, x[i], w[i]);
-    for (int i = wk; i < new_tiles; i += S::WK) new_tile(WIN ? win.at(i) : win.high - 1 - i);
-    // the stages whose tiles every query sees whole, then those at the window's border and the sinks
+    // the stages whose tiles every query sees whole end there; then those at the window's border and the sinks
     const int s_whole = WIN ? max(s_first, max(win.high - max(win.low, win.clean), 0) / S::WK) : nst;
-    Ids nx = x[AHEAD];
-    auto stages = [&](int from, int to, auto masked) {
-        int s = from;
-        auto turn = [&](int i) {
-            if (use[i] != 0) compute(s, use[i], w[i], masked);
-            use[i] = load(s + AHEAD, nx, w[i]);
-            nx = ids(s + AHEAD + 1);
-            ++s;
-        };
-        while (s < to) {
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) turn(i);
+    auto new_tokens = [&]() INLINE {
+        for (int i = wk; i < new_tiles; i += S::WK) {
+            const int u0 = ((WIN ? win.at(i) : win.high - 1 - i) - nct) * KT;
+#pragma unroll 1
+            for (int u = u0 + KT - 32; u >= u0; u -= 32) new_rows_at(u);
         }
-        return s;
     };
-    // (a turn past `to` belongs to the next kind: the counts are rounded so that masks are asked where they may count)
-    if constexpr (WIN) {
-        const int at = stages(s_first, s_first + (s_whole - s_first) / AHEAD * AHEAD, std::false_type{});
-        stages(at, nst, std::true_type{});
+    if constexpr (SHARED) {
+        new_tokens();
+        // stage s is computed while s + 1 is converted and s + 2 is on its way: one barrier a stage
+        Raw w;
+        uint64_t use = load(s_first, ids(s_first), w), here = use, next;
+        Ids x = ids(s_first + 1);
+        convert(s_first, use, w);
+        next = load(s_first + 1, x, w);
+        x = ids(s_first + 2);
+        auto stage = [&](int s, auto masked) INLINE {
+            __syncthreads();
+            if (here != 0) compute(s, here, w, masked);
+            convert(s + 1, next, w);
+            here = next;
+            next = load(s + 2, x, w);
+            x = ids(s + 3);
+        };
+        for (int s = s_first; s < s_whole; ++s) stage(s, std::false_type{});
+        if constexpr (WIN)
+            for (int s = s_whole; s < nst; ++s) stage(s, std::true_type{});
     } else {
-        stages(s_first, nst, std::false_type{});
+        constexpr int AHEAD = S::waves(std::is_same_v<T, BF16>) == 3 || (WIN && QT == 2) ? 1 : 2;
+        Raw w[AHEAD];
+        uint64_t use[AHEAD];
+        Ids nx;
+        auto start = [&]() INLINE {
+            Ids x[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) x[i] = ids(s_first + i);
+            nx = ids(s_first + AHEAD);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) use[i] = load(s_first + i, x[i], w[i]);
+        };
+        // (the cached rows' first loads run beside the new tokens where the registers reach for both)
+        if constexpr (QT == 1) start();
+        new_tokens();
+        if constexpr (QT > 1) start();
+        auto stages = [&](int s, int to, auto masked) INLINE {
+            while (s < to) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    if (use[i] != 0) compute(s, use[i], w[i], masked);
+                    use[i] = load(s + AHEAD, nx, w[i]);
+                    nx = ids(s + AHEAD + 1);
+                    ++s;
+                }
+            }
+            return s;
+        };
+        if constexpr (WIN) {
+            // (by whole turns of the registers)
+            const int at = stages(s_first, s_first + (s_whole - s_first) / AHEAD * AHEAD, std::false_type{});
+            stages(at, nst, std::true_type{});
+        } else {
+            stages(s_first, nst, std::false_type{});
+        }
     }
 
     float L[QT];
@@ -722,7 +886,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
         m[qt] *= c;
         L[qt] = sum_across_rows(l[qt]);
     }
-    auto store4 = [&](int r, int d, f32x4 v, float M, float sum) {
+    auto store4 = [&](int r, int d, f32x4 v, float M, float sum) INLINE {
         const int t = r / a.G, gh = r - t * a.G;
         if (r >= R || t >= tn) return;
         if (whole) {
@@ -741,7 +905,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
         }
     };
     // channels (4 g + r) D / 16 and on of a query, four at a time
-    auto each4 = [&](auto f) {
+    auto each4 = [&](auto f) INLINE {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
@@ -754,7 +918,7 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
         each4([&](int qt, int d, f32x4 v) { store4(r0 + wr * 16 * QT + qt * 16 + l16, d, v, m[qt], L[qt]); });
     } else {
         // the key groups' results side by side in LDS, then joined
-        float *so = s_epi, *sm = so + S::WK * S::RW * S::OLD;
+        float *so = reinterpret_cast<float*>(smem), *sm = so + S::WK * S::RW * S::OLD;
         each4([&](int qt, int d, f32x4 v) { *reinterpret_cast<f32x4*>(so + (wk * S::RW + wr * 16 * QT + qt * 16 + l16) * S::OLD + d) = v; });
         if (g == 0) {
 #pragma unroll
@@ -764,7 +928,8 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
                 sm[2 * row + 1] = L[qt];
             }
         }
-        __syncthreads();
+        // (LDS alone: the loads of tiles behind the last are not waited for)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         for (int i = tid; i < S::RW * D / 4; i += 256) {
             const int row = i / (D / 4), d = i % (D / 4) * 4;
             float M = -INFINITY, sum = 0.f;
@@ -783,19 +948,21 @@ __global__ __launch_bounds__(256, 2) void paged_q4_kernel(PagedArgs a) {
     }
 }
 
-// How a call is cut (plan_of, with tiles of 32 rows whatever the workgroup's shape).
-Plan plan_q4(int B, int Hkv, int G, int T, int d, int columns, int page, int window, int sinks) {
+// How a call is cut (plan_of, for the shapes of paged_q4_kernel).
+Plan plan_q4(int dtype, int B, int Hkv, int G, int T, int d, int columns, int page, int window, int sinks) {
     Plan p;
     const int64_t rows = (int64_t)T * G;
-    p.qt = rows <= 16 ? 1 : 2;
-    p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-    p.kt = 32;
+    // 16 rows of a wave (bfloat16: 32) leave the tiles to the four; more share them. 32 rows of a wave where there are more
+    // than 64 and the queries' pieces leave the registers
+    const bool few = rows <= (dtype == YTHIP_BF16 ? 32 : 16);
+    p.wr = few ? 1 : 4;
+    p.qt = few ? (rows <= 16 ? 1 : 2) : rows <= 64 || dtype == YTHIP_F32 ? 1 : 2;
+    p.kt = few ? 32 : 64;
     const int rw = 16 * p.qt * p.wr;
     p.row_tiles = (int)((rows + rw - 1) / rw);
     const int64_t per = (int64_t)Hkv * p.row_tiles;
     p.stage = 4 / p.wr;
-    const bool many = p.wr == 1 && SLOTS / per >= 8 * (int64_t)B;
-    const int64_t slots = many ? SLOTS / 2 : SLOTS;
+    const int64_t slots = p.wr == 1 && p.qt == 1 && (dtype == YTHIP_BF16 || d == 64) ? SLOTS / 2 * 3 : SLOTS;
     p.short_run = p.wr > 1 ? 4 : 0;
     int64_t seq_rows = (int64_t)columns * page;
     if (window > 0) seq_rows = std::min(seq_rows, (int64_t)window + sinks + 2 * p.kt);
@@ -828,10 +995,12 @@ int launch_q4(const PagedArgs& a, const Plan& p, hipStream_t s) {
 }
 template <class T, int D, bool WIN>
 int run_q4(const PagedArgs& a, const Plan& p, hipStream_t s) {
-    if (p.qt == 1) return launch_q4<T, D, 1, 1, WIN>(a, p, s);
-    if (p.wr == 1) return launch_q4<T, D, 2, 1, WIN>(a, p, s);
-    if (p.wr == 2) return launch_q4<T, D, 2, 2, WIN>(a, p, s);
-    return launch_q4<T, D, 2, 4, WIN>(a, p, s);
+    if (p.wr == 1 && p.qt == 1) return launch_q4<T, D, 1, 1, WIN>(a, p, s);
+    if constexpr (std::is_same_v<T, BF16>)
+        if (p.wr == 1) return launch_q4<T, D, 2, 1, WIN>(a, p, s);
+    if constexpr (!std::is_same_v<T, F32>)
+        if (p.qt == 2) return launch_q4<T, D, 2, 4, WIN>(a, p, s);
+    return launch_q4<T, D, 1, 4, WIN>(a, p, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -951,7 +1120,7 @@ __attribute__((visibility("default"))) size_t ythip_paged_attn_q4_workspace_size
                                                                                  int sinks) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || d <= 0 || columns < 0 || page <= 0 || window < 0 || sinks < 0 || Hq % Hkv != 0) return 0;
     trim_window(T, columns, page, window, sinks);
-    return plan_q4(B, Hkv, Hq / Hkv, T, d, columns, page, window, sinks).bytes();
+    return plan_q4(dtype, B, Hkv, Hq / Hkv, T, d, columns, page, window, sinks).bytes();
 }
 
 __attribute__((visibility("default"))) int ythip_paged_attn_q4(
@@ -975,9 +1144,14 @@ __attribute__((visibility("default"))) int ythip_paged_attn_q4(
     if (columns > 0)
         if (const int e = check_blocks(who, 1, pages, Hkv, page, d, Kp, Vp, str, ps)) return e;
     a.ps[0] = ps[1], a.ps[1] = ps[2], a.ps[2] = 0;
+    if (pages == 0) {
+        void* none = nullptr;
+        if (const int e = status_of(hipGetSymbolAddress(&none, HIP_SYMBOL(no_pages)))) return e;
+        a.Kp = a.Vp = none;
+    }
     trim_window(T, columns, page, window, sinks);
     a.window = window, a.sinks = sinks;
-    const Plan p = plan_q4(B, Hkv, a.G, T, d, columns, page, window, sinks);
+    const Plan p = plan_q4(dtype, B, Hkv, a.G, T, d, columns, page, window, sinks);
     if (const int e = check_workspace(who, p.bytes(), workspace_, ws_bytes)) return e;
     if (!launchable((p.items * a.Hkv + 8) * p.row_tiles, 256))
         return fail(YTHIP_EUNSUPPORTED, "%s: %lld workgroups (2^24 - 1 at most)", who, (long long)(p.items * a.Hkv * p.row_tiles));
