@@ -10,9 +10,13 @@ def mass(x: float) -> float:
     return x if 0.0 < x < math.inf else 0.0
 
 
+def masses(row):
+    return torch.where((row > 0) & (row < math.inf), row, 0.0)
+
+
 def draw(weights, x):
     """The first entry at which the sum passes x times all; -1 without a weight."""
-    w = torch.tensor([mass(v) for v in weights], dtype=torch.float64)
+    w = masses(weights)
     cum = torch.cumsum(w, 0)
     if not cum[-1] > 0:
         return -1
@@ -44,7 +48,7 @@ def verify(target, tokens, u, u_next, draft=None, parents=None, tree_len=None):
                 if 0 <= x < V and u[b][t] * q < mass(float(row[x])):
                     path.append(t)
                     continue
-                left = [max(mass(float(p)) - mass(float(d)), 0.0) for p, d in zip(row, draft[b, t])]
+                left = (masses(row) - masses(draft[b, t])).clamp(min=0.0)
             else:
                 kids = [t for t in range(n + 1, tn) if parents[b][t] == n and 0 <= tokens[b][t] < V]
                 low, met, went = 0.0, set(), None
@@ -61,10 +65,10 @@ def verify(target, tokens, u, u_next, draft=None, parents=None, tree_len=None):
                     continue
                 left = row.clone()
                 left[list(met)] = 0.0
-                left = left.tolist()
-            rest = left if any(mass(v) for v in left) else None
+                left = masses(left)
+            rest = left if (left > 0).any() else None
             break
         paths.append(path + [-1] * (T - len(path)))
         counts.append(len(path))
-        nexts.append(-1 if not path else draw(rest if rest is not None else target[b, path[-1]].tolist(), u_next[b]))
+        nexts.append(-1 if not path else draw(rest if rest is not None else target[b, path[-1]], u_next[b]))
     return paths, counts, nexts

@@ -110,6 +110,16 @@ def test_verify(kind, B, T, V, dtype):
               tree_len=ints([max(0, T - b) for b in range(B)]) if seed else None)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["draft", "chain", "tree"])
+@pytest.mark.parametrize("V", [(1 << 18) - 5, 1 << 18, (1 << 18) + 1, 300007])
+def test_verify_of_long_rows(kind, V, dtype):
+    """Rows of more runs than lanes, whole and not."""
+    args, near, above = drafts(V, 2, 4, V, dtype, kind != "tree", spread=2.0)
+    for u_next in (args[3], torch.tensor([0.0, 1 - 2.0 ** -24], device="cuda")):
+        check((*args[:3], u_next), draft=near if kind == "draft" else None, parents=above if kind == "tree" else None)
+
+
 @pytest.mark.parametrize("kind", ["draft", "chain", "tree"])
 def test_verify_keeps_long_paths(kind):
     """A target that is all but sure of the drafted tokens, up to the last of 1024."""
@@ -154,11 +164,11 @@ def test_verify_of_siblings_with_one_token_and_bad_tokens():
             check((p, tokens, u, torch.tensor([c], device="cuda")), parents=ints([[5, 7, 1, -1, 9, 0, 2]]))
 
 
+@pytest.mark.parametrize("V", [5000, 270000])
 @pytest.mark.parametrize("kind", ["draft", "tree"])
-def test_verify_where_nothing_is_left(kind):
+def test_verify_where_nothing_is_left(kind, V):
     """A draft row that is the target's, a node whose children hold all of it, rows without a weight, with NaN, negative
     and infinite entries, and random numbers of 0, all but 1, 1 and NaN."""
-    V = 5000
     target = torch.zeros(6, 3, V)
     target[:, :, 7], target[:, :, 4500] = 0.25, 0.75
     target[3] = 0.0

@@ -176,9 +176,10 @@ ProbsPlan probs_plan(int rows, int n) {
 constexpr int MAX_DRAFTS = 1024;   // tokens of a sequence: their probabilities lie in LDS
 constexpr int SLICE = 4096;        // vocabulary entries of a workgroup
 constexpr int MAX_SLICES = 1024;
+constexpr int RUN = 512;           // of a wave at a time: what has a sum of its own
 
 struct VerifyArgs {
-    int B, T, V, slices;
+    int B, T, V, slices, runs;
     const void *target, *draft;
     int64_t ts[2], ds[2];  // elements
     const int32_t *tokens, *parents, *tree_len;
@@ -187,7 +188,8 @@ struct VerifyArgs {
     int64_t ld_u;
     int32_t *path, *kept, *next;
     int64_t ld_path;
-    double* sums;  // [B][slices] of (what is left, the row as it is)
+    double* sums;   // [B][2][runs]: what is left of every RUN entries, then the row as it is
+    int32_t* walk;  // [B][4]: kept, last, behind
 };
 
 // What a probability weighs: one that is not a positive number has no weight.
@@ -199,11 +201,11 @@ struct Walk {
     int n, last;  // kept tokens, the last of them
     int behind;   // the chain's first refused token, whose draft row is taken off the target's (0: none)
 };
-template <class T>
+template <class T, int NT>
 __device__ __forceinline__ Walk walk_drafts(const VerifyArgs& a, int b, double* s_p, int16_t* s_up, int32_t* s_tok,
                                             int32_t* s_walk, int32_t* path) {
     const int tn = a.tree_len != nullptr ? min(max(a.tree_len[b], 0), a.T) : a.T;
-    for (int t = threadIdx.x; t < tn; t += 256) {
+    for (int t = threadIdx.x; t < tn; t += NT) {
         const int up = a.parents != nullptr ? a.parents[b * a.ld_par + t] : t - 1;
         const int x = a.tokens[b * a.ld_tok + t];
         const bool is = t > 0 && up >= 0 && up < t && x >= 0 && x < a.V;
@@ -220,7 +222,7 @@ __device__ __forceinline__ Walk walk_drafts(const VerifyArgs& a, int b, double* 
     __syncthreads();
     if (a.draft == nullptr) {
         // of siblings with one token the first has its probability
-        for (int t = threadIdx.x; t < tn; t += 256) {
+        for (int t = threadIdx.x; t < tn; t += NT) {
             bool twice = false;
             for (int o = 1; o < t && !twice; ++o) twice = s_up[o] == s_up[t] && s_tok[o] == s_tok[t];
             if (twice && s_up[t] >= 0) s_p[t] = 0.0;
@@ -311,14 +313,15 @@ struct Weights {
     }
 };
 
-// Bits of a slice's entries that are children's tokens of the last token that was kept.
-__device__ __forceinline__ void mark_children(const Walk& w, int tn, const int16_t* s_up, const int32_t* s_tok, int v0,
+// Bits of `width` entries from v0 on that are children's tokens of the last token that was kept.
+template <int NT>
+__device__ __forceinline__ void mark_children(const Walk& w, int tn, const int16_t* s_up, const int32_t* s_tok, int v0, int width,
                                               uint32_t* s_gone) {
-    for (int i = threadIdx.x; i < SLICE / 32; i += 256) s_gone[i] = 0;
+    for (int i = threadIdx.x; i < width / 32; i += NT) s_gone[i] = 0;
     __syncthreads();
-    for (int t = threadIdx.x; t < tn; t += 256) {
+    for (int t = threadIdx.x; t < tn; t += NT) {
         const int v = s_tok[t] - v0;
-        if (s_up[t] == w.last && v >= 0 && v < SLICE) atomicOr(&s_gone[v / 32], 1u << (v % 32));
+        if (s_up[t] == w.last && v >= 0 && v < width) atomicOr(&s_gone[v / 32], 1u << (v % 32));
     }
     __syncthreads();
 }
@@ -333,9 +336,41 @@ struct Rows {
     }
 };
 
+// Of n numbers a lane, in the lanes' order, behind `sum`: the first at which the sum passes x, or the last that adds to
+// it. `base`: the sum before it.
+template <class F>
+__device__ __forceinline__ int find_in_wave(F&& number, int n, double sum, double x, double& base) {
+    int first = -1, last = -1;
+    double at_first = 0.0, at_last = 0.0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+        const double m = number(i);
+        if (m > 0.0) {
+            last = i, at_last = sum;
+            if (first < 0 && sum + m > x) first = i, at_first = sum;
+        }
+        sum += m;
+    }
+    const uint64_t hit = __ballot(first >= 0), some = __ballot(last >= 0);
+    const int lane = hit != 0 ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some | 1);
+    base = __shfl(hit != 0 ? at_first : at_last, lane, 64);
+    return lane * n + __shfl(hit != 0 ? first : last, lane, 64);
+}
+__device__ __forceinline__ double before_in_wave(double v, double& total) {
+    double inc = v;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const double x = __shfl_up(inc, off, 64);
+        if (lane >= off) inc += x;
+    }
+    total = __shfl(inc, 63, 64);
+    const double x = __shfl_up(inc, 1, 64);
+    return lane > 0 ? x : 0.0;
+}
+
 // A slice's sums of both weights. Every workgroup of a sequence walks its drafts by itself: the T probabilities are
-// loads that lie side by side, and a launch would cost more. Sums are in 64 bits: which entry the random number falls on
-// does not depend on how 150000 numbers of 24 bits were added up. Bound by the round trips (lengths, tokens, their
+// loads that lie side by side, and a launch would cost more. Bound by the round trips (lengths, tokens, their
 // probabilities, a slice).
 template <class T>
 __global__ __launch_bounds__(256) void verify_sum_kernel(VerifyArgs a) {
@@ -343,143 +378,105 @@ __global__ __launch_bounds__(256) void verify_sum_kernel(VerifyArgs a) {
     __shared__ int32_t s_tok[MAX_DRAFTS], s_walk[3];
     __shared__ int16_t s_up[MAX_DRAFTS];
     __shared__ uint32_t s_gone[SLICE / 32];
-    __shared__ double s_sum[4][2];
-    const int b = blockIdx.y, v0 = blockIdx.x * SLICE, end = min(v0 + SLICE, a.V);
+    const int b = blockIdx.y, v0 = blockIdx.x * SLICE;
     const int tn = a.tree_len != nullptr ? min(max(a.tree_len[b], 0), a.T) : a.T;
     int32_t* path = blockIdx.x == 0 ? a.path + b * a.ld_path : nullptr;
-    const Walk w = walk_drafts<T>(a, b, s_p, s_up, s_tok, s_walk, path);
+    const Walk w = walk_drafts<T, 256>(a, b, s_p, s_up, s_tok, s_walk, path);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.kept[b] = w.n;
     if (w.n == 0) {
         if (blockIdx.x == 0 && threadIdx.x == 0) a.next[b] = -1;
         return;
     }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        int32_t* out = a.walk + 4 * b;
+        out[1] = w.last, out[2] = w.behind;
+    }
     const Rows<T> rows(a, b, w);
-    Weights<T> x[SLICE / 2048];
+    constexpr int EACH = SLICE / (4 * RUN);  // runs of a wave
+    const int lane = threadIdx.x & 63, run0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * EACH;
+    Weights<T> x[EACH];
 #pragma unroll
-    for (int i = 0; i < SLICE / 2048; ++i) x[i].load(a, rows.p, rows.q, min(v0 + i * 2048 + (int)threadIdx.x * 8, end), end);
-    if (a.draft == nullptr) mark_children(w, tn, s_up, s_tok, v0, s_gone);
-    double left = 0.0, whole = 0.0;
+    for (int i = 0; i < EACH; ++i) x[i].load(a, rows.p, rows.q, min((run0 + i) * RUN + lane * 8, a.V), a.V);
+    if (a.draft == nullptr) mark_children<256>(w, tn, s_up, s_tok, v0, SLICE, s_gone);
 #pragma unroll
-    for (int i = 0; i < SLICE / 2048; ++i) {
-        const int at = i * 2048 + threadIdx.x * 8;
+    for (int i = 0; i < EACH; ++i) {
+        if (run0 + i >= a.runs) break;
+        const int at = (run0 + i) * RUN + lane * 8 - v0;
         const uint32_t gone = a.draft == nullptr ? s_gone[at / 32] >> (at % 32) : 0;
+        double left = 0.0, whole = 0.0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) left += x[i].left(e, gone), whole += x[i].whole(e);
-    }
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) left += __shfl_xor(left, off, 64), whole += __shfl_xor(whole, off, 64);
-    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6][0] = left, s_sum[threadIdx.x >> 6][1] = whole;
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        double t = 0.0;
-        for (int i = 0; i < 4; ++i) t += s_sum[i][threadIdx.x];
-        a.sums[2 * ((int64_t)b * a.slices + blockIdx.x) + threadIdx.x] = t;
+        for (int off = 32; off >= 1; off >>= 1) left += __shfl_xor(left, off, 64), whole += __shfl_xor(whole, off, 64);
+        if (lane == 0) {
+            double* out = a.sums + (int64_t)b * 2 * a.runs + run0 + i;
+            out[0] = left, out[a.runs] = whole;
+        }
     }
 }
 
-// Sum of v over the threads before this one, and over all 256.
-__device__ __forceinline__ double scan256(double v, double* lds, double& total) {
-    double inc = v;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double x = __shfl_up(inc, off, 64);
-        if (lane >= off) inc += x;
-    }
-    __syncthreads();  // the last call's totals are read
-    if (lane == 63) lds[wave] = inc;
-    __syncthreads();
-    double before = 0.0;
-    for (int w = 0; w < wave; ++w) before += lds[w];
-    total = ((lds[0] + lds[1]) + lds[2]) + lds[3];
-    return before + (inc - v);
-}
-
-// The next token: the slice that the random number falls on by the slices' sums, then the entry. A number that the
-// sums' own rounding leaves behind the last entry takes the last with a weight.
+// The next token, by one wave a sequence: the run that the random number falls on by the runs' sums, then the entry, the
+// run read again. A number that the sums' own rounding leaves behind the last entry takes the last with a weight. Three
+// round trips (the walk's end and the first sums, the row, the token): as a workgroup that walked by itself and searched
+// whole slices, 13 us for 16 trees of 16.
 template <class T>
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a) {
-    __shared__ double s_p[MAX_DRAFTS];
-    __shared__ int32_t s_tok[MAX_DRAFTS], s_walk[3];
-    __shared__ int16_t s_up[MAX_DRAFTS];
-    __shared__ uint32_t s_gone[SLICE / 32];
-    __shared__ double s_scan[4], s_base;
-    __shared__ int s_first, s_last;
-    const int b = blockIdx.x;
+__global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
+    const int b = blockIdx.x, lane = threadIdx.x;
     const int tn = a.tree_len != nullptr ? min(max(a.tree_len[b], 0), a.T) : a.T;
-    const Walk w = walk_drafts<T>(a, b, s_p, s_up, s_tok, s_walk, nullptr);
-    if (w.n == 0) return;
-    constexpr int PER = MAX_SLICES / 256;
-    const double* sums = a.sums + 2 * (int64_t)b * a.slices;
-    double mine[PER][2], left = 0.0, whole = 0.0, total, before;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int at = (int)threadIdx.x * PER + i;
-        mine[i][0] = at < a.slices ? sums[2 * at] : 0.0;
-        mine[i][1] = at < a.slices ? sums[2 * at + 1] : 0.0;
-        left += mine[i][0], whole += mine[i][1];
+    if (tn == 0) {
+        if (lane == 0) a.next[b] = -1;
+        return;
     }
+    const int32_t* walk = a.walk + 4 * b;
+    const Walk w = {1, walk[1], walk[2]};
+    const float u = a.u_next[b];
+    // lane l has `per` runs in a row
+    const int per = (a.runs + 63) / 64;
+    const double* sums = a.sums + (int64_t)b * 2 * a.runs;
+    double before, total;
     int which = 0;
-    before = scan256(left, s_scan, total);
+    auto sum_of = [&](const double* from) {
+        double sum = 0.0;
+        for (int i = 0; i < per; ++i) sum += lane * per + i < a.runs ? from[lane * per + i] : 0.0;
+        before = before_in_wave(sum, total);
+    };
+    sum_of(sums);
     if (!(total > 0.0)) {
         // nothing is left (the draft's row is the target's, up to its rounding): the row as it is
         which = 1;
-        before = scan256(whole, s_scan, total);
+        sums += a.runs;
+        sum_of(sums);
         if (!(total > 0.0)) {
-            if (threadIdx.x == 0) a.next[b] = -1;
+            if (lane == 0) a.next[b] = -1;
             return;
         }
     }
-    // the first place where the sum passes x, and the last that adds to it
-    const double x = (double)a.u_next[b] * total;
-    auto search = [&](double sum, auto weight, int n) {
-        if (threadIdx.x == 0) s_first = INT_MAX, s_last = -1;
-        __syncthreads();
-        int first = INT_MAX, last = -1;
-        double at_first = 0.0, at_last = 0.0;
-        for (int i = 0; i < n; ++i) {
-            const double m = weight(i);
-            if (m > 0.0) {
-                last = (int)threadIdx.x * n + i, at_last = sum;
-                if (first == INT_MAX && sum + m > x) first = last, at_first = sum;
-            }
-            sum += m;
-        }
-        if (first != INT_MAX) atomicMin(&s_first, first);
-        if (last >= 0) atomicMax(&s_last, last);
-        __syncthreads();
-        const int at = s_first != INT_MAX ? s_first : s_last;
-        if (at == first) s_base = at_first;
-        else if (at == last) s_base = at_last;
-        __syncthreads();
-        return at;
-    };
-    const int slice = search(before, [&](int i) { return which ? mine[i][1] : mine[i][0]; }, PER);
-    const double base = s_base;
-    const int v0 = slice * SLICE, end = min(v0 + SLICE, a.V);
-    if (a.draft == nullptr) mark_children(w, tn, s_up, s_tok, v0, s_gone);
+    const double x = (double)u * total;
+    double base, unused;
+    const int run = find_in_wave([&](int i) { return lane * per + i < a.runs ? sums[lane * per + i] : 0.0; }, per, before, x, base);
     const Rows<T> rows(a, b, w);
-    constexpr int EACH = SLICE / 256;
-    double m[EACH], sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < EACH / 8; ++i) {
-        const int at = (int)threadIdx.x * EACH + i * 8;
-        Weights<T> y;
-        y.load(a, rows.p, rows.q, min(v0 + at, end), end);
-        const uint32_t gone = a.draft == nullptr ? s_gone[at / 32] >> (at % 32) : 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            m[i * 8 + e] = which ? y.whole(e) : y.left(e, gone);
-            sum += m[i * 8 + e];
+    const int v = run * RUN + lane * 8;
+    Weights<T> y;
+    y.load(a, rows.p, rows.q, min(v, a.V), a.V);
+    uint32_t gone = 0;
+    if (a.draft == nullptr)
+        for (int t = w.last + 1; t < tn; ++t) {
+            const int up = a.parents != nullptr ? a.parents[b * a.ld_par + t] : t - 1, e = a.tokens[b * a.ld_tok + t] - v;
+            if (up == w.last && e >= 0 && e < 8) gone |= 1u << e;
         }
+    double m[8], sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        m[e] = which ? y.whole(e) : y.left(e, gone);
+        sum += m[e];
     }
-    before = scan256(sum, s_scan, total);
-    const int at = search(base + before, [&](int i) { return m[i]; }, EACH);
-    if (threadIdx.x == 0) a.next[b] = at >= 0 ? v0 + at : -1;
+    before = before_in_wave(sum, total);
+    const int token = run * RUN + find_in_wave([&](int i) { return m[i]; }, 8, base + before, x, unused);
+    if (lane == 0) a.next[b] = token;
 }
 
 size_t verify_bytes(int B, int V) {
-    return B > 0 && V > 0 ? (size_t)B * ((V + SLICE - 1) / SLICE) * 2 * sizeof(double) : 0;
+    return B > 0 && V > 0 ? (size_t)B * (((V + RUN - 1) / RUN) * 2 * sizeof(double) + 4 * sizeof(int32_t)) : 0;
 }
 
 }  // namespace
@@ -561,7 +558,7 @@ __attribute__((visibility("default"))) int ythip_verify_drafts(
     if (workspace == nullptr || ws_bytes < need || ((uintptr_t)workspace & 7) != 0)
         return fail(YTHIP_EINVAL, "%s: needs an 8-byte aligned workspace of %zu bytes, got %zu", who, need, ws_bytes);
     VerifyArgs a;
-    a.B = B, a.T = T, a.V = V, a.slices = (V + SLICE - 1) / SLICE;
+    a.B = B, a.T = T, a.V = V, a.slices = (V + SLICE - 1) / SLICE, a.runs = (V + RUN - 1) / RUN;
     a.target = target, a.draft = draft;
     for (int i = 0; i < 2; ++i) {
         a.ts[i] = (i == 0 ? B : T) > 1 ? target_str[i] : 0;
@@ -570,11 +567,12 @@ __attribute__((visibility("default"))) int ythip_verify_drafts(
     a.tokens = tokens, a.parents = parents, a.tree_len = tree_len, a.ld_tok = ld_tokens, a.ld_par = ld_parents;
     a.u = u, a.u_next = u_next, a.ld_u = ld_u, a.path = path, a.ld_path = ld_path, a.kept = kept, a.next = next;
     a.sums = static_cast<double*>(workspace);
+    a.walk = reinterpret_cast<int32_t*>(a.sums + (int64_t)B * 2 * a.runs);
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto t) {
         using T_ = decltype(t);
         verify_sum_kernel<T_><<<dim3(a.slices, B), 256, 0, s>>>(a);
-        verify_pick_kernel<T_><<<B, 256, 0, s>>>(a);
+        verify_pick_kernel<T_><<<B, 64, 0, s>>>(a);
     };
     if (dtype == YTHIP_F32) run(F32{});
     else if (dtype == YTHIP_F16) run(F16{});

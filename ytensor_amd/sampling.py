@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import check
 from .ops import _code, _stream
-from .paged import _away, _device, _ints, _packed, _real
+from .paged import _away, _device, _i64, _ints, _packed, _real
 
 
 def token_probs(logits: torch.Tensor, temperature: float = 1.0, out: torch.Tensor | None = None,
@@ -36,17 +36,28 @@ def token_probs(logits: torch.Tensor, temperature: float = 1.0, out: torch.Tenso
     elif out.dtype != torch.float32 or out.shape != shape:
         raise ValueError(f"out must be float32 {list(shape)}")
     n = shape[-1]
+    if logits.is_contiguous() and out.is_contiguous() and n:
+        x, o, rows, ld, ld_out = logits, out, logits.numel() // n, n, n
+    else:
+        x, o, rows, ld, ld_out = _matrices(logits, out, n)
+    at, size, need = None, 0, _probs_workspace(rows, n)
+    if need:
+        workspace, at, size = _space(workspace, need, logits.device)
+    st = _lib.lib().ythip_token_probs(code, rows, n, x.data_ptr(), ld, float(temperature), o.data_ptr(), ld_out, at, size,
+                                      _stream())
+    if st:
+        check(st, "ythip_token_probs")
+    return out
+
+
+def _matrices(logits, out, n):
+    """logits and out as rows: (logits, or a copy, out, rows, their strides)"""
     x, o = _matrix(logits), _matrix(out)
     if x is None:
         x = logits.contiguous().reshape(-1, n)
     if o is None:
         raise ValueError("out must have rows at one stride, with the last dim contiguous")
-    rows = x.shape[0]
-    need = _probs_workspace(rows, n)
-    workspace, at, size = _space(workspace, need, logits.device)
-    check(_lib.lib().ythip_token_probs(code, rows, n, x.data_ptr(), x.stride(0), float(temperature), o.data_ptr(),
-                                       o.stride(0), at, size, _stream()), "ythip_token_probs")
-    return out
+    return x, o, x.shape[0], x.stride(0), o.stride(0)
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor | None:
@@ -136,17 +147,20 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, u
     if tree_len is not None:
         tree_len = _packed(_ints("tree_len", tree_len, (B,)))
     if out is None:
-        out = (torch.empty((B, T), dtype=torch.int32, device=target.device),
-               *torch.empty((2, B), dtype=torch.int32, device=target.device))
-    path, kept, token = out
-    for name, t, shape in (("path", path, (B, T)), ("kept", kept, (B,)), ("token", token, (B,))):
-        if not _ints(name, t, shape).is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+        dev = target.device
+        path, kept = torch.empty((B, T), dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int32, device=dev)
+        token = torch.empty_like(kept)
+    else:
+        path, kept, token = out
+        for name, t, shape in (("path", path, (B, T)), ("kept", kept, (B,)), ("token", token, (B,))):
+            if not _ints(name, t, shape).is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
     workspace, at, size = _space(workspace, _verify_workspace(B, V), target.device)
-    strides = lambda t: _lib.i64array(_real(t)[:2])  # noqa: E731
-    check(_lib.lib().ythip_verify_drafts(
-        code, B, T, V, target.data_ptr(), strides(target), None if draft is None else draft.data_ptr(),
-        None if draft is None else strides(draft), tokens.data_ptr(), T, None if parents is None else parents.data_ptr(),
+    st = _lib.lib().ythip_verify_drafts(
+        code, B, T, V, target.data_ptr(), _i64(_real(target)), None if draft is None else draft.data_ptr(),
+        None if draft is None else _i64(_real(draft)), tokens.data_ptr(), T, None if parents is None else parents.data_ptr(),
         T, None if tree_len is None else tree_len.data_ptr(), u.data_ptr(), T, u_next.data_ptr(), path.data_ptr(), T,
-        kept.data_ptr(), token.data_ptr(), at, size, _stream()), "ythip_verify_drafts")
+        kept.data_ptr(), token.data_ptr(), at, size, _stream())
+    if st:
+        check(st, "ythip_verify_drafts")
     return path, kept, token
