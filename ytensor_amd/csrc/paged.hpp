@@ -362,6 +362,10 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     p.wr = rows <= 32 || top_k > 0 ? 1 : rows <= 64 ? 2 : 4;
     p.kt = 16 * p.wr;
     const int64_t all_rows = top_k > 0 ? G : (int64_t)T * G;
+    // a window leaves a row tile few keys: half the rows a workgroup where that fills the second place of the CUs
+    const bool windowed = window > 0 && p.wr == 4;
+    if (windowed && (int64_t)B * Hkv * ((all_rows + 127) / 128) < SLOTS && (int64_t)B * Hkv * ((all_rows + 63) / 64) >= SLOTS / 2)
+        p.wr = 2, p.kt = 32;
     const int rw = 16 * p.qt * p.wr;
     p.row_tiles = (int)((all_rows + rw - 1) / rw);
     const int64_t per = (int64_t)Hkv * p.row_tiles;
@@ -384,7 +388,11 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     if (window > 0) seq_rows = std::min(seq_rows, (int64_t)window + sinks + 2 * p.kt);  // (a tile more at either end)
     const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + new_tiles, most = (tiles + p.stage - 1) / p.stage;
     int64_t part_items = 0;
-    if (top_k > 0) {
+    if (windowed && B * per >= SLOTS / 2) {
+        // (each row tile sees tiles of its own: ranges of all that one of them sees would leave most workgroups few)
+        p.target = 0;
+        p.items = B;
+    } else if (top_k > 0) {
         // (a token's pages in ranges of at least the stages that least_stages explains)
         const int64_t root = std::max<int64_t>(1, (int64_t)std::ceil(std::sqrt((double)most / 20)));
         p.target = (int)std::max<int64_t>(1, std::min((most + root - 1) / root, (slots + per * B * T - 1) / (per * B * T)));

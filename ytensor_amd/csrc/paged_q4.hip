@@ -667,6 +667,10 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
     auto clean_scales = [&](u32x2& vs, uint32_t use, bool some, int c) INLINE {
         const uint32_t mine = use >> (8 * g);
         uint32_t odd = 0;
+        // (a byte of 255: bit 7 of it, and of its complement less 1)
+        const uint32_t none = vs[0] & (~vs[0] - 0x01010101u) & 0x80808080u, none1 = vs[1] & (~vs[1] - 0x01010101u) & 0x80808080u;
+        some = some && __ballot((none | none1) != 0) != 0;
+        if (!some && use == ~0u) return odd;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint32_t byte = vs[e / 4] >> (8 * (e % 4)) & 255;
@@ -953,10 +957,11 @@ Plan plan_q4(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     Plan p;
     const int64_t rows = (int64_t)T * G;
     // 16 rows of a wave (bfloat16: 32) leave the tiles to the four; more share them. 32 rows of a wave where there are more
-    // than 64 and the queries' pieces leave the registers
+    // than 64 and one piece a query leaves the registers; with a window 16 where that fills the second place of the CUs
     const bool few = rows <= (dtype == YTHIP_BF16 ? 32 : 16);
     p.wr = few ? 1 : 4;
-    p.qt = few ? (rows <= 16 ? 1 : 2) : rows <= 64 || dtype == YTHIP_F32 ? 1 : 2;
+    p.qt = few ? (rows <= 16 ? 1 : 2) : rows <= 64 || dtype != YTHIP_BF16 ? 1 : 2;
+    if (window > 0 && !few && (int64_t)B * Hkv * ((rows + 127) / 128) < SLOTS) p.qt = 1;
     p.kt = few ? 32 : 64;
     const int rw = 16 * p.qt * p.wr;
     p.row_tiles = (int)((rows + rw - 1) / rw);
@@ -968,7 +973,7 @@ Plan plan_q4(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     if (window > 0) seq_rows = std::min(seq_rows, (int64_t)window + sinks + 2 * p.kt);
     const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + ((int64_t)T + p.kt - 1) / p.kt, most = (tiles + p.stage - 1) / p.stage;
     int64_t part_items = 0;
-    if (most <= WHOLE) {
+    if (most <= WHOLE || (window > 0 && !few && B * per >= SLOTS / 2)) {  // (as plan_of has it)
         p.target = 0;
         p.items = B;
     } else {
@@ -996,10 +1001,10 @@ int launch_q4(const PagedArgs& a, const Plan& p, hipStream_t s) {
 template <class T, int D, bool WIN>
 int run_q4(const PagedArgs& a, const Plan& p, hipStream_t s) {
     if (p.wr == 1 && p.qt == 1) return launch_q4<T, D, 1, 1, WIN>(a, p, s);
-    if constexpr (std::is_same_v<T, BF16>)
+    if constexpr (std::is_same_v<T, BF16>) {
         if (p.wr == 1) return launch_q4<T, D, 2, 1, WIN>(a, p, s);
-    if constexpr (!std::is_same_v<T, F32>)
         if (p.qt == 2) return launch_q4<T, D, 2, 4, WIN>(a, p, s);
+    }
     return launch_q4<T, D, 1, 4, WIN>(a, p, s);
 }
 

@@ -43,8 +43,8 @@ def _blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, dims: int) -> tuple:
     if k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 or k_pool.dim() != dims or v_pool.shape != k_pool.shape:
         raise ValueError(f"4-bit pools must be uint8 [{'L, ' if dims == 4 else ''}P, Hkv, bytes], got {k_pool.dtype} "
                          f"{list(k_pool.shape)} and {v_pool.dtype} {list(v_pool.shape)}")
-    st = _real(k_pool)
-    if k_pool.stride(-1) != 1 or v_pool.stride(-1) != 1 or _real(v_pool) != st:
+    st = k_pool.stride()
+    if st[-1] != 1 or (v_pool.stride() != st and (v_pool.stride(-1) != 1 or _real(v_pool) != _real(k_pool))):
         raise ValueError("k_pool and v_pool must share strides, with a block contiguous")
     return st
 

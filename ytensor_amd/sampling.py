@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import check
 from .ops import _code, _stream
-from .paged import _away, _device, _i64, _ints, _packed, _real
+from .paged import _away, _device, _i64, _ints, _packed
 
 
 def token_probs(logits: torch.Tensor, temperature: float = 1.0, out: torch.Tensor | None = None,
@@ -157,8 +157,8 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, u
                 raise ValueError(f"{name} must be contiguous")
     workspace, at, size = _space(workspace, _verify_workspace(B, V), target.device)
     st = _lib.lib().ythip_verify_drafts(
-        code, B, T, V, target.data_ptr(), _i64(_real(target)), None if draft is None else draft.data_ptr(),
-        None if draft is None else _i64(_real(draft)), tokens.data_ptr(), T, None if parents is None else parents.data_ptr(),
+        code, B, T, V, target.data_ptr(), _i64(target.stride()), None if draft is None else draft.data_ptr(),
+        None if draft is None else _i64(draft.stride()), tokens.data_ptr(), T, None if parents is None else parents.data_ptr(),
         T, None if tree_len is None else tree_len.data_ptr(), u.data_ptr(), T, u_next.data_ptr(), path.data_ptr(), T,
         kept.data_ptr(), token.data_ptr(), at, size, _stream())
     if st:
