@@ -70,7 +70,7 @@ __device__ __forceinline__ int tiles_of(const PagedArgs& a, int len, int tn, int
 
 // What of a sequence's tiles (seen_rows', then those of the new tokens) one workgroup's tokens see under a window, of
 // its range [c0, c1): those from `low` on, then, downwards too, those below `sink_end`. at(i): the i-th, c0 - 1 behind
-// the last. `clean`: all its tokens see the cached tiles from there on whole.
+// the last. `clean`: all its tokens see the tiles from there on whole, up to their own.
 struct Window {
     int c0, high, low, sink_end, clean;
     __device__ __forceinline__ int count() const { return max(high - low, 0) + max(sink_end - c0, 0); }
@@ -95,7 +95,7 @@ __device__ __forceinline__ Window window_of(const PagedArgs& a, const Seen& seen
     w.low = max(max(low, end), c0);
     w.sink_end = min(end, w.high);
     const int64_t whole = (int64_t)len + t_last + 1 - a.window;
-    w.clean = whole <= 0 ? 0 : (int)min((whole + kt - 1) / kt - seen.gap, (int64_t)INT_MAX);
+    w.clean = whole <= 0 ? 0 : whole <= len ? (int)((whole + kt - 1) / kt) - seen.gap : seen.tiles + (int)((whole - len + kt - 1) / kt);
     return w;
 }
 

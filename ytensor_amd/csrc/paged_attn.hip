@@ -587,7 +587,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
     };
 
     uint32_t here = 0, next = 0;  // what is staged for s and s + 1
-    auto step = [&](int s, auto with_new) {
+    auto step = [&](int s, auto issue_new, auto with_new) {
         // the lookups of stage s + 2 run beside the arithmetic of stage s
         ids(s + 2);
 #pragma unroll
@@ -601,11 +601,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
         if constexpr (WR > 1) wg_barrier();
         else asm volatile("" ::: "memory");
         here = next;
-        next = s + 2 < nst ? issue(s + 2, with_new) : 0;
+        next = s + 2 < nst ? issue(s + 2, issue_new) : 0;
     };
     // stages with new tokens, then those of cached rows alone: a loop of its own, that holds none of
     // the paths' state in registers
-    const int s_new = WIN ? (max(win.high - max(win.low, nct), 0) + max(win.sink_end - max(c0, nct), 0) + S::WK - 1) / S::WK
+    // (with a window and no tree, new tokens before the first query's are as cached rows are)
+    const int own = WIN && a.parents == nullptr && a.sinks <= len ? (t_first + 1) / KT : 0;
+    const int s_new = WIN ? (max(win.high - max(win.low, nct + own), 0) + max(win.sink_end - max(c0, nct), 0) + S::WK - 1) / S::WK
                           : (max(c1 - max(c0, nct), 0) + S::WK - 1) / S::WK;
     const int s_whole = WIN ? max(s_new, max(win.high - max(win.low, win.clean), 0) / S::WK) : nst;
     {
@@ -638,10 +640,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedArgs a) {
             next = s < nst ? issue(s, std::true_type{}) : 0;
         }
     }
-    for (int s = 0; s < s_new; ++s) step(s, std::true_type{});
-    for (int s = s_new; s < s_whole; ++s) step(s, std::false_type{});
+    for (int s = 0; s < s_new; ++s) step(s, std::true_type{}, std::true_type{});
+    for (int s = s_new; s < s_whole; ++s) step(s, std::bool_constant<WIN>{}, std::false_type{});
     if constexpr (WIN)
-        for (int s = s_whole; s < nst; ++s) step(s, std::true_type{});
+        for (int s = s_whole; s < nst; ++s) step(s, std::true_type{}, std::true_type{});
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) m[qt] *= c;
     // the place of row r's result: O itself, or this item's partial
