@@ -277,6 +277,27 @@ def test_strides_and_bad_pages(dtype, d):
             yt.paged_attention_q4(**(dict(q=q, k_new=kn, v_new=vn, k_pool=k, v_pool=v, table=table, kv_len=kv_len, page=page) | bad))
 
 
+@pytest.mark.parametrize("columns,pages", [(3, 0), (0, 0), (0, 5)])
+@pytest.mark.parametrize("page", [16, 128, 8192])
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 64)])
+def test_no_pages_and_no_columns(dtype, d, page, columns, pages):
+    """Every cached row is hidden, or there is none: the new tokens alone, and zeros without them."""
+    dt, Hkv, G, B = DT[dtype], 2, 4, 2
+    g = torch.Generator().manual_seed(page + columns)
+    k, v = (torch.full((pages, Hkv, yt.cache_q4_bytes(page, d)), 255, dtype=torch.uint8, device="cuda") for _ in range(2))
+    table = torch.randint(-2, 4, (B, columns), generator=g).int().cuda()
+    kv_len = ints([2 * page + 9, 5])
+    rows = Rows(*(torch.zeros(pages, Hkv, page, d) for _ in range(2)), table, ints([2 * page + 9, 5] if columns else [0, 0]))
+    used = kv_len if columns else ints([0, 0])
+    for T in (1, 5, 70):
+        for window, sinks in ((0, 0), (3, 40)):
+            q, kn, vn = tokens(g, B, Hkv * G, Hkv, T, d, dt)
+            out = yt.paged_attention_q4(q, kn, vn, k, v, table, kv_len, page, window=window, sinks=sinks)
+            want, tol = attention(q, kn, vn, rows, used, None, None, window, sinks)
+            compare(out, want, tol)
+            assert (yt.paged_attention_q4(q, None, None, k, v, table, kv_len, page, window=window, sinks=sinks) == 0).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("T", [1, 9, 40, 140])
 @pytest.mark.parametrize("d", [64, 128])

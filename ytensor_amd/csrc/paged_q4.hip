@@ -259,8 +259,9 @@ __device__ __forceinline__ float sum_across_rows(float v) {
     return __uint_as_float(p32[0]) + __uint_as_float(p32[1]);
 }
 
-// What stands in for a pool that has no pages: a tile's loads go there.
-static __device__ const u32x4 no_pages[2 * 64 * 64 / 16] = {};
+// What stands in for a pool that has no pages, or where no sequence has a column: one page of 16 rows, which a tile's
+// loads go to.
+static __device__ const u32x4 no_pages[16 * (128 / 2 + 128 / 32) / 16] = {};
 
 // (a lambda that is not inlined has its arrays in memory)
 #define INLINE __attribute__((always_inline))
@@ -360,8 +361,12 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
     }
 
     // ---- tiles of cached rows: lookups and loads
-    const int page = 1 << a.shift;
-    const uint8_t *Kp = static_cast<const uint8_t*>(a.Kp) + h * a.ps[1], *Vp = static_cast<const uint8_t*>(a.Vp) + h * a.ps[1];
+    // (where there is none, no id is one of a page: all loads are within page 0, the stand-in)
+    const bool none = a.pages == 0;
+    const int page = none ? 16 : 1 << a.shift;
+    const int64_t page_str = none ? 0 : a.ps[0], head = none ? 0 : h * a.ps[1];
+    const uint8_t* stand_in = reinterpret_cast<const uint8_t*>(no_pages);
+    const uint8_t *Kp = (none ? stand_in : static_cast<const uint8_t*>(a.Kp)) + head, *Vp = (none ? stand_in : static_cast<const uint8_t*>(a.Vp)) + head;
     auto tile_at = [&](int s) { return WIN ? win.at(s * S::WK + wk) : win.high - 1 - (s * S::WK + wk); };
     struct Ids {
         int id[SUB];  // of the tile's 16 rows each
@@ -410,7 +415,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             const int q = SHARED ? wave >> 1 : i;
             // where the 32 rows begin in a block, as their two halves have it: with pages of 16 rows those lie in two
             const int first = row + 32 * q, low = first & (page - 1), high = ((first + 16) & (page - 1)) - 16;
-            const int64_t p0 = page_of(SHARED ? (wave >> 1 ? 2 : 0) : 2 * i) * a.ps[0], p1 = page_of(SHARED ? (wave >> 1 ? 3 : 1) : 2 * i + 1) * a.ps[0];
+            const int64_t p0 = page_of(SHARED ? (wave >> 1 ? 2 : 0) : 2 * i) * page_str, p1 = page_of(SHARED ? (wave >> 1 ? 3 : 1) : 2 * i + 1) * page_str;
             const int64_t codes[2] = {p0 + low * (D / 2), p1 + high * (D / 2)};
             const int64_t scales[2] = {p0 + page * (D / 2) + low * (D / 32), p1 + page * (D / 2) + high * (D / 32)};
             const uint8_t *kc = Kp + (l16 >> 3 ? codes[1] : codes[0]) + k_at, *kx = Kp + (l16 >> 3 ? scales[1] : scales[0]) + ks_at;
@@ -1146,14 +1151,12 @@ __attribute__((visibility("default"))) int ythip_paged_attn_q4(
     if (st || done) return st;
     int64_t ps[3] = {0, 0, 0};
     const int64_t str[3] = {0, pool_str[0], pool_str[1]};
-    if (columns > 0)
+    if (columns > 0) {
         if (const int e = check_blocks(who, 1, pages, Hkv, page, d, Kp, Vp, str, ps)) return e;
-    a.ps[0] = ps[1], a.ps[1] = ps[2], a.ps[2] = 0;
-    if (pages == 0) {
-        void* none = nullptr;
-        if (const int e = status_of(hipGetSymbolAddress(&none, HIP_SYMBOL(no_pages)))) return e;
-        a.Kp = a.Vp = none;
+    } else {
+        a.pages = 0;  // the pools may be NULL
     }
+    a.ps[0] = ps[1], a.ps[1] = ps[2], a.ps[2] = 0;
     trim_window(T, columns, page, window, sinks);
     a.window = window, a.sinks = sinks;
     const Plan p = plan_q4(dtype, B, Hkv, a.G, T, d, columns, page, window, sinks);
