@@ -306,6 +306,11 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
     __shared__ u32x4 smem[S::LDS];
     __shared__ int16_t s_up[MAX_TREE];
     __shared__ uint32_t s_odd[SHARED ? 2 * 4 * 2 : 1];  // of a converted tile: bits of rows without a value, by channel group
+    __shared__ int s_inf[4];  // of the tiles of new tokens there, by stage: V holds what is not finite
+    // New tokens go through LDS too where one piece holds their values: a wave reads a quarter of a tile, not all of it
+    // (chunk of 2048 after 2048 rows, window 1024: 219 -> 78 us; 4096 after 64, window 2048: 560 -> 221; two chunks of 512
+    // over 8192: 116 -> 96). float16 and float32 would take two or three pieces, which LDS has no room for.
+    constexpr bool SHARED_NEW = SHARED && std::is_same_v<T, BF16>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR;
     const int l16 = lane & 15, g = lane >> 4;
@@ -726,13 +731,77 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         });
     };
 
+    // The same for a tile of new tokens: what a wave has of it, and its share into LDS
+    struct RawNew {
+        u32x4 k[SHARED_NEW ? KS : 1];
+        uint32_t v[SHARED_NEW ? 8 : 1][SHARED_NEW ? DT / 4 : 1];
+    };
+    auto load_new = [&](int s, RawNew& w) INLINE {
+        const int u0 = (tile_at(s) - nct) * KT, half = u0 + 32 * (wave >> 1);
+        const char* k = Kn + min(half + k_row + 4 * (wave & 1), tn - 1) * a.kns[2] * ES + g * (D / 4) * ES;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) w.k[ks] = *reinterpret_cast<const u32x4*>(k + ks * 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const char* v = Vn + min(half + 8 * g + e, tn - 1) * a.vns[2] * ES + l16 * (D / 16) * ES + 4 * (wave & 1);
+#pragma unroll
+            for (int i = 0; i < DT / 4; ++i) w.v[e][i] = *reinterpret_cast<const uint32_t*>(v + 8 * i);
+        }
+    };
+    auto convert_new = [&](int s, RawNew& w) INLINE {
+        u32x4* to = smem + (s & 1) * 64 * (S::KF + S::VF) + lane;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) to[(wave * KS + ks) * 64] = w.k[ks];
+        to += (S::KF + (wave >> 1) * DT + 2 * (wave & 1)) * 64;
+        // 0 . V is NaN for a V that is not finite: such elements are left out, and added for the queries that see them
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < DT / 4; ++i) {
+            uint32_t v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t odd = (((w.v[e][i] & 0x7f807f80u) + 0x00800080u) >> 15) & 0x00010001u;  // an exponent of ones
+                bad = bad || odd != 0;
+                v[e] = w.v[e][i] & ~(odd * 0xffffu);
+            }
+            u32x4 even, odd;
+            pair_rows(v, even, odd);
+            to[4 * i * 64] = even, to[(4 * i + 1) * 64] = odd;
+        }
+        if (__ballot(bad) != 0 && lane == 0) s_inf[s & 3] = 1;
+    };
+
     auto compute = [&](int s, uint64_t use, Raw& w, auto masked) INLINE {
         constexpr bool MASKED = decltype(masked)::value;
         uint64_t see[QT];
         bool hide = use != FULL, some = false;  // some: a query sees rows of it that another does not
+        const bool is_new = SHARED_NEW && MASKED && tile_at(s) >= nct;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) see[qt] = use;
-        if constexpr (MASKED) {
+        if (is_new) {
+            const int u0 = (tile_at(s) - nct) * KT;
+            bool any = false;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+                uint64_t mine = 0;
+                if (walk) {
+                    while (cur[qt] >= u0) {
+                        const bool in = !WIN || up[qt] < a.window || deep[qt] - up[qt] < a.sinks - len;
+                        if (in && cur[qt] < u0 + KT) mine |= 1ull << (cur[qt] - u0);
+                        cur[qt] = s_up[cur[qt]];
+                        ++up[qt];
+                    }
+                } else if (tok[qt] >= u0) {
+                    mine = ~from_bit(tok[qt] + 1 - u0);
+                    if constexpr (WIN) mine &= from_bit((int64_t)tok[qt] + 1 - a.window - u0) | ~from_bit((int64_t)a.sinks - len - u0);
+                }
+                see[qt] &= mine;
+                any = any || see[qt] != 0;
+                some = some || see[qt] != use;
+            }
+            if (__ballot(any) == 0) return;
+            hide = hide || __ballot(some) != 0;
+        } else if constexpr (MASKED && WIN) {
             const int j0 = seen.row(tile_at(s), KT);
             bool any = false;
 #pragma unroll
@@ -781,7 +850,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
                 for (int kk = 0; kk < KG; ++kk) odd[kk] = clean_scales(w.vs[kk], mine[kk], some, g * (D / 4) / 32);
             }
         }
-        if constexpr (SHARED && WIN) {
+        if (SHARED && WIN && !is_new) {
 #pragma unroll
             for (int kk = 0; kk < KG; ++kk) odd[kk] = s_odd[((s & 1) * 4 + g * (D / 4) / 32) * 2 + kk];
         }
@@ -805,6 +874,21 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
                         o[qt][2 * Q + 1] = mfma_chunk(BF16{}, odd_, pw[qt][n], o[qt][2 * Q + 1]);
                     }
             });
+        }
+        if (is_new && s_inf[s & 3] != 0) {
+            const int u0 = (tile_at(s) - nct) * KT;
+            for (int u = 0; u < min(tn - u0, KT); ++u) {
+                const int64_t row = (u0 + u) * a.vns[2];
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float x = load_as_f32<T>(Vn, row + (4 * g + r) * (D / 16) + t);
+#pragma unroll
+                        for (int qt = 0; qt < QT; ++qt)
+                            if (!(fabsf(x) < INFINITY) && (see[qt] >> u & 1)) o[qt][t][r] += x;
+                    }
+            }
         }
         if constexpr (SHARED ? WIN : MASKED) {
             const uint64_t none = odd[0] | (KG == 2 ? (uint64_t)odd[KG - 1] << 32 : 0);
@@ -831,7 +915,49 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             for (int u = u0 + KT - 32; u >= u0; u -= 32) new_rows_at(u);
         }
     };
-    if constexpr (SHARED) {
+    if constexpr (SHARED_NEW) {
+        // as below, from the new tokens' tiles on
+        if (tid < 4) s_inf[tid] = 0;
+        __syncthreads();
+        Raw w;
+        RawNew fresh;
+        uint64_t here, next = 0;
+        auto there = [&](int s) { return from_bit(tn - (tile_at(s) - nct) * KT); };  // rows behind the last new token
+        Ids x = ids(0);
+        uint64_t use = load(0, x, w);
+        if (new_tiles > 0) {
+            load_new(0, fresh);
+            convert_new(0, fresh);
+            here = ~there(0);
+        } else {
+            convert(0, use, w);
+            here = use;
+        }
+        x = ids(1);
+        next = load(1, x, w);
+        x = ids(2);
+        auto stage = [&](int s, auto masked, auto more_new) INLINE {
+            __syncthreads();
+            const bool fresh_next = decltype(more_new)::value && s + 1 < new_tiles;
+            if (fresh_next) load_new(s + 1, fresh);
+            if (here != 0) compute(s, here, w, masked);
+            // (read two stages ago, written again in the next)
+            if (decltype(more_new)::value && tid == 0) s_inf[(s + 2) & 3] = 0;
+            if (fresh_next) {
+                convert_new(s + 1, fresh);
+                here = ~there(s + 1);
+            } else {
+                convert(s + 1, next, w);
+                here = next;
+            }
+            next = load(s + 2, x, w);
+            x = ids(s + 3);
+        };
+        for (int s = 0; s < new_tiles; ++s) stage(s, std::true_type{}, std::true_type{});
+        for (int s = new_tiles; s < s_whole; ++s) stage(s, std::false_type{}, std::false_type{});
+        if constexpr (WIN)
+            for (int s = s_whole; s < nst; ++s) stage(s, std::true_type{}, std::false_type{});
+    } else if constexpr (SHARED) {
         new_tokens();
         // stage s is computed while s + 1 is converted and s + 2 is on its way: one barrier a stage
         Raw w;
