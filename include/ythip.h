@@ -707,7 +707,7 @@ int ythip_paged_attn_q4(int dtype, int B, int Hq, int Hkv, int T, int d, const v
 /*
  * probs[r] = softmax(logits[r] / temperature) over n columns, in fp32, of rows at strides
  * ld and ld_out (>= n; any alignment of an element). -inf has probability 0, a row of them
- * zeros; NaN or +inf makes its row NaN. temperature > 0. rows < 2^22. Workspace:
+ * zeros; NaN or +inf makes its row NaN. temperature > 0 (YTHIP_EUNSUPPORTED from about 1e36). rows < 2^22. Workspace:
  * ythip_token_probs_workspace_size bytes, 8-byte aligned (0: NULL is accepted).
  */
 size_t ythip_token_probs_workspace_size(int rows, int n);

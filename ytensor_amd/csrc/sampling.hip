@@ -20,17 +20,20 @@ struct ProbsArgs {
     int64_t ld, ld_out;
     float scale;  // log2(e) / temperature
     float scale_low;  // what scale lacks to it
+    float least;      // -200 / scale: what lies further below the largest has no weight in 32 bits
     float* p;
     float* part;  // [rows][parts] of (max, sum)
 };
 
-// 2^((x - top) scale) with the product's rounding put back: a logit 30 below the largest is else off by 2^-19.
-__device__ __forceinline__ float weight(float x, float top, float scale, float low) {
-    const float d = x - top, t = d * scale, rest = fmaf(d, scale, -t) + d * low;
+// 2^((x - top) scale) with the product's rounding put back: a logit 30 below the largest is else off by 2^-19. 0 for an x
+// of -inf; where x or top is NaN or +inf the row is NaN, which its maximum says (see write_row).
+__device__ __forceinline__ float weight(const ProbsArgs& a, float x, float top) {
+    const float d = __builtin_fmaxf(x - top, a.least), t = d * a.scale;
+    const float rest = fmaf(d, a.scale_low, fmaf(d, a.scale, -t));
     const float w = __builtin_amdgcn_exp2f(t);
-    // (below 2^-126 the product has nothing to put back, and -inf has none)
-    return t > -126.f ? fmaf(w, rest * 0.6931471805599453f, w) : t == t ? w : t;
+    return fmaf(w, rest * 0.6931471805599453f, w);
 }
+__device__ __forceinline__ float finite(float top) { return top == -INFINITY ? 0.f : top; }
 
 template <class T>
 struct Eight {  // 8 neighbouring logits
@@ -45,27 +48,31 @@ struct Eight {  // 8 neighbouring logits
         if constexpr (std::is_same_v<T, F32>) return __uint_as_float(w[i / 4][i % 4]);
         else return i & 1 ? hi_as_f32(T{}, w[0][i / 2]) : lo_as_f32(T{}, w[0][i / 2]);
     }
+    // (the compiler keeps no converted logits from one pass for the next: they take twice the registers)
+    __device__ __forceinline__ void again() {
+#pragma unroll
+        for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
+    }
 };
 
 // (M, L) of two parts: the larger maximum, and the sums in its unit
-__device__ __forceinline__ void join(float& M, float& L, float M2, float L2, float scale, float low) {
-    const float top = __builtin_elementwise_maximum(M, M2);
-    const float ref = top == -INFINITY ? 0.f : top;
-    L = L * weight(M, ref, scale, low) + L2 * weight(M2, ref, scale, low);
+__device__ __forceinline__ void join(const ProbsArgs& a, float& M, float& L, float M2, float L2) {
+    const float top = __builtin_elementwise_maximum(M, M2), ref = finite(top);
+    L = L * weight(a, M, ref) + L2 * weight(a, M2, ref);
     M = top;
 }
 template <int NT>
-__device__ __forceinline__ void join_block(float& M, float& L, float (&lds)[2 * NT / 64], float scale, float low) {
+__device__ __forceinline__ void join_block(const ProbsArgs& a, float& M, float& L, float (&lds)[2 * NT / 64]) {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) {
         const float M2 = __shfl_xor(M, off, 64), L2 = __shfl_xor(L, off, 64);
-        join(M, L, M2, L2, scale, low);
+        join(a, M, L, M2, L2);
     }
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) lds[2 * wave] = M, lds[2 * wave + 1] = L;
     __syncthreads();
     M = lds[0], L = lds[1];
-    for (int w = 1; w < NT / 64; ++w) join(M, L, lds[2 * w], lds[2 * w + 1], scale, low);
+    for (int w = 1; w < NT / 64; ++w) join(a, M, L, lds[2 * w], lds[2 * w + 1]);
 }
 
 // This thread's maximum and sum over columns [c0, c1) of a row.
@@ -83,23 +90,38 @@ __device__ __forceinline__ void scan_row(const ProbsArgs& a, int64_t row, int c0
         for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = __builtin_elementwise_maximum(top, v[u][e]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        L *= weight(M, ref, a.scale, a.scale_low);
+        const float ref = finite(top);
+        L *= weight(a, M, ref);
         M = top;
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
             if (c + u * NT * 8 < whole) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) L += weight(v[u][e], ref, a.scale, a.scale_low);
+                for (int e = 0; e < 8; ++e) L += weight(a, v[u][e], ref);
             }
     }
     const int c = whole + (int)threadIdx.x;
-    if (c < c1) join(M, L, load_as_f32<T>(a.x, row * a.ld + c), 1.f, a.scale, a.scale_low);
+    if (c < c1) join(a, M, L, load_as_f32<T>(a.x, row * a.ld + c), 1.f);
+}
+
+// Eight probabilities from their logits.
+template <class T>
+__device__ __forceinline__ void write_eight(const ProbsArgs& a, const Eight<T>& v, int64_t at, float ref, float inv) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        f32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = weight(a, v[4 * q + e], ref) * inv;
+        *reinterpret_cast<f32x4_any*>(a.p + at + 4 * q) = o;
+    }
+}
+// 1 / the sum; 0 for a row of -inf, NaN for one with a NaN or +inf
+__device__ __forceinline__ float inverse(float M, float L) {
+    return M == -INFINITY ? 0.f : M < INFINITY ? 1.0f / L : __builtin_nanf("");
 }
 template <class T, int NT>
-__device__ __forceinline__ void write_row(const ProbsArgs& a, int64_t row, int c0, int c1, float M, float L) {
+__device__ __forceinline__ void write_row(const ProbsArgs& a, int64_t row, int c0, int c1, float ref, float inv) {
     constexpr int AHEAD = 4;
-    const float ref = M == -INFINITY ? 0.f : M, inv = M == -INFINITY ? 0.f : 1.0f / L;
     const int whole = c0 + (c1 - c0) / 8 * 8;
     for (int c = c0 + (int)threadIdx.x * 8; c < whole; c += AHEAD * NT * 8) {
         Eight<T> v[AHEAD];
@@ -108,29 +130,56 @@ __device__ __forceinline__ void write_row(const ProbsArgs& a, int64_t row, int c
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (c + u * NT * 8 >= whole) break;
-            float* out = a.p + row * a.ld_out + c + u * NT * 8;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                f32x4 o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = weight(v[u][4 * q + e], ref, a.scale, a.scale_low) * inv;
-                *reinterpret_cast<f32x4_any*>(out + 4 * q) = o;
-            }
+            write_eight<T>(a, v[u], row * a.ld_out + c + u * NT * 8, ref, inv);
         }
     }
     const int c = whole + (int)threadIdx.x;
-    if (c < c1) a.p[row * a.ld_out + c] = weight(load_as_f32<T>(a.x, row * a.ld + c), ref, a.scale, a.scale_low) * inv;
+    if (c < c1) a.p[row * a.ld_out + c] = weight(a, load_as_f32<T>(a.x, row * a.ld + c), ref) * inv;
 }
 
-// Many rows: a workgroup has one, and reads it twice (the second time out of the caches).
+// Many rows: a workgroup has one. What of it the registers hold is read once (HELD times 8 columns a thread: 155648 columns
+// of 16 bits, 73728 of 32), and all of that is on its way before the first maximum; the rest is read twice. Bound by the
+// writes, and a third of the time by the exponentials, once for the sum and once to write: 256 rows of 151936 bfloat16
+// 51.6 us, 4.5 TB/s (read twice, and a weight of eleven operations where it has eight: 73).
 template <class T>
 __global__ __launch_bounds__(1024) void probs_row_kernel(ProbsArgs a) {
-    __shared__ float lds[2 * 1024 / 64];
+    constexpr int NT = 1024, HELD = std::is_same_v<T, F32> ? 9 : 19;
+    __shared__ float lds[2 * NT / 64];
     const int64_t row = blockIdx.x;
+    const int held = min(a.n / 8, HELD * NT) * 8;
+    Eight<T> v[HELD];
     float M, L;
-    scan_row<T, 1024>(a, row, 0, a.n, M, L);
-    join_block<1024>(M, L, lds, a.scale, a.scale_low);
-    write_row<T, 1024>(a, row, 0, a.n, M, L);
+#pragma unroll
+    for (int u = 0; u < HELD; ++u)
+        if (u * NT * 8 < held) v[u].load(a.x, row * a.ld + min((u * NT + (int)threadIdx.x) * 8, held - 8));
+    scan_row<T, NT>(a, row, held, a.n, M, L);
+    float top = M;
+#pragma unroll
+    for (int u = 0; u < HELD; ++u)
+        if (u * NT * 8 < held) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = __builtin_elementwise_maximum(top, v[u][e]);
+        }
+    float ref = finite(top);
+    L *= weight(a, M, ref);
+    M = top;
+#pragma unroll
+    for (int u = 0; u < HELD; ++u)
+        if ((u * NT + (int)threadIdx.x) * 8 < held) {
+            v[u].again();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) L += weight(a, v[u][e], ref);
+        }
+    join_block<NT>(a, M, L, lds);
+    ref = finite(M);
+    const float inv = inverse(M, L);
+#pragma unroll
+    for (int u = 0; u < HELD; ++u)
+        if ((u * NT + (int)threadIdx.x) * 8 < held) {
+            v[u].again();
+            write_eight<T>(a, v[u], row * a.ld_out + (u * NT + (int)threadIdx.x) * 8, ref, inv);
+        }
+    write_row<T, NT>(a, row, held, a.n, ref, inv);
 }
 // Few rows: `parts` workgroups a row, whose maxima and sums the second launch joins, each workgroup for itself.
 template <class T>
@@ -140,7 +189,7 @@ __global__ __launch_bounds__(256) void probs_part_kernel(ProbsArgs a) {
     const int c0 = blockIdx.x * a.run, c1 = min(c0 + a.run, a.n);
     float M, L;
     scan_row<T, 256>(a, row, c0, c1, M, L);
-    join_block<256>(M, L, lds, a.scale, a.scale_low);
+    join_block<256>(a, M, L, lds);
     if (threadIdx.x == 0) *reinterpret_cast<f32x2*>(a.part + 2 * (row * a.parts + blockIdx.x)) = f32x2{M, L};
 }
 template <class T>
@@ -151,19 +200,21 @@ __global__ __launch_bounds__(256) void probs_write_kernel(ProbsArgs a) {
     float M = -INFINITY, L = 0.f;
     for (int i = threadIdx.x; i < a.parts; i += 256) {
         const f32x2 v = *reinterpret_cast<const f32x2*>(a.part + 2 * (row * a.parts + i));
-        join(M, L, v[0], v[1], a.scale, a.scale_low);
+        join(a, M, L, v[0], v[1]);
     }
-    join_block<256>(M, L, lds, a.scale, a.scale_low);
-    write_row<T, 256>(a, row, c0, c1, M, L);
+    join_block<256>(a, M, L, lds);
+    write_row<T, 256>(a, row, c0, c1, finite(M), inverse(M, L));
 }
 
-constexpr int ROWS_ALONE = 192;  // rows from which a workgroup has one to itself
+// Rows from which a workgroup has one to itself (bfloat16, alone and in parts: 151936 columns, 128 rows 40.4 and 36.5 us,
+// 192 50.3 and 55.1, 256 60.1 and 68.8; 32000 columns 14.6 and 12.7, 15.7 and 17.0, 17.2 and 18.9).
+constexpr int ROWS_ALONE = 192;
 struct ProbsPlan {
     int parts, run;
 };
 ProbsPlan probs_plan(int rows, int n) {
     if (rows >= ROWS_ALONE || n <= 4096) return {1, n};
-    // 512 workgroups, of at least 1024 columns each
+    // 512 workgroups, of at least 1024 columns each (64 rows of 151936: 256 workgroups 23.3 us, 512 21.7, 1024 22.4)
     const int want = std::max(1, std::min((n + 1023) / 1024, (512 + rows - 1) / rows));
     const int run = ((n + want - 1) / want + 7) / 8 * 8;
     return {(n + run - 1) / run, run};
@@ -512,8 +563,8 @@ __attribute__((visibility("default"))) int ythip_token_probs(int dtype, int rows
     if (need > 0 && (workspace == nullptr || ws_bytes < need || ((uintptr_t)workspace & 7) != 0))
         return fail(YTHIP_EINVAL, "%s: needs an 8-byte aligned workspace of %zu bytes, got %zu", who, need, ws_bytes);
     const double scale = 1.4426950408889634 / (double)temperature;
-    if (!(scale < 1e38) || !(scale > 1e-37)) return fail(YTHIP_EUNSUPPORTED, "%s: temperature %g", who, temperature);
-    const ProbsArgs a = {rows, n, p.parts, p.run, logits, ld, ld_out, (float)scale, (float)(scale - (double)(float)scale), probs,
+    if (!(scale < 1e38) || !(scale > 1e-36)) return fail(YTHIP_EUNSUPPORTED, "%s: temperature %g", who, temperature);
+    const ProbsArgs a = {rows, n, p.parts, p.run, logits, ld, ld_out, (float)scale, (float)(scale - (double)(float)scale), (float)(-200.0 / scale), probs,
                          static_cast<float*>(workspace)};
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto t) {
