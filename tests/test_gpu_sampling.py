@@ -77,6 +77,25 @@ def test_probs_of_rows_with_infinities(dtype, n):
     assert p[5, 3] == 1 and p[5].sum() == 1
 
 
+@pytest.mark.parametrize("dtype,n", [("bf16", 8191), ("bf16", 155648), ("f16", 155661), ("bf16", 170003), ("f32", 73731), ("f32", 73728), ("f32", 100007)])
+def test_probs_of_many_rows(dtype, n):
+    """Rows with a workgroup each: within what its registers hold, to the last of it, and beyond; at an odd stride too."""
+    x = (3.0 * torch.randn(8, n, generator=torch.Generator().manual_seed(n))).to(DT[dtype])
+    x[1, n - 1] = math.inf
+    x[2, n - 1] = math.nan
+    x[3] = -math.inf
+    x[4, : n - 3] = -math.inf
+    x[5, n - 9] = 60.0
+    for wide in (0, 1):
+        rows = torch.zeros(200, n + wide, dtype=DT[dtype])
+        rows[:, :n] = x.repeat(25, 1)
+        p = yt.token_probs(rows.cuda()[:, :n], 0.7).cpu()
+        assert p[1:3].isnan().all() and (p[3] == 0).all() and (p[4, : n - 3] == 0).all()
+        for r in (0, 4, 5, 6, 7):
+            check_probs(p[r], x[r], 0.7)
+        assert torch.equal(p.view(25, 8, n).view(torch.int32), p[:8].view(torch.int32).expand(25, 8, n))
+
+
 def drafts(seed, B, T, V, dtype, chain, spread=3.0):
     g = torch.Generator().manual_seed(seed)
     logits = spread * torch.randn(B, T, V, generator=g)

@@ -138,9 +138,9 @@ __device__ __forceinline__ void write_row(const ProbsArgs& a, int64_t row, int c
 }
 
 // Many rows: a workgroup has one. What of it the registers hold is read once (HELD times 8 columns a thread: 155648 columns
-// of 16 bits, 73728 of 32), and all of that is on its way before the first maximum; the rest is read twice. Bound by the
-// writes, and a third of the time by the exponentials, once for the sum and once to write: 256 rows of 151936 bfloat16
-// 51.6 us, 4.5 TB/s (read twice, and a weight of eleven operations where it has eight: 73).
+// of 16 bits, 73728 of 32), and all of that is on its way before the first maximum; the rest is read twice. Bound by
+// memory: 256 rows of 151936 bfloat16 51.6 us, 4.5 TB/s (read twice, and a weight of eleven operations where it has eight:
+// 73).
 template <class T>
 __global__ __launch_bounds__(1024) void probs_row_kernel(ProbsArgs a) {
     constexpr int NT = 1024, HELD = std::is_same_v<T, F32> ? 9 : 19;
