@@ -360,6 +360,34 @@ def test_new_tokens_that_are_not_finite(dtype, T):
     compare(out[:, :, rest], want[:, :, rest], tol[:, :, rest])
 
 
+@pytest.mark.parametrize("kind,window,sinks", [("chain", 0, 0), ("tree", 0, 0), ("chain", 70, 0), ("chain", 100, 90), ("tree", 5, 40)])
+@pytest.mark.parametrize("dtype,d,G", [("bf16", 128, 1), ("bf16", 64, 3), ("f16", 128, 1), ("f32", 64, 2)])
+def test_long_chunks_with_values_that_are_not_finite(dtype, d, G, kind, window, sinks):
+    """Infinities and NaN in V of new tokens, in tiles next to each other and apart: NaN or that infinity where a token sees
+    one, and within the bound everywhere else."""
+    dt, Hkv, page, T, lens = DT[dtype], 1, 16, 330, [37, 0]
+    g, k, v, table, kv_len = cache4(T + window, lens, Hkv, page, d, dt)
+    q, kn, vn = tokens(g, 2, Hkv * G, Hkv, T, d, dt)
+    parents = tree(g, 2, T, 40) if kind == "tree" else None
+    tree_len = ints([T, T - 9])
+    bad = vn.clone()
+    for b, t, ch, x in ((0, 0, 3, math.inf), (0, 70, 9, -math.inf), (0, 140, 3, -math.inf), (0, 329, d - 1, math.nan), (1, 64, 0, math.nan),
+                        (1, 130, 17, math.inf), (1, 131, 40, math.inf), (1, 325, 5, math.nan)):
+        bad[b, 0, t, ch] = x
+    out = yt.paged_attention_q4(q, kn, bad, k, v, table, kv_len, page, parents=parents, tree_len=tree_len, window=window, sinks=sinks)
+    rows = rows4(k, v, table, kv_len, page, d)
+    want, _ = attention(q, kn, bad, rows, kv_len, parents, tree_len, window, sinks)
+    zeros = torch.where(torch.isfinite(bad), bad, 0.0)
+    fine, tol = attention(q, kn, zeros, rows, kv_len, parents, tree_len, window, sinks)
+    o = out.cpu().double()
+    for b in range(2):
+        n = int(tree_len[b])
+        w, f, tl, got = want[b, :, :n], fine[b, :, :n], tol[b, :, :n], o[b, :, :n]
+        assert torch.equal(w.isnan(), got.isnan()) and torch.equal(w[w.isinf()], got[w.isinf()])
+        ok = torch.isfinite(w)
+        assert ((got - f).abs()[ok] <= tl[ok]).all()
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32", "bf16"])
 def test_large_and_close_scores(dtype):
     """Queries whose scores are far from 0 and near each other: the weights keep their order."""
