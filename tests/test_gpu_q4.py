@@ -514,3 +514,46 @@ def test_a_served_step():
     _, _, live = yt.cache_compact((k, v), ref, table, kv_len, page)
     check_cache()
     assert status.item() == 0 and live.item() == int((ref > 0).sum()) and int(table[0, 0]) < live.item()
+
+
+def test_two_streams_at_once():
+    """Calls on two streams that overlap, each with a workspace of its own, over one pool: what each gives alone, bit for bit,
+    in eager calls and as two graphs."""
+    cases = []
+    for dtype, T, Hkv, G, window in (("bf16", 1, 2, 2, 0), ("bf16", 300, 1, 2, 0), ("f16", 25, 2, 5, 700), ("f32", 40, 1, 4, 0)):
+        dt, page, d = DT[dtype], 32, 128
+        g, k, v, table, kv_len = cache4(T, [4000, 1777], Hkv, page, d, dt)
+        q, kn, vn = tokens(g, 2, Hkv * G, Hkv, T, d, dt)
+        want = yt.paged_attention_q4(q, kn, vn, k, v, table, kv_len, page, window=window, sinks=4)
+        need = yt.paged_q4_workspace_bytes(dt, 2, Hkv * G, Hkv, T, d, table.shape[1], page, window, 4)
+        cases.append((want, [(torch.empty_like(want), torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")) for _ in range(2)],
+                      lambda out, ws, a=(q, kn, vn, k, v, table, kv_len, page), w=window: yt.paged_attention_q4(*a, window=w, sinks=4, out=out, workspace=ws)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            for _, to, call in cases:
+                call(*to[i])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            for _, to, call in cases if i else reversed(cases):
+                call(*to[i])
+        graphs.append(graph)
+    for kind in ("eager", "graphs", "eager", "graphs"):
+        for _, to, _ in cases:
+            for out, _ in to:
+                out.fill_(7.0)
+        torch.cuda.synchronize()
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                if kind == "graphs":
+                    graphs[i].replay()
+                else:
+                    for _, to, call in cases if i else reversed(cases):
+                        call(*to[i])
+        torch.cuda.synchronize()
+        for want, to, _ in cases:
+            for out, _ in to:
+                assert torch.equal(out, want)

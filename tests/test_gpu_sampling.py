@@ -254,3 +254,27 @@ def test_a_captured_step():
         check_probs(p, logits, 0.8)
         want = model(p, tokens, u, un, parents=above, tree_len=lens)
         assert [x.tolist() for x in out] == [want[0], want[1], want[2]]
+
+
+def test_two_streams_at_once():
+    """Steps on two streams that overlap: what each gives alone, bit for bit."""
+    B, T, V = 4, 5, 60001
+    steps = []
+    for seed in range(2):
+        (_, tokens, u, un), _, above = drafts(seed, B, T, V, "f32", False)
+        logits = torch.randn(B, T, V, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).cuda()
+
+        def step(logits=logits, tokens=tokens, u=u, un=un, above=above):
+            p = yt.token_probs(logits, 0.5)
+            return (p, *yt.verify_drafts(p, tokens, u, un, parents=above))
+        steps.append((step, step()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for st, (step, _) in zip(streams, steps):
+            with torch.cuda.stream(st):
+                got.append(step())
+        torch.cuda.synchronize()
+        for out, (_, want) in zip(got, steps):
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
