@@ -363,6 +363,7 @@ Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     p.kt = 16 * p.wr;
     const int64_t all_rows = top_k > 0 ? G : (int64_t)T * G;
     // a window leaves a row tile few keys: half the rows a workgroup where that fills the second place of the CUs
+    // (float32, d 64, 1024 tokens, window 256: 62 -> 25.7 us; 4 chunks of 512 after 4096 rows, window 4096: 196 -> 135)
     const bool windowed = window > 0 && p.wr == 4;
     if (windowed && (int64_t)B * Hkv * ((all_rows + 127) / 128) < SLOTS && (int64_t)B * Hkv * ((all_rows + 63) / 64) >= SLOTS / 2)
         p.wr = 2, p.kt = 32;

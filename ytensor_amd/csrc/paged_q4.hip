@@ -531,6 +531,18 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             for (int n = 0; n < NW; ++n) pw[n][i] = w[n];
         }
     };
+    auto half_weights = [&](const f32x4& p0, const f32x4& p1, u32x4 (&pw)[NW]) INLINE {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4& p = i < 2 ? p0 : p1;
+            const float x = p[2 * (i & 1)] * 0x1p14f, y = p[2 * (i & 1) + 1] * 0x1p14f;
+#if defined(__HIP_DEVICE_COMPILE__)
+            const uint32_t first = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+            pw[0][i] = first;
+            pw[NW - 1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - lo_as_f32(F16{}, first), y - hi_as_f32(F16{}, first)));
+#endif
+        }
+    };
     auto hide_rows = [&](f32x4 (&p)[2], uint32_t see) INLINE {
         const uint32_t mine = see >> (8 * g);
 #pragma unroll
@@ -583,8 +595,9 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         for (int e = 0; e < 8; ++e) at[e] = min(u0 + 8 * g + e, tn - 1) * a.vns[2] * ES;
         using Pair = std::conditional_t<F, u32x2, uint32_t>;
         auto pair_at = [&](int e, int q) INLINE { return *reinterpret_cast<const Pair*>(v + at[e] + q * (int)sizeof(Pair)); };
-        // (in flight beside K where the registers reach for it: all at once, or a pair at a time)
-        constexpr bool EARLY = QT == 1 && !SHARED && (std::is_same_v<T, BF16> || D == 64);
+        // (in flight beside K where the registers reach for it, all at once, else a pair at a time: 2048 float16 tokens 309 ->
+        // 183 us)
+        constexpr bool EARLY = QT == 1 && (SHARED || std::is_same_v<T, BF16> || D == 64);
         Pair ahead[EARLY ? 8 : 1][EARLY ? DT / 2 : 1];
         if constexpr (EARLY) {
 #pragma unroll
@@ -609,23 +622,33 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) p[qt][j] *= flip;
         }
+        // float16's V as it is takes fewer instructions than as bfloat16 pieces (which the other types' conversion is bound by);
+        // the weights are two float16 numbers then, in a unit of 2^14, so that none above 2^-38 of the largest is lost
+        constexpr bool HALF = std::is_same_v<T, F16>;
         u32x4 pw[QT][NW];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
             hide_rows(p[qt], see[qt]);
             weigh(p[qt], qt);
-            split_weights(p[qt][0], p[qt][1], pw[qt]);
+            if constexpr (HALF) half_weights(p[qt][0], p[qt][1], pw[qt]);
+            else split_weights(p[qt][0], p[qt][1], pw[qt]);
         }
         bool bad = false;  // 0 . V is NaN for a V that is not finite: such elements are left out and added to those that see them
 #pragma unroll
         for (int q = 0; q < DT / 2; ++q) {
-            constexpr int NP = pieces<T>();
+            constexpr int NP = HALF ? 1 : pieces<T>();
             uint32_t part[NP][8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 Pair in;
                 if constexpr (EARLY) in = ahead[e][q];
                 else in = pair_at(e, q);
+                if constexpr (HALF) {
+                    const uint32_t none = (((in & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u;  // an exponent of ones
+                    bad = bad || none != 0;
+                    part[0][e] = in & ~(none * 0xffffu);
+                    continue;
+                }
                 float x, y;
                 if constexpr (F) x = __uint_as_float(in[0]), y = __uint_as_float(in[1]);
                 else x = lo_as_f32(T{}, in), y = hi_as_f32(T{}, in);
@@ -640,13 +663,25 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             for (int i = 0; i < NP; ++i) {
                 u32x4 even, odd;
                 pair_rows(part[i], even, odd);
-#pragma unroll
-                for (int n = 0; n < NW; ++n)
+                if constexpr (HALF) {
 #pragma unroll
                     for (int qt = 0; qt < QT; ++qt) {
-                        o[qt][2 * q] = mfma_chunk(BF16{}, even, pw[qt][n], o[qt][2 * q]);
-                        o[qt][2 * q + 1] = mfma_chunk(BF16{}, odd, pw[qt][n], o[qt][2 * q + 1]);
+                        f32x4 y[2] = {};
+#pragma unroll
+                        for (int n = 0; n < NW; ++n) y[0] = mfma_chunk(T{}, even, pw[qt][n], y[0]), y[1] = mfma_chunk(T{}, odd, pw[qt][n], y[1]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            o[qt][2 * q][r] = fmaf(y[0][r], 0x1p-14f, o[qt][2 * q][r]), o[qt][2 * q + 1][r] = fmaf(y[1][r], 0x1p-14f, o[qt][2 * q + 1][r]);
                     }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NW; ++n)
+#pragma unroll
+                        for (int qt = 0; qt < QT; ++qt) {
+                            o[qt][2 * q] = mfma_chunk(BF16{}, even, pw[qt][n], o[qt][2 * q]);
+                            o[qt][2 * q + 1] = mfma_chunk(BF16{}, odd, pw[qt][n], o[qt][2 * q + 1]);
+                        }
+                }
             }
             if constexpr (!EARLY) __builtin_amdgcn_sched_barrier(0);
         }
@@ -1087,8 +1122,10 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
 Plan plan_q4(int dtype, int B, int Hkv, int G, int T, int d, int columns, int page, int window, int sinks) {
     Plan p;
     const int64_t rows = (int64_t)T * G;
-    // 16 rows of a wave (bfloat16: 32) leave the tiles to the four; more share them. 32 rows of a wave where there are more
-    // than 64 and one piece a query leaves the registers; with a window 16 where that fills the second place of the CUs
+    // 16 rows of a wave (bfloat16: 32) leave the tiles to the four; more share them (8 sequences, 32 rows over 8192: 32.9 us,
+    // shared 41.1). 32 rows of a wave where there are more than 64 and one piece a query leaves the registers (two chunks of
+    // 512 over 8192 rows 101.6 us, with 16 115; 16 x 200 rows over 4096 133 and 146); with a window 16 where that fills the
+    // second place of the CUs (chunk of 2048, window 1024: 78.9 us, with 32 96.5; 4 chunks of 512, window 4096 147 and 182)
     const bool few = rows <= (dtype == YTHIP_BF16 ? 32 : 16);
     p.wr = few ? 1 : 4;
     p.qt = few ? (rows <= 16 ? 1 : 2) : rows <= 64 || dtype != YTHIP_BF16 ? 1 : 2;
@@ -1104,7 +1141,8 @@ Plan plan_q4(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     if (window > 0) seq_rows = std::min(seq_rows, (int64_t)window + sinks + 2 * p.kt);
     const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + ((int64_t)T + p.kt - 1) / p.kt, most = (tiles + p.stage - 1) / p.stage;
     int64_t part_items = 0;
-    if (most <= WHOLE || (window > 0 && !few && B * per >= SLOTS / 2)) {  // (as plan_of has it)
+    // (as plan_of has it: 8 chunks of 256, window 1024 46.5 us, in ranges 56.3)
+    if (most <= WHOLE || (window > 0 && !few && B * per >= SLOTS / 2)) {
         p.target = 0;
         p.items = B;
     } else {
