@@ -300,17 +300,17 @@ template <class T, int D, int QT, int WR, bool WIN>
 __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, BF16>))) void paged_q4_kernel(PagedArgs a) {
     using S = Q4Shape<D, QT, WR>;
     using raw = typename T::raw;
-    constexpr bool F = std::is_same_v<T, F32>, SHARED = S::SHARED;
+    constexpr bool F = std::is_same_v<T, F32>, SHARED = S::SHARED, HALF = std::is_same_v<T, F16>;
     constexpr int KT = S::KT, SUB = KT / 16, KG = KT / 32, KS = S::KS, DT = S::DT, NQ = pieces<T>(), NW = F ? 3 : 2, GROUPS = S::GROUPS;
     constexpr int ES = sizeof(raw);
     __shared__ u32x4 smem[S::LDS];
     __shared__ int16_t s_up[MAX_TREE];
     __shared__ uint32_t s_odd[SHARED ? 2 * 4 * 2 : 1];  // of a converted tile: bits of rows without a value, by channel group
     __shared__ int s_inf[4];  // of the tiles of new tokens there, by stage: V holds what is not finite
-    // New tokens go through LDS too where one piece holds their values: a wave reads a quarter of a tile, not all of it
-    // (chunk of 2048 after 2048 rows, window 1024: 219 -> 78 us; 4096 after 64, window 2048: 560 -> 221; two chunks of 512
-    // over 8192: 116 -> 96). float16 and float32 would take two or three pieces, which LDS has no room for.
-    constexpr bool SHARED_NEW = SHARED && std::is_same_v<T, BF16>;
+    // New tokens of 16 bits go through LDS too, as they are: a wave reads a quarter of a tile, not all of it (chunk of 2048
+    // after 2048 rows, window 1024: 219 -> 78 us; 4096 after 64, window 2048: 560 -> 221; two chunks of 512 over 8192: 116
+    // -> 96). LDS has no room for float32's.
+    constexpr bool SHARED_NEW = SHARED && !F;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR;
     const int l16 = lane & 15, g = lane >> 4;
@@ -561,6 +561,22 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         }
     };
 
+    // Two 16-bit numbers, 0 in the place of one that is not finite
+    auto finite_pair = [](uint32_t w, bool& bad) INLINE {
+        constexpr uint32_t ONES = std::is_same_v<T, F16> ? 0x7c007c00u : 0x7f807f80u, LOW = 0x80008000u - ONES;
+        const uint32_t none = (((w & ONES) + LOW) >> 15) & 0x00010001u;  // an exponent of ones
+        bad = bad || none != 0;
+        return w & ~(none * 0xffffu);
+    };
+    // The sums of one piece of V (two channel tiles) with the weights' two: float16's are in a unit of 2^14
+    auto add_half = [&](int qt, int t, u32x4 even, u32x4 odd, const u32x4 (&pw)[NW]) INLINE {
+        f32x4 y[2] = {};
+#pragma unroll
+        for (int n = 0; n < NW; ++n) y[0] = mfma_chunk(T{}, even, pw[n], y[0]), y[1] = mfma_chunk(T{}, odd, pw[n], y[1]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[qt][t][r] = fmaf(y[0][r], 0x1p-14f, o[qt][t][r]), o[qt][t + 1][r] = fmaf(y[1][r], 0x1p-14f, o[qt][t + 1][r]);
+    };
+
     // ---- tiles of new tokens, by halves of 32
     const char* Kn = static_cast<const char*>(a.Kn) + (b * a.kns[0] + h * a.kns[1]) * ES;
     const char* Vn = static_cast<const char*>(a.Vn) + (b * a.vns[0] + h * a.vns[1]) * ES;
@@ -624,7 +640,6 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         }
         // float16's V as it is takes fewer instructions than as bfloat16 pieces (which the other types' conversion is bound by);
         // the weights are two float16 numbers then, in a unit of 2^14, so that none above 2^-38 of the largest is lost
-        constexpr bool HALF = std::is_same_v<T, F16>;
         u32x4 pw[QT][NW];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
@@ -644,9 +659,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
                 if constexpr (EARLY) in = ahead[e][q];
                 else in = pair_at(e, q);
                 if constexpr (HALF) {
-                    const uint32_t none = (((in & 0x7c007c00u) + 0x04000400u) >> 15) & 0x00010001u;  // an exponent of ones
-                    bad = bad || none != 0;
-                    part[0][e] = in & ~(none * 0xffffu);
+                    part[0][e] = finite_pair(in, bad);
                     continue;
                 }
                 float x, y;
@@ -665,14 +678,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
                 pair_rows(part[i], even, odd);
                 if constexpr (HALF) {
 #pragma unroll
-                    for (int qt = 0; qt < QT; ++qt) {
-                        f32x4 y[2] = {};
-#pragma unroll
-                        for (int n = 0; n < NW; ++n) y[0] = mfma_chunk(T{}, even, pw[qt][n], y[0]), y[1] = mfma_chunk(T{}, odd, pw[qt][n], y[1]);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            o[qt][2 * q][r] = fmaf(y[0][r], 0x1p-14f, o[qt][2 * q][r]), o[qt][2 * q + 1][r] = fmaf(y[1][r], 0x1p-14f, o[qt][2 * q + 1][r]);
-                    }
+                    for (int qt = 0; qt < QT; ++qt) add_half(qt, 2 * q, even, odd, pw[qt]);
                 } else {
 #pragma unroll
                     for (int n = 0; n < NW; ++n)
@@ -795,9 +801,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             uint32_t v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t odd = (((w.v[e][i] & 0x7f807f80u) + 0x00800080u) >> 15) & 0x00010001u;  // an exponent of ones
-                bad = bad || odd != 0;
-                v[e] = w.v[e][i] & ~(odd * 0xffffu);
+                v[e] = finite_pair(w.v[e][i], bad);
             }
             u32x4 even, odd;
             pair_rows(v, even, odd);
@@ -806,14 +810,25 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         if (__ballot(bad) != 0 && lane == 0) s_inf[s & 3] = 1;
     };
 
-    auto compute = [&](int s, uint64_t use, Raw& w, auto masked) INLINE {
-        constexpr bool MASKED = decltype(masked)::value;
+    // new tokens first, from the last: their paths are walked down once
+    const int new_tiles = WIN ? max(win.high - max(win.low, nct), 0) + max(win.sink_end - max(c0, nct), 0) : max(win.high - max(c0, nct), 0);
+    // float16's queries as they are, which its new tokens meet
+    u32x4 qr[SHARED_NEW && HALF ? KS : 1];
+    if constexpr (SHARED_NEW && HALF) {
+        static_assert(QT == 1);
+        if (new_tiles > 0) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) qr[ks] = *reinterpret_cast<const u32x4*>(qp[0] + ks * 8);
+        }
+    }
+
+    auto compute = [&](int s, uint64_t use, Raw& w, auto masked, auto fresh) INLINE {
+        constexpr bool MASKED = decltype(masked)::value, is_new = decltype(fresh)::value;
         uint64_t see[QT];
         bool hide = use != FULL, some = false;  // some: a query sees rows of it that another does not
-        const bool is_new = SHARED_NEW && MASKED && tile_at(s) >= nct;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) see[qt] = use;
-        if (is_new) {
+        if constexpr (is_new) {
             const int u0 = (tile_at(s) - nct) * KT;
             bool any = false;
 #pragma unroll
@@ -860,11 +875,16 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
                 u32x4 kf;
                 if constexpr (SHARED) kf = from[(j * KS + ks) * 64];
                 else kf = k_frag(w, j, ks);
+                if constexpr (is_new && HALF) {
+                    p[0][j] = mfma_chunk(T{}, kf, qr[ks], p[0][j]);
+                } else {
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
+                    for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                    for (int qt = 0; qt < QT; ++qt) p[qt][j] = mfma_chunk(BF16{}, kf, qf[qt][n][ks], p[qt][j]);
+                        for (int qt = 0; qt < QT; ++qt) p[qt][j] = mfma_chunk(BF16{}, kf, qf[qt][n][ks], p[qt][j]);
+                }
             }
+            if constexpr (is_new && HALF) p[0][j] *= flip;
         }
         uint32_t odd[KG] = {};  // rows without a value in this lane's channels that not every query sees
         if (hide) {
@@ -885,7 +905,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
                 for (int kk = 0; kk < KG; ++kk) odd[kk] = clean_scales(w.vs[kk], mine[kk], some, g * (D / 4) / 32);
             }
         }
-        if (SHARED && WIN && !is_new) {
+        if constexpr (SHARED && WIN && !is_new) {
 #pragma unroll
             for (int kk = 0; kk < KG; ++kk) odd[kk] = s_odd[((s & 1) * 4 + g * (D / 4) / 32) * 2 + kk];
         }
@@ -895,22 +915,29 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         for (int kk = 0; kk < KG; ++kk) {
             u32x4 pw[QT][NW];
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) split_weights(p[qt][2 * kk], p[qt][2 * kk + 1], pw[qt]);
+            for (int qt = 0; qt < QT; ++qt) {
+                if constexpr (is_new && HALF) half_weights(p[qt][2 * kk], p[qt][2 * kk + 1], pw[qt]);
+                else split_weights(p[qt][2 * kk], p[qt][2 * kk + 1], pw[qt]);
+            }
             static_for<0, DT / 2>([&](auto q) {
                 constexpr int Q = decltype(q)::value;
                 u32x4 even, odd_;
                 if constexpr (SHARED) even = from[(S::KF + kk * DT + 2 * Q) * 64], odd_ = from[(S::KF + kk * DT + 2 * Q + 1) * 64];
                 else v_frags(w, kk, q, even, odd_);
+                if constexpr (is_new && HALF) {
+                    add_half(0, 2 * Q, even, odd_, pw[0]);
+                } else {
 #pragma unroll
-                for (int n = 0; n < NW; ++n)
+                    for (int n = 0; n < NW; ++n)
 #pragma unroll
-                    for (int qt = 0; qt < QT; ++qt) {
-                        o[qt][2 * Q] = mfma_chunk(BF16{}, even, pw[qt][n], o[qt][2 * Q]);
-                        o[qt][2 * Q + 1] = mfma_chunk(BF16{}, odd_, pw[qt][n], o[qt][2 * Q + 1]);
-                    }
+                        for (int qt = 0; qt < QT; ++qt) {
+                            o[qt][2 * Q] = mfma_chunk(BF16{}, even, pw[qt][n], o[qt][2 * Q]);
+                            o[qt][2 * Q + 1] = mfma_chunk(BF16{}, odd_, pw[qt][n], o[qt][2 * Q + 1]);
+                        }
+                }
             });
         }
-        if (is_new && s_inf[s & 3] != 0) {
+        if (is_new && s_inf[s & 3] != 0) {  // (of all waves' shares)
             const int u0 = (tile_at(s) - nct) * KT;
             for (int u = 0; u < min(tn - u0, KT); ++u) {
                 const int64_t row = (u0 + u) * a.vns[2];
@@ -938,8 +965,6 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         }
     };
 
-    // new tokens first, from the last: their paths are walked down once
-    const int new_tiles = WIN ? max(win.high - max(win.low, nct), 0) + max(win.sink_end - max(c0, nct), 0) : max(win.high - max(c0, nct), 0);
     const int s_first = new_tiles / S::WK;  // the first stage with a tile of cached rows (for some wave)
     // the stages whose tiles every query sees whole end there; then those at the window's border and the sinks
     const int s_whole = WIN ? max(s_first, max(win.high - max(win.low, win.clean), 0) / S::WK) : nst;
@@ -975,7 +1000,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             __syncthreads();
             const bool fresh_next = decltype(more_new)::value && s + 1 < new_tiles;
             if (fresh_next) load_new(s + 1, fresh);
-            if (here != 0) compute(s, here, w, masked);
+            if (here != 0) compute(s, here, w, masked, more_new);
             // (read two stages ago, written again in the next)
             if (decltype(more_new)::value && tid == 0) s_inf[(s + 2) & 3] = 0;
             if (fresh_next) {
@@ -1003,7 +1028,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         x = ids(s_first + 2);
         auto stage = [&](int s, auto masked) INLINE {
             __syncthreads();
-            if (here != 0) compute(s, here, w, masked);
+            if (here != 0) compute(s, here, w, masked, std::false_type{});
             convert(s + 1, next, w);
             here = next;
             next = load(s + 2, x, w);
@@ -1033,7 +1058,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             while (s < to) {
 #pragma unroll
                 for (int i = 0; i < AHEAD; ++i) {
-                    if (use[i] != 0) compute(s, use[i], w[i], masked);
+                    if (use[i] != 0) compute(s, use[i], w[i], masked, std::false_type{});
                     use[i] = load(s + AHEAD, nx, w[i]);
                     nx = ids(s + AHEAD + 1);
                     ++s;
