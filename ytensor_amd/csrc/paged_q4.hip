@@ -291,7 +291,8 @@ struct Q4Shape {
 //   O^T = V^T . P^T: the lane has rows 8 g .. 8 g + 7 of channels l16 D / 16 and on, 32 (16) consecutive bytes of a V block
 //     and 8 scales; converted row by row, then paired by row (v_perm), it has each of its channels over 8 rows, which is
 //     row l16 of channel tile t. So tile t's row i is channel i D / 16 + t.
-//   New tokens are of the queries' type: their scores on its own matrix instruction, their V as bfloat16 pieces.
+//   New tokens are of the queries' type: their scores on its own matrix instruction, so their V, but float32's, which is
+//     three bfloat16 pieces.
 // Numerics: queries and weights as bfloat16 pieces (split) that hold all bits of the queries and 16 (24 for fp32) of the
 //   weights; scores, maxima, sums and O in fp32. (The matrix cores' scaled product would take K's codes as they are, with
 //   the queries as e4m3 pieces, but of every 8 products it drops what is 2^13 below the largest: fp32 scores were off by
@@ -307,9 +308,10 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
     __shared__ int16_t s_up[MAX_TREE];
     __shared__ uint32_t s_odd[SHARED ? 2 * 4 * 2 : 1];  // of a converted tile: bits of rows without a value, by channel group
     __shared__ int s_inf[4];  // of the tiles of new tokens there, by stage: V holds what is not finite
-    // New tokens of 16 bits go through LDS too, as they are: a wave reads a quarter of a tile, not all of it (chunk of 2048
-    // after 2048 rows, window 1024: 219 -> 78 us; 4096 after 64, window 2048: 560 -> 221; two chunks of 512 over 8192: 116
-    // -> 96). LDS has no room for float32's.
+    // New tokens of 16 bits go through LDS too, as they are: a wave reads a quarter of a tile, not all of it (bfloat16, chunk
+    // of 2048 after 2048 rows, window 1024: 219 -> 78 us; 4096 after 64, window 2048: 560 -> 221; two chunks of 512 over 8192:
+    // 116 -> 96; float16, 2048 after 64: 169 -> 106). A single tile gains nothing, and loses nothing: five trees of 25 39.0 us,
+    // each wave by itself 39.2. LDS has no room for float32's.
     constexpr bool SHARED_NEW = SHARED && !F;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR;
@@ -611,8 +613,8 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         for (int e = 0; e < 8; ++e) at[e] = min(u0 + 8 * g + e, tn - 1) * a.vns[2] * ES;
         using Pair = std::conditional_t<F, u32x2, uint32_t>;
         auto pair_at = [&](int e, int q) INLINE { return *reinterpret_cast<const Pair*>(v + at[e] + q * (int)sizeof(Pair)); };
-        // (in flight beside K where the registers reach for it, all at once, else a pair at a time: 2048 float16 tokens 309 ->
-        // 183 us)
+        // (in flight beside K where the registers reach for it, all at once, else a pair at a time: 1024 float32 tokens 153 ->
+        // 142 us)
         constexpr bool EARLY = QT == 1 && (SHARED || std::is_same_v<T, BF16> || D == 64);
         Pair ahead[EARLY ? 8 : 1][EARLY ? DT / 2 : 1];
         if constexpr (EARLY) {
@@ -638,8 +640,9 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) p[qt][j] *= flip;
         }
-        // float16's V as it is takes fewer instructions than as bfloat16 pieces (which the other types' conversion is bound by);
-        // the weights are two float16 numbers then, in a unit of 2^14, so that none above 2^-38 of the largest is lost
+        // float16's V as it is takes fewer instructions than as two bfloat16 pieces (2048 tokens, each wave by itself: 183 -> 169
+        // us); the weights are two float16 numbers then, truncated, 2^-20 of themselves away at most, in a unit of 2^14, so that none above
+        // 2^-38 of the largest is lost
         u32x4 pw[QT][NW];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
