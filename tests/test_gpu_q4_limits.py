@@ -1,0 +1,61 @@
+"""4-bit attention on the GPU where its numbers end: queries that are not finite, weights far below the largest, what two
+pieces of a weight hold."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import q4_ref
+import ytensor_amd as yt
+from window_ref import Rows, attention, compare
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def pool(k, v, page):
+    """Rows k and v [B, Hkv, n, d] as 4-bit pools, a table and lengths, and the values that the pools hold."""
+    B, Hkv, n, d = k.shape
+    pages = max(1, -(-n // page))
+    pools, values = [], []
+    for x, which in ((k, "k"), (v, "v")):
+        x = torch.nn.functional.pad(x, (0, 0, 0, pages * page - n))
+        blocks = q4_ref.pack(x.unflatten(2, (pages, page)).transpose(1, 2).flatten(0, 1), which)
+        pools.append(blocks.cuda())
+        values.append(q4_ref.values(blocks, page, d, which))
+    table, kv_len = ints([[b * pages + c for c in range(pages)] for b in range(B)]), ints([n] * B)
+    return (*pools, table, kv_len), Rows(*values, table, kv_len)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 64), ("f16", 128), ("f32", 64)])
+@pytest.mark.parametrize("T", [1, 5, 40, 140])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_queries_with_an_infinity(dtype, d, T, sign):
+    """One channel of a query is infinite, and every cached key is below 0 there: all scores are -inf, so the row is zero;
+    with a new key above 0, or an infinity of the other sign, it is NaN. Other heads and tokens are as ever."""
+    dt, page, n, Hq, c = DT[dtype], 16, 45, 3, 5
+    g = torch.Generator().manual_seed(T + d)
+    k, v = (torch.randn(1, 1, n, d, generator=g).to(dt) for _ in range(2))
+    q, kn, vn = (torch.randn(1, h, T, d, generator=g).to(dt) for h in (Hq, 1, 1))
+    k[..., c], kn[..., c] = -2.0, -1.0
+    kn[0, 0, T // 2, c] = sign
+    where = torch.zeros(1, Hq, T, dtype=torch.bool)
+    where[0, 0, 0] = where[0, 1, T - 1] = where[0, 2, T // 2] = where[0, 2, 0] = True
+    q[where] = torch.where(torch.arange(d) == c, torch.inf, q[where])
+    q[0, 2, 0, c] = -torch.inf
+    q, kn, vn = q.cuda(), kn.cuda(), vn.cuda()
+    args, rows = pool(k, v, page)
+    out = yt.paged_attention_q4(q, kn, vn, *args, page).cpu()
+    want, tol = attention(q, kn, vn, rows, args[-1])
+    assert want[0, 2, 0].isnan().all() and ((want[where] == 0) | want[where].isnan()).all()
+    assert (want[0, 1, T - 1] == 0).all() == (sign < 0)
+    assert torch.equal(want.isnan(), out.isnan())
+    here = out[where].double()
+    assert torch.equal(here[~here.isnan()], want[where][~want[where].isnan()])
+    compare(out[~where], want[~where], tol[~where])

@@ -152,7 +152,8 @@ def paged_attention_q4(q: torch.Tensor, k_new: torch.Tensor | None, v_new: torch
     """paged_attention over a layer's 4-bit pools [P, Hkv, cache_q4_bytes(page, d)]: T new tokens a sequence, q [B, Hq, T,
     d] of any of the three types, over the kv_len[b] cached rows' values and the tokens' own k_new / v_new [B, Hkv, T, d] of
     q's type (None: the cache alone). parents, tree_len, scale, out, window and sinks as there. The cached values take part
-    as they are, whatever q's type is; a query with a NaN or an infinity gives NaN where it sees one. Returns out [B, Hq, T, d]."""
+    as they are, whatever q's type is. An infinity or a NaN in a query has the scores that follow from it: -inf has no
+    weight (a row that has nothing else is zero), +inf and NaN make the row NaN. Returns out [B, Hq, T, d]."""
     away = _away(_device(q, k_new, v_new, k_pool, v_pool, table, kv_len, parents, tree_len, out, workspace))
     if away is not None:
         with away:
