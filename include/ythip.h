@@ -684,10 +684,11 @@ int ythip_cache_unpack_q4(int dtype, int layers, int pages, int Hkv, int page, i
 
 /*
  * ythip_paged_attn_window (window 0: ythip_paged_attn) over 4-bit pages. Q, Kn, Vn and O are of
- * dtype; the cached values take part as they are. Weights keep 16 bits (fp32: 24), queries all
- * of theirs (fp32: what of a channel lies below 2^-126 may be lost), the rest is fp32. A query
- * that holds an infinity or a NaN has the scores that follow from it: -inf has no weight (zeros
- * where no key has another), +inf and NaN make O's row NaN.
+ * dtype; the cached values take part as they are. Weights keep 16 bits (fp32: 24; of new fp16
+ * tokens what is above 2^-50 of the largest), queries all of theirs (fp32: what of a channel
+ * lies below 2^-126 may be lost), the rest is fp32. A query that holds an infinity or a NaN has
+ * the scores that follow from it: -inf has no weight (zeros where no key has another), +inf and
+ * NaN make O's row NaN.
  */
 size_t ythip_paged_attn_q4_workspace_size(int dtype, int B, int Hq, int Hkv, int T, int d, int columns, int page,
                                           int window, int sinks);

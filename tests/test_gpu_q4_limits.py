@@ -59,3 +59,35 @@ def test_queries_with_an_infinity(dtype, d, T, sign):
     here = out[where].double()
     assert torch.equal(here[~here.isnan()], want[where][~want[where].isnan()])
     compare(out[~where], want[~where], tol[~where])
+
+
+@pytest.mark.parametrize("dtype,steps", [("f16", 20.0), ("f16", 27.75), ("f16", 31.0), ("bf16", 27.75), ("f32", 27.75)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T,n", [(9, 0), (66, 0), (200, 40)])
+def test_weights_far_below_the_largest(dtype, steps, d, T, n):
+    """The key with the largest weight has a V of 0: what the others add, e^-steps (2^-29, 2^-40, 2^-45) of it each, is all
+    of the result. A weight keeps 16 bits (fp32: 24): 2^-16 (2^-24) of sum p |v|; a score of two products and its
+    exponential are (steps + 4) 2^-23 off, a sum of n keys n 2^-24; the result is half a step of its type, at least of its
+    smallest number. A new float16 token's weight is a float16 number times 2^25 and its largest is 1, so half a step of the
+    smallest, 2^-24, is 2^-50: with |v| that much a key."""
+    dt, page = DT[dtype], 16
+    g = torch.Generator().manual_seed(T)
+    q, kn, k = torch.zeros(1, 2, T, d), torch.zeros(1, 1, T, d), torch.zeros(1, 1, n, d)
+    q[..., 0], kn[:, :, 0, 0] = 4.0, steps / 4.0
+    vn, v = (40000.0 + 20000.0 * torch.rand(1, 1, m, d, generator=g) for m in (T, n))
+    vn[:, :, 0] = 0.0
+    q, kn, vn, k, v = (x.to(dt) for x in (q, kn, vn, k, v))
+    args, rows = pool(k, v, page)
+    out = yt.paged_attention_q4(q.cuda(), kn.cuda(), vn.cuda(), *args, page, scale=1.0).cpu().double()
+    _, _, vc = rows(0, 0)
+    values = torch.cat([vn[0, 0].double(), vc])
+    f = torch.finfo(dt)
+    least = f.smallest_normal * f.eps
+    for t in range(T):
+        keys = torch.cat([torch.arange(t + 1), T + torch.arange(n)])
+        w = torch.where(keys == 0, 1.0, math.exp(-steps)).double()
+        want = (w[:, None] * values[keys]).sum(0) / w.sum()
+        off = 2.0 ** (-24 if dt == torch.float32 else -16) + 2.0 ** -23 * (steps + 4) + 2.0 ** -24 * len(keys)
+        tol = (f.eps / 2 + off) * want + least / 2 + (2.0 ** -50 * values[keys].sum(0) if dt == torch.float16 else 0.0)
+        worst = ((out[0, :, t] - want).abs() / tol).max().item()
+        assert worst <= 1.0, (t, worst)

@@ -533,6 +533,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             for (int n = 0; n < NW; ++n) pw[n][i] = w[n];
         }
     };
+    // (float16's: the first piece in a unit of 2^14, what is left in one of 2^25, below 2^15 as the first is)
     auto half_weights = [&](const f32x4& p0, const f32x4& p1, u32x4 (&pw)[NW]) INLINE {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
 #if defined(__HIP_DEVICE_COMPILE__)
             const uint32_t first = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
             pw[0][i] = first;
-            pw[NW - 1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - lo_as_f32(F16{}, first), y - hi_as_f32(F16{}, first)));
+            pw[NW - 1][i] = pack2<F16>((x - lo_as_f32(F16{}, first)) * 0x1p11f, (y - hi_as_f32(F16{}, first)) * 0x1p11f);
 #endif
         }
     };
@@ -570,13 +571,16 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
         bad = bad || none != 0;
         return w & ~(none * 0xffffu);
     };
-    // The sums of one piece of V (two channel tiles) with the weights' two: float16's are in a unit of 2^14
+    // The sums of one piece of V (two channel tiles) with the weights' two, each in its unit
     auto add_half = [&](int qt, int t, u32x4 even, u32x4 odd, const u32x4 (&pw)[NW]) INLINE {
-        f32x4 y[2] = {};
+        static_assert(!HALF || NW == 2);
+        f32x4 y[2][NW] = {};
 #pragma unroll
-        for (int n = 0; n < NW; ++n) y[0] = mfma_chunk(T{}, even, pw[n], y[0]), y[1] = mfma_chunk(T{}, odd, pw[n], y[1]);
+        for (int n = 0; n < NW; ++n) y[0][n] = mfma_chunk(T{}, even, pw[n], y[0][n]), y[1][n] = mfma_chunk(T{}, odd, pw[n], y[1][n]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[qt][t][r] = fmaf(y[0][r], 0x1p-14f, o[qt][t][r]), o[qt][t + 1][r] = fmaf(y[1][r], 0x1p-14f, o[qt][t + 1][r]);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[qt][t + i][r] = fmaf(y[i][0][r], 0x1p-14f, fmaf(y[i][NW - 1][r], 0x1p-25f, o[qt][t + i][r]));
     };
 
     // ---- tiles of new tokens, by halves of 32
@@ -641,8 +645,8 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
             for (int qt = 0; qt < QT; ++qt) p[qt][j] *= flip;
         }
         // float16's V as it is takes fewer instructions than as two bfloat16 pieces (2048 tokens, each wave by itself: 183 -> 169
-        // us); the weights are two float16 numbers then, truncated, 2^-20 of themselves away at most, in a unit of 2^14, so that none above
-        // 2^-38 of the largest is lost
+        // us); the weights are two float16 numbers then, each in a unit of its own (half_weights): 2^-22 of a weight is lost,
+        // or 2^-50 of the largest. (In one unit, of 2^14, a weight below 2^-28 of the largest keeps less than 16 bits.)
         u32x4 pw[QT][NW];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
