@@ -14,6 +14,14 @@ namespace {
 // softmax(logits / temperature)
 // ---------------------------------------------------------------------------
 
+// A part of a row. Its sum is of up to 2^30 weights: eight are added in 32 bits, those in 64 (256 rows of 151936: 0.8e-7 of a
+// probability, that of its own roundings; with sums in 32 bits and parts joined two by two, their lower one brought to the
+// other's unit each time, up to 3.4e-7: an exponential's error is not centred).
+struct Part {
+    double sum;
+    float max;
+};
+
 struct ProbsArgs {
     int rows, n, parts, run;  // columns; workgroups of a row; columns of a workgroup, a multiple of 8
     const void* x;
@@ -22,11 +30,11 @@ struct ProbsArgs {
     float scale_low;  // what scale lacks to it
     float least;      // -200 / scale: what lies further below the largest has no weight in 32 bits
     float* p;
-    float* part;  // [rows][parts] of (max, sum)
+    Part* part;  // [rows][parts]
 };
 
 // 2^((x - top) scale) with the product's rounding put back: a logit 30 below the largest is else off by 2^-19. 0 for an x
-// of -inf; where x or top is NaN or +inf the row is NaN, which its maximum says (see write_row).
+// of -inf; where x or top is NaN or +inf the row is NaN, which its maximum says (see inverse).
 __device__ __forceinline__ float weight(const ProbsArgs& a, float x, float top) {
     const float d = __builtin_fmaxf(x - top, a.least), t = d * a.scale;
     const float rest = fmaf(d, a.scale_low, fmaf(d, a.scale, -t));
@@ -56,30 +64,45 @@ struct Eight {  // 8 neighbouring logits
 };
 
 // (M, L) of two parts: the larger maximum, and the sums in its unit
-__device__ __forceinline__ void join(const ProbsArgs& a, float& M, float& L, float M2, float L2) {
+__device__ __forceinline__ void join(const ProbsArgs& a, float& M, double& L, float M2, double L2) {
     const float top = __builtin_elementwise_maximum(M, M2), ref = finite(top);
-    L = L * weight(a, M, ref) + L2 * weight(a, M2, ref);
+    L = L * (double)weight(a, M, ref) + L2 * (double)weight(a, M2, ref);
     M = top;
 }
+// Over a wave, then a workgroup: the largest maximum first, so that a sum is brought to another unit twice.
 template <int NT>
-__device__ __forceinline__ void join_block(const ProbsArgs& a, float& M, float& L, float (&lds)[2 * NT / 64]) {
+__device__ __forceinline__ void join_block(const ProbsArgs& a, float& M, double& L, Part (&lds)[NT / 64]) {
+    float top = M;
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        const float M2 = __shfl_xor(M, off, 64), L2 = __shfl_xor(L, off, 64);
-        join(a, M, L, M2, L2);
-    }
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) lds[2 * wave] = M, lds[2 * wave + 1] = L;
+    for (int off = 32; off >= 1; off >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, off, 64));
+    L *= (double)weight(a, M, finite(top));
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) L += __shfl_xor(L, off, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = {L, top};
     __syncthreads();
-    M = lds[0], L = lds[1];
-    for (int w = 1; w < NT / 64; ++w) join(a, M, L, lds[2 * w], lds[2 * w + 1]);
+    // lane l has wave l % (NT / 64)
+    const Part mine = lds[threadIdx.x % (NT / 64)];
+    M = mine.max;
+#pragma unroll
+    for (int off = NT / 128; off >= 1; off >>= 1) M = __builtin_elementwise_maximum(M, __shfl_xor(M, off, 64));
+    L = mine.sum * (double)weight(a, mine.max, finite(M));
+#pragma unroll
+    for (int off = NT / 128; off >= 1; off >>= 1) L += __shfl_xor(L, off, 64);
+}
+// The sum of eight neighbouring logits' weights
+template <class T>
+__device__ __forceinline__ double sum_eight(const ProbsArgs& a, const Eight<T>& v, float ref) {
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = weight(a, v[e], ref);
+    return (double)(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
 }
 
 // This thread's maximum and sum over columns [c0, c1) of a row.
 template <class T, int NT>
-__device__ __forceinline__ void scan_row(const ProbsArgs& a, int64_t row, int c0, int c1, float& M, float& L) {
+__device__ __forceinline__ void scan_row(const ProbsArgs& a, int64_t row, int c0, int c1, float& M, double& L) {
     constexpr int AHEAD = 4;
-    M = -INFINITY, L = 0.f;
+    M = -INFINITY, L = 0.0;
     const int whole = c0 + (c1 - c0) / 8 * 8;
     for (int c = c0 + (int)threadIdx.x * 8; c < whole; c += AHEAD * NT * 8) {
         Eight<T> v[AHEAD];
@@ -91,17 +114,14 @@ __device__ __forceinline__ void scan_row(const ProbsArgs& a, int64_t row, int c0
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = __builtin_elementwise_maximum(top, v[u][e]);
         const float ref = finite(top);
-        L *= weight(a, M, ref);
+        L *= (double)weight(a, M, ref);
         M = top;
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
-            if (c + u * NT * 8 < whole) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) L += weight(a, v[u][e], ref);
-            }
+            if (c + u * NT * 8 < whole) L += sum_eight<T>(a, v[u], ref);
     }
     const int c = whole + (int)threadIdx.x;
-    if (c < c1) join(a, M, L, load_as_f32<T>(a.x, row * a.ld + c), 1.f);
+    if (c < c1) join(a, M, L, load_as_f32<T>(a.x, row * a.ld + c), 1.0);
 }
 
 // Eight probabilities from their logits.
@@ -116,8 +136,8 @@ __device__ __forceinline__ void write_eight(const ProbsArgs& a, const Eight<T>& 
     }
 }
 // 1 / the sum; 0 for a row of -inf, NaN for one with a NaN or +inf
-__device__ __forceinline__ float inverse(float M, float L) {
-    return M == -INFINITY ? 0.f : M < INFINITY ? 1.0f / L : __builtin_nanf("");
+__device__ __forceinline__ float inverse(float M, double L) {
+    return M == -INFINITY ? 0.f : M < INFINITY ? (float)(1.0 / L) : __builtin_nanf("");
 }
 template <class T, int NT>
 __device__ __forceinline__ void write_row(const ProbsArgs& a, int64_t row, int c0, int c1, float ref, float inv) {
@@ -139,16 +159,17 @@ __device__ __forceinline__ void write_row(const ProbsArgs& a, int64_t row, int c
 
 // Many rows: a workgroup has one. What of it the registers hold is read once (HELD times 8 columns a thread: 155648 columns
 // of 16 bits, 73728 of 32), and all of that is on its way before the first maximum; the rest is read twice. Bound by
-// memory: 256 rows of 151936 bfloat16 51.6 us, 4.5 TB/s (read twice, and a weight of eleven operations where it has eight:
-// 73).
+// memory: 256 rows of 151936 bfloat16 49.6 us, 4.7 TB/s (read twice, and a weight of eleven operations where it has eight:
+// 73; with the workgroup's maximum before any sum, a barrier more: 55).
 template <class T>
 __global__ __launch_bounds__(1024) void probs_row_kernel(ProbsArgs a) {
     constexpr int NT = 1024, HELD = std::is_same_v<T, F32> ? 9 : 19;
-    __shared__ float lds[2 * NT / 64];
+    __shared__ Part lds[NT / 64];
     const int64_t row = blockIdx.x;
     const int held = min(a.n / 8, HELD * NT) * 8;
     Eight<T> v[HELD];
-    float M, L;
+    float M;
+    double L;
 #pragma unroll
     for (int u = 0; u < HELD; ++u)
         if (u * NT * 8 < held) v[u].load(a.x, row * a.ld + min((u * NT + (int)threadIdx.x) * 8, held - 8));
@@ -161,14 +182,13 @@ __global__ __launch_bounds__(1024) void probs_row_kernel(ProbsArgs a) {
             for (int e = 0; e < 8; ++e) top = __builtin_elementwise_maximum(top, v[u][e]);
         }
     float ref = finite(top);
-    L *= weight(a, M, ref);
+    L *= (double)weight(a, M, ref);
     M = top;
 #pragma unroll
     for (int u = 0; u < HELD; ++u)
         if ((u * NT + (int)threadIdx.x) * 8 < held) {
             v[u].again();
-#pragma unroll
-            for (int e = 0; e < 8; ++e) L += weight(a, v[u][e], ref);
+            L += sum_eight<T>(a, v[u], ref);
         }
     join_block<NT>(a, M, L, lds);
     ref = finite(M);
@@ -184,23 +204,25 @@ __global__ __launch_bounds__(1024) void probs_row_kernel(ProbsArgs a) {
 // Few rows: `parts` workgroups a row, whose maxima and sums the second launch joins, each workgroup for itself.
 template <class T>
 __global__ __launch_bounds__(256) void probs_part_kernel(ProbsArgs a) {
-    __shared__ float lds[2 * 256 / 64];
+    __shared__ Part lds[256 / 64];
     const int64_t row = blockIdx.y;
     const int c0 = blockIdx.x * a.run, c1 = min(c0 + a.run, a.n);
-    float M, L;
+    float M;
+    double L;
     scan_row<T, 256>(a, row, c0, c1, M, L);
     join_block<256>(a, M, L, lds);
-    if (threadIdx.x == 0) *reinterpret_cast<f32x2*>(a.part + 2 * (row * a.parts + blockIdx.x)) = f32x2{M, L};
+    if (threadIdx.x == 0) a.part[row * a.parts + blockIdx.x] = {L, M};
 }
 template <class T>
 __global__ __launch_bounds__(256) void probs_write_kernel(ProbsArgs a) {
-    __shared__ float lds[2 * 256 / 64];
+    __shared__ Part lds[256 / 64];
     const int64_t row = blockIdx.y;
     const int c0 = blockIdx.x * a.run, c1 = min(c0 + a.run, a.n);
-    float M = -INFINITY, L = 0.f;
+    float M = -INFINITY;
+    double L = 0.0;
     for (int i = threadIdx.x; i < a.parts; i += 256) {
-        const f32x2 v = *reinterpret_cast<const f32x2*>(a.part + 2 * (row * a.parts + i));
-        join(a, M, L, v[0], v[1]);
+        const Part v = a.part[row * a.parts + i];
+        join(a, M, L, v.max, v.sum);
     }
     join_block<256>(a, M, L, lds);
     write_row<T, 256>(a, row, c0, c1, finite(M), inverse(M, L));
@@ -540,7 +562,7 @@ extern "C" {
 __attribute__((visibility("default"))) size_t ythip_token_probs_workspace_size(int rows, int n) {
     if (rows <= 0 || n <= 0) return 0;
     const ProbsPlan p = probs_plan(rows, n);
-    return p.parts > 1 ? (size_t)rows * p.parts * 2 * sizeof(float) : 0;
+    return p.parts > 1 ? (size_t)rows * p.parts * sizeof(Part) : 0;
 }
 
 __attribute__((visibility("default"))) int ythip_token_probs(int dtype, int rows, int n, const void* logits, int64_t ld,
@@ -565,7 +587,7 @@ __attribute__((visibility("default"))) int ythip_token_probs(int dtype, int rows
     const double scale = 1.4426950408889634 / (double)temperature;
     if (!(scale < 1e38) || !(scale > 1e-36)) return fail(YTHIP_EUNSUPPORTED, "%s: temperature %g", who, temperature);
     const ProbsArgs a = {rows, n, p.parts, p.run, logits, ld, ld_out, (float)scale, (float)(scale - (double)(float)scale), (float)(-200.0 / scale), probs,
-                         static_cast<float*>(workspace)};
+                         static_cast<Part*>(workspace)};
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto t) {
         using T = decltype(t);
