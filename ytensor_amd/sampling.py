@@ -61,16 +61,18 @@ def _matrices(logits, out, n):
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor | None:
-    """t as [rows, n] without a copy; None where its rows do not lie at one stride, or its last dim is not contiguous."""
+    """t as [rows, n] without a copy; None where its rows do not lie at one stride, one behind the other, or its last dim is
+    not contiguous."""
     n = t.shape[-1]
     if n > 1 and t.stride(-1) != 1:
         return None
     if t.numel() == 0:
         return t.new_empty((0, n))
     try:
-        return t.view(-1, n)
+        m = t.view(-1, n)
     except RuntimeError:
         return None
+    return m if m.shape[0] == 1 or m.stride(0) >= n else None
 
 
 @functools.lru_cache(maxsize=4096)
