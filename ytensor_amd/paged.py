@@ -57,6 +57,13 @@ def _device(first: torch.Tensor, *rest) -> int:
     return dev
 
 
+def _sizes(*sizes: int) -> tuple:
+    """The sizes, which the C calls take in 32 bits."""
+    if max(sizes) > 2 ** 31 - 1:
+        raise ValueError(f"sizes of {list(sizes)}: 2^31 - 1 at most")
+    return sizes
+
+
 def _away(dev: int):
     """A context that makes `dev` the current GPU, or None where it is that."""
     return None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
@@ -173,7 +180,7 @@ def _table(table: torch.Tensor, B: int) -> tuple[torch.Tensor, int, int]:
     """(table, row stride, columns)"""
     if table.dim() != 2:
         raise ValueError("table must be int32 [B, columns]")
-    columns = table.shape[1]
+    _, columns = _sizes(*table.shape)
     _ints("table", table, (B, columns))
     ld, step = table.stride()
     if step != 1 and columns > 1:
