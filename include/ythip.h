@@ -709,7 +709,8 @@ int ythip_paged_attn_q4(int dtype, int B, int Hq, int Hkv, int T, int d, const v
 /*
  * probs[r] = softmax(logits[r] / temperature) over n columns, in fp32, of rows at strides
  * ld and ld_out (>= n; any alignment of an element). -inf has probability 0, a row of them
- * zeros; NaN or +inf makes its row NaN. temperature > 0 (YTHIP_EUNSUPPORTED from about 1e36). rows < 2^22. Workspace:
+ * zeros; NaN or +inf makes its row NaN. temperature > 0 (YTHIP_EUNSUPPORTED from about 1e36). rows < 2^22. probs may
+ * be logits (fp32, the same strides), else they share no memory. Workspace:
  * ythip_token_probs_workspace_size bytes, 8-byte aligned (0: NULL is accepted).
  */
 size_t ythip_token_probs_workspace_size(int rows, int n);
@@ -734,7 +735,9 @@ int ythip_token_probs(int dtype, int rows, int n, const void* logits, int64_t ld
  * all of them. What is not a positive number has no weight; a token outside [0, V) is never
  * kept. All of it in 64 bits. path int32 [B][T]: the kept tokens' numbers, then -1; kept
  * int32 [B]; next int32 [B], -1 where tree_len is 0 or the row has no weight. T <= 1024,
- * V <= 2^22, B <= 65535. Workspace: ythip_verify_drafts_workspace_size bytes, 8-byte aligned.
+ * V <= 2^22, B <= 65535. path, kept and next share no memory with each other nor with what is
+ * read (next may be tokens where T is 1). Workspace: ythip_verify_drafts_workspace_size bytes,
+ * 8-byte aligned.
  */
 size_t ythip_verify_drafts_workspace_size(int B, int V);
 int ythip_verify_drafts(int dtype, int B, int T, int V, const void* target, const int64_t target_str[2],

@@ -49,3 +49,51 @@ def test_sizes_past_32_bits():
     new = torch.zeros(1, 1, 1, 1, 64, device="cuda").expand(1, 1, 1, much, 64)
     with pytest.raises(ValueError, match="2\\^31"):
         yt.cache_append_q4(new, new, pool, pool, ints([[0]]), ints([0]), 16)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 33), (3, 151936), (200, 33), (200, 80001)])
+def test_probs_in_place(rows, n):
+    """float32 logits as their own output, in parts and a workgroup a row, and the two halves of one buffer's rows."""
+    x = logits((rows, n), torch.float32, n)
+    want = yt.token_probs(x, 0.8)
+    both = torch.cat([x, torch.zeros_like(x)], 1)
+    assert yt.token_probs(both[:, :n], 0.8, out=both[:, n:]).data_ptr() == both.data_ptr() + 4 * n
+    assert torch.equal(both[:, n:], want) and torch.equal(both[:, :n], x)
+    assert yt.token_probs(both[:, :n], 0.8, out=both[:, :n]).data_ptr() == both.data_ptr()
+    assert torch.equal(both[:, :n], want)
+    yt.token_probs(x, 0.8, out=x)
+    assert torch.equal(x, want)
+    if rows > 1:
+        with pytest.raises(yt.YthipError):
+            yt.token_probs(x[:-1], out=x[1:])
+
+
+def step(B, T, V, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    target = torch.softmax(3.0 * torch.randn(B, T, V, generator=g), -1).cuda()
+    tokens = torch.multinomial(target.reshape(-1, V).cpu(), 1, generator=g).reshape(B, T).int().cuda()
+    return target, tokens, torch.rand(B, T, generator=g).cuda(), torch.rand(B, generator=g).cuda()
+
+
+def test_outputs_of_a_verification_share_nothing():
+    """Outputs over inputs or over each other are refused; those in the gaps of a buffer's rows, and the next token over the
+    only one, are as those in memory of their own."""
+    B, T, V = 4, 5, 40
+    args = step(B, T, V)
+    lens = ints([5, 4, 0, 1])
+    parents = ints([[0, 0, 1, 1, 2]] * B)
+    want = yt.verify_drafts(*args, parents=parents, tree_len=lens)
+    ok = lambda: [torch.zeros_like(t) for t in want]  # noqa: E731
+    for out in ((args[1], ok()[1], ok()[2]), (parents, ok()[1], ok()[2]), (ok()[0], lens, ok()[2]), (ok()[0], want[1], want[1])):
+        with pytest.raises(yt.YthipError):
+            yt.verify_drafts(*args, parents=parents, tree_len=lens, out=tuple(out))
+    flat = torch.zeros(B * T + 2 * B, dtype=torch.int32, device="cuda")
+    out = (flat[: B * T].view(B, T), flat[B * T: B * T + B], flat[B * T + B:])
+    yt.verify_drafts(*args, parents=parents, tree_len=lens, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    # the next token over the only one
+    args = step(B, 1, V, 1)
+    want = yt.verify_drafts(*args, tree_len=ints([1, 1, 0, 1]))
+    out = (torch.zeros_like(want[0]), torch.zeros_like(want[1]), args[1][:, 0])
+    yt.verify_drafts(*args, tree_len=ints([1, 1, 0, 1]), out=out)
+    assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -548,6 +548,20 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
     if (lane == 0) a.next[b] = token;
 }
 
+// Rows of `width` bytes at a stride of `ld`; whether two such share a byte (taken to where rows lie side by side at strides
+// that differ).
+struct Block {
+    const void* at;
+    int64_t rows, ld, width;
+};
+bool meet(const Block& a, const Block& b) {
+    if (a.at == nullptr || b.at == nullptr || !overlap(span_of(a.at, 1, {{a.rows, a.ld}, {a.width, 1}}), span_of(b.at, 1, {{b.rows, b.ld}, {b.width, 1}}))) return false;
+    if (a.rows > 1 && b.rows > 1 && a.ld != b.ld) return true;
+    if (a.rows == 1 && b.rows == 1) return true;
+    const int64_t ld = a.rows > 1 ? a.ld : b.ld, apart = (int64_t)((uintptr_t)b.at - (uintptr_t)a.at) % ld, off = apart < 0 ? apart + ld : apart;
+    return off < a.width || ld - off < b.width;
+}
+
 size_t verify_bytes(int B, int V) {
     return B > 0 && V > 0 ? (size_t)B * (((V + RUN - 1) / RUN) * 2 * sizeof(double) + 4 * sizeof(int32_t)) : 0;
 }
@@ -586,6 +600,10 @@ __attribute__((visibility("default"))) int ythip_token_probs(int dtype, int rows
         return fail(YTHIP_EINVAL, "%s: needs an 8-byte aligned workspace of %zu bytes, got %zu", who, need, ws_bytes);
     const double scale = 1.4426950408889634 / (double)temperature;
     if (!(scale < 1e38) || !(scale > 1e-36)) return fail(YTHIP_EUNSUPPORTED, "%s: temperature %g", who, temperature);
+    const Block from = {logits, rows, ld * (int64_t)es, n * (int64_t)es}, to = {probs, rows, ld_out * 4, n * 4ll};
+    // (in place each element is read before it is written, by one thread)
+    if (meet(from, to) && !(logits == probs && dtype == YTHIP_F32 && (rows == 1 || ld == ld_out)))
+        return fail(YTHIP_EINVAL, "%s: probs lies over logits (float32 alone, element on element, may)", who);
     const ProbsArgs a = {rows, n, p.parts, p.run, logits, ld, ld_out, (float)scale, (float)(scale - (double)(float)scale), (float)(-200.0 / scale), probs,
                          static_cast<Part*>(workspace)};
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -630,6 +648,20 @@ __attribute__((visibility("default"))) int ythip_verify_drafts(
     const size_t need = verify_bytes(B, V);
     if (workspace == nullptr || ws_bytes < need || ((uintptr_t)workspace & 7) != 0)
         return fail(YTHIP_EINVAL, "%s: needs an 8-byte aligned workspace of %zu bytes, got %zu", who, need, ws_bytes);
+    const Block row = {nullptr, 1, 0, B * 4ll};
+    auto at = [](Block b, const void* p) { return Block{p, b.rows, b.ld, b.width}; };
+    auto tokens_at = [&](const void* p, int64_t ld) { return Block{p, B, ld * 4, T * 4ll}; };
+    const Block read[] = {tokens_at(tokens, ld_tokens), tokens_at(parents, ld_parents), tokens_at(u, ld_u), at(row, tree_len), at(row, u_next),
+                          {workspace, 1, 0, (int64_t)need}};
+    const Block written[] = {tokens_at(path, ld_path), at(row, kept), at(row, next)};
+    for (const Block& w : written) {
+        // (the last launch writes next[b] behind its own reads: it may be the tokens where there is one a sequence)
+        const bool same = w.at == next && T == 1 && tokens == next && (B == 1 || ld_tokens == 1);
+        for (const Block& x : read)
+            if (meet(w, x) && !(same && x.at == tokens)) return fail(YTHIP_EINVAL, "%s: path, kept or next lies over what is read", who);
+        for (const Block& x : written)
+            if (&x != &w && meet(w, x)) return fail(YTHIP_EINVAL, "%s: path, kept and next lie over each other", who);
+    }
     VerifyArgs a;
     a.B = B, a.T = T, a.V = V, a.slices = (V + SLICE - 1) / SLICE, a.runs = (V + RUN - 1) / RUN;
     a.target = target, a.draft = draft;

@@ -23,7 +23,8 @@ from .paged import _away, _device, _i64, _ints, _packed, _sizes
 def token_probs(logits: torch.Tensor, temperature: float = 1.0, out: torch.Tensor | None = None,
                 workspace: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(logits / temperature) over the last dim, in float32 (out: float32 of logits' shape). A logit of -inf has
-    probability 0, a row of them zeros; a NaN or +inf makes its row NaN. temperature > 0."""
+    probability 0, a row of them zeros; a NaN or +inf makes its row NaN. temperature > 0. out may be float32 logits
+    themselves, else it shares no memory with them."""
     away = _away(_device(logits, out, workspace))
     if away is not None:
         with away:
@@ -125,8 +126,8 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, u
     no weight. Decided in 64 bits.
 
     Returns (path, kept, token), int32 [B, T], [B], [B]: the kept tokens' numbers, then -1; how many; the next token (-1
-    where tree_len is 0 or the row has no weight). out: three such tensors to write. At most 1024 tokens a sequence and
-    2^22 entries."""
+    where tree_len is 0 or the row has no weight). out: three such tensors to write, in memory of their own (the last may
+    be the tokens where T is 1). At most 1024 tokens a sequence and 2^22 entries."""
     away = _away(_device(target, tokens, u, u_next, draft, parents, tree_len, workspace, *(out or ())))
     if away is not None:
         with away:
