@@ -678,7 +678,8 @@ int ythip_cache_append_q4(int dtype, int layers, int B, int Hkv, int T, int d, c
                           const int32_t* n_new, const int32_t* new_len, const int32_t* path, int64_t ld_path,
                           int32_t* status, void* stream);
 
-/* The values of whole pools, in dtype: K and V contiguous [layers][pages][Hkv][page][d]. */
+/* The values of whole pools, in dtype: K and V contiguous [layers][pages][Hkv][page][d], in
+ * memory of their own. */
 int ythip_cache_unpack_q4(int dtype, int layers, int pages, int Hkv, int page, int d, const void* Kp, const void* Vp,
                           const int64_t pool_str[3], void* K, void* V, void* stream);
 

@@ -1309,6 +1309,13 @@ __attribute__((visibility("default"))) int ythip_cache_unpack_q4(int dtype, int 
     a.K = static_cast<char*>(K), a.V = static_cast<char*>(V);
     const double grid = 2.0 * layers * pages * Hkv * (page / 16);
     if (grid >= 2147483648.0 / (16 * d / 8)) return fail(YTHIP_EUNSUPPORTED, "%s: %.0f workgroups", who, grid);
+    const int64_t values = (int64_t)layers * pages * Hkv * page * d, es = dtype == YTHIP_F32 ? 4 : 2;
+    const Span k = span_of(K, es, {{values, 1}}), v = span_of(V, es, {{values, 1}});
+    for (const void* pool : {Kp, Vp}) {
+        const Span from = span_of(pool, 1, {{layers, a.ps[0]}, {pages, a.ps[1]}, {Hkv, a.ps[2]}, {block_bytes(page, d), 1}});
+        if (overlap(k, from) || overlap(v, from)) return fail(YTHIP_EINVAL, "%s: K or V lies over the pools", who);
+    }
+    if (overlap(k, v)) return fail(YTHIP_EINVAL, "%s: K and V lie over each other", who);
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto t) {
         using T_ = decltype(t);

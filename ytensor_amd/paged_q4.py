@@ -111,7 +111,7 @@ def cache_append_q4(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
 def cache_unpack_q4(k_pool: torch.Tensor, v_pool: torch.Tensor, page: int, dtype: torch.dtype = torch.float32,
                     out=None) -> tuple[torch.Tensor, torch.Tensor]:
     """What 4-bit pools [L, P, Hkv, bytes] hold, as K and V [L, P, Hkv, page, d] of `dtype` (out: two such contiguous
-    tensors to write), whatever their rows are in use for. Values that the type cannot hold are rounded to it."""
+    tensors to write, in memory of their own), whatever their rows are in use for. Values that the type cannot hold are rounded to it."""
     away = _away(_device(k_pool, v_pool, *(out or ())))
     if away is not None:
         with away:
