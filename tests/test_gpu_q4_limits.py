@@ -91,3 +91,50 @@ def test_weights_far_below_the_largest(dtype, steps, d, T, n):
         tol = (f.eps / 2 + off) * want + least / 2 + (2.0 ** -50 * values[keys].sum(0) if dt == torch.float16 else 0.0)
         worst = ((out[0, :, t] - want).abs() / tol).max().item()
         assert worst <= 1.0, (t, worst)
+
+
+def cancelling(g, T, n, d, dt, scale):
+    """One head: q, new rows and n cached ones, where each token's own V is such that its result is all but 0: what is
+    left of it is the weights' error, for the result's own rounding is as small as the result."""
+    q, k, v = torch.randn(T, d, generator=g).to(dt), torch.randn(n, d, generator=g).to(dt), torch.randn(n, d, generator=g).to(dt)
+    # a score of log(n + t) + 1: a third or so of the weight is the token's own
+    long = torch.log(n + 1.0 + torch.arange(T)).add(1)[:, None] / (scale * q.float().square().sum(-1, keepdim=True))
+    kn, vn = (q.float() * long).to(dt), torch.zeros(T, d, dtype=dt)
+    return q, k, v, kn, vn
+
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 16), ("f16", 16), ("f32", 24)])
+@pytest.mark.parametrize("T", [1, 10, 40, 140])
+@pytest.mark.parametrize("d,pages", [(64, "4 bits"), (128, "4 bits"), (64, "values"), (128, "values")])
+def test_weights_keep_their_bits(dtype, bits, T, d, pages):
+    """Results that cancel, within 2^-bits of sum p |v| for the weights; a score and its exponential (d + 3) 2^-24 S and
+    2^-22, S = scale sum |q k|, sums over n keys n 2^-24, each for the numerator and the denominator; half a step of the
+    result. (With a weight's first 8 bits alone, or with the bits behind them of another key, it is 14 to 110 times the bound.)"""
+    dt, page, n, scale = DT[dtype], 16, 37, 1.0 / math.sqrt(d)
+    g = torch.Generator().manual_seed(10 * T + d)
+    q, k, v, kn, vn = cancelling(g, T, n, d, dt, scale)
+    if pages == "values":
+        pad = lambda x: torch.nn.functional.pad(x, (0, 0, 0, -n % page)).view(-1, 1, page, d)  # noqa: E731
+        pools = (pad(k).cuda(), pad(v).cuda(), ints([list(range(-(-n // page)))]), ints([n]))
+        kc, vc = k.double(), v.double()
+    else:
+        pools, rows = pool(k[None, None], v[None, None], page)
+        _, kc, vc = rows(0, 0)
+    want, tol = torch.zeros(T, d, dtype=torch.float64), torch.zeros(T, d, dtype=torch.float64)
+    for t in range(T):
+        keys = torch.cat([kc, kn[:t + 1].double()])
+        p = torch.softmax(scale * (keys @ q[t].double()), 0)
+        vn[t] = (-(p[:-1] @ torch.cat([vc, vn[:t].double()])) / p[-1]).to(dt)
+        values = torch.cat([vc, vn[:t + 1].double()])
+        want[t] = p @ values
+        S = (scale * (keys.abs() @ q[t].double().abs())).max()
+        size = p @ values.abs()
+        tol[t] = torch.finfo(dt).eps / 2 * want[t].abs() + size * (2.0 ** -bits + 2.0 ** -24 * (2 * (d + 3) * S + 8 + 2 * len(keys)))
+    new = (q[None, None].cuda(), kn[None, None].cuda(), vn[None, None].cuda())
+    if pages == "values":
+        out = yt.paged_attention(*new, *pools)
+    else:
+        out = yt.paged_attention_q4(*new, *pools, page)
+    worst = ((out[0, 0].cpu().double() - want).abs() / tol).max().item()
+    print(f"worst error / bound {worst:.3f}, result / sum p |v| {(want.abs().max() / size.max()).item():.1e}", flush=True)
+    assert worst <= 1.0
