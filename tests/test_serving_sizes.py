@@ -27,3 +27,12 @@ def test_sizes_are_handed_on():
     assert _sizes(0, 5, (1 << 31) - 1) == (0, 5, (1 << 31) - 1)
     with pytest.raises(ValueError):
         _sizes(1, 1 << 31)
+
+
+def test_no_workspace_for_chosen_pages_with_a_window():
+    """There is no such attention: the size of one with a window alone is not that of one over chosen pages."""
+    args = (torch.bfloat16, 1, 8, 2, 1, 64, 400, 16)
+    assert yt.paged_workspace_bytes(*args, top_k=9) > 0 and yt.paged_workspace_bytes(*args, window=99, sinks=3) >= 0
+    assert yt.paged_workspace_bytes(*args, top_k=9, sinks=3) == yt.paged_workspace_bytes(*args, top_k=9)
+    with pytest.raises(ValueError, match="window"):
+        yt.paged_workspace_bytes(*args, top_k=9, window=99)

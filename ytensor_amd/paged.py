@@ -199,7 +199,9 @@ def _workspace(code, B, Hq, Hkv, T, d, columns, page, top_k, window=0, sinks=0) 
 
 def paged_workspace_bytes(dtype: torch.dtype, B: int, Hq: int, Hkv: int, T: int, d: int, columns: int, page: int,
                           top_k: int = 0, window: int = 0, sinks: int = 0) -> int:
-    """Bytes that paged_attention (top_k 0) or paged_sparse_attention writes."""
+    """Bytes that paged_attention (top_k 0) or paged_sparse_attention, which has no window, writes."""
+    if top_k and window:
+        raise ValueError(f"top_k = {top_k} and a window of {window}: attention over chosen pages has no window")
     return _workspace(_DT[dtype], B, Hq, Hkv, T, d, columns, page, top_k, *_window(window, sinks))
 
 
