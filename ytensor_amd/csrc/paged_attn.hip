@@ -910,6 +910,77 @@ __global__ __launch_bounds__(SEL) void paged_select_kernel(PagedArgs a) {
     });
 }
 
+// How a call is cut (plan_q4 in paged_q4.hip: for 4-bit pages).
+Plan plan_of(int dtype, int B, int Hkv, int G, int T, int d, int columns, int page, int top_k, int window, int sinks) {
+    const int rows = top_k > 0 ? G : (int)std::min<int64_t>((int64_t)T * G, 1 << 20);
+    Plan p;
+    // 16 rows or 32 leave the keys to the four waves; more share each staged tile between
+    // two or four of them
+    p.qt = rows <= 16 ? 1 : 2;
+    p.wr = rows <= 32 || top_k > 0 ? 1 : rows <= 64 ? 2 : 4;
+    p.kt = 16 * p.wr;
+    const int64_t all_rows = top_k > 0 ? G : (int64_t)T * G;
+    // a window leaves a row tile few keys: half the rows a workgroup where that fills the second place of the CUs
+    // (float32, d 64, 1024 tokens, window 256: 62 -> 25.7 us; 4 chunks of 512 after 4096 rows, window 4096: 196 -> 135)
+    const bool windowed = window > 0 && p.wr == 4;
+    if (windowed && (int64_t)B * Hkv * ((all_rows + 127) / 128) < SLOTS && (int64_t)B * Hkv * ((all_rows + 63) / 64) >= SLOTS / 2)
+        p.wr = 2, p.kt = 32;
+    const int rw = 16 * p.qt * p.wr;
+    p.row_tiles = (int)((all_rows + rw - 1) / rw);
+    const int64_t per = (int64_t)Hkv * p.row_tiles;
+    p.stage = 4 / p.wr;
+    // Workgroups that the work is dealt to: the 512 that run at once (of 768 that stream their own rows
+    // a third waits: 16 sequences, 1 token, up to 8192 rows 60 -> 63 us; 1024 that share tiles: a tree of 64 over
+    // 131072 rows 126 -> 146 us).
+    // Half of them where a workgroup has a CU to itself (128 rows of fp32, d 128: 136 KB of LDS) and the
+    // sequences are few, whose items are alike (a tree of 64 over 32768 rows 219 -> 198 us; 16 ragged
+    // sequences 152 -> 188 us, left as they were).
+    const bool alone = dtype == YTHIP_F32 && d == 128 && p.wr > 1 && B <= EVEN_SEQS;
+    // And half where rows are streamed and a sequence has many ranges, which are alike then and whose
+    // partials cost more than the second workgroup of a CU brings (1 token, 4 KV heads, 60000 rows 32 ->
+    // 29 us; 16 sequences, 8 heads, 4 ranges each 60 -> 67 us, left as they were).
+    const bool many = p.wr == 1 && SLOTS / per >= 8 * (int64_t)B * (top_k > 0 ? T : 1);
+    const int64_t slots = alone || many ? SLOTS / 2 : SLOTS;
+    p.short_run = p.wr > 1 ? 4 : 0;
+    const int64_t new_tiles = ((int64_t)T + p.kt - 1) / p.kt;
+    int64_t seq_rows = (int64_t)std::min(top_k > 0 ? top_k : columns, columns) * page;
+    if (window > 0) seq_rows = std::min(seq_rows, (int64_t)window + sinks + 2 * p.kt);  // (a tile more at either end)
+    const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + new_tiles, most = (tiles + p.stage - 1) / p.stage;
+    int64_t part_items = 0;
+    if (windowed && B * per >= SLOTS / 2) {
+        // Each row tile sees tiles of its own: ranges of all that one of them sees would leave most workgroups few (4 chunks
+        // of 512, window 1024 51 us, cut into ranges 72; 16 of 128, window 4096 148 and 217). That takes items of about one
+        // length: a window that is long beside most of the sequences leaves one of them nearly all of the work (chunks of
+        // 512, window 4096: over 4 times 4096 rows 154 us either way, over 4096 and three times 600 126 us, cut 82; window
+        // 16384 over 16384 and three times 600 442 and 158).
+        p.target = 0;
+        p.items = B;
+    } else if (top_k > 0) {
+        // (a token's pages in ranges of at least the stages that least_stages explains)
+        const int64_t root = std::max<int64_t>(1, (int64_t)std::ceil(std::sqrt((double)most / 20)));
+        p.target = (int)std::max<int64_t>(1, std::min((most + root - 1) / root, (slots + per * B * T - 1) / (per * B * T)));
+        p.items = (int64_t)B * T * p.target;
+        if (p.target > 1) part_items = p.items;
+    } else if (most <= WHOLE) {
+        p.target = 0;
+        p.items = B;
+    } else {
+        int64_t ranges = slots / per;
+        p.even = B <= EVEN_SEQS && B <= ranges && ranges <= 8 * B;
+        // the items at the ends of a few sequences count among the slots too
+        if (!p.even && B - 1 <= ranges / 2) ranges -= B - 1;
+        p.target = (int)std::min(std::max<int64_t>(1, ranges), B * most);
+        p.items = (int64_t)p.target + (p.even ? 0 : B - 1);
+        if (p.target > 1) part_items = p.items;  // one range holds every sequence whole
+    }
+    const int64_t part_rows = part_items * Hkv * all_rows;
+    p.part_bytes = (size_t)part_rows * d * sizeof(float);
+    p.ml_bytes = ((size_t)part_rows * 2 * sizeof(float) + 15) / 16 * 16;
+    // (the partials behind them are read 16 bytes at a time)
+    p.rank_bytes = top_k > 0 ? ((size_t)B * Hkv * T * columns * sizeof(uint64_t) + 15) / 16 * 16 : 0;
+    return p;
+}
+
 template <class T, int D, int QT, int WR, bool SPARSE, bool WIN>
 int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
     const int64_t groups = (p.items * a.Hkv + 7) / 8 * 8;

@@ -122,7 +122,6 @@ __global__ __launch_bounds__(APPEND_ROWS * D / 8) void cache_append_q4_kernel(Ap
                 if (!is) v[q] = u32x4{0u, 0u, 0u, 0u};
             }
             float top = 0.f;
-            bool odd = false;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if constexpr (W == 2) x[e] = __uint_as_float(v[e / 4][e % 4]);
@@ -1173,7 +1172,8 @@ Plan plan_q4(int dtype, int B, int Hkv, int G, int T, int d, int columns, int pa
     if (window > 0) seq_rows = std::min(seq_rows, (int64_t)window + sinks + 2 * p.kt);
     const int64_t tiles = (seq_rows + p.kt - 1) / p.kt + ((int64_t)T + p.kt - 1) / p.kt, most = (tiles + p.stage - 1) / p.stage;
     int64_t part_items = 0;
-    // (as plan_of has it: 8 chunks of 256, window 1024 46.5 us, in ranges 56.3)
+    // (no ranges, as in plan_of: 8 chunks of 256, window 1024 58 us, cut into ranges 78; with a window that is long beside
+    // most of the sequences they would be better: chunks of 512 over 4096 and three times 600 rows, window 4096 138 us, cut 91)
     if (most <= WHOLE || (window > 0 && !few && B * per >= SLOTS / 2)) {
         p.target = 0;
         p.items = B;

@@ -262,7 +262,7 @@ struct VerifyArgs {
     int32_t *path, *kept, *next;
     int64_t ld_path;
     double* sums;   // [B][2][runs]: what is left of every RUN entries, then the row as it is
-    int32_t* walk;  // [B][4]: kept, last, behind
+    int32_t* walk;  // [B][2]: last, behind
 };
 
 // What a probability weighs: one that is not a positive number has no weight.
@@ -461,8 +461,7 @@ __global__ __launch_bounds__(256) void verify_sum_kernel(VerifyArgs a) {
         return;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) {
-        int32_t* out = a.walk + 4 * b;
-        out[1] = w.last, out[2] = w.behind;
+        a.walk[2 * b] = w.last, a.walk[2 * b + 1] = w.behind;
     }
     const Rows<T> rows(a, b, w);
     constexpr int EACH = SLICE / (4 * RUN);  // runs of a wave
@@ -500,8 +499,7 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
         if (lane == 0) a.next[b] = -1;
         return;
     }
-    const int32_t* walk = a.walk + 4 * b;
-    const Walk w = {1, walk[1], walk[2]};
+    const Walk w = {1, a.walk[2 * b], a.walk[2 * b + 1]};
     const float u = a.u_next[b];
     // lane l has `per` runs in a row
     const int per = (a.runs + 63) / 64;
@@ -563,7 +561,7 @@ bool meet(const Block& a, const Block& b) {
 }
 
 size_t verify_bytes(int B, int V) {
-    return B > 0 && V > 0 ? (size_t)B * (((V + RUN - 1) / RUN) * 2 * sizeof(double) + 4 * sizeof(int32_t)) : 0;
+    return B > 0 && V > 0 ? (size_t)B * (((V + RUN - 1) / RUN) * 2 * sizeof(double) + 2 * sizeof(int32_t)) : 0;
 }
 
 }  // namespace

@@ -57,9 +57,12 @@ def _device(first: torch.Tensor, *rest) -> int:
     return dev
 
 
+MOST = 2 ** 31 - 1
+
+
 def _sizes(*sizes: int) -> tuple:
-    """The sizes, which the C calls take in 32 bits."""
-    if max(sizes) > 2 ** 31 - 1:
+    """The sizes, which the C calls take in 32 bits (asked where there are more than MOST elements: it counts in a call)."""
+    if max(sizes) > MOST:
         raise ValueError(f"sizes of {list(sizes)}: 2^31 - 1 at most")
     return sizes
 
@@ -180,7 +183,9 @@ def _table(table: torch.Tensor, B: int) -> tuple[torch.Tensor, int, int]:
     """(table, row stride, columns)"""
     if table.dim() != 2:
         raise ValueError("table must be int32 [B, columns]")
-    _, columns = _sizes(*table.shape)
+    columns = table.shape[1]
+    if table.numel() > MOST:
+        _sizes(*table.shape)
     _ints("table", table, (B, columns))
     ld, step = table.stride()
     if step != 1 and columns > 1:

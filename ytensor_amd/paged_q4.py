@@ -26,7 +26,7 @@ import torch
 from . import _lib
 from ._lib import check
 from .ops import _DT, _code, _stream
-from .paged import _away, _device, _i64, _ints, _packed, _real, _rows, _sizes, _table, _window
+from .paged import MOST, _away, _device, _i64, _ints, _packed, _real, _rows, _sizes, _table, _window
 
 
 @functools.lru_cache(maxsize=256)
@@ -77,7 +77,9 @@ def cache_append_q4(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
         raise ValueError("n_new and new_len both say how many rows there are: give one")
     if k_new.dim() != 5:
         raise ValueError("k_new must be [L, B, Hkv, T, d]")
-    L, B, Hkv, T, d = _sizes(*k_new.shape)
+    L, B, Hkv, T, d = k_new.shape
+    if k_new.numel() > MOST:
+        _sizes(*k_new.shape)
     pool_st = _blocks(k_pool, v_pool, 4)
     P = k_pool.shape[1]
     if tuple(k_pool.shape) != (L, P, Hkv, cache_q4_bytes(page, d)) or v_new.shape != k_new.shape or v_new.dtype != k_new.dtype:

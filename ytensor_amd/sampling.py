@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import check
 from .ops import _code, _stream
-from .paged import _away, _device, _i64, _ints, _packed, _sizes
+from .paged import MOST, _away, _device, _i64, _ints, _packed, _sizes
 
 
 def token_probs(logits: torch.Tensor, temperature: float = 1.0, out: torch.Tensor | None = None,
@@ -32,7 +32,7 @@ def token_probs(logits: torch.Tensor, temperature: float = 1.0, out: torch.Tenso
     code, shape = _code(logits), logits.shape
     if logits.dim() < 1:
         raise ValueError("logits must be [..., V]")
-    if logits.numel() >= 1 << 31:
+    if logits.numel() > MOST:
         _sizes(logits.numel() // shape[-1], shape[-1])
     if out is None:
         out = torch.empty(shape, dtype=torch.float32, device=logits.device)
@@ -134,7 +134,9 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, u
             return verify_drafts(target, tokens, u, u_next, draft, parents, tree_len, out, workspace)
     if target.dim() != 3:
         raise ValueError("target must be [B, T, V]")
-    B, T, V = _sizes(*target.shape)
+    B, T, V = target.shape
+    if target.numel() > MOST:
+        _sizes(B, T, V)
     code = _code(target)
     if target.stride(2) != 1 and V > 1:
         target = target.contiguous()
