@@ -530,7 +530,8 @@ enum ythip_cache_status {
  * nothing, or only scores of -inf, is zero; K and V of what a row does not see never reach
  * it, NaN and infinities included. scale == 0: 1 / sqrt(d). d in {64, 128}; strides (batch,
  * head, token), d contiguous, 16-byte aligned rows. Any of Q's type. The weights p of 16-bit
- * inputs keep 16 bits (bf16) or 21 (fp16), the rest is fp32. At most 65535 sequences and query
+ * inputs keep 16 bits (bf16) or 21 (fp16; below 2^-17 of the largest what of them is above
+ * 2^-39 of it), the rest is fp32. At most 65535 sequences and query
  * heads, T * Hq <= 2^30, fewer than 2^24 workgroups. Workspace:
  * ythip_paged_attn_workspace_size bytes (0: NULL is accepted).
  */

@@ -61,6 +61,33 @@ def test_queries_with_an_infinity(dtype, d, T, sign):
     compare(out[~where], want[~where], tol[~where])
 
 
+@pytest.mark.parametrize("window", [0, 1000])
+@pytest.mark.parametrize("steps", [8.0, 16.0, 20.0, 24.0])
+@pytest.mark.parametrize("T", [2, 66])
+def test_float16_weights_over_pools_of_values(steps, T, window):
+    """The same over float16 pools, whose weights have one unit: 21 bits of a weight, at best 2^-39 of the largest, so with
+    |v| that much a key; the rest as there."""
+    d, page, n = 64, 16, 40
+    g = torch.Generator().manual_seed(T)
+    q, kn, k = torch.zeros(1, 2, T, d), torch.zeros(1, 1, T, d), torch.zeros(1, 1, n, d)
+    q[..., 0], kn[:, :, 0, 0] = 4.0, steps / 4.0
+    vn, v = (40000.0 + 20000.0 * torch.rand(1, 1, m, d, generator=g) for m in (T, n))
+    vn[:, :, 0] = 0.0
+    q, kn, vn, k, v = (x.half() for x in (q, kn, vn, k, v))
+    pad = lambda x: torch.nn.functional.pad(x[0, 0], (0, 0, 0, -n % page)).view(-1, 1, page, d).cuda()  # noqa: E731
+    out = yt.paged_attention(q.cuda(), kn.cuda(), vn.cuda(), pad(k), pad(v), ints([list(range(-(-n // page)))]), ints([n]), scale=1.0,
+                             window=window).cpu().double()
+    values = torch.cat([vn[0, 0].double(), v[0, 0].double()])
+    for t in range(T):
+        keys = torch.cat([torch.arange(t + 1), T + torch.arange(n)])
+        w = torch.where(keys == 0, 1.0, math.exp(-steps)).double()
+        want = (w[:, None] * values[keys]).sum(0) / w.sum()
+        off = 2.0 ** -21 + 2.0 ** -23 * (steps + 4) + 2.0 ** -24 * len(keys)
+        tol = (2.0 ** -11 + off) * want + 2.0 ** -25 + 2.0 ** -39 * values[keys].sum(0)
+        worst = ((out[0, :, t] - want).abs() / tol).max().item()
+        assert worst <= 1.0, (t, worst)
+
+
 @pytest.mark.parametrize("dtype,steps", [("f16", 20.0), ("f16", 27.75), ("f16", 31.0), ("bf16", 27.75), ("f32", 27.75)])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("T,n", [(9, 0), (66, 0), (200, 40)])

@@ -309,7 +309,7 @@ __global__ __launch_bounds__(256, (Q4Shape<D, QT, WR>::waves(std::is_same_v<T, B
     __shared__ int s_inf[4];  // of the tiles of new tokens there, by stage: V holds what is not finite
     // New tokens of 16 bits go through LDS too, as they are: a wave reads a quarter of a tile, not all of it (bfloat16, chunk
     // of 2048 after 2048 rows, window 1024: 219 -> 78 us; 4096 after 64, window 2048: 560 -> 221; two chunks of 512 over 8192:
-    // 116 -> 96; float16, 2048 after 64: 169 -> 106). A single tile gains nothing, and loses nothing: five trees of 25 39.0 us,
+    // 116 -> 96; float16, 2048 after 64: 169 -> 107). A single tile gains nothing, and loses nothing: five trees of 25 39.0 us,
     // each wave by itself 39.2. LDS has no room for float32's.
     constexpr bool SHARED_NEW = SHARED && !F;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
