@@ -162,6 +162,7 @@ __global__ __launch_bounds__(APPEND_ROWS * D / 8) void cache_append_q4_kernel(Ap
 
 struct UnpackArgs {
     int layers, pages, Hkv, page;
+    int64_t first;  // workgroups of earlier launches
     const uint8_t *Kp, *Vp;
     int64_t ps[3];  // bytes
     char *K, *V;    // [layers][pages][Hkv][page][d] in a row
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(16 * D / 8) void cache_unpack_q4_kernel(UnpackArgs 
     constexpr int LPR = D / 8;
     using raw = typename T::raw;
     const int runs = a.page / 16;
-    int64_t w = blockIdx.x;
+    int64_t w = a.first + blockIdx.x;
     const int r0 = (int)(w % runs) * 16;
     w /= runs;
     const bool is_v = w % 2;
@@ -1307,8 +1308,9 @@ __attribute__((visibility("default"))) int ythip_cache_unpack_q4(int dtype, int 
     a.layers = layers, a.pages = pages, a.Hkv = Hkv, a.page = page;
     a.Kp = static_cast<const uint8_t*>(Kp), a.Vp = static_cast<const uint8_t*>(Vp);
     a.K = static_cast<char*>(K), a.V = static_cast<char*>(V);
-    const double grid = 2.0 * layers * pages * Hkv * (page / 16);
-    if (grid >= 2147483648.0 / (16 * d / 8)) return fail(YTHIP_EUNSUPPORTED, "%s: %.0f workgroups", who, grid);
+    if (2.0 * layers * pages * Hkv * (page / 16) >= 2147483648.0)
+        return fail(YTHIP_EUNSUPPORTED, "%s: %.0f workgroups (2^31 - 1 at most)", who, 2.0 * layers * pages * Hkv * (page / 16));
+    const int64_t grid = 2ll * layers * pages * Hkv * (page / 16);
     const int64_t values = (int64_t)layers * pages * Hkv * page * d, es = dtype == YTHIP_F32 ? 4 : 2;
     const Span k = span_of(K, es, {{values, 1}}), v = span_of(V, es, {{values, 1}});
     for (const void* pool : {Kp, Vp}) {
@@ -1319,8 +1321,13 @@ __attribute__((visibility("default"))) int ythip_cache_unpack_q4(int dtype, int 
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto run = [&](auto t) {
         using T_ = decltype(t);
-        if (d == 64) cache_unpack_q4_kernel<T_, 64><<<(int)grid, 128, 0, s>>>(a);
-        else cache_unpack_q4_kernel<T_, 128><<<(int)grid, 256, 0, s>>>(a);
+        // (a launch holds fewer than 2^32 threads)
+        constexpr int64_t MOST = 1 << 23;
+        for (a.first = 0; a.first < grid; a.first += MOST) {
+            const int n = (int)std::min(grid - a.first, MOST);
+            if (d == 64) cache_unpack_q4_kernel<T_, 64><<<n, 128, 0, s>>>(a);
+            else cache_unpack_q4_kernel<T_, 128><<<n, 256, 0, s>>>(a);
+        }
     };
     if (dtype == YTHIP_F32) run(F32{});
     else if (dtype == YTHIP_F16) run(F16{});
